@@ -226,6 +226,151 @@ int zs_decode_attention_paged(void* stream, const uint16_t* d_q, const ZsKvPool*
                               float softmax_scale, int num_splits, float* d_ws, size_t ws_bytes, uint16_t* d_out,
                               int* splits_used, unsigned* d_err);
 
+/* ---- Uncompressed paged KV cache: the operators of a decode step ------------
+ * No counterpart in the reference, whose serving runs on its host engine's own
+ * paged cache. Each call takes a struct of arguments (fill every field; unused
+ * pointers are NULL), reads it before it returns and works in stream order.
+ *
+ * One layout for all of them: a pool of num_blocks pages of page_size tokens (a
+ * power of two, 16..256) of num_heads KV heads, element (block, token, head, d)
+ * at block * stride_block + token * stride_token + head * stride_head + d
+ * (strides in elements, multiples of 8; base 16-byte aligned), so a page may hold
+ * its heads or its tokens outermost. Logical page p of sequence b is block
+ * block_table[b * table_stride + p], p < width. Kernels check every index that
+ * they read from a table, a list or the slots against the pool; a bad one is
+ * skipped and sets bit 2 in *err (nullable). Pointers are device memory. */
+enum { ZS_BF16 = 0, ZS_FP16 = 1 };
+typedef struct ZsPagePool {
+    void* data;
+    int64_t stride_block, stride_token, stride_head;
+    int num_blocks, page_size, num_heads, head_dim, dtype;
+} ZsPagePool;
+
+/* Block tables, slots and positions of one step, from request lengths. Request
+ * r of R (<= 8192) has seq_lens[r] tokens and gets new_lens[r] more; negative: it
+ * has ended, and its pages go back to the free list. The free list is
+ * free_blocks[0 .. *free_count), room for `capacity` entries; pages are given
+ * back at its end in order of request and page, then taken from its end. In
+ * request order, a request is admitted when the tokens asked for up to and
+ * including it are at most max_tokens (<= 2^30), its pages fit the table's width,
+ * and the pages needed up to and including it are free; one that is not admitted
+ * keeps its state, is marked in `refused` and sets bit 4 in *err. Outputs:
+ * out_lens [R], *out_count, out_cu [R + 1] (prefix sums of the admitted tokens),
+ * refused [R], and for each of max_tokens tokens its slot (block * page_size +
+ * row), request and position (-1, -1 and 0 past the last). block_table and
+ * free_blocks are updated in place; seq_lens and free_count are not (out_lens
+ * and out_count are other buffers), so a repeated call gives the same result. */
+typedef struct ZsPlanStep {
+    void* stream;
+    int* block_table;
+    int64_t table_stride;
+    const int* seq_lens;
+    const int* new_lens;
+    int* free_blocks;
+    const int* free_count;
+    int* out_lens;
+    int* out_count;
+    int* out_cu;
+    int64_t* slots;
+    int* token_seq;
+    int* positions;
+    uint8_t* refused;
+    unsigned* err;
+    int R, width, capacity, page_size, max_tokens, reserved;
+} ZsPlanStep;
+int zs_plan_step(const ZsPlanStep* args);
+
+/* Rotary positions on q and k, and k and v to their slots. q is [N][Hq][D], k
+ * and v [N][Hkv][D] with token and head strides in elements (multiples of 8);
+ * q_out [N][Hq][D] contiguous (may be q). The first `rot` (a multiple of 16)
+ * channels turn, in pairs (j, j + rot / 2) or (2j, 2j + 1) when interleaved, pair
+ * j by row positions[axis * pos_axis + n] of cos_sin [table_rows][rot] fp32 (rot
+ * / 2 cosines, then rot / 2 sines), axis the one of the `axes` (1..4) sections
+ * (sum rot / 2) that j falls in. Slots of -1 are skipped; the slots of one call
+ * are distinct. D is a multiple of 16, up to 512. */
+typedef struct ZsRopeWrite {
+    void* stream;
+    const uint16_t *q, *k, *v;
+    int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
+    uint16_t* q_out;
+    const int* positions;
+    int64_t pos_axis;
+    const float* cos_sin;
+    const int64_t* slots;
+    unsigned* err;
+    ZsPagePool k_pool, v_pool;
+    int N, Hq, axes, sections[4], table_rows, rot, interleaved;
+} ZsRopeWrite;
+int zs_rope_write(const ZsRopeWrite* args);
+
+/* Attention of one new token per sequence: out[b][i] = softmax(softmax_scale
+ * q[b][i] . K^T) V over the first seq_lens[b] tokens of the cache, KV head i /
+ * (Hq / Hkv); D is 64 or 128; q and out are [B][Hq][D], 16-byte aligned. With
+ * pages ([B][Hkv][top] distinct logical pages) and counts ([B][Hkv]) only the
+ * tokens of the listed pages count. A sequence with nothing to attend gets zeros.
+ * lse (nullable, [B][Hq]) receives log sum exp(softmax_scale q.k), -inf where
+ * nothing counts. ws: 16-byte aligned workspace of
+ * zs_paged_attention_workspace_bytes. */
+typedef struct ZsPagedAttention {
+    void* stream;
+    const uint16_t* q;
+    const int* block_table;
+    int64_t table_stride;
+    const int* seq_lens;
+    const int* pages;
+    const int* counts;
+    void* ws;
+    size_t ws_bytes;
+    uint16_t* out;
+    float* lse;
+    unsigned* err;
+    ZsPagePool k_pool, v_pool;
+    int B, Hq, width, top;
+    float softmax_scale;
+    int reserved;
+} ZsPagedAttention;
+size_t zs_paged_attention_workspace_bytes(int B, int Hq, int Hkv, int D);
+int zs_paged_attention(const ZsPagedAttention* args);
+
+/* Bounds of the pages that sequences completed between lens_before[b] and
+ * seq_lens[b] tokens (at most max_new tokens each): codes [num_blocks][num_heads]
+ * [2][D] int8 (16-byte aligned), upper then lower bound of the keys per channel in
+ * units of scales [num_blocks][num_heads], a power of two (infinite, with codes
+ * of zero, for a page with a non-finite key). D is 64, 128 or 256. */
+typedef struct ZsPageBounds {
+    void* stream;
+    const int* block_table;
+    int64_t table_stride;
+    const int* lens_before;
+    const int* seq_lens;
+    int8_t* codes;
+    float* scales;
+    unsigned* err;
+    ZsPagePool k_pool;
+    int B, width, max_new, reserved;
+} ZsPageBounds;
+int zs_page_bounds(const ZsPageBounds* args);
+
+/* Choice of up to `top` pages per (sequence, KV head) for sparse attention: the
+ * first `sinks` pages, the last `local` (>= 1) and the best of the others by the
+ * bound max_g sum_d max(q_gd up_d, q_gd lo_d) * scale, q in whole numbers, ties
+ * to the lowest page. pages [B][Hkv][top]: ascending, -1 past counts [B][Hkv].
+ * width <= 32768, Hq / Hkv <= 128, top >= sinks + local; D is 64, 128 or 256. */
+typedef struct ZsSelectPages {
+    void* stream;
+    const uint16_t* q;
+    const int8_t* codes;
+    const float* scales;
+    const int* block_table;
+    int64_t table_stride;
+    const int* seq_lens;
+    int* pages;
+    int* counts;
+    unsigned* err;
+    int dtype, B, Hq, Hkv, D, num_blocks, width, page_size, top, sinks, local, reserved;
+} ZsSelectPages;
+int zs_select_pages(const ZsSelectPages* args);
+
 /* ---- On-disk TCA-TBE container (file format version 1) -------------------
  * No counterpart in the reference, which keeps no serialised compressed form
  * (its benchmarks re-encode the dense checkpoint at start-up,

@@ -1,0 +1,248 @@
+// Step plan of a paged KV cache: block tables, slots and positions from request
+// lengths, on the GPU (zs_plan_step).
+//
+// With page size P, request r of length len[r] gets new[r] tokens (negative: it
+// has ended). In request order:
+//   back[r]  = pages of an ended request, appended to the free list
+//   fits[r]  = its tokens fit the step's room, its pages the table's width, and
+//              its new pages the free list (by inclusive prefix sums)
+//   need[r]  = ceil((len + new) / P) - ceil(len / P) where it fits
+//   page j of the step (exclusive prefix of need) = free[have - 1 - j]
+//   token t of the step: request by the prefix sums of the admitted tokens,
+//   position len + rank, slot = table[r][pos / P] * P + pos % P.
+//
+// What bounds it: nothing but latency (16 bytes a token; 131 thousand tokens
+// are 2 MB, 0.3 us of HBM). So it is one launch: every CTA repeats the three
+// prefix sums over the requests in shared memory, each thread holding a
+// contiguous run of them (three block scans whatever the request count), and
+// then writes its share of the tokens, table entries and free-list entries by
+// binary search in the prefix sums. No CTA reads what another writes: inputs
+// `lens` and `count` are not updated in place, taken pages are looked up by
+// formula and not in the table, and a taken page that was given back in the
+// same step is found in the ended request's row and not in the free list.
+#include <algorithm>
+
+#include "paged.cuh"
+
+namespace zs {
+namespace {
+
+constexpr int kPlanThreads = 512;
+constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kPlanMaxRequests = 8192;
+
+struct PlanArgs {
+    int* table;
+    long long table_stride;
+    int R, width, page_shift, max_tokens, capacity;
+    const int* lens;
+    const int* fresh;
+    int* free_list;
+    const int* count;
+    int* out_lens;
+    int* out_count;
+    int* out_cu;
+    long long* slots;
+    int* token_seq;
+    int* positions;
+    uint8_t* refused;
+    unsigned* err;
+};
+
+// Exclusive prefix of v over the block's threads; *total gets the block's sum.
+// `part` is this scan's own kPlanWarps entries of shared memory.
+__device__ __forceinline__ long long block_scan(long long v, long long* part, long long* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(~0u, inc, o);
+        if (lane >= o) inc += u;
+    }
+    if (lane == 31) part[warp] = inc;
+    __syncthreads();
+    long long w = lane < kPlanWarps ? part[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < kPlanWarps; o <<= 1) {
+        const long long u = __shfl_up_sync(~0u, w, o);
+        if (lane >= o) w += u;
+    }
+    const long long before = __shfl_sync(~0u, w, warp ? warp - 1 : 0);
+    *total = __shfl_sync(~0u, w, kPlanWarps - 1);
+    return inc - v + (warp ? before : 0);
+}
+
+// Largest r in [0, n) with pre[r] <= x (pre ascending, pre[0] == 0).
+__device__ __forceinline__ int owner(const int* pre, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pre[mid] <= x) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
+    extern __shared__ int plan_smem[];
+    __shared__ long long parts[4][kPlanWarps];
+    __shared__ int s_taken;            // pages taken by the step
+    if (threadIdx.x == 0) s_taken = 0;
+    int* cu = plan_smem;               // [R + 1] admitted tokens before request r
+    int* need0 = cu + a.R + 1;         // [R] pages taken before request r
+    int* back0 = need0 + a.R + 1;      // [R + 1] pages given back before request r
+    const int R = a.R, sh = a.page_shift, P1 = (1 << sh) - 1;
+    const int per = (R + kPlanThreads - 1) / kPlanThreads;
+    const int r0 = min(R, (int)threadIdx.x * per), r1 = min(R, r0 + per);
+    const int len_cap = (int)min((long long)a.width << sh, (long long)INT_MAX - P1);
+
+    auto length = [&](int r) { return max(0, min(a.lens[r], len_cap)); };
+    // 1. pages given back, tokens asked for
+    long long back_sum = 0, want_sum = 0;
+    for (int r = r0; r < r1; ++r) {
+        const int f = a.fresh[r];
+        if (f < 0) back_sum += (length(r) + P1) >> sh;
+        else want_sum += f;
+    }
+    long long back_total, want_total, need_total, got_total;
+    long long back = block_scan(back_sum, parts[0], &back_total);
+    long long want = block_scan(want_sum, parts[1], &want_total);
+    const int count0 = max(0, min(*a.count, a.capacity));
+    const long long have = min((long long)count0 + back_total, (long long)a.capacity);
+    // 2. pages needed by the requests that fit the step and the table
+    auto pages_needed = [&](int r, long long want_end) -> int {
+        const int f = a.fresh[r], len = length(r);
+        const long long pages = ((long long)len + max(f, 0) + P1) >> sh;
+        if (f < 0 || want_end > a.max_tokens || pages > a.width) return -1;
+        return (int)(pages - ((len + P1) >> sh));
+    };
+    long long need_sum = 0;
+    long long w = want;
+    for (int r = r0; r < r1; ++r) {
+        w += max(a.fresh[r], 0);
+        need_sum += max(pages_needed(r, w), 0);
+    }
+    long long need = block_scan(need_sum, parts[2], &need_total);
+    // 3. admitted tokens
+    long long got_sum = 0;
+    w = want;
+    long long n = need;
+    for (int r = r0; r < r1; ++r) {
+        const int f = a.fresh[r];
+        w += max(f, 0);
+        const int p = pages_needed(r, w);
+        n += max(p, 0);
+        if (p == 0 || (p > 0 && n <= have)) got_sum += f;
+    }
+    long long got = block_scan(got_sum, parts[3], &got_total);
+    w = want;
+    n = need;
+    const bool first = blockIdx.x == 0;
+    bool any_refused = false;
+    int end = 0;
+    for (int r = r0; r < r1; ++r) {
+        const int f = a.fresh[r], len = length(r);
+        w += max(f, 0);
+        const int p = pages_needed(r, w);
+        const bool ok = p == 0 || (p > 0 && n + p <= have);
+        cu[r] = (int)got;
+        need0[r] = (int)min(n, have);       // exact for every admitted request that takes pages
+        back0[r] = (int)back;
+        if (first) {
+            a.out_lens[r] = f < 0 ? 0 : len + (ok ? f : 0);
+            a.out_cu[r] = (int)got;
+            a.refused[r] = !ok && f > 0;
+        }
+        any_refused |= !ok && f > 0;
+        n += max(p, 0);
+        if (ok && p > 0) end = (int)n;
+        if (ok) got += f;
+        if (f < 0) back += (len + P1) >> sh;
+    }
+    // Admission is by inclusive prefix, so the requests refused for want of
+    // pages are the last ones that need any: the pages taken end where the last
+    // admitted request's do.
+    if (end) atomicMax(&s_taken, end);
+    if (threadIdx.x == 0) {
+        cu[R] = (int)got_total;
+        back0[R] = (int)back_total;
+    }
+    if (first && any_refused) set_err(a.err, kErrPagedFull);
+    __syncthreads();
+    const int used = s_taken;
+    if (first && threadIdx.x == 0) {
+        a.out_cu[R] = cu[R];
+        *a.out_count = (int)have - used;
+        if (back_total + count0 > a.capacity) set_err(a.err, kErrPagedIndex);
+    }
+
+    // the page at position x of the free list once the ended requests' pages are on it
+    auto free_page = [&](int x) -> int {
+        if (x < count0) return a.free_list[x];
+        const int b = x - count0;
+        const int r = owner(back0, R, b);
+        return a.table[(long long)r * a.table_stride + (b - back0[r])];
+    };
+    const int gid = blockIdx.x * kPlanThreads + threadIdx.x, gsize = gridDim.x * kPlanThreads;
+    // give pages back (the free list has room for every page of the pool)
+    const int nback = (int)(have - count0);
+    for (int i = gid; i < nback; i += gsize) a.free_list[count0 + i] = free_page(count0 + i);
+    // new table entries
+    for (int j = gid; j < used; j += gsize) {
+        const int r = owner(need0, R, j);
+        const int col = ((length(r) + P1) >> sh) + (j - need0[r]);
+        a.table[(long long)r * a.table_stride + col] = free_page((int)have - 1 - j);
+    }
+    // tokens
+    const int tokens = cu[R];
+    for (int t = gid; t < a.max_tokens; t += gsize) {
+        long long slot = -1;
+        int r = -1, pos = 0;
+        if (t < tokens) {
+            r = owner(cu, R, t);
+            const int len = length(r);
+            pos = len + (t - cu[r]);
+            const int col = pos >> sh, old = (len + P1) >> sh;
+            const int blk = col < old ? a.table[(long long)r * a.table_stride + col]
+                                      : free_page((int)have - 1 - (need0[r] + col - old));
+            slot = ((long long)blk << sh) + (pos & P1);
+        }
+        a.slots[t] = slot;
+        a.token_seq[t] = r;
+        a.positions[t] = pos;
+    }
+}
+
+}  // namespace
+}  // namespace zs
+
+extern "C" int zs_plan_step(const ZsPlanStep* p) {
+    using namespace zs;
+    if (!p || p->R <= 0 || p->R > kPlanMaxRequests || p->width <= 0 || p->capacity <= 0 || p->max_tokens < 0 ||
+        p->max_tokens > (1 << 30))
+        return cudaErrorInvalidValue;
+    const int R = p->R, page_size = p->page_size, max_tokens = p->max_tokens;
+    if ((int64_t)R * p->width > INT32_MAX || p->table_stride < p->width) return cudaErrorInvalidValue;
+    if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1))) return cudaErrorInvalidValue;
+    if (!p->block_table || !p->seq_lens || !p->new_lens || !p->free_blocks || !p->free_count || !p->out_lens ||
+        !p->out_count || !p->out_cu || !p->refused || (max_tokens && (!p->slots || !p->token_seq || !p->positions)))
+        return cudaErrorInvalidValue;
+    // every CTA repeats the prefix sums from these; the outputs are other buffers
+    if (p->out_lens == p->seq_lens || p->out_count == p->free_count) return cudaErrorInvalidValue;
+    PlanArgs a{p->block_table, p->table_stride, R, p->width, 0, max_tokens, p->capacity, p->seq_lens, p->new_lens,
+               p->free_blocks, p->free_count, p->out_lens, p->out_count, p->out_cu,
+               reinterpret_cast<long long*>(p->slots), p->token_seq, p->positions, p->refused, p->err};
+    while ((1 << a.page_shift) < page_size) ++a.page_shift;
+    const size_t smem = 3 * sizeof(int) * ((size_t)R + 1);
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+    }
+    const int grid = std::max(1, std::min(148, (max_tokens + kPlanThreads - 1) / kPlanThreads));
+    plan_kernel<<<grid, kPlanThreads, smem, (cudaStream_t)p->stream>>>(a);
+    return cudaGetLastError();
+}
+
+// The argument structs' sizes, as bindings pack them.
+static_assert(sizeof(ZsPagePool) == 56 && sizeof(ZsPlanStep) == 144 && sizeof(ZsRopeWrite) == 280 &&
+                  sizeof(ZsPagedAttention) == 232 && sizeof(ZsPageBounds) == 136 && sizeof(ZsSelectPages) == 128,
+              "argument struct layout");

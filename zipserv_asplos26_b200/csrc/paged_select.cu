@@ -1,0 +1,390 @@
+// Bounds of complete pages in 8 bits (zs_page_bounds) and the choice of a
+// sequence's pages by those bounds (zs_select_pages).
+//
+// Bounds, per page and KV head, from its keys k[t][d]: with
+//   s    = 2^floor(log2 max |k|) / 64            (a power of two: dividing by it is exact)
+//   up_d = ceil(max_t k[t][d] / s), lo_d = floor(min_t k[t][d] / s), within +-127
+// so up_d * s and lo_d * s bound every key of the page but for the clamp.
+//
+// Score of a page for a query group of G heads sharing the KV head: with q
+// rounded to whole numbers within +-127 by a power of two common to the group,
+//   score = max_g sum_d (q_gd > 0 ? q_gd * up_d : q_gd * lo_d) * s.
+// The sums are whole numbers below 2^24 for head dims up to 512 and s is a power
+// of two, so a score is exact in fp32 in any order of summation and the choice
+// is the same on every run and in every implementation. A page with a NaN or an
+// infinity has s = inf and is chosen before all scored ones.
+#include <algorithm>
+#include <cmath>
+
+#include "paged.cuh"
+
+namespace zs {
+namespace {
+
+// ------------------------------------------------------------------ bounds
+// One warp reduces one page of one KV head: a lane holds 8 channels of every
+// (32 / (D / 8))-th token, running maximum and minimum as packed 16-bit pairs
+// (exact), 16-byte loads. Bound by HBM: the keys are read once.
+constexpr int kBoundsThreads = 256;
+
+struct BoundsArgs {
+    PoolView kp;
+    const int* table;
+    long long table_stride;
+    int B, width, per_seq;
+    const int* before;
+    const int* lens;
+    int8_t* codes;     // [num_blocks][heads][2][D]
+    float* scales;     // [num_blocks][heads]
+    unsigned* err;
+};
+
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b, __nv_bfloat16) {
+    const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b, __nv_bfloat16) {
+    const __nv_bfloat162 r = __hmin2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b, __half) {
+    const __half2 r = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b, __half) {
+    const __half2 r = __hmin2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const BoundsArgs a) {
+    constexpr int kLanes = D / 8;            // lanes a token
+    constexpr int kRows = 32 / kLanes;       // tokens a pass
+    const int lane = threadIdx.x & 31;
+    const long long warp = (long long)blockIdx.x * (kBoundsThreads / 32) + (threadIdx.x >> 5);
+    const int h = (int)(warp % a.kp.heads);
+    const long long bj = warp / a.kp.heads;
+    const int b = (int)(bj / a.per_seq), j = (int)(bj % a.per_seq);
+    if (b >= a.B) return;
+    const int sh = a.kp.page_shift;
+    const int before = max(a.before[b], 0);
+    const int last = min(a.lens[b] >> sh, a.width);
+    const int p = (before >> sh) + j;        // pages [before / P, len / P) became complete
+    if (p >= last) return;
+    const int blk = a.table[b * a.table_stride + p];
+    if (blk < 0 || blk >= a.kp.num_blocks) {
+        if (lane == 0) set_err(a.err, kErrPagedIndex);
+        return;
+    }
+    const int c = lane % kLanes, r0 = lane / kLanes;
+    const uint16_t* base = static_cast<const uint16_t*>(a.kp.data) + blk * a.kp.s_block + h * a.kp.s_head + c * 8;
+    uint4 hi = ld_nc16(base + r0 * a.kp.s_token), lo = hi;
+    auto fold = [&](const uint4& x) {
+        hi.x = max2_nan(hi.x, x.x, T()); hi.y = max2_nan(hi.y, x.y, T());
+        hi.z = max2_nan(hi.z, x.z, T()); hi.w = max2_nan(hi.w, x.w, T());
+        lo.x = min2_nan(lo.x, x.x, T()); lo.y = min2_nan(lo.y, x.y, T());
+        lo.z = min2_nan(lo.z, x.z, T()); lo.w = min2_nan(lo.w, x.w, T());
+    };
+    const int page = 1 << sh;
+#pragma unroll 8
+    for (int r = r0 + kRows; r < page; r += kRows) fold(ld_nc16(base + r * a.kp.s_token));
+#pragma unroll
+    for (int o = kLanes; o < 32; o <<= 1) {
+        hi.x = max2_nan(hi.x, __shfl_xor_sync(~0u, hi.x, o), T()); hi.y = max2_nan(hi.y, __shfl_xor_sync(~0u, hi.y, o), T());
+        hi.z = max2_nan(hi.z, __shfl_xor_sync(~0u, hi.z, o), T()); hi.w = max2_nan(hi.w, __shfl_xor_sync(~0u, hi.w, o), T());
+        lo.x = min2_nan(lo.x, __shfl_xor_sync(~0u, lo.x, o), T()); lo.y = min2_nan(lo.y, __shfl_xor_sync(~0u, lo.y, o), T());
+        lo.z = min2_nan(lo.z, __shfl_xor_sync(~0u, lo.z, o), T()); lo.w = min2_nan(lo.w, __shfl_xor_sync(~0u, lo.w, o), T());
+    }
+    float up[8], dn[8];
+    const uint32_t hw[4] = {hi.x, hi.y, hi.z, hi.w}, lw[4] = {lo.x, lo.y, lo.z, lo.w};
+    uint32_t most = 0;       // bits of max |k|: unsigned order is magnitude order, NaN above infinity
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 u = unpack2<T>(hw[i]), w = unpack2<T>(lw[i]);
+        up[2 * i] = u.x; up[2 * i + 1] = u.y;
+        dn[2 * i] = w.x; dn[2 * i + 1] = w.y;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        most = max(most, max(__float_as_uint(up[i]) & 0x7FFFFFFFu, __float_as_uint(dn[i]) & 0x7FFFFFFFu));
+    most = __reduce_max_sync(~0u, most);
+    const bool finite = most < 0x7F800000u;
+    const float power = __uint_as_float(most & 0x7F800000u);      // 2^floor(log2 max), 0 for zero and subnormals
+    const bool live = finite && power > 0.f;
+    const float s = finite ? power * 0.015625f : INFINITY;
+    if (r0 == 0) {
+        uint32_t cu[2] = {0, 0}, cl[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float d = live ? s : 1.f;
+            const int u = live ? max(-127, min(127, (int)ceilf(up[i] / d))) : 0;
+            const int w = live ? max(-127, min(127, (int)floorf(dn[i] / d))) : 0;
+            cu[i / 4] |= (uint32_t)(u & 0xFF) << (8 * (i % 4));
+            cl[i / 4] |= (uint32_t)(w & 0xFF) << (8 * (i % 4));
+        }
+        int8_t* out = a.codes + ((long long)blk * a.kp.heads + h) * (2 * D) + c * 8;
+        *reinterpret_cast<uint2*>(out) = make_uint2(cu[0], cu[1]);
+        *reinterpret_cast<uint2*>(out + D) = make_uint2(cl[0], cl[1]);
+    }
+    if (lane == 0) a.scales[(long long)blk * a.kp.heads + h] = s;
+}
+
+// ------------------------------------------------------------------ choice
+// One CTA a (sequence, KV head): scores of its pages into shared memory as
+// order-preserving 32-bit keys, the K-th largest key by four 8-bit radix
+// passes, then the chosen pages in ascending order, ties to the lowest page.
+constexpr int kSelectThreads = 512;
+constexpr int kSelectWarps = kSelectThreads / 32;
+constexpr int kSelectMaxPages = 32768;
+constexpr int kSelectMaxGroup = 128;
+
+struct SelectArgs {
+    const uint16_t* q;       // [B][Hq][D]
+    const int8_t* codes;
+    const float* scales;
+    const int* table;
+    long long table_stride;
+    const int* lens;
+    int B, Hq, Hkv, width, page_shift, num_blocks, top, sinks, local;
+    int* pages;              // [B][Hkv][top]
+    int* counts;             // [B][Hkv]
+    unsigned* err;
+};
+
+__device__ __forceinline__ uint32_t order_key(float f) {
+    const uint32_t u = __float_as_uint(f + 0.f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// Sum of a 32-bit value over the block, exclusive prefix per thread.
+__device__ __forceinline__ uint32_t select_scan(uint32_t v, uint32_t* part, uint32_t* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(~0u, inc, o);
+        if (lane >= o) inc += u;
+    }
+    if (lane == 31) part[warp] = inc;
+    __syncthreads();
+    uint32_t w = lane < kSelectWarps ? part[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < kSelectWarps; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(~0u, w, o);
+        if (lane >= o) w += u;
+    }
+    const uint32_t before = __shfl_sync(~0u, w, warp ? warp - 1 : 0);
+    *total = __shfl_sync(~0u, w, kSelectWarps - 1);
+    __syncthreads();
+    return inc - v + (warp ? before : 0);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kSelectThreads) select_kernel(const SelectArgs a) {
+    constexpr int kPieces = 2 * D / 16;              // 16-byte pieces of a page's codes
+    constexpr int kPagesPerWarp = 32 / kPieces;
+    extern __shared__ uint4 select_smem[];
+    __shared__ uint32_t s_part[kSelectWarps], s_hist[256], s_pick[2];
+    __shared__ uint32_t s_most;
+    const int b = blockIdx.x / a.Hkv, h = blockIdx.x % a.Hkv;
+    const int G = a.Hq / a.Hkv, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int sh = a.page_shift;
+    const int len = max(0, min(a.lens[b], (int)min((long long)a.width << sh, (long long)INT_MAX)));
+    const int n = (int)(((long long)len + (1 << sh) - 1) >> sh);
+    int* out = a.pages + (long long)blockIdx.x * a.top;
+    const int chosen = min(n, a.top);
+    if (tid == 0) a.counts[blockIdx.x] = chosen;
+    if (n <= a.top) {
+        for (int i = tid; i < a.top; i += kSelectThreads) out[i] = i < n ? i : -1;
+        return;
+    }
+    int8_t* q8 = reinterpret_cast<int8_t*>(select_smem);              // [G][2 D]: positive part, negative part
+    uint32_t* keys = reinterpret_cast<uint32_t*>(select_smem + G * kPieces);
+    // q to whole numbers
+    if (tid == 0) s_most = 0;
+    __syncthreads();
+    const uint16_t* q = a.q + ((long long)b * a.Hq + (long long)h * G) * D;
+    uint32_t most = 0;
+    for (int i = tid; i < G * D / 2; i += kSelectThreads) {
+        const float2 f = unpack2<T>(reinterpret_cast<const uint32_t*>(q)[i]);
+        most = max(most, max(__float_as_uint(f.x) & 0x7FFFFFFFu, __float_as_uint(f.y) & 0x7FFFFFFFu));
+    }
+    most = __reduce_max_sync(~0u, most);
+    if (lane == 0) atomicMax(&s_most, most);
+    __syncthreads();
+    most = s_most;
+    const float step = __uint_as_float(most & 0x7F800000u) * 0.015625f;
+    const bool live = most < 0x7F800000u && step > 0.f;
+    for (int i = tid; i < G * D; i += kSelectThreads) {
+        const float2 f = unpack2<T>(q[i]);
+        const int v = live ? max(-127, min(127, (int)rintf(f.x / step))) : 0;
+        const int g = i / D, d = i % D;
+        q8[g * 2 * D + d] = (int8_t)max(v, 0);
+        q8[g * 2 * D + D + d] = (int8_t)min(v, 0);
+    }
+    __syncthreads();
+    // scores: kPieces lanes a page
+    const int piece = lane % kPieces, sub = lane / kPieces;
+    for (int p0 = warp * kPagesPerWarp; p0 < n; p0 += kSelectWarps * kPagesPerWarp) {
+        const int p = p0 + sub;
+        uint4 c = make_uint4(0, 0, 0, 0);
+        float s = 0.f;
+        if (p < n) {
+            const int blk = a.table[b * a.table_stride + p];
+            if (blk >= 0 && blk < a.num_blocks) {
+                const long long at = (long long)blk * a.Hkv + h;
+                c = ld_nc16(a.codes + at * (2 * D) + piece * 16);
+                s = a.scales[at];
+            } else if (piece == 0) {
+                set_err(a.err, kErrPagedIndex);
+            }
+        }
+        int best = INT_MIN;
+        for (int g = 0; g < G; ++g) {
+            const uint4 w = select_smem[g * kPieces + piece];
+            int sum = __dp4a((int)c.x, (int)w.x, 0);
+            sum = __dp4a((int)c.y, (int)w.y, sum);
+            sum = __dp4a((int)c.z, (int)w.z, sum);
+            sum = __dp4a((int)c.w, (int)w.w, sum);
+#pragma unroll
+            for (int o = 1; o < kPieces; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
+            best = max(best, sum);
+        }
+        if (p < n && piece == 0) {
+            const bool forced = p < a.sinks || p >= n - a.local;
+            const float score = s < INFINITY ? (float)best * s : INFINITY;
+            keys[p] = forced ? 0xFFFFFFFFu : order_key(score);
+        }
+    }
+    // the key of rank `top`: four passes over 8 bits
+    uint32_t prefix = 0, mask = 0, want = (uint32_t)a.top;
+#pragma unroll 1
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        for (int i = tid; i < 256; i += kSelectThreads) s_hist[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += kSelectThreads)
+            if ((keys[i] & mask) == prefix) atomicAdd(&s_hist[(keys[i] >> shift) & 255], 1u);
+        __syncthreads();
+        // thread t looks at bin 255 - t: keys in higher bins before it
+        const uint32_t mine = tid < 256 ? s_hist[255 - tid] : 0;
+        uint32_t total;
+        const uint32_t above = select_scan(mine, s_part, &total);
+        if (tid < 256 && above < want && above + mine >= want) {
+            s_pick[0] = 255 - tid;
+            s_pick[1] = want - above;
+        }
+        __syncthreads();
+        prefix |= s_pick[0] << shift;
+        mask |= 255u << shift;
+        want = s_pick[1];
+    }
+    // keys above `prefix` are in; of its equals the first `want` pages
+    const int per = (n + kSelectThreads - 1) / kSelectThreads;
+    const int i0 = min(n, tid * per), i1 = min(n, i0 + per);
+    uint32_t above = 0, equal = 0;
+    for (int i = i0; i < i1; ++i) {
+        above += keys[i] > prefix;
+        equal += keys[i] == prefix;
+    }
+    uint32_t total;
+    const uint32_t before = select_scan(above << 16 | equal, s_part, &total);
+    uint32_t at_above = before >> 16, at_equal = before & 0xFFFFu;
+    for (int i = i0; i < i1; ++i) {
+        const bool gt = keys[i] > prefix, eq = keys[i] == prefix;
+        if (gt || (eq && at_equal < want)) out[at_above + min(at_equal, want)] = i;
+        at_above += gt;
+        at_equal += eq;
+    }
+}
+
+template <typename T>
+cudaError_t launch_select(const SelectArgs& a, int D, cudaStream_t s) {
+    const int G = a.Hq / a.Hkv;
+    const size_t smem = (size_t)G * 2 * D + sizeof(uint32_t) * (size_t)a.width;
+    auto go = [&](auto kernel) -> cudaError_t {
+        if (smem > 40 * 1024) {
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (e != cudaSuccess) return e;
+        }
+        kernel<<<(unsigned)(a.B * a.Hkv), kSelectThreads, smem, s>>>(a);
+        return cudaGetLastError();
+    };
+    switch (D) {
+        case 64: return go(select_kernel<T, 64>);
+        case 128: return go(select_kernel<T, 128>);
+        case 256: return go(select_kernel<T, 256>);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace
+}  // namespace zs
+
+extern "C" int zs_page_bounds(const ZsPageBounds* p) {
+    using namespace zs;
+    BoundsArgs a{};
+    if (!p || !make_pool(&p->k_pool, &a.kp) || p->B < 0 || p->width <= 0 || p->table_stride < p->width ||
+        p->max_new < 0)
+        return cudaErrorInvalidValue;
+    if (a.kp.dim != 64 && a.kp.dim != 128 && a.kp.dim != 256) return cudaErrorInvalidValue;
+    if (p->B == 0 || p->max_new == 0) return cudaSuccess;
+    if (!p->block_table || !p->lens_before || !p->seq_lens || !p->codes || !p->scales || !aligned16p(p->codes))
+        return cudaErrorInvalidValue;
+    const int B = p->B;
+    a.table = p->block_table;
+    a.table_stride = p->table_stride;
+    a.B = B;
+    a.width = p->width;
+    // max_new tokens complete at most this many pages of a sequence
+    a.per_seq = (int)std::min<long long>(p->width, ((long long)p->max_new + (1 << a.kp.page_shift) - 1) >>
+                                                       a.kp.page_shift);
+    a.before = p->lens_before;
+    a.lens = p->seq_lens;
+    a.codes = p->codes;
+    a.scales = p->scales;
+    a.err = p->err;
+    const long long warps = (long long)B * a.per_seq * a.kp.heads;
+    const long long grid = (warps + kBoundsThreads / 32 - 1) / (kBoundsThreads / 32);
+    if (grid > INT32_MAX) return cudaErrorInvalidValue;
+    cudaStream_t s = (cudaStream_t)p->stream;
+    const bool bf = p->k_pool.dtype == ZS_BF16;
+    switch (a.kp.dim) {
+        case 64:
+            if (bf) page_bounds_kernel<__nv_bfloat16, 64><<<(unsigned)grid, kBoundsThreads, 0, s>>>(a);
+            else page_bounds_kernel<__half, 64><<<(unsigned)grid, kBoundsThreads, 0, s>>>(a);
+            break;
+        case 128:
+            if (bf) page_bounds_kernel<__nv_bfloat16, 128><<<(unsigned)grid, kBoundsThreads, 0, s>>>(a);
+            else page_bounds_kernel<__half, 128><<<(unsigned)grid, kBoundsThreads, 0, s>>>(a);
+            break;
+        case 256:
+            if (bf) page_bounds_kernel<__nv_bfloat16, 256><<<(unsigned)grid, kBoundsThreads, 0, s>>>(a);
+            else page_bounds_kernel<__half, 256><<<(unsigned)grid, kBoundsThreads, 0, s>>>(a);
+            break;
+        default: return cudaErrorInvalidValue;
+    }
+    return cudaGetLastError();
+}
+
+extern "C" int zs_select_pages(const ZsSelectPages* p) {
+    using namespace zs;
+    if (!p) return cudaErrorInvalidValue;
+    const int B = p->B, Hq = p->Hq, Hkv = p->Hkv, page_size = p->page_size;
+    if (B < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > kSelectMaxGroup || p->width <= 0 ||
+        p->width > kSelectMaxPages || p->table_stride < p->width || p->num_blocks <= 0)
+        return cudaErrorInvalidValue;
+    if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1))) return cudaErrorInvalidValue;
+    if (p->sinks < 0 || p->local < 1 || p->top < (long long)p->sinks + p->local ||
+        (p->dtype != ZS_BF16 && p->dtype != ZS_FP16) || (p->D != 64 && p->D != 128 && p->D != 256))
+        return cudaErrorInvalidValue;
+    if ((long long)B * Hkv > INT32_MAX) return cudaErrorInvalidValue;
+    if (B == 0) return cudaSuccess;
+    if (!p->q || !p->codes || !p->scales || !p->block_table || !p->seq_lens || !p->pages || !p->counts ||
+        !aligned16p(p->codes) || !aligned16p(p->q))
+        return cudaErrorInvalidValue;
+    SelectArgs a{p->q, p->codes, p->scales, p->block_table, p->table_stride, p->seq_lens, B, Hq, Hkv, p->width, 0,
+                 p->num_blocks, p->top, p->sinks, p->local, p->pages, p->counts, p->err};
+    while ((1 << a.page_shift) < page_size) ++a.page_shift;
+    return p->dtype == ZS_BF16 ? launch_select<__nv_bfloat16>(a, p->D, (cudaStream_t)p->stream)
+                               : launch_select<__half>(a, p->D, (cudaStream_t)p->stream);
+}
