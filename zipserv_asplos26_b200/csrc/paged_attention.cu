@@ -130,9 +130,12 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const PaArgs a) 
     constexpr int kKs = D / 16;
     extern __shared__ __align__(1024) uint8_t pa_smem[];
     __shared__ long long s_red[kPaWarps];
-    __shared__ long long s_pos[2];
+    __shared__ long long s_lo;
+    __shared__ int s_entry, s_chunks;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t ring = smem_u32(pa_smem) + warp * C::kRing;
+    grid_dep_launch();
+    grid_dep_wait();
 
     // ---- this CTA's run of chunks
     const int entries = kListed ? a.B * a.Hkv : a.B;
@@ -171,23 +174,23 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const PaArgs a) 
         }
         const long long lo = (before + inc - n) * per_entry, hi = (before + inc) * per_entry;
         if (lo <= c_begin && c_begin < hi) {
-            s_pos[0] = e;
-            s_pos[1] = lo;
+            s_entry = e;
+            s_chunks = n;
+            s_lo = lo;
         }
         if (base * per_entry > c_begin) break;
     }
     __syncthreads();
-    int e = (int)s_pos[0];
-    long long e_lo = s_pos[1];
+    int e = s_entry, n = s_chunks;
+    long long e_lo = s_lo;
 
     long long c = c_begin;
     while (c < c_end) {
-        int n = entry_chunks<kListed>(a, e);
         while (n == 0 || e_lo + (long long)n * per_entry <= c) {     // next entry with chunks left
             e_lo += (long long)n * per_entry;
             n = entry_chunks<kListed>(a, ++e);
         }
-        const int in_e = (int)((c - e_lo) / n);                        // unit of the entry
+        const int in_e = (int)div_nonneg(c - e_lo, n);                 // unit of the entry
         const long long u_lo = e_lo + (long long)in_e * n;
         const int first = (int)(c - u_lo);
         const int last = (int)min((long long)n, c_end - u_lo);
@@ -199,26 +202,6 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const PaArgs a) 
         if (first == 0 && tid == 0) a.plan[1 + unit] = u_lo;
         const long long cap = (long long)a.width << a.kp.page_shift;
         const int len = (int)max(0ll, min((long long)a.lens[b], cap));
-
-        // ---- Q fragments
-        uint32_t qf[kKs][4];
-        {
-            const uint16_t* q = a.q + ((long long)b * a.Hq + (long long)h * a.G + g0) * D;
-            const int r = lane >> 2, cc = (lane & 3) * 2;
-#pragma unroll
-            for (int ks = 0; ks < kKs; ++ks)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = r + (i & 1) * 8, col = ks * 16 + (i >> 1) * 8 + cc;
-                    qf[ks][i] = row < rows ? *reinterpret_cast<const uint32_t*>(q + (long long)row * D + col) : 0u;
-                }
-        }
-        float o[D / 8][4];
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
         // ---- chunks first + warp, + 4, ...
         const int steps = (last - first - warp + kPaWarps - 1) / kPaWarps;
@@ -273,6 +256,26 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const PaArgs a) 
             produce(s);
             lim_at[s] = __shfl_sync(~0u, lims, s & 31);
         }
+        // ---- Q fragments, while the first chunks are on their way
+        uint32_t qf[kKs][4];
+        {
+            const uint16_t* q = a.q + ((long long)b * a.Hq + (long long)h * a.G + g0) * D;
+            const int r = lane >> 2, cc = (lane & 3) * 2;
+#pragma unroll
+            for (int ks = 0; ks < kKs; ++ks)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = r + (i & 1) * 8, col = ks * 16 + (i >> 1) * 8 + cc;
+                    qf[ks][i] = row < rows ? *reinterpret_cast<const uint32_t*>(q + (long long)row * D + col) : 0u;
+                }
+        }
+        float o[D / 8][4];
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
         for (int s = 0; s < steps; ++s) {
             cp_wait<C::kStages - 2>();
             __syncwarp();
@@ -421,35 +424,79 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const PaArgs a) 
     }
 }
 
-// Joins the pieces of the units that the runs cut, in order, and writes zeros
-// where nothing is attended. One CTA a query head, one thread a channel.
+// Joins the pieces of the units that the runs cut and writes zeros where nothing
+// is attended. A warp takes a query head, D / 32 channels a lane; with few heads
+// (long sequences: up to one piece a CTA of the attention kernel) the eight warps
+// of a CTA share one head's pieces, so that their loads are in flight together,
+// and add their sums in order.
+constexpr int kJoinWarps = 8;
+
 template <typename T, int D, bool kListed>
-__global__ void __launch_bounds__(D) paged_join_kernel(const PaArgs a) {
-    const int b = blockIdx.x / a.Hq, i = blockIdx.x % a.Hq, h = i / a.G, g = i % a.G;
-    const int tile = g / kPaRows, row = g % kPaRows, d = threadIdx.x;
-    const int n = entry_chunks<kListed>(a, kListed ? b * a.Hkv + h : b);
-    T* out = reinterpret_cast<T*>(a.out) + (long long)blockIdx.x * D + d;
-    if (n == 0) {
-        *out = T(0.f);
-        if (a.lse && d == 0) a.lse[blockIdx.x] = -INFINITY;
-        return;
-    }
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PaArgs a, int share) {
+    constexpr int kVec = D / 32;
+    __shared__ float s_acc[kJoinWarps][D], s_m[kJoinWarps], s_l[kJoinWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int head = share ? (int)blockIdx.x : (int)blockIdx.x * kJoinWarps + warp;
+    if (head >= a.B * a.Hq) return;
+    const int b = head / a.Hq, i = head % a.Hq, h = i / a.G, g = i % a.G;
+    const int tile = g / kPaRows, row = g % kPaRows;
+    grid_dep_wait();
     const long long run = a.plan[0], lo = a.plan[1 + (b * a.Hkv + h) * a.tiles + tile];
-    const long long w0 = lo / run, w1 = (lo + n - 1) / run;
-    if (w0 == w1) return;
-    auto slot_of = [&](long long w) { return (2 * w + (w == w0 && lo % run != 0 ? 1 : 0)) * kPaRows + row; };
-    float m = -INFINITY;
-    for (long long w = w0; w <= w1; ++w) m = fmaxf(m, a.part_ml[slot_of(w) * 2]);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f, acc = 0.f;
-    for (long long w = w0; w <= w1; ++w) {
-        const long long s = slot_of(w);
-        const float f = exp2f(a.part_ml[s * 2] - ref);
-        l += a.part_ml[s * 2 + 1] * f;
-        acc += a.part_o[s * D + d] * f;
+    const int n = entry_chunks<kListed>(a, kListed ? b * a.Hkv + h : b);
+    float m = -INFINITY, l = 0.f, acc[kVec];
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) acc[j] = 0.f;
+    if (n > 0) {
+        const int w0 = (int)div_nonneg(lo, run), w1 = (int)div_nonneg(lo + n - 1, run);
+        if (w0 == w1) return;                   // written whole
+        // the first piece is the last of its CTA's run unless it starts that run
+        const bool second = lo != w0 * run;
+        const int first = share ? warp : 0, by = share ? kJoinWarps : 1;
+#pragma unroll 4
+        for (int w = w0 + first; w <= w1; w += by) {
+            const long long s = (2ll * w + (w == w0 && second ? 1 : 0)) * kPaRows + row;
+            const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + s * 2);
+            float o[kVec];
+            const float* src = a.part_o + s * D + lane * kVec;
+            if constexpr (kVec == 4) *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(src);
+            else *reinterpret_cast<float2*>(o) = *reinterpret_cast<const float2*>(src);
+            const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.f : mn;
+            const float f0 = exp2f(m - ref), f1 = exp2f(ml.x - ref);
+            l = l * f0 + ml.y * f1;
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) acc[j] = acc[j] * f0 + o[j] * f1;
+            m = mn;
+        }
     }
-    *out = T(l == 0.f ? 0.f : acc * (1.f / l));
-    if (a.lse && d == 0) a.lse[blockIdx.x] = l == 0.f ? -INFINITY : (m + log2f(l) - kPBias<T>) / kLog2e;
+    if (share) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) s_acc[warp][lane * kVec + j] = acc[j];
+        if (lane == 0) {
+            s_m[warp] = m;
+            s_l[warp] = l;
+        }
+        __syncthreads();
+        if (warp) return;
+        m = s_m[0];
+#pragma unroll
+        for (int w = 1; w < kJoinWarps; ++w) m = fmaxf(m, s_m[w]);
+        const float ref = m == -INFINITY ? 0.f : m;
+        l = 0.f;
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) acc[j] = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) {
+            const float f = exp2f(s_m[w] - ref);
+            l += s_l[w] * f;
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) acc[j] += s_acc[w][lane * kVec + j] * f;
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint32_t* out = reinterpret_cast<uint32_t*>(a.out + (long long)head * D + lane * kVec);
+#pragma unroll
+    for (int j = 0; j < kVec; j += 2) out[j / 2] = pack2<T>(acc[j] * inv, acc[j + 1] * inv);
+    if (a.lse && lane == 0) a.lse[head] = l == 0.f ? -INFINITY : (m + log2f(l) - kPBias<T>) / kLog2e;
 }
 
 constexpr int kPaMaxCtas = 148 * 4;      // the workspace's bound on the grid
@@ -484,11 +531,16 @@ cudaError_t launch_paged(const PaArgs& a, cudaStream_t s) {
     int ctas = 0;
     cudaError_t e = resident_ctas<T, D, kListed>(&ctas);
     if (e != cudaSuccess) return e;
-    paged_attn_kernel<T, D, kListed><<<ctas, kPaThreads, PaCfg<D>::kSmem, s>>>(a);
-    e = cudaGetLastError();
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr;
+    pdl_config(&cfg, &attr, dim3(ctas), dim3(kPaThreads), PaCfg<D>::kSmem, s);
+    e = cudaLaunchKernelEx(&cfg, paged_attn_kernel<T, D, kListed>, a);
     if (e != cudaSuccess) return e;
-    paged_join_kernel<T, D, kListed><<<(unsigned)(a.B * a.Hq), D, 0, s>>>(a);
-    return cudaGetLastError();
+    // heads enough to fill the GPU by a warp each, or a CTA each
+    const int heads = a.B * a.Hq, share = heads < 148 * kJoinWarps ? 1 : 0;
+    pdl_config(&cfg, &attr, dim3((unsigned)(share ? heads : (heads + kJoinWarps - 1) / kJoinWarps)),
+               dim3(kJoinWarps * 32), 0, s);
+    return cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D, kListed>, a, share);
 }
 
 template <typename T, bool kListed>

@@ -130,13 +130,19 @@ __global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const Bound
 }
 
 // ------------------------------------------------------------------ choice
-// One CTA a (sequence, KV head): scores of its pages into shared memory as
-// order-preserving 32-bit keys, the K-th largest key by four 8-bit radix
-// passes, then the chosen pages in ascending order, ties to the lowest page.
+// A cluster of CTAs a (sequence, KV head): each scores its share of the pages and
+// stores the scores, as order-preserving 32-bit keys, in the first CTA's shared
+// memory; that one finds the K-th largest key by histograms over the range of the
+// keys (1024 bins of it, then of the bin that holds the K-th, until a bin ends at
+// the K-th or is one key wide) and writes the chosen pages in ascending order,
+// ties to the lowest page. Scoring is bound by HBM (2 D + 4 bytes a page and
+// head), choosing by the latency of some ten barriers.
 constexpr int kSelectThreads = 512;
 constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kSelectMaxPages = 32768;
 constexpr int kSelectMaxGroup = 128;
+constexpr int kSelectBins = 1024;
+constexpr int kSelectMaxCluster = 8;
 
 struct SelectArgs {
     const uint16_t* q;       // [B][Hq][D]
@@ -156,8 +162,12 @@ __device__ __forceinline__ uint32_t order_key(float f) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sum of a 32-bit value over the block, exclusive prefix per thread.
-__device__ __forceinline__ uint32_t select_scan(uint32_t v, uint32_t* part, uint32_t* total) {
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+// Exclusive prefix of a 32-bit value over the block's threads.
+__device__ __forceinline__ uint32_t select_scan(uint32_t v, uint32_t* part) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t inc = v;
 #pragma unroll
@@ -174,123 +184,187 @@ __device__ __forceinline__ uint32_t select_scan(uint32_t v, uint32_t* part, uint
         if (lane >= o) w += u;
     }
     const uint32_t before = __shfl_sync(~0u, w, warp ? warp - 1 : 0);
-    *total = __shfl_sync(~0u, w, kSelectWarps - 1);
-    __syncthreads();
     return inc - v + (warp ? before : 0);
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kSelectThreads) select_kernel(const SelectArgs a) {
+__global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectArgs a, int cluster) {
     constexpr int kPieces = 2 * D / 16;              // 16-byte pieces of a page's codes
-    constexpr int kPagesPerWarp = 32 / kPieces;
+    constexpr int kLanes = 4;                        // lanes a page
+    constexpr int kLoads = kPieces / kLanes;
+    constexpr int kPages = 32 / kLanes;              // pages a warp pass
     extern __shared__ uint4 select_smem[];
-    __shared__ uint32_t s_part[kSelectWarps], s_hist[256], s_pick[2];
+    __shared__ uint32_t s_part[2][kSelectWarps], s_hist[kSelectBins], s_pick[3], s_lo, s_hi;
     __shared__ uint32_t s_most;
-    const int b = blockIdx.x / a.Hkv, h = blockIdx.x % a.Hkv;
+    const int unit = blockIdx.x / cluster, rank = blockIdx.x % cluster;
+    const int b = unit / a.Hkv, h = unit % a.Hkv;
     const int G = a.Hq / a.Hkv, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int sh = a.page_shift;
+    grid_dep_launch();
+    grid_dep_wait();
     const int len = max(0, min(a.lens[b], (int)min((long long)a.width << sh, (long long)INT_MAX)));
     const int n = (int)(((long long)len + (1 << sh) - 1) >> sh);
-    int* out = a.pages + (long long)blockIdx.x * a.top;
-    const int chosen = min(n, a.top);
-    if (tid == 0) a.counts[blockIdx.x] = chosen;
-    if (n <= a.top) {
-        for (int i = tid; i < a.top; i += kSelectThreads) out[i] = i < n ? i : -1;
+    int* out = a.pages + (long long)unit * a.top;
+    if (rank == 0 && tid == 0) a.counts[unit] = min(n, a.top);
+    if (n <= a.top) {                                // the same for the whole cluster
+        for (int i = rank * kSelectThreads + tid; i < a.top; i += cluster * kSelectThreads) out[i] = i < n ? i : -1;
         return;
     }
+    // no CTA writes into the first one's shared memory before that one runs
+    if (cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     int8_t* q8 = reinterpret_cast<int8_t*>(select_smem);              // [G][2 D]: positive part, negative part
     uint32_t* keys = reinterpret_cast<uint32_t*>(select_smem + G * kPieces);
     // q to whole numbers
-    if (tid == 0) s_most = 0;
+    if (tid == 0) {
+        s_most = 0;
+        s_lo = 0xFFFFFFFFu;
+        s_hi = 0;
+    }
     __syncthreads();
-    const uint16_t* q = a.q + ((long long)b * a.Hq + (long long)h * G) * D;
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(a.q + ((long long)b * a.Hq + (long long)h * G) * D);
     uint32_t most = 0;
     for (int i = tid; i < G * D / 2; i += kSelectThreads) {
-        const float2 f = unpack2<T>(reinterpret_cast<const uint32_t*>(q)[i]);
+        const float2 f = unpack2<T>(q[i]);
         most = max(most, max(__float_as_uint(f.x) & 0x7FFFFFFFu, __float_as_uint(f.y) & 0x7FFFFFFFu));
     }
     most = __reduce_max_sync(~0u, most);
-    if (lane == 0) atomicMax(&s_most, most);
+    if (lane == 0 && most) atomicMax(&s_most, most);
     __syncthreads();
     most = s_most;
     const float step = __uint_as_float(most & 0x7F800000u) * 0.015625f;
     const bool live = most < 0x7F800000u && step > 0.f;
-    for (int i = tid; i < G * D; i += kSelectThreads) {
+    for (int i = tid; i < G * D / 2; i += kSelectThreads) {
         const float2 f = unpack2<T>(q[i]);
-        const int v = live ? max(-127, min(127, (int)rintf(f.x / step))) : 0;
-        const int g = i / D, d = i % D;
-        q8[g * 2 * D + d] = (int8_t)max(v, 0);
-        q8[g * 2 * D + D + d] = (int8_t)min(v, 0);
+        const int x = live ? max(-127, min(127, (int)rintf(f.x / step))) : 0;
+        const int y = live ? max(-127, min(127, (int)rintf(f.y / step))) : 0;
+        char2* at = reinterpret_cast<char2*>(q8 + (i / (D / 2)) * 2 * D + i % (D / 2) * 2);
+        at[0] = make_char2((signed char)max(x, 0), (signed char)max(y, 0));
+        at[D / 2] = make_char2((signed char)min(x, 0), (signed char)min(y, 0));
     }
     __syncthreads();
-    // scores: kPieces lanes a page
-    const int piece = lane % kPieces, sub = lane / kPieces;
-    for (int p0 = warp * kPagesPerWarp; p0 < n; p0 += kSelectWarps * kPagesPerWarp) {
-        const int p = p0 + sub;
-        uint4 c = make_uint4(0, 0, 0, 0);
+    // scores of this CTA's pages, kLanes lanes a page
+    const uint32_t keys0 = cluster > 1 ? mapa_shared(smem_u32(keys), 0) : 0;
+    if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    const int share = (n + cluster - 1) / cluster;
+    const int p_end = min(n, (rank + 1) * share);
+    const int sub = lane / kLanes, l4 = lane % kLanes;
+    for (int p0 = rank * share + warp * 32; p0 < p_end; p0 += kSelectWarps * 32) {
+        // 32 pages a warp: their blocks, then kPages at a time
+        long long at = -1;
         float s = 0.f;
-        if (p < n) {
-            const int blk = a.table[b * a.table_stride + p];
+        if (p0 + lane < p_end) {
+            const int blk = a.table[b * a.table_stride + p0 + lane];
             if (blk >= 0 && blk < a.num_blocks) {
-                const long long at = (long long)blk * a.Hkv + h;
-                c = ld_nc16(a.codes + at * (2 * D) + piece * 16);
+                at = (long long)blk * a.Hkv + h;
                 s = a.scales[at];
-            } else if (piece == 0) {
+            } else {
                 set_err(a.err, kErrPagedIndex);
             }
         }
-        int best = INT_MIN;
-        for (int g = 0; g < G; ++g) {
-            const uint4 w = select_smem[g * kPieces + piece];
-            int sum = __dp4a((int)c.x, (int)w.x, 0);
-            sum = __dp4a((int)c.y, (int)w.y, sum);
-            sum = __dp4a((int)c.z, (int)w.z, sum);
-            sum = __dp4a((int)c.w, (int)w.w, sum);
+        int best = 0;
+#pragma unroll 2
+        for (int j = 0; j < kLanes; ++j) {
+            const long long from = __shfl_sync(~0u, at, j * kPages + sub);
+            uint4 c[kLoads];
 #pragma unroll
-            for (int o = 1; o < kPieces; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
-            best = max(best, sum);
+            for (int i = 0; i < kLoads; ++i)
+                c[i] = from >= 0 ? ld_nc16(a.codes + from * (2 * D) + (i * kLanes + l4) * 16) : make_uint4(0, 0, 0, 0);
+            int mx = INT_MIN;
+            for (int g = 0; g < G; ++g) {
+                int sum = 0;
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    const uint4 w = select_smem[g * kPieces + i * kLanes + l4];
+                    sum = __dp4a((int)c[i].x, (int)w.x, sum);
+                    sum = __dp4a((int)c[i].y, (int)w.y, sum);
+                    sum = __dp4a((int)c[i].z, (int)w.z, sum);
+                    sum = __dp4a((int)c[i].w, (int)w.w, sum);
+                }
+                sum += __shfl_xor_sync(~0u, sum, 1);
+                sum += __shfl_xor_sync(~0u, sum, 2);
+                mx = max(mx, sum);
+            }
+            // page j * kPages + i is scored by lanes 4 i ..; lane j * kPages + i keeps it
+            const int got = __shfl_sync(~0u, mx, (lane % kPages) * kLanes);
+            if (lane / kPages == j) best = got;
         }
-        if (p < n && piece == 0) {
+        const int p = p0 + lane;
+        if (p < p_end) {
             const bool forced = p < a.sinks || p >= n - a.local;
             const float score = s < INFINITY ? (float)best * s : INFINITY;
-            keys[p] = forced ? 0xFFFFFFFFu : order_key(score);
+            const uint32_t key = forced ? 0xFFFFFFFFu : order_key(score);
+            if (cluster > 1) st_cluster(keys0 + p * 4, key);
+            else keys[p] = key;
         }
     }
-    // the key of rank `top`: four passes over 8 bits
-    uint32_t prefix = 0, mask = 0, want = (uint32_t)a.top;
-#pragma unroll 1
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += kSelectThreads) s_hist[i] = 0;
+    if (cluster > 1) cluster_sync();
+    else __syncthreads();
+    if (rank) return;
+    // range of the scored keys
+    uint32_t lo = 0xFFFFFFFFu, hi = 0;
+    for (int i = tid; i < n; i += kSelectThreads) {
+        const uint32_t k = keys[i];
+        if (k != 0xFFFFFFFFu) {
+            lo = min(lo, k);
+            hi = max(hi, k);
+        }
+    }
+    lo = __reduce_min_sync(~0u, lo);
+    hi = __reduce_max_sync(~0u, hi);
+    if (lane == 0) {
+        atomicMin(&s_lo, lo);
+        atomicMax(&s_hi, hi);
+    }
+    __syncthreads();
+    lo = s_lo;
+    hi = s_hi;
+    // top < n and the forced pages are sinks + local <= top, all different, so
+    // at least one page is scored and `want` of the scored ones are chosen
+    uint32_t want = (uint32_t)(a.top - a.sinks - a.local);
+    while (want && lo != hi) {
+        const int shift = max(0, 22 - __clz(hi - lo));          // (hi - lo) >> shift is below 1024
+        for (int i = tid; i < kSelectBins; i += kSelectThreads) s_hist[i] = 0;
         __syncthreads();
-        for (int i = tid; i < n; i += kSelectThreads)
-            if ((keys[i] & mask) == prefix) atomicAdd(&s_hist[(keys[i] >> shift) & 255], 1u);
-        __syncthreads();
-        // thread t looks at bin 255 - t: keys in higher bins before it
-        const uint32_t mine = tid < 256 ? s_hist[255 - tid] : 0;
-        uint32_t total;
-        const uint32_t above = select_scan(mine, s_part, &total);
-        if (tid < 256 && above < want && above + mine >= want) {
-            s_pick[0] = 255 - tid;
-            s_pick[1] = want - above;
+        for (int i = tid; i < n; i += kSelectThreads) {
+            const uint32_t k = keys[i];
+            if (k >= lo && k <= hi) atomicAdd(&s_hist[(k - lo) >> shift], 1u);
         }
         __syncthreads();
-        prefix |= s_pick[0] << shift;
-        mask |= 255u << shift;
+        // thread t looks at the bins kBins - 1 - 2 t and the one below, from the top
+        const int top_bin = kSelectBins - 1 - 2 * tid;
+        const uint32_t c0 = s_hist[top_bin], c1 = s_hist[top_bin - 1];
+        const uint32_t above = select_scan(c0 + c1, s_part[0]);
+        if (above < want && above + c0 + c1 >= want) {
+            const bool upper = above + c0 >= want;
+            s_pick[0] = upper ? top_bin : top_bin - 1;
+            s_pick[1] = want - above - (upper ? 0 : c0);
+            s_pick[2] = upper ? c0 : c1;
+        }
+        __syncthreads();
+        const uint32_t from = lo + (s_pick[0] << shift);
         want = s_pick[1];
+        if (want == s_pick[2]) {        // the whole bin is chosen: everything from its start on
+            lo = from - 1;
+            want = 0;
+            break;
+        }
+        hi = min(hi, from + ((1u << shift) - 1));
+        lo = from;
+        __syncthreads();                // before the bins and the pick are written again
     }
-    // keys above `prefix` are in; of its equals the first `want` pages
+    // keys above lo are in; of its equals the first `want` pages
+    if (a.top == a.sinks + a.local) lo = 0xFFFFFFFEu;
     const int per = (n + kSelectThreads - 1) / kSelectThreads;
     const int i0 = min(n, tid * per), i1 = min(n, i0 + per);
     uint32_t above = 0, equal = 0;
     for (int i = i0; i < i1; ++i) {
-        above += keys[i] > prefix;
-        equal += keys[i] == prefix;
+        above += keys[i] > lo;
+        equal += keys[i] == lo;
     }
-    uint32_t total;
-    const uint32_t before = select_scan(above << 16 | equal, s_part, &total);
+    const uint32_t before = select_scan(above << 16 | equal, s_part[1]);
     uint32_t at_above = before >> 16, at_equal = before & 0xFFFFu;
     for (int i = i0; i < i1; ++i) {
-        const bool gt = keys[i] > prefix, eq = keys[i] == prefix;
+        const bool gt = keys[i] > lo, eq = keys[i] == lo;
         if (gt || (eq && at_equal < want)) out[at_above + min(at_equal, want)] = i;
         at_above += gt;
         at_equal += eq;
@@ -301,13 +375,24 @@ template <typename T>
 cudaError_t launch_select(const SelectArgs& a, int D, cudaStream_t s) {
     const int G = a.Hq / a.Hkv;
     const size_t smem = (size_t)G * 2 * D + sizeof(uint32_t) * (size_t)a.width;
+    // CTAs a (sequence, KV head): as many as the GPU holds at once (two an SM), while
+    // each still has 32 pages for a part of its 16 warps
+    int cluster = 1;
+    while (cluster < kSelectMaxCluster && (long long)a.B * a.Hkv * cluster * 2 <= 296 && a.width / (2 * cluster) >= 64) cluster *= 2;
+    if ((long long)a.B * a.Hkv * cluster > INT32_MAX) return cudaErrorInvalidValue;
     auto go = [&](auto kernel) -> cudaError_t {
         if (smem > 40 * 1024) {
             const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
             if (e != cudaSuccess) return e;
         }
-        kernel<<<(unsigned)(a.B * a.Hkv), kSelectThreads, smem, s>>>(a);
-        return cudaGetLastError();
+        cudaLaunchConfig_t cfg;
+        cudaLaunchAttribute attr[2];
+        pdl_config(&cfg, attr, dim3((unsigned)(a.B * a.Hkv * cluster)), dim3(kSelectThreads), smem, s);
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = cluster;
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.numAttrs = 2;
+        return cudaLaunchKernelEx(&cfg, kernel, a, cluster);
     };
     switch (D) {
         case 64: return go(select_kernel<T, 64>);
