@@ -103,6 +103,15 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
 
 __device__ __forceinline__ uint4 ld_nc16(const void* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 
+// read once: no place in L1
+__device__ __forceinline__ uint4 ld_stream16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+
 __device__ __forceinline__ void set_err(unsigned* err, unsigned bit) {
     if (err) atomicOr(err, bit);
 }

@@ -19,6 +19,7 @@ namespace {
 
 constexpr int kRopeThreads = 256;
 constexpr int kRopeMaxAxes = 4;
+constexpr int kRopeBatch = 2;       // heads whose loads are in flight together
 
 struct RopeArgs {
     const uint16_t* q;
@@ -118,52 +119,62 @@ __global__ void __launch_bounds__(kRopeThreads) rope_write_kernel(const RopeArgs
     if (slot >= cap && lane == 0) set_err(a.err, kErrPagedIndex);
     const long long blk = slot >> a.kp.page_shift, row = slot & ((1 << a.kp.page_shift) - 1);
     if (!on) return;
+    uint16_t* kdst = static_cast<uint16_t*>(a.kp.data) + blk * a.kp.s_block + row * a.kp.s_token;
+    uint16_t* vdst = static_cast<uint16_t*>(a.vp.data) + blk * a.vp.s_block + row * a.vp.s_token;
     const int rows = a.Hq + 2 * a.Hkv;                       // heads of q, then k, then v
     const int passes = (rows + heads_per - 1) / heads_per;
-    for (int i = part; i < passes; i += a.parts) {
-        const int h = i * heads_per + sub;
-        if (h >= rows) break;
-        const uint16_t* src;
-        uint16_t* dst;
-        if (h < a.Hq) {
-            src = a.q + n * a.q_tok + h * a.q_head;
-            dst = a.q_out + n * a.qo_tok + h * a.qo_head;
-        } else {
-            if (!live) break;
-            const int kh = h - a.Hq;
-            if (kh < a.Hkv) {
-                src = a.k + n * a.k_tok + kh * a.k_head;
-                dst = static_cast<uint16_t*>(a.kp.data) + blk * a.kp.s_block + row * a.kp.s_token + kh * a.kp.s_head;
-            } else {
-                const int vh = kh - a.Hkv;
-                src = a.v + n * a.v_tok + vh * a.v_head;
-                dst = static_cast<uint16_t*>(a.vp.data) + blk * a.vp.s_block + row * a.vp.s_token + vh * a.vp.s_head;
-            }
-        }
-        // plain loads: q may be turned in place
-        uint4 x = *reinterpret_cast<const uint4*>(src + c0), y = *reinterpret_cast<const uint4*>(src + c1);
-        if (turns && h < a.Hq + a.Hkv) {
-            uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-            if (a.interleaved) {
+    for (int i0 = part; i0 < passes; i0 += kRopeBatch * a.parts) {
+        uint4 x[kRopeBatch], y[kRopeBatch];
+        uint16_t* dst[kRopeBatch];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 u = unpack2<T>(xs[j]), w = unpack2<T>(ys[j]);
-                    xs[j] = pack2<T>(u.x * cs[j] - u.y * sn[j], u.y * cs[j] + u.x * sn[j]);
-                    ys[j] = pack2<T>(w.x * cs[4 + j] - w.y * sn[4 + j], w.y * cs[4 + j] + w.x * sn[4 + j]);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 u = unpack2<T>(xs[j]), w = unpack2<T>(ys[j]);
-                    xs[j] = pack2<T>(u.x * cs[2 * j] - w.x * sn[2 * j], u.y * cs[2 * j + 1] - w.y * sn[2 * j + 1]);
-                    ys[j] = pack2<T>(w.x * cs[2 * j] + u.x * sn[2 * j], w.y * cs[2 * j + 1] + u.y * sn[2 * j + 1]);
+        for (int u = 0; u < kRopeBatch; ++u) {
+            const int h = (i0 + u * a.parts) * heads_per + sub;
+            const uint16_t* src = nullptr;
+            dst[u] = nullptr;
+            if (h < a.Hq) {
+                src = a.q + n * a.q_tok + h * a.q_head;
+                dst[u] = a.q_out + n * a.qo_tok + h * a.qo_head;
+            } else if (h < rows && live) {
+                const int kh = h - a.Hq, vh = kh - a.Hkv;
+                if (vh < 0) {
+                    src = a.k + n * a.k_tok + kh * a.k_head;
+                    dst[u] = kdst + kh * a.kp.s_head;
+                } else {
+                    src = a.v + n * a.v_tok + vh * a.v_head;
+                    dst[u] = vdst + vh * a.vp.s_head;
                 }
             }
-            x = make_uint4(xs[0], xs[1], xs[2], xs[3]);
-            y = make_uint4(ys[0], ys[1], ys[2], ys[3]);
+            if (src) {               // plain loads: q may be turned in place
+                x[u] = __ldcs(reinterpret_cast<const uint4*>(src + c0));
+                y[u] = __ldcs(reinterpret_cast<const uint4*>(src + c1));
+            }
         }
-        *reinterpret_cast<uint4*>(dst + c0) = x;
-        *reinterpret_cast<uint4*>(dst + c1) = y;
+#pragma unroll
+        for (int u = 0; u < kRopeBatch; ++u) {
+            if (!dst[u]) continue;
+            if (turns && (i0 + u * a.parts) * heads_per + sub < a.Hq + a.Hkv) {
+                uint32_t xs[4] = {x[u].x, x[u].y, x[u].z, x[u].w}, ys[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
+                if (a.interleaved) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 f = unpack2<T>(xs[j]), w = unpack2<T>(ys[j]);
+                        xs[j] = pack2<T>(f.x * cs[j] - f.y * sn[j], f.y * cs[j] + f.x * sn[j]);
+                        ys[j] = pack2<T>(w.x * cs[4 + j] - w.y * sn[4 + j], w.y * cs[4 + j] + w.x * sn[4 + j]);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 f = unpack2<T>(xs[j]), w = unpack2<T>(ys[j]);
+                        xs[j] = pack2<T>(f.x * cs[2 * j] - w.x * sn[2 * j], f.y * cs[2 * j + 1] - w.y * sn[2 * j + 1]);
+                        ys[j] = pack2<T>(w.x * cs[2 * j] + f.x * sn[2 * j], w.y * cs[2 * j + 1] + f.y * sn[2 * j + 1]);
+                    }
+                }
+                x[u] = make_uint4(xs[0], xs[1], xs[2], xs[3]);
+                y[u] = make_uint4(ys[0], ys[1], ys[2], ys[3]);
+            }
+            __stcs(reinterpret_cast<uint4*>(dst[u] + c0), x[u]);
+            __stcs(reinterpret_cast<uint4*>(dst[u] + c1), y[u]);
+        }
     }
 }
 

@@ -15,6 +15,7 @@
 // infinity has s = inf and is chosen before all scored ones.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -25,7 +26,8 @@ namespace {
 // One warp reduces one page of one KV head: a lane holds 8 channels of every
 // (32 / (D / 8))-th token, running maximum and minimum as packed 16-bit pairs
 // (exact), 16-byte loads. Bound by HBM: the keys are read once.
-constexpr int kBoundsThreads = 256;
+constexpr int kBoundsThreads = 128;
+constexpr int kBoundsBatch = 8;
 
 struct BoundsArgs {
     PoolView kp;
@@ -78,16 +80,31 @@ __global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const Bound
     }
     const int c = lane % kLanes, r0 = lane / kLanes;
     const uint16_t* base = static_cast<const uint16_t*>(a.kp.data) + blk * a.kp.s_block + h * a.kp.s_head + c * 8;
-    uint4 hi = ld_nc16(base + r0 * a.kp.s_token), lo = hi;
+    // (-inf, +inf) pairs of the type
+    const uint32_t ninf = std::is_same<T, __nv_bfloat16>::value ? 0xFF80FF80u : 0xFC00FC00u, pinf = ninf & 0x7FFF7FFFu;
+    uint4 hi = make_uint4(ninf, ninf, ninf, ninf), lo = make_uint4(pinf, pinf, pinf, pinf);
     auto fold = [&](const uint4& x) {
         hi.x = max2_nan(hi.x, x.x, T()); hi.y = max2_nan(hi.y, x.y, T());
         hi.z = max2_nan(hi.z, x.z, T()); hi.w = max2_nan(hi.w, x.w, T());
         lo.x = min2_nan(lo.x, x.x, T()); lo.y = min2_nan(lo.y, x.y, T());
         lo.z = min2_nan(lo.z, x.z, T()); lo.w = min2_nan(lo.w, x.w, T());
     };
-    const int page = 1 << sh;
-#pragma unroll 8
-    for (int r = r0 + kRows; r < page; r += kRows) fold(ld_nc16(base + r * a.kp.s_token));
+    // batches of loads in flight; a page is 4 passes (16 tokens of 64 channels) or a multiple of 8
+    const int passes = (1 << sh) / kRows;
+    const uint16_t* at = base + r0 * a.kp.s_token;
+    const long long step = kRows * a.kp.s_token;
+    if (passes < kBoundsBatch) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fold(ld_stream16(at + i * step));
+    } else {
+        for (int i = 0; i < passes; i += kBoundsBatch) {
+            uint4 x[kBoundsBatch];
+#pragma unroll
+            for (int j = 0; j < kBoundsBatch; ++j) x[j] = ld_stream16(at + (i + j) * step);
+#pragma unroll
+            for (int j = 0; j < kBoundsBatch; ++j) fold(x[j]);
+        }
+    }
 #pragma unroll
     for (int o = kLanes; o < 32; o <<= 1) {
         hi.x = max2_nan(hi.x, __shfl_xor_sync(~0u, hi.x, o), T()); hi.y = max2_nan(hi.y, __shfl_xor_sync(~0u, hi.y, o), T());
