@@ -1,8 +1,9 @@
-"""Paged-cache operators without a GPU: the argument structs of the C ABI as the
-Python side packs them, and refusals before anything is launched."""
+"""Paged-cache operators without a GPU: the argument structs of the C ABI as a
+ctypes caller packs them, and refusals before anything is launched."""
 import ctypes as C
 import os
 import re
+import struct
 import subprocess
 
 import pytest
@@ -21,8 +22,17 @@ def zlib():
     return lib()
 
 
-STRUCTS = {"ZsPlanStep": paged._PLAN, "ZsRopeWrite": paged._ROPE, "ZsPagedAttention": paged._ATTN,
-           "ZsPageBounds": paged._BOUNDS, "ZsSelectPages": paged._SELECT}
+_POOL = "Qqqqiiiii4x"
+STRUCTS = {"ZsPlanStep": struct.Struct("<QQq12Q6i"), "ZsRopeWrite": struct.Struct("<QQQQ6qQQqQQQ" + _POOL * 2 + "3i4i3i"),
+           "ZsPagedAttention": struct.Struct("<QQQqQQQQQQQQ" + _POOL * 2 + "4ifi"),
+           "ZsPageBounds": struct.Struct("<QQqQQQQQ" + _POOL + "4i"),
+           "ZsSelectPages": struct.Struct("<QQQQQqQQQQ12i")}
+
+
+def _fn(zlib, name, args=(C.c_char_p,), res=C.c_int):
+    f = getattr(zlib, name)
+    f.argtypes, f.restype = list(args), res
+    return f
 
 
 def test_packed_structs_match_the_header(tmp_path):
@@ -46,7 +56,6 @@ def test_packed_structs_match_the_header(tmp_path):
     for line in subprocess.check_output([str(tmp_path / "sizes")], text=True).splitlines():
         s, f, off = line.split()
         seen.setdefault(s, []).append((f, int(off)))
-    import struct
     for s, fmt in STRUCTS.items():
         got = dict(seen[s])
         assert got.pop(".") == fmt.size, s
@@ -67,7 +76,7 @@ def test_packed_structs_match_the_header(tmp_path):
 
 def test_null_and_bad_arguments_are_refused(zlib):
     for name in ("zs_plan_step", "zs_rope_write", "zs_paged_attention", "zs_page_bounds", "zs_select_pages"):
-        f = paged._fn(name)
+        f = _fn(zlib, name)
         assert f(None) == 1, name
         size = {"zs_plan_step": 144, "zs_rope_write": 280, "zs_paged_attention": 232, "zs_page_bounds": 136,
                 "zs_select_pages": 128}[name]
@@ -76,14 +85,14 @@ def test_null_and_bad_arguments_are_refused(zlib):
     for i, bad in ((0, 0), (0, (1 << 20) + 8), (1, 2049), (2, -8), (4, 0), (5, 24), (5, 512), (6, 0), (8, 2)):
         pool = list(ok)
         pool[i] = bad
-        args = paged._BOUNDS.pack(0, 1 << 20, 4, 1 << 20, 1 << 20, 1 << 20, 1 << 20, 0, *pool, 0, 4, 8, 0)
-        assert paged._fn("zs_page_bounds")(args) == 1, (i, bad)
-    assert paged._fn("zs_page_bounds")(paged._BOUNDS.pack(0, 1 << 20, 4, 1 << 20, 1 << 20, 1 << 20, 1 << 20, 0, *ok,
+        args = STRUCTS["ZsPageBounds"].pack(0, 1 << 20, 4, 1 << 20, 1 << 20, 1 << 20, 1 << 20, 0, *pool, 0, 4, 8, 0)
+        assert _fn(zlib, "zs_page_bounds")(args) == 1, (i, bad)
+    assert _fn(zlib, "zs_page_bounds")(STRUCTS["ZsPageBounds"].pack(0, 1 << 20, 4, 1 << 20, 1 << 20, 1 << 20, 1 << 20, 0, *ok,
                                                           0, 4, 8, 0)) == 0          # no sequences: nothing to do
 
 
 def test_workspace_bytes(zlib):
-    f = paged._fn("zs_paged_attention_workspace_bytes")
+    f = _fn(zlib, "zs_paged_attention_workspace_bytes", [C.c_int] * 4, C.c_size_t)
     assert f(0, 32, 8, 128) == 0 and f(1, 30, 8, 128) == 0
     assert f(1, 32, 8, 128) >= 2 * 148 * 16 * (128 + 2) * 4
     assert f(1 << 20, 32, 8, 128) > f(1, 32, 8, 128)

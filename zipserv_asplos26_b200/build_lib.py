@@ -1,8 +1,10 @@
 """Build libzipserv_b200.so (sm_100a) in-tree with nvcc / g++.
 
 The library is the product: CUDA kernels, the reference's C++ ABI
-(include/L_API.cuh) and the plain C ABI (include/zipserv_b200.h). The build is
-incremental (objects are rebuilt when a source or header is newer).
+(include/L_API.cuh) and the plain C ABI (include/zipserv_b200.h). Beside it goes
+the Python binding of the paged-cache operators (csrc/binding), a CPython module
+over the C ABI. The build is incremental (objects are rebuilt when a source or
+header is newer).
 """
 from __future__ import annotations
 
@@ -18,6 +20,7 @@ INCLUDE = os.path.join(ROOT, "include")
 LIBDIR = os.path.join(PKG, "lib")
 OBJDIR = os.path.join(LIBDIR, "obj")
 LIB = os.path.join(LIBDIR, "libzipserv_b200.so")
+BINDING = os.path.join(LIBDIR, "_paged_native.so")
 CUDA = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA, "bin", "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -72,7 +75,31 @@ def build(verbose: bool = False) -> str:
         os.replace(tmp, LIB)
         if verbose:
             print(f"[zipserv build] linked {LIB}")
+    _build_binding(verbose)
     return LIB
+
+
+def _build_binding(verbose: bool) -> str:
+    src = os.path.join(CSRC, "binding", "paged_bind.cpp")
+    if not _stale(BINDING, [src, LIB, os.path.join(INCLUDE, "zipserv_b200.h")]):
+        return BINDING
+    import sysconfig
+
+    import torch
+    tdir = os.path.dirname(torch.__file__)
+    tmp = BINDING + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f"-I{INCLUDE}", f"-I{CUDA}/include",
+           f"-I{sysconfig.get_paths()['include']}", "-isystem", f"{tdir}/include", "-isystem",
+           f"{tdir}/include/torch/csrc/api/include", src, "-o", tmp, f"-L{LIBDIR}", "-lzipserv_b200", f"-L{tdir}/lib",
+           "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: {src}\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, BINDING)
+    if verbose:
+        print(f"[zipserv build] linked {BINDING}")
+    return BINDING
 
 
 if __name__ == "__main__":

@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const PaArgs a) 
     constexpr int kPieces = D / 8;                 // 16-byte pieces a row
     constexpr int kKs = D / 16;
     extern __shared__ __align__(1024) uint8_t pa_smem[];
-    __shared__ long long s_red[kPaWarps];
+    __shared__ long long s_red[2][kPaWarps];
     __shared__ long long s_lo;
     __shared__ int s_entry, s_chunks;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -140,37 +140,50 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const PaArgs a) 
     // ---- this CTA's run of chunks
     const int entries = kListed ? a.B * a.Hkv : a.B;
     const int per_entry = kListed ? a.tiles : a.Hkv * a.tiles;     // units an entry
-    long long mine = 0;
-    for (int e = tid; e < entries; e += kPaThreads) mine += entry_chunks<kListed>(a, e);
-    mine = warp_sum(mine);
-    if (lane == 0) s_red[warp] = mine;
+    // chunks in all, and (one load for up to kPaThreads entries) this thread's first entry's
+    const int n0 = tid < entries ? entry_chunks<kListed>(a, tid) : 0;
+    long long mine = n0;
+    for (int e = tid + kPaThreads; e < entries; e += kPaThreads) mine += entry_chunks<kListed>(a, e);
+    long long inc0 = n0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(~0u, inc0, o);
+        if (lane >= o) inc0 += u;
+    }
+    mine = entries <= kPaThreads ? __shfl_sync(~0u, inc0, 31) : warp_sum(mine);
+    if (lane == 31) s_red[0][warp] = inc0;
+    if (lane == 0) s_red[1][warp] = mine;
     __syncthreads();
     long long total = 0;
 #pragma unroll
-    for (int w = 0; w < kPaWarps; ++w) total += s_red[w];
+    for (int w = 0; w < kPaWarps; ++w) total += s_red[1][w];
     total *= per_entry;
-    const long long run = max((total + gridDim.x - 1) / gridDim.x, (long long)kPaWarps);
+    const long long run = max(div_nonneg(total + gridDim.x - 1, gridDim.x), (long long)kPaWarps);
     if (blockIdx.x == 0 && tid == 0) a.plan[0] = run;
     const long long c_begin = run * blockIdx.x, c_end = min(total, c_begin + run);
     if (c_begin >= c_end) return;
     // the entry that holds c_begin
     long long base = 0;
     for (int e0 = 0; e0 < entries; e0 += kPaThreads) {
-        __syncthreads();
         const int e = e0 + tid;
-        const int n = e < entries ? entry_chunks<kListed>(a, e) : 0;
-        long long inc = n;
+        int n = n0;
+        long long inc = inc0;
+        if (e0) {
+            __syncthreads();
+            n = e < entries ? entry_chunks<kListed>(a, e) : 0;
+            inc = n;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long u = __shfl_up_sync(~0u, inc, o);
-            if (lane >= o) inc += u;
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long u = __shfl_up_sync(~0u, inc, o);
+                if (lane >= o) inc += u;
+            }
+            if (lane == 31) s_red[0][warp] = inc;
+            __syncthreads();
         }
-        if (lane == 31) s_red[warp] = inc;
-        __syncthreads();
         long long before = base;
         for (int w = 0; w < kPaWarps; ++w) {
-            if (w < warp) before += s_red[w];
-            base += s_red[w];
+            if (w < warp) before += s_red[0][w];
+            base += s_red[0][w];
         }
         const long long lo = (before + inc - n) * per_entry, hi = (before + inc) * per_entry;
         if (lo <= c_begin && c_begin < hi) {
@@ -202,6 +215,26 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const PaArgs a) 
         if (first == 0 && tid == 0) a.plan[1 + unit] = u_lo;
         const long long cap = (long long)a.width << a.kp.page_shift;
         const int len = (int)max(0ll, min((long long)a.lens[b], cap));
+
+        // ---- Q fragments (on their way while the first chunks' blocks are looked up)
+        uint32_t qf[kKs][4];
+        {
+            const uint16_t* q = a.q + ((long long)b * a.Hq + (long long)h * a.G + g0) * D;
+            const int r = lane >> 2, cc = (lane & 3) * 2;
+#pragma unroll
+            for (int ks = 0; ks < kKs; ++ks)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = r + (i & 1) * 8, col = ks * 16 + (i >> 1) * 8 + cc;
+                    qf[ks][i] = row < rows ? *reinterpret_cast<const uint32_t*>(q + (long long)row * D + col) : 0u;
+                }
+        }
+        float o[D / 8][4];
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
         // ---- chunks first + warp, + 4, ...
         const int steps = (last - first - warp + kPaWarps - 1) / kPaWarps;
@@ -256,26 +289,6 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const PaArgs a) 
             produce(s);
             lim_at[s] = __shfl_sync(~0u, lims, s & 31);
         }
-        // ---- Q fragments, while the first chunks are on their way
-        uint32_t qf[kKs][4];
-        {
-            const uint16_t* q = a.q + ((long long)b * a.Hq + (long long)h * a.G + g0) * D;
-            const int r = lane >> 2, cc = (lane & 3) * 2;
-#pragma unroll
-            for (int ks = 0; ks < kKs; ++ks)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = r + (i & 1) * 8, col = ks * 16 + (i >> 1) * 8 + cc;
-                    qf[ks][i] = row < rows ? *reinterpret_cast<const uint32_t*>(q + (long long)row * D + col) : 0u;
-                }
-        }
-        float o[D / 8][4];
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-
         for (int s = 0; s < steps; ++s) {
             cp_wait<C::kStages - 2>();
             __syncwarp();
