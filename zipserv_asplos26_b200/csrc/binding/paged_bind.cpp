@@ -161,6 +161,15 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, int index) {
                                   std::nullopt);
 }
 
+// n elements of `type` from byte `offset` of a byte tensor's storage, as a tensor of their own.
+at::Tensor part_of(const at::Tensor& block, int64_t offset, int64_t n, at::ScalarType type) {
+    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(block.storage()), block.key_set(),
+                                                     c10::scalarTypeToTypeMeta(type));
+    impl->set_storage_offset(offset / static_cast<int64_t>(c10::elementSize(type)));
+    impl->set_sizes_contiguous(at::IntArrayRef(&n, 1));
+    return at::Tensor(std::move(impl));
+}
+
 void* current_stream(int index) {
     return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(index)).stream();
 }
@@ -237,10 +246,17 @@ PyObject* plan_step(PyObject* const* a) {
         Py_INCREF(a[7]);
         return a[7];
     }
-    at::Tensor out[7] = {fresh({R}, at::kInt, index),     fresh({1}, at::kInt, index),
-                         fresh({R + 1}, at::kInt, index), fresh({room}, at::kLong, index),
-                         fresh({room}, at::kInt, index),  fresh({room}, at::kInt, index),
-                         fresh({R}, at::kBool, index)};
+    // one allocation for the seven outputs, each on a 16-byte boundary
+    const int64_t sizes[7] = {R, 1, R + 1, room, room, room, R};
+    const at::ScalarType types[7] = {at::kInt, at::kInt, at::kInt, at::kLong, at::kInt, at::kInt, at::kBool};
+    int64_t at_byte[7], bytes = 0;
+    for (int i = 0; i < 7; ++i) {
+        at_byte[i] = bytes;
+        bytes += (sizes[i] * static_cast<int64_t>(c10::elementSize(types[i])) + 15) / 16 * 16;
+    }
+    const at::Tensor block = fresh({bytes}, at::kByte, index);
+    at::Tensor out[7];
+    for (int i = 0; i < 7; ++i) out[i] = part_of(block, at_byte[i], sizes[i], types[i]);
     p.out_lens = ptr<int>(out[0]);
     p.out_count = ptr<int>(out[1]);
     p.out_cu = ptr<int>(out[2]);
