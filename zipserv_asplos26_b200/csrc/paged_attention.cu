@@ -49,9 +49,10 @@ struct PaArgs {
     float scale2;             // softmax scale * log2(e)
     uint16_t* out;            // [B][Hq][D]
     float* lse;               // nullable: [B][Hq]
-    long long* plan;          // workspace: [0] chunks a CTA, [1 + unit] first chunk of the unit
-    float* part_ml;           // [2 W][16][2]
-    float* part_o;            // [2 W][16][D]
+    long long* plan;          // workspace: [0] chunks a warp, [1 + unit] first chunk of the unit
+    int prow;                 // rows of a piece: min(G, 16)
+    float* part_ml;           // [2 W][prow][2], W warps
+    float* part_o;            // [2 W][prow][D]
     unsigned* err;
 };
 
@@ -117,27 +118,41 @@ template <int D>
 struct PaCfg {
     static constexpr int kRowBytes = D * 2;
     static constexpr int kTile = kPaChunk * kRowBytes;             // one K or V chunk
-    static constexpr int kStages = D <= 64 ? 6 : (D <= 128 ? 3 : 2);
+    static constexpr int kStages = D <= 64 ? 6 : 3;
     static constexpr int kRing = kStages * 2 * kTile;              // a warp's ring
-    static constexpr int kMerge = kPaWarps * kPaRows * (D + 2) * 4;
-    static constexpr int kSmem = kPaWarps * kRing > kMerge ? kPaWarps * kRing : kMerge;
+    static constexpr int kSmem = kPaWarps * kRing;
 };
 
+// Where a warp is in the sequence of all chunks: chunk `ch` of the n chunks of
+// unit `in_e` of entry e.
+struct PaCursor {
+    int e, n, in_e, ch;
+};
+
+// To the next unit that has chunks (there is one: the caller has chunks left).
+template <bool kListed>
+__device__ __forceinline__ void next_unit(const PaArgs& a, int per_entry, PaCursor& c) {
+    c.ch = 0;
+    if (++c.in_e < per_entry) return;
+    c.in_e = 0;
+    do c.n = entry_chunks<kListed>(a, ++c.e);
+    while (c.n == 0);
+}
+
 template <typename T, int D, bool kListed>
-__global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const PaArgs a) {
+__global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const PaArgs a) {
     using C = PaCfg<D>;
     constexpr int kPieces = D / 8;                 // 16-byte pieces a row
     constexpr int kKs = D / 16;
     extern __shared__ __align__(1024) uint8_t pa_smem[];
-    __shared__ long long s_red[2][kPaWarps];
-    __shared__ long long s_lo;
-    __shared__ int s_entry, s_chunks;
+    __shared__ long long s_red[2][kPaWarps], s_lo[kPaWarps];
+    __shared__ int s_entry[kPaWarps], s_chunks[kPaWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t ring = smem_u32(pa_smem) + warp * C::kRing;
     grid_dep_launch();
     grid_dep_wait();
 
-    // ---- this CTA's run of chunks
+    // ---- each warp's run of chunks
     const int entries = kListed ? a.B * a.Hkv : a.B;
     const int per_entry = kListed ? a.tiles : a.Hkv * a.tiles;     // units an entry
     // chunks in all, and (one load for up to kPaThreads entries) this thread's first entry's
@@ -158,11 +173,12 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const PaArgs a) 
 #pragma unroll
     for (int w = 0; w < kPaWarps; ++w) total += s_red[1][w];
     total *= per_entry;
-    const long long run = max(div_nonneg(total + gridDim.x - 1, gridDim.x), (long long)kPaWarps);
+    const int warps = gridDim.x * kPaWarps;
+    const long long run = max(div_nonneg(total + warps - 1, warps), 1ll);
     if (blockIdx.x == 0 && tid == 0) a.plan[0] = run;
-    const long long c_begin = run * blockIdx.x, c_end = min(total, c_begin + run);
-    if (c_begin >= c_end) return;
-    // the entry that holds c_begin
+    // neighbouring runs go to different CTAs, so that few chunks spread over the SMs
+    const int id = warp * (int)gridDim.x + (int)blockIdx.x;
+    // the entries that hold the four warps' first chunks
     long long base = 0;
     for (int e0 = 0; e0 < entries; e0 += kPaThreads) {
         const int e = e0 + tid;
@@ -181,45 +197,122 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const PaArgs a) 
             __syncthreads();
         }
         long long before = base;
+#pragma unroll
         for (int w = 0; w < kPaWarps; ++w) {
             if (w < warp) before += s_red[0][w];
             base += s_red[0][w];
         }
         const long long lo = (before + inc - n) * per_entry, hi = (before + inc) * per_entry;
-        if (lo <= c_begin && c_begin < hi) {
-            s_entry = e;
-            s_chunks = n;
-            s_lo = lo;
+#pragma unroll
+        for (int w = 0; w < kPaWarps; ++w) {
+            const long long at = run * (w * (int)gridDim.x + (int)blockIdx.x);
+            if (lo <= at && at < hi) {
+                s_entry[w] = e;
+                s_chunks[w] = n;
+                s_lo[w] = lo;
+            }
         }
-        if (base * per_entry > c_begin) break;
+        if (base * per_entry > run * ((kPaWarps - 1) * (int)gridDim.x + (int)blockIdx.x)) break;
     }
     __syncthreads();
-    int e = s_entry, n = s_chunks;
-    long long e_lo = s_lo;
+    const long long c_begin = run * id;
+    if (c_begin >= total) return;
+    const int steps = (int)min(run, total - c_begin);
 
-    long long c = c_begin;
-    while (c < c_end) {
-        while (n == 0 || e_lo + (long long)n * per_entry <= c) {     // next entry with chunks left
-            e_lo += (long long)n * per_entry;
-            n = entry_chunks<kListed>(a, ++e);
+    PaCursor at;                   // of the copies
+    at.e = s_entry[warp];
+    at.n = s_chunks[warp];
+    at.in_e = (int)div_nonneg(c_begin - s_lo[warp], at.n);
+    at.ch = (int)(c_begin - s_lo[warp] - (long long)at.in_e * at.n);
+    PaCursor cur = at;             // of the products
+    long long u_lo = c_begin - at.ch;
+
+    // ---- copies: batches of up to 32 chunks of one unit, a lane holding the block
+    // and the number of valid tokens of one chunk; the next batch is looked up
+    // while the present one is copied
+    const int cps = a.kp.page_shift - 4;                               // log2 chunks a page
+    const int table_len = (int)min((long long)a.width << a.kp.page_shift, (long long)INT_MAX);
+    struct Batch {
+        int ids, lims, count, h, ch;
+    } now, next;
+    int looked = 0;                // chunks looked up
+    auto look = [&](Batch& t) {
+        t.count = min(32, min(at.n - at.ch, steps - looked));
+        t.ids = 0;
+        t.lims = 0;
+        t.ch = at.ch;
+        t.h = kListed ? at.e % a.Hkv : at.in_e / a.tiles;
+        if (t.count <= 0) return;
+        if (lane < t.count) {
+            const int b = kListed ? at.e / a.Hkv : at.e;
+            const int ch = at.ch + lane;
+            int p = ch >> cps;
+            if (kListed) p = a.pages[(long long)at.e * a.top + p];
+            const int t0 = ((p << cps) + (ch & ((1 << cps) - 1))) * kPaChunk;
+            const int len = min(a.lens[b], table_len);
+            if (p >= 0 && p < a.width && t0 < len) {
+                t.ids = a.table[b * a.table_stride + p];
+                t.lims = min(kPaChunk, len - t0);
+                if (t.ids < 0 || t.ids >= a.kp.num_blocks) {
+                    set_err(a.err, kErrPagedIndex);
+                    t.ids = 0;
+                    t.lims = 0;
+                }
+            }
         }
-        const int in_e = (int)div_nonneg(c - e_lo, n);                 // unit of the entry
-        const long long u_lo = e_lo + (long long)in_e * n;
-        const int first = (int)(c - u_lo);
-        const int last = (int)min((long long)n, c_end - u_lo);
-        const int b = kListed ? e / a.Hkv : e;
-        const int h = kListed ? e % a.Hkv : in_e / a.tiles;
-        const int tile = kListed ? in_e : in_e % a.tiles;
-        const int g0 = tile * kPaRows, rows = min(kPaRows, a.G - g0);
-        const int unit = (b * a.Hkv + h) * a.tiles + tile;
-        if (first == 0 && tid == 0) a.plan[1 + unit] = u_lo;
-        const long long cap = (long long)a.width << a.kp.page_shift;
-        const int len = (int)max(0ll, min((long long)a.lens[b], cap));
+        looked += t.count;
+        at.ch += t.count;
+        if (at.ch == at.n && looked < steps) next_unit<kListed>(a, per_entry, at);
+    };
+    look(now);
+    look(next);
+    int in_batch = 0;
+    // starts the copies of step s; returns its number of valid tokens
+    auto produce = [&](int s) {
+        int lim = 0;
+        if (s < steps) {
+            if (in_batch == now.count) {
+                now = next;
+                in_batch = 0;
+                look(next);
+            }
+            const int blk = __shfl_sync(~0u, now.ids, in_batch);
+            lim = __shfl_sync(~0u, now.lims, in_batch);
+            const int row0 = ((now.ch + in_batch) & ((1 << cps) - 1)) * kPaChunk;
+            ++in_batch;
+            const uint16_t* ks = static_cast<const uint16_t*>(a.kp.data) + now.h * a.kp.s_head + blk * a.kp.s_block +
+                                 row0 * a.kp.s_token;
+            const uint16_t* vs = static_cast<const uint16_t*>(a.vp.data) + now.h * a.vp.s_head + blk * a.vp.s_block +
+                                 row0 * a.vp.s_token;
+            const uint32_t dst = ring + (s % C::kStages) * 2 * C::kTile;
+#pragma unroll
+            for (int i = 0; i < kPaChunk * kPieces / 32; ++i) {
+                const int x = i * 32 + lane, r = x / kPieces, pc = x % kPieces;
+                const uint32_t to = dst + r * C::kRowBytes + ((pc ^ (r & 7)) * 16);
+                cp16(to, ks + r * a.kp.s_token + pc * 8, r < lim);
+                cp16(to + C::kTile, vs + r * a.vp.s_token + pc * 8, r < lim);
+            }
+        }
+        cp_commit();
+        return lim;
+    };
+    int lim_at[C::kStages];        // of the steps in flight, oldest first
+#pragma unroll
+    for (int s = 0; s < C::kStages - 1; ++s) lim_at[s] = produce(s);
 
-        // ---- Q fragments (on their way while the first chunks' blocks are looked up)
+    int s = 0;
+    while (true) {
+        // ---- a unit, or the part of it in this run
+        const int first = cur.ch, count = min(cur.n - first, steps - s);
+        const int b = kListed ? cur.e / a.Hkv : cur.e;
+        const int h = kListed ? cur.e % a.Hkv : cur.in_e / a.tiles;
+        const int tile = kListed ? cur.in_e : cur.in_e % a.tiles;
+        const int g0 = tile * kPaRows, rows = min(kPaRows, a.G - g0);
+        if (first == 0 && lane == 0) a.plan[1 + (b * a.Hkv + h) * a.tiles + tile] = u_lo;
+        const long long head0 = (long long)b * a.Hq + (long long)h * a.G + g0;
         uint32_t qf[kKs][4];
         {
-            const uint16_t* q = a.q + ((long long)b * a.Hq + (long long)h * a.G + g0) * D;
+            const uint16_t* q = a.q + head0 * D;
             const int r = lane >> 2, cc = (lane & 3) * 2;
 #pragma unroll
             for (int ks = 0; ks < kKs; ++ks)
@@ -236,67 +329,13 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const PaArgs a) 
             for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-        // ---- chunks first + warp, + 4, ...
-        const int steps = (last - first - warp + kPaWarps - 1) / kPaWarps;
-        const int cps = a.kp.page_shift - 4;                           // log2 chunks a page
-        // tokens of the step's chunk that count, and its block; lane 0..31 hold 32 steps' worth
-        int ids = 0, lims = 0;
-        auto fetch = [&](int s0) {
-            const int s = s0 + lane;
-            ids = 0;
-            lims = 0;
-            if (s < steps) {
-                const int ch = first + warp + s * kPaWarps;
-                int p = ch >> cps;
-                if (kListed) p = a.pages[(long long)e * a.top + p];
-                const int t0 = ((p << cps) + (ch & ((1 << cps) - 1))) * kPaChunk;
-                if (p >= 0 && p < a.width && t0 < len) {
-                    ids = a.table[b * a.table_stride + p];
-                    lims = min(kPaChunk, len - t0);
-                    if (ids < 0 || ids >= a.kp.num_blocks) {
-                        set_err(a.err, kErrPagedIndex);
-                        ids = 0;
-                        lims = 0;
-                    }
-                }
-            }
-        };
-        const uint16_t* kbase = static_cast<const uint16_t*>(a.kp.data) + h * a.kp.s_head;
-        const uint16_t* vbase = static_cast<const uint16_t*>(a.vp.data) + h * a.vp.s_head;
-        auto produce = [&](int s) {
-            if (s < steps) {
-                if (s > 0 && (s & 31) == 0) fetch(s);
-                const int blk = __shfl_sync(~0u, ids, s & 31), lim = __shfl_sync(~0u, lims, s & 31);
-                const int row0 = ((first + warp + s * kPaWarps) & ((1 << cps) - 1)) * kPaChunk;
-                const uint16_t* ks = kbase + blk * a.kp.s_block + row0 * a.kp.s_token;
-                const uint16_t* vs = vbase + blk * a.vp.s_block + row0 * a.vp.s_token;
-                const uint32_t dst = ring + (s % C::kStages) * 2 * C::kTile;
-#pragma unroll
-                for (int i = 0; i < kPaChunk * kPieces / 32; ++i) {
-                    const int x = i * 32 + lane, r = x / kPieces, pc = x % kPieces;
-                    const uint32_t at = dst + r * C::kRowBytes + ((pc ^ (r & 7)) * 16);
-                    cp16(at, ks + r * a.kp.s_token + pc * 8, r < lim);
-                    cp16(at + C::kTile, vs + r * a.vp.s_token + pc * 8, r < lim);
-                }
-            }
-            cp_commit();
-        };
-        fetch(0);
-        // limits of the steps in flight, oldest first
-        int lim_at[C::kStages];
-#pragma unroll
-        for (int s = 0; s < C::kStages - 1; ++s) {
-            produce(s);
-            lim_at[s] = __shfl_sync(~0u, lims, s & 31);
-        }
-        for (int s = 0; s < steps; ++s) {
+        for (const int end = s + count; s < end; ++s) {
             cp_wait<C::kStages - 2>();
             __syncwarp();
-            produce(s + C::kStages - 1);
-            lim_at[C::kStages - 1] = __shfl_sync(~0u, lims, (s + C::kStages - 1) & 31);
             const int lim = lim_at[0];
 #pragma unroll
             for (int i = 0; i + 1 < C::kStages; ++i) lim_at[i] = lim_at[i + 1];
+            lim_at[C::kStages - 2] = produce(s + C::kStages - 1);
             const uint32_t kt = ring + (s % C::kStages) * 2 * C::kTile, vt = kt + C::kTile;
             // S = Q K^T: 16 heads x 16 tokens
             float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -378,78 +417,56 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const PaArgs a) 
             }
             __syncwarp();
         }
-        cp_wait<0>();
-        __syncthreads();
-        // ---- join the four warps through shared memory
-        float* mo = reinterpret_cast<float*>(pa_smem);                  // [warp][16][D]
-        float* ml = mo + kPaWarps * kPaRows * D;                        // [warp][16][2]
+        // ---- out, or to the workspace where the run cuts the unit
+        const bool whole = first == 0 && count == cur.n;
+        const long long slot = 2ll * id + (s == count ? 0 : 1);       // the run's first part, or its last
+        const int d0 = (lane & 3) * 2;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             l[r] += __shfl_xor_sync(~0u, l[r], 1);
             l[r] += __shfl_xor_sync(~0u, l[r], 2);
             const int row = (lane >> 2) + r * 8;
-            if ((lane & 3) == 0) {
-                ml[(warp * kPaRows + row) * 2] = m[r];
-                ml[(warp * kPaRows + row) * 2 + 1] = l[r];
-            }
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i)
-                *reinterpret_cast<float2*>(mo + (warp * kPaRows + row) * D + i * 8 + (lane & 3) * 2) =
-                    make_float2(o[i][r * 2], o[i][r * 2 + 1]);
-        }
-        __syncthreads();
-        const bool whole = first == 0 && last == n;
-        const long long slot = 2ll * blockIdx.x + (c == c_begin ? 0 : 1);
-        for (int x = tid; x < rows * (D / 4); x += kPaThreads) {
-            const int row = x / (D / 4), d4 = x % (D / 4) * 4;
-            float mm = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kPaWarps; ++w) mm = fmaxf(mm, ml[(w * kPaRows + row) * 2]);
-            const float ref = mm == -INFINITY ? 0.f : mm;
-            float ll = 0.f;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < kPaWarps; ++w) {
-                const float f = exp2f(ml[(w * kPaRows + row) * 2] - ref);
-                ll += ml[(w * kPaRows + row) * 2 + 1] * f;
-                const float4 v = *reinterpret_cast<const float4*>(mo + (w * kPaRows + row) * D + d4);
-                acc.x += v.x * f;
-                acc.y += v.y * f;
-                acc.z += v.z * f;
-                acc.w += v.w * f;
-            }
+            if (row >= rows) continue;
             if (whole) {
-                const float inv = ll == 0.f ? 0.f : 1.f / ll;
-                const long long at = (long long)b * a.Hq + (long long)h * a.G + g0 + row;
-                *reinterpret_cast<uint2*>(a.out + at * D + d4) =
-                    make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-                if (a.lse && d4 == 0) a.lse[at] = ll == 0.f ? -INFINITY : (mm + log2f(ll) - kPBias<T>) / kLog2e;
+                const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+                uint16_t* out = a.out + (head0 + row) * D + d0;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i)
+                    *reinterpret_cast<uint32_t*>(out + i * 8) = pack2<T>(o[i][r * 2] * inv, o[i][r * 2 + 1] * inv);
+                if (a.lse && d0 == 0)
+                    a.lse[head0 + row] = l[r] == 0.f ? -INFINITY : (m[r] + log2f(l[r]) - kPBias<T>) / kLog2e;
             } else {
-                *reinterpret_cast<float4*>(a.part_o + (slot * kPaRows + row) * D + d4) = acc;
-                if (d4 == 0) {
-                    a.part_ml[(slot * kPaRows + row) * 2] = mm;
-                    a.part_ml[(slot * kPaRows + row) * 2 + 1] = ll;
-                }
+                float* po = a.part_o + (slot * a.prow + row) * D + d0;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i)
+                    *reinterpret_cast<float2*>(po + i * 8) = make_float2(o[i][r * 2], o[i][r * 2 + 1]);
+                if (d0 == 0)
+                    *reinterpret_cast<float2*>(a.part_ml + (slot * a.prow + row) * 2) = make_float2(m[r], l[r]);
             }
         }
-        __syncthreads();
-        c = u_lo + last;
+        if (s == steps) break;
+        u_lo += cur.n;
+        next_unit<kListed>(a, per_entry, cur);
     }
+    cp_wait<0>();
 }
 
 // Joins the pieces of the units that the runs cut and writes zeros where nothing
-// is attended. A warp takes a query head, D / 32 channels a lane; with few heads
-// (long sequences: up to one piece a CTA of the attention kernel) the eight warps
-// of a CTA share one head's pieces, so that their loads are in flight together,
-// and add their sums in order.
-constexpr int kJoinWarps = 8;
+// is attended. Its time is a few dependent reads of what other SMs wrote, so the
+// pieces are read in batches, weights and outputs together. A warp takes a query
+// head, D / 32 channels a lane; with few heads (long sequences: up to a piece a
+// warp of the attention kernel) the warps of a CTA share a head's pieces and add
+// their sums in order.
+constexpr int kJoinWarps = 16;
+constexpr int kJoinShare = 148;        // heads joined by a CTA each
+constexpr int kJoinBatch = 8;
 
 template <typename T, int D, bool kListed>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PaArgs a, int share) {
     constexpr int kVec = D / 32;
     __shared__ float s_acc[kJoinWarps][D], s_m[kJoinWarps], s_l[kJoinWarps];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int head = share ? (int)blockIdx.x : (int)blockIdx.x * kJoinWarps + warp;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int head = share ? (int)blockIdx.x : (int)blockIdx.x * warps + warp;
     if (head >= a.B * a.Hq) return;
     const int b = head / a.Hq, i = head % a.Hq, h = i / a.G, g = i % a.G;
     const int tile = g / kPaRows, row = g % kPaRows;
@@ -462,22 +479,40 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PaArg
     if (n > 0) {
         const int w0 = (int)div_nonneg(lo, run), w1 = (int)div_nonneg(lo + n - 1, run);
         if (w0 == w1) return;                   // written whole
-        // the first piece is the last of its CTA's run unless it starts that run
+        // the first piece is the last of its warp's run unless it starts that run
         const bool second = lo != w0 * run;
-        const int first = share ? warp : 0, by = share ? kJoinWarps : 1;
-#pragma unroll 4
-        for (int w = w0 + first; w <= w1; w += by) {
-            const long long s = (2ll * w + (w == w0 && second ? 1 : 0)) * kPaRows + row;
-            const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + s * 2);
-            float o[kVec];
-            const float* src = a.part_o + s * D + lane * kVec;
-            if constexpr (kVec == 4) *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(src);
-            else *reinterpret_cast<float2*>(o) = *reinterpret_cast<const float2*>(src);
-            const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.f : mn;
-            const float f0 = exp2f(m - ref), f1 = exp2f(ml.x - ref);
-            l = l * f0 + ml.y * f1;
+        const int by = share ? warps : 1;
+        for (int v = w0 + (share ? warp : 0); v <= w1; v += kJoinBatch * by) {
+            float2 ml[kJoinBatch];
+            float o[kJoinBatch][kVec];
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) acc[j] = acc[j] * f0 + o[j] * f1;
+            for (int x = 0; x < kJoinBatch; ++x) {
+                const int w = v + x * by;
+                const long long s = (2ll * w + (w == w0 && second ? 1 : 0)) * a.prow + row;
+                ml[x] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) o[x][j] = 0.f;
+                if (w <= w1) {
+                    ml[x] = *reinterpret_cast<const float2*>(a.part_ml + s * 2);
+                    const float* src = a.part_o + s * D + lane * kVec;
+                    if constexpr (kVec == 4) *reinterpret_cast<float4*>(o[x]) = *reinterpret_cast<const float4*>(src);
+                    else *reinterpret_cast<float2*>(o[x]) = *reinterpret_cast<const float2*>(src);
+                }
+            }
+            float mn = m;
+#pragma unroll
+            for (int x = 0; x < kJoinBatch; ++x) mn = fmaxf(mn, ml[x].x);
+            const float ref = mn == -INFINITY ? 0.f : mn, f0 = exp2f(m - ref);
+            l *= f0;
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) acc[j] *= f0;
+#pragma unroll
+            for (int x = 0; x < kJoinBatch; ++x) {
+                const float f = exp2f(ml[x].x - ref);
+                l += ml[x].y * f;
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) acc[j] += o[x][j] * f;
+            }
             m = mn;
         }
     }
@@ -490,16 +525,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PaArg
         }
         __syncthreads();
         if (warp) return;
-        m = s_m[0];
+        const float mw = lane < warps ? s_m[lane] : -INFINITY;
+        m = mw;
 #pragma unroll
-        for (int w = 1; w < kJoinWarps; ++w) m = fmaxf(m, s_m[w]);
-        const float ref = m == -INFINITY ? 0.f : m;
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+        const float fw = lane < warps ? exp2f(mw - (m == -INFINITY ? 0.f : m)) : 0.f;
         l = 0.f;
 #pragma unroll
         for (int j = 0; j < kVec; ++j) acc[j] = 0.f;
-#pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) {
-            const float f = exp2f(s_m[w] - ref);
+        for (int w = 0; w < warps; ++w) {
+            const float f = __shfl_sync(~0u, fw, w);
             l += s_l[w] * f;
 #pragma unroll
             for (int j = 0; j < kVec; ++j) acc[j] += s_acc[w][lane * kVec + j] * f;
@@ -512,10 +547,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PaArg
     if (a.lse && lane == 0) a.lse[head] = l == 0.f ? -INFINITY : (m + log2f(l) - kPBias<T>) / kLog2e;
 }
 
-constexpr int kPaMaxCtas = 148 * 4;      // the workspace's bound on the grid
+constexpr int kPaMaxCtas = 148 * 2;      // the workspace's bound on the grid
 
 size_t plan_bytes(long long units) { return ((size_t)(1 + units) * 8 + 255) / 256 * 256; }
-size_t ml_bytes() { return (size_t)2 * kPaMaxCtas * kPaRows * 2 * 4; }
+size_t ml_bytes(int prow) { return (size_t)2 * kPaMaxCtas * kPaWarps * prow * 2 * 4; }
 
 // The attention kernel's grid: the CTAs that the GPU holds at once (looked up once per device).
 template <typename T, int D, bool kListed>
@@ -549,10 +584,9 @@ cudaError_t launch_paged(const PaArgs& a, cudaStream_t s) {
     pdl_config(&cfg, &attr, dim3(ctas), dim3(kPaThreads), PaCfg<D>::kSmem, s);
     e = cudaLaunchKernelEx(&cfg, paged_attn_kernel<T, D, kListed>, a);
     if (e != cudaSuccess) return e;
-    // heads enough to fill the GPU by a warp each, or a CTA each
-    const int heads = a.B * a.Hq, share = heads < 148 * kJoinWarps ? 1 : 0;
-    pdl_config(&cfg, &attr, dim3((unsigned)(share ? heads : (heads + kJoinWarps - 1) / kJoinWarps)),
-               dim3(kJoinWarps * 32), 0, s);
+    // a head a CTA while there are SMs for it, else a head a warp in small CTAs
+    const int heads = a.B * a.Hq, share = heads <= kJoinShare ? 1 : 0;
+    pdl_config(&cfg, &attr, dim3((unsigned)(share ? heads : (heads + 3) / 4)), dim3(share ? kJoinWarps * 32 : 128), 0, s);
     return cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D, kListed>, a, share);
 }
 
@@ -572,7 +606,8 @@ extern "C" size_t zs_paged_attention_workspace_bytes(int B, int Hq, int Hkv, int
     using namespace zs;
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0) return 0;
     const long long tiles = (Hq / Hkv + kPaRows - 1) / kPaRows;
-    return plan_bytes((long long)B * Hkv * tiles) + ml_bytes() + (size_t)2 * kPaMaxCtas * kPaRows * D * 4;
+    const int prow = std::min(Hq / Hkv, kPaRows);
+    return plan_bytes((long long)B * Hkv * tiles) + ml_bytes(prow) + (size_t)2 * kPaMaxCtas * kPaWarps * prow * D * 4;
 }
 
 extern "C" int zs_paged_attention(const ZsPagedAttention* p) {
@@ -600,6 +635,7 @@ extern "C" int zs_paged_attention(const ZsPagedAttention* p) {
     a.pages = p->pages;
     a.counts = p->counts;
     a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.width = p->width; a.top = top;
+    a.prow = std::min(a.G, kPaRows);
     a.scale2 = p->softmax_scale * kLog2e;
     a.out = p->out;
     a.lse = p->lse;
@@ -607,7 +643,7 @@ extern "C" int zs_paged_attention(const ZsPagedAttention* p) {
     a.plan = reinterpret_cast<long long*>(ws);
     ws += plan_bytes((long long)B * Hkv * a.tiles);
     a.part_ml = reinterpret_cast<float*>(ws);
-    ws += ml_bytes();
+    ws += ml_bytes(a.prow);
     a.part_o = reinterpret_cast<float*>(ws);
     a.err = p->err;
     cudaStream_t s = (cudaStream_t)p->stream;
