@@ -150,15 +150,15 @@ __global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const Bound
 // A cluster of CTAs a (sequence, KV head): each scores its share of the pages and
 // stores the scores, as order-preserving 32-bit keys, in the first CTA's shared
 // memory; that one finds the K-th largest key by histograms over the range of the
-// keys (1024 bins of it, then of the bin that holds the K-th, until a bin ends at
+// keys (512 bins of it, then of the bin that holds the K-th, until a bin ends at
 // the K-th or is one key wide) and writes the chosen pages in ascending order,
 // ties to the lowest page. Scoring is bound by HBM (2 D + 4 bytes a page and
 // head), choosing by the latency of some ten barriers.
-constexpr int kSelectThreads = 512;
+constexpr int kSelectThreads = 256;
 constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kSelectMaxPages = 32768;
 constexpr int kSelectMaxGroup = 128;
-constexpr int kSelectBins = 1024;
+constexpr int kSelectBins = 512;         // two a thread
 constexpr int kSelectMaxCluster = 8;
 
 struct SelectArgs {
@@ -181,6 +181,13 @@ __device__ __forceinline__ uint32_t order_key(float f) {
 
 __device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+__device__ __forceinline__ void red_cluster_min(uint32_t addr, uint32_t v) {
+    asm volatile("red.relaxed.cluster.shared::cluster.min.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void red_cluster_max(uint32_t addr, uint32_t v) {
+    asm volatile("red.relaxed.cluster.shared::cluster.max.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
 // Exclusive prefix of a 32-bit value over the block's threads.
@@ -209,10 +216,10 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectA
     constexpr int kPieces = 2 * D / 16;              // 16-byte pieces of a page's codes
     constexpr int kLanes = 4;                        // lanes a page
     constexpr int kLoads = kPieces / kLanes;
-    constexpr int kPages = 32 / kLanes;              // pages a warp pass
+    constexpr int kPages = 32 / kLanes;              // pages scored together
+    constexpr int kGroups = D <= 128 ? 4 : 2;        // of them a warp pass, loads in flight together
     extern __shared__ uint4 select_smem[];
-    __shared__ uint32_t s_part[2][kSelectWarps], s_hist[kSelectBins], s_pick[3], s_lo, s_hi;
-    __shared__ uint32_t s_most;
+    __shared__ uint32_t s_part[2][kSelectWarps], s_hist[kSelectBins], s_pick[3], s_lo, s_hi, s_most;
     const int unit = blockIdx.x / cluster, rank = blockIdx.x % cluster;
     const int b = unit / a.Hkv, h = unit % a.Hkv;
     const int G = a.Hq / a.Hkv, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -227,8 +234,16 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectA
         for (int i = rank * kSelectThreads + tid; i < a.top; i += cluster * kSelectThreads) out[i] = i < n ? i : -1;
         return;
     }
-    // no CTA writes into the first one's shared memory before that one runs
-    if (cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    // This CTA's pages; a warp passes over `pass` of them at a time, few where
+    // there are few. The blocks of the first pass are on their way during q's
+    // rounding.
+    const int share = (n + cluster - 1) / cluster;
+    const int p_end = min(n, (rank + 1) * share);
+    const int groups = min(kGroups, (share + kSelectWarps * kPages - 1) / (kSelectWarps * kPages));
+    const int pass = groups * kPages;
+    const int* row = a.table + b * a.table_stride;
+    int p0 = rank * share + warp * pass;
+    int blk = lane < pass && p0 + lane < p_end ? row[p0 + lane] : -1;
     int8_t* q8 = reinterpret_cast<int8_t*>(select_smem);              // [G][2 D]: positive part, negative part
     uint32_t* keys = reinterpret_cast<uint32_t*>(select_smem + G * kPieces);
     // q to whole numbers
@@ -238,6 +253,8 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectA
         s_hi = 0;
     }
     __syncthreads();
+    // no CTA writes into the first one's shared memory before that one has set it up
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     const uint32_t* q = reinterpret_cast<const uint32_t*>(a.q + ((long long)b * a.Hq + (long long)h * G) * D);
     uint32_t most = 0;
     for (int i = tid; i < G * D / 2; i += kSelectThreads) {
@@ -259,87 +276,86 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectA
         at[D / 2] = make_char2((signed char)min(x, 0), (signed char)min(y, 0));
     }
     __syncthreads();
-    // scores of this CTA's pages, kLanes lanes a page
-    const uint32_t keys0 = cluster > 1 ? mapa_shared(smem_u32(keys), 0) : 0;
-    if (cluster > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    const int share = (n + cluster - 1) / cluster;
-    const int p_end = min(n, (rank + 1) * share);
+    const uint32_t keys0 = mapa_shared(smem_u32(keys), 0);
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    // scores, kLanes lanes a page
     const int sub = lane / kLanes, l4 = lane % kLanes;
-    for (int p0 = rank * share + warp * 32; p0 < p_end; p0 += kSelectWarps * 32) {
-        // 32 pages a warp: their blocks, then kPages at a time
-        long long at = -1;
-        float s = 0.f;
-        if (p0 + lane < p_end) {
-            const int blk = a.table[b * a.table_stride + p0 + lane];
-            if (blk >= 0 && blk < a.num_blocks) {
-                at = (long long)blk * a.Hkv + h;
-                s = a.scales[at];
-            } else {
-                set_err(a.err, kErrPagedIndex);
-            }
+    uint32_t lo = 0xFFFFFFFFu, hi = 0;               // range of the scored keys
+    for (; p0 < p_end; p0 += kSelectWarps * pass) {
+        const int p = p0 + lane;
+        const bool mine = lane < pass && p < p_end;
+        if (mine && (blk < 0 || blk >= a.num_blocks)) {
+            set_err(a.err, kErrPagedIndex);
+            blk = -1;
         }
-        int best = 0;
-#pragma unroll 2
-        for (int j = 0; j < kLanes; ++j) {
-            const long long from = __shfl_sync(~0u, at, j * kPages + sub);
-            uint4 c[kLoads];
+        const long long at = blk >= 0 ? (long long)blk * a.Hkv + h : -1;
+        const float s = at >= 0 ? a.scales[at] : 0.f;
+        uint4 c[kGroups][kLoads];
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) {
+            const long long from = __shfl_sync(~0u, at, (j * kPages + sub) & 31);
 #pragma unroll
             for (int i = 0; i < kLoads; ++i)
-                c[i] = from >= 0 ? ld_nc16(a.codes + from * (2 * D) + (i * kLanes + l4) * 16) : make_uint4(0, 0, 0, 0);
-            int mx = INT_MIN;
-            for (int g = 0; g < G; ++g) {
+                c[j][i] = j < groups && from >= 0 ? ld_nc16(a.codes + from * (2 * D) + (i * kLanes + l4) * 16)
+                                                  : make_uint4(0, 0, 0, 0);
+        }
+        const int ahead = p0 + kSelectWarps * pass + lane;
+        blk = lane < pass && ahead < p_end ? row[ahead] : -1;
+        int mx[kGroups];
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) mx[j] = INT_MIN;
+        for (int g = 0; g < G; ++g) {
+            uint4 w[kLoads];                         // read once for the groups: shared memory would bound the scores
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) w[i] = select_smem[g * kPieces + i * kLanes + l4];
+#pragma unroll
+            for (int j = 0; j < kGroups; ++j) {
+                if (j >= groups) break;
                 int sum = 0;
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
-                    const uint4 w = select_smem[g * kPieces + i * kLanes + l4];
-                    sum = __dp4a((int)c[i].x, (int)w.x, sum);
-                    sum = __dp4a((int)c[i].y, (int)w.y, sum);
-                    sum = __dp4a((int)c[i].z, (int)w.z, sum);
-                    sum = __dp4a((int)c[i].w, (int)w.w, sum);
+                    sum = __dp4a((int)c[j][i].x, (int)w[i].x, sum);
+                    sum = __dp4a((int)c[j][i].y, (int)w[i].y, sum);
+                    sum = __dp4a((int)c[j][i].z, (int)w[i].z, sum);
+                    sum = __dp4a((int)c[j][i].w, (int)w[i].w, sum);
                 }
                 sum += __shfl_xor_sync(~0u, sum, 1);
                 sum += __shfl_xor_sync(~0u, sum, 2);
-                mx = max(mx, sum);
+                mx[j] = max(mx[j], sum);
             }
+        }
+        int best = 0;
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) {
             // page j * kPages + i is scored by lanes 4 i ..; lane j * kPages + i keeps it
-            const int got = __shfl_sync(~0u, mx, (lane % kPages) * kLanes);
+            const int got = __shfl_sync(~0u, mx[j], (lane % kPages) * kLanes);
             if (lane / kPages == j) best = got;
         }
-        const int p = p0 + lane;
-        if (p < p_end) {
-            const bool forced = p < a.sinks || p >= n - a.local;
-            const float score = s < INFINITY ? (float)best * s : INFINITY;
-            const uint32_t key = forced ? 0xFFFFFFFFu : order_key(score);
-            if (cluster > 1) st_cluster(keys0 + p * 4, key);
-            else keys[p] = key;
-        }
-    }
-    if (cluster > 1) cluster_sync();
-    else __syncthreads();
-    if (rank) return;
-    // range of the scored keys
-    uint32_t lo = 0xFFFFFFFFu, hi = 0;
-    for (int i = tid; i < n; i += kSelectThreads) {
-        const uint32_t k = keys[i];
-        if (k != 0xFFFFFFFFu) {
-            lo = min(lo, k);
-            hi = max(hi, k);
+        if (mine) {
+            uint32_t key = 0xFFFFFFFFu;              // the first and last pages are chosen in any case
+            if (p >= a.sinks && p < n - a.local) {
+                key = order_key(s < INFINITY ? (float)best * s : INFINITY);
+                lo = min(lo, key);
+                hi = max(hi, key);
+            }
+            st_cluster(keys0 + p * 4, key);
         }
     }
     lo = __reduce_min_sync(~0u, lo);
     hi = __reduce_max_sync(~0u, hi);
-    if (lane == 0) {
-        atomicMin(&s_lo, lo);
-        atomicMax(&s_hi, hi);
+    if (lane == 0 && hi) {
+        red_cluster_min(mapa_shared(smem_u32(&s_lo), 0), lo);
+        red_cluster_max(mapa_shared(smem_u32(&s_hi), 0), hi);
     }
-    __syncthreads();
+    cluster_sync();
+    if (rank) return;
     lo = s_lo;
     hi = s_hi;
     // top < n and the forced pages are sinks + local <= top, all different, so
     // at least one page is scored and `want` of the scored ones are chosen
     uint32_t want = (uint32_t)(a.top - a.sinks - a.local);
     while (want && lo != hi) {
-        const int shift = max(0, 22 - __clz(hi - lo));          // (hi - lo) >> shift is below 1024
+        const int shift = max(0, 23 - __clz(hi - lo));          // (hi - lo) >> shift is below 512
         for (int i = tid; i < kSelectBins; i += kSelectThreads) s_hist[i] = 0;
         __syncthreads();
         for (int i = tid; i < n; i += kSelectThreads) {
@@ -347,7 +363,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectA
             if (k >= lo && k <= hi) atomicAdd(&s_hist[(k - lo) >> shift], 1u);
         }
         __syncthreads();
-        // thread t looks at the bins kBins - 1 - 2 t and the one below, from the top
+        // thread t looks at bin kSelectBins - 1 - 2 t and the one below it
         const int top_bin = kSelectBins - 1 - 2 * tid;
         const uint32_t c0 = s_hist[top_bin], c1 = s_hist[top_bin - 1];
         const uint32_t above = select_scan(c0 + c1, s_part[0]);
