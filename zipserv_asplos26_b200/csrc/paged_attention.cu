@@ -108,9 +108,13 @@ __device__ __forceinline__ int entry_chunks(const PaArgs& a, int e) {
     return (max(0, min(a.lens[e], cap)) + kPaChunk - 1) / kPaChunk;
 }
 
-__device__ __forceinline__ long long warp_sum(long long v) {
+// Inclusive prefix over the warp's lanes.
+__device__ __forceinline__ long long warp_prefix(long long v) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(~0u, v, o);
+        if ((int)(threadIdx.x & 31) >= o) v += u;
+    }
     return v;
 }
 
@@ -145,8 +149,6 @@ __global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const PaArgs 
     constexpr int kPieces = D / 8;                 // 16-byte pieces a row
     constexpr int kKs = D / 16;
     extern __shared__ __align__(1024) uint8_t pa_smem[];
-    __shared__ long long s_red[2][kPaWarps], s_lo[kPaWarps];
-    __shared__ int s_entry[kPaWarps], s_chunks[kPaWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t ring = smem_u32(pa_smem) + warp * C::kRing;
     grid_dep_launch();
@@ -155,75 +157,54 @@ __global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const PaArgs 
     // ---- each warp's run of chunks
     const int entries = kListed ? a.B * a.Hkv : a.B;
     const int per_entry = kListed ? a.tiles : a.Hkv * a.tiles;     // units an entry
-    // chunks in all, and (one load for up to kPaThreads entries) this thread's first entry's
-    const int n0 = tid < entries ? entry_chunks<kListed>(a, tid) : 0;
-    long long mine = n0;
-    for (int e = tid + kPaThreads; e < entries; e += kPaThreads) mine += entry_chunks<kListed>(a, e);
-    long long inc0 = n0;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(~0u, inc0, o);
-        if (lane >= o) inc0 += u;
+    // Each warp by itself: lane i sums the chunks of entries [i per, (i + 1) per),
+    // a prefix over the lanes gives the total and the lane whose entries hold the
+    // warp's first chunk, a second one over those entries the entry.
+    const int per = (entries + 31) / 32;
+    long long mine = 0;
+    int n1 = 0;                    // the lane's last entry's (its only one up to 32 entries)
+#pragma unroll 4
+    for (int i = 0; i < per; ++i) {
+        const int e = lane * per + i;
+        n1 = e < entries ? entry_chunks<kListed>(a, e) : 0;
+        mine += n1;
     }
-    mine = entries <= kPaThreads ? __shfl_sync(~0u, inc0, 31) : warp_sum(mine);
-    if (lane == 31) s_red[0][warp] = inc0;
-    if (lane == 0) s_red[1][warp] = mine;
-    __syncthreads();
-    long long total = 0;
-#pragma unroll
-    for (int w = 0; w < kPaWarps; ++w) total += s_red[1][w];
-    total *= per_entry;
+    const long long inc = warp_prefix(mine);
+    const long long total = __shfl_sync(~0u, inc, 31) * per_entry;
     const int warps = gridDim.x * kPaWarps;
     const long long run = max(div_nonneg(total + warps - 1, warps), 1ll);
     if (blockIdx.x == 0 && tid == 0) a.plan[0] = run;
     // neighbouring runs go to different CTAs, so that few chunks spread over the SMs
     const int id = warp * (int)gridDim.x + (int)blockIdx.x;
-    // the entries that hold the four warps' first chunks
-    long long base = 0;
-    for (int e0 = 0; e0 < entries; e0 += kPaThreads) {
-        const int e = e0 + tid;
-        int n = n0;
-        long long inc = inc0;
-        if (e0) {
-            __syncthreads();
-            n = e < entries ? entry_chunks<kListed>(a, e) : 0;
-            inc = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long u = __shfl_up_sync(~0u, inc, o);
-                if (lane >= o) inc += u;
-            }
-            if (lane == 31) s_red[0][warp] = inc;
-            __syncthreads();
-        }
-        long long before = base;
-#pragma unroll
-        for (int w = 0; w < kPaWarps; ++w) {
-            if (w < warp) before += s_red[0][w];
-            base += s_red[0][w];
-        }
-        const long long lo = (before + inc - n) * per_entry, hi = (before + inc) * per_entry;
-#pragma unroll
-        for (int w = 0; w < kPaWarps; ++w) {
-            const long long at = run * (w * (int)gridDim.x + (int)blockIdx.x);
-            if (lo <= at && at < hi) {
-                s_entry[w] = e;
-                s_chunks[w] = n;
-                s_lo[w] = lo;
-            }
-        }
-        if (base * per_entry > run * ((kPaWarps - 1) * (int)gridDim.x + (int)blockIdx.x)) break;
-    }
-    __syncthreads();
     const long long c_begin = run * id;
     if (c_begin >= total) return;
     const int steps = (int)min(run, total - c_begin);
+    const int owner = __ffs(__ballot_sync(~0u, inc * per_entry > c_begin)) - 1;
+    long long lo = __shfl_sync(~0u, inc - mine, owner);            // entry chunks before, per unit
+    int entry = owner * per, n = __shfl_sync(~0u, n1, owner);
+    if (per > 1) {
+        for (;; entry += 32) {
+            const int e = entry + lane;
+            const int ne = e < min(entries, (owner + 1) * per) ? entry_chunks<kListed>(a, e) : 0;
+            const long long ie = warp_prefix((long long)ne);
+            const unsigned past = __ballot_sync(~0u, (lo + ie) * per_entry > c_begin);
+            if (past) {
+                const int l = __ffs(past) - 1;
+                entry += l;
+                n = __shfl_sync(~0u, ne, l);
+                lo += __shfl_sync(~0u, ie - ne, l);
+                break;
+            }
+            lo += __shfl_sync(~0u, ie, 31);
+        }
+    }
+    const long long into = c_begin - lo * per_entry;               // chunks into the entry
 
     PaCursor at;                   // of the copies
-    at.e = s_entry[warp];
-    at.n = s_chunks[warp];
-    at.in_e = (int)div_nonneg(c_begin - s_lo[warp], at.n);
-    at.ch = (int)(c_begin - s_lo[warp] - (long long)at.in_e * at.n);
+    at.e = entry;
+    at.n = n;
+    at.in_e = (int)div_nonneg(into, n);
+    at.ch = (int)(into - (long long)at.in_e * n);
     PaCursor cur = at;             // of the products
     long long u_lo = c_begin - at.ch;
 
@@ -265,7 +246,6 @@ __global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const PaArgs 
         if (at.ch == at.n && looked < steps) next_unit<kListed>(a, per_entry, at);
     };
     look(now);
-    look(next);
     int in_batch = 0;
     // starts the copies of step s; returns its number of valid tokens
     auto produce = [&](int s) {
@@ -297,8 +277,10 @@ __global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const PaArgs 
         return lim;
     };
     int lim_at[C::kStages];        // of the steps in flight, oldest first
+    lim_at[0] = produce(0);        // on its way while the next batch is looked up
+    look(next);
 #pragma unroll
-    for (int s = 0; s < C::kStages - 1; ++s) lim_at[s] = produce(s);
+    for (int s = 1; s < C::kStages - 1; ++s) lim_at[s] = produce(s);
 
     int s = 0;
     while (true) {

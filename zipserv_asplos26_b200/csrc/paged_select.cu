@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const Bound
 // A cluster of CTAs a (sequence, KV head): each scores its share of the pages and
 // stores the scores, as order-preserving 32-bit keys, in the first CTA's shared
 // memory; that one finds the K-th largest key by histograms over the range of the
-// keys (512 bins of it, then of the bin that holds the K-th, until a bin ends at
+// keys (1024 bins of it, then of the bin that holds the K-th, until a bin ends at
 // the K-th or is one key wide) and writes the chosen pages in ascending order,
 // ties to the lowest page. Scoring is bound by HBM (2 D + 4 bytes a page and
 // head), choosing by the latency of some ten barriers.
@@ -158,7 +158,7 @@ constexpr int kSelectThreads = 256;
 constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kSelectMaxPages = 32768;
 constexpr int kSelectMaxGroup = 128;
-constexpr int kSelectBins = 512;         // two a thread
+constexpr int kSelectBins = 1024;        // four a thread
 constexpr int kSelectMaxCluster = 8;
 
 struct SelectArgs {
@@ -190,6 +190,15 @@ __device__ __forceinline__ void red_cluster_max(uint32_t addr, uint32_t v) {
     asm volatile("red.relaxed.cluster.shared::cluster.max.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+        "%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 // Exclusive prefix of a 32-bit value over the block's threads.
 __device__ __forceinline__ uint32_t select_scan(uint32_t v, uint32_t* part) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -219,13 +228,16 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectA
     constexpr int kPages = 32 / kLanes;              // pages scored together
     constexpr int kGroups = D <= 128 ? 4 : 2;        // of them a warp pass, loads in flight together
     extern __shared__ uint4 select_smem[];
-    __shared__ uint32_t s_part[2][kSelectWarps], s_hist[kSelectBins], s_pick[3], s_lo, s_hi, s_most;
+    __shared__ __align__(16) uint32_t s_hist[kSelectBins];
+    __shared__ uint32_t s_part[2][kSelectWarps], s_pick[3], s_lo, s_hi, s_most;
     const int unit = blockIdx.x / cluster, rank = blockIdx.x % cluster;
     const int b = unit / a.Hkv, h = unit % a.Hkv;
     const int G = a.Hq / a.Hkv, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int sh = a.page_shift;
     grid_dep_launch();
     grid_dep_wait();
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(a.q + ((long long)b * a.Hq + (long long)h * G) * D);
+    const uint32_t q0 = tid < G * D / 2 ? q[tid] : 0;              // beside the length
     const int len = max(0, min(a.lens[b], (int)min((long long)a.width << sh, (long long)INT_MAX)));
     const int n = (int)(((long long)len + (1 << sh) - 1) >> sh);
     int* out = a.pages + (long long)unit * a.top;
@@ -255,10 +267,9 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectA
     __syncthreads();
     // no CTA writes into the first one's shared memory before that one has set it up
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    const uint32_t* q = reinterpret_cast<const uint32_t*>(a.q + ((long long)b * a.Hq + (long long)h * G) * D);
     uint32_t most = 0;
     for (int i = tid; i < G * D / 2; i += kSelectThreads) {
-        const float2 f = unpack2<T>(q[i]);
+        const float2 f = unpack2<T>(i == tid ? q0 : q[i]);
         most = max(most, max(__float_as_uint(f.x) & 0x7FFFFFFFu, __float_as_uint(f.y) & 0x7FFFFFFFu));
     }
     most = __reduce_max_sync(~0u, most);
@@ -268,7 +279,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectA
     const float step = __uint_as_float(most & 0x7F800000u) * 0.015625f;
     const bool live = most < 0x7F800000u && step > 0.f;
     for (int i = tid; i < G * D / 2; i += kSelectThreads) {
-        const float2 f = unpack2<T>(q[i]);
+        const float2 f = unpack2<T>(i == tid ? q0 : q[i]);
         const int x = live ? max(-127, min(127, (int)rintf(f.x / step))) : 0;
         const int y = live ? max(-127, min(127, (int)rintf(f.y / step))) : 0;
         char2* at = reinterpret_cast<char2*>(q8 + (i / (D / 2)) * 2 * D + i % (D / 2) * 2);
@@ -301,35 +312,42 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectA
         }
         const int ahead = p0 + kSelectWarps * pass + lane;
         blk = lane < pass && ahead < p_end ? row[ahead] : -1;
-        int mx[kGroups];
+        // Products of 8-bit matrices, 16 heads x 32 codes x 8 pages: as the order of
+        // the codes does not matter, a lane's 16-byte pieces are used as they lie.
+        int best = INT_MIN;
+        for (int g0 = 0; g0 < G; g0 += 16) {
+            int sum[kGroups][4];
 #pragma unroll
-        for (int j = 0; j < kGroups; ++j) mx[j] = INT_MIN;
-        for (int g = 0; g < G; ++g) {
-            uint4 w[kLoads];                         // read once for the groups: shared memory would bound the scores
+            for (int j = 0; j < kGroups; ++j)
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) w[i] = select_smem[g * kPieces + i * kLanes + l4];
+                for (int x = 0; x < 4; ++x) sum[j][x] = 0;
+            const bool r0 = g0 + sub < G, r1 = g0 + sub + 8 < G;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const uint4 zero = make_uint4(0, 0, 0, 0);
+                const uint4 w0 = r0 ? select_smem[(g0 + sub) * kPieces + i * kLanes + l4] : zero;
+                const uint4 w1 = r1 ? select_smem[(g0 + sub + 8) * kPieces + i * kLanes + l4] : zero;
+#pragma unroll
+                for (int j = 0; j < kGroups; ++j) {
+                    mma_s8(sum[j], w0.x, w1.x, w0.y, w1.y, c[j][i].x, c[j][i].y);
+                    mma_s8(sum[j], w0.z, w1.z, w0.w, w1.w, c[j][i].z, c[j][i].w);
+                }
+            }
+            // heads sub and sub + 8, pages 2 l4 and 2 l4 + 1 of each group
 #pragma unroll
             for (int j = 0; j < kGroups; ++j) {
-                if (j >= groups) break;
-                int sum = 0;
+                int x = max(r0 ? sum[j][0] : INT_MIN, r1 ? sum[j][2] : INT_MIN);
+                int y = max(r0 ? sum[j][1] : INT_MIN, r1 ? sum[j][3] : INT_MIN);
 #pragma unroll
-                for (int i = 0; i < kLoads; ++i) {
-                    sum = __dp4a((int)c[j][i].x, (int)w[i].x, sum);
-                    sum = __dp4a((int)c[j][i].y, (int)w[i].y, sum);
-                    sum = __dp4a((int)c[j][i].z, (int)w[i].z, sum);
-                    sum = __dp4a((int)c[j][i].w, (int)w[i].w, sum);
+                for (int o = kLanes; o < 32; o <<= 1) {
+                    x = max(x, __shfl_xor_sync(~0u, x, o));
+                    y = max(y, __shfl_xor_sync(~0u, y, o));
                 }
-                sum += __shfl_xor_sync(~0u, sum, 1);
-                sum += __shfl_xor_sync(~0u, sum, 2);
-                mx[j] = max(mx[j], sum);
+                // lane j * kPages + i keeps page i of group j
+                const int from = (lane % kPages) / 2;
+                const int gx = __shfl_sync(~0u, x, from), gy = __shfl_sync(~0u, y, from);
+                if (lane / kPages == j) best = max(best, lane & 1 ? gy : gx);
             }
-        }
-        int best = 0;
-#pragma unroll
-        for (int j = 0; j < kGroups; ++j) {
-            // page j * kPages + i is scored by lanes 4 i ..; lane j * kPages + i keeps it
-            const int got = __shfl_sync(~0u, mx[j], (lane % kPages) * kLanes);
-            if (lane / kPages == j) best = got;
         }
         if (mine) {
             uint32_t key = 0xFFFFFFFFu;              // the first and last pages are chosen in any case
@@ -355,7 +373,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectA
     // at least one page is scored and `want` of the scored ones are chosen
     uint32_t want = (uint32_t)(a.top - a.sinks - a.local);
     while (want && lo != hi) {
-        const int shift = max(0, 23 - __clz(hi - lo));          // (hi - lo) >> shift is below 512
+        const int shift = max(0, 22 - __clz(hi - lo));          // (hi - lo) >> shift is below 1024
         for (int i = tid; i < kSelectBins; i += kSelectThreads) s_hist[i] = 0;
         __syncthreads();
         for (int i = tid; i < n; i += kSelectThreads) {
@@ -363,15 +381,18 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectA
             if (k >= lo && k <= hi) atomicAdd(&s_hist[(k - lo) >> shift], 1u);
         }
         __syncthreads();
-        // thread t looks at bin kSelectBins - 1 - 2 t and the one below it
-        const int top_bin = kSelectBins - 1 - 2 * tid;
-        const uint32_t c0 = s_hist[top_bin], c1 = s_hist[top_bin - 1];
-        const uint32_t above = select_scan(c0 + c1, s_part[0]);
-        if (above < want && above + c0 + c1 >= want) {
-            const bool upper = above + c0 >= want;
-            s_pick[0] = upper ? top_bin : top_bin - 1;
-            s_pick[1] = want - above - (upper ? 0 : c0);
-            s_pick[2] = upper ? c0 : c1;
+        // thread t looks at four bins, from kSelectBins - 1 - 4 t down
+        const uint4 bins = reinterpret_cast<const uint4*>(s_hist)[kSelectThreads - 1 - tid];
+        uint32_t above = select_scan(bins.x + bins.y + bins.z + bins.w, s_part[0]);
+        const uint32_t count[4] = {bins.w, bins.z, bins.y, bins.x};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (above < want && above + count[i] >= want) {
+                s_pick[0] = kSelectBins - 1 - 4 * tid - i;
+                s_pick[1] = want - above;
+                s_pick[2] = count[i];
+            }
+            above += count[i];
         }
         __syncthreads();
         const uint32_t from = lo + (s_pick[0] << shift);
