@@ -56,8 +56,18 @@ struct PaArgs {
     unsigned* err;
 };
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+// The keys and values pass through L2 once: marked to leave it first, they do not
+// push out what the kernels around share through it (tables, q, pieces, the next
+// layer's weights).
+__device__ __forceinline__ uint64_t evict_first_policy() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint.L2::256B [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src),
+                 "r"(on ? 16 : 0), "l"(policy)
+                 : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -153,6 +163,8 @@ __global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const PaArgs 
     const uint32_t ring = smem_u32(pa_smem) + warp * C::kRing;
     grid_dep_launch();
     grid_dep_wait();
+
+    const uint64_t policy = evict_first_policy();
 
     // ---- each warp's run of chunks
     const int entries = kListed ? a.B * a.Hkv : a.B;
@@ -269,8 +281,8 @@ __global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const PaArgs 
             for (int i = 0; i < kPaChunk * kPieces / 32; ++i) {
                 const int x = i * 32 + lane, r = x / kPieces, pc = x % kPieces;
                 const uint32_t to = dst + r * C::kRowBytes + ((pc ^ (r & 7)) * 16);
-                cp16(to, ks + r * a.kp.s_token + pc * 8, r < lim);
-                cp16(to + C::kTile, vs + r * a.vp.s_token + pc * 8, r < lim);
+                cp16(to, ks + r * a.kp.s_token + pc * 8, r < lim, policy);
+                cp16(to + C::kTile, vs + r * a.vp.s_token + pc * 8, r < lim, policy);
             }
         }
         cp_commit();
