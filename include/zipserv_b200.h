@@ -333,8 +333,8 @@ size_t zs_paged_attention_workspace_bytes(int B, int Hq, int Hkv, int D);
 int zs_paged_attention(const ZsPagedAttention* args);
 
 /* Bounds of the pages that sequences completed between lens_before[b] and
- * seq_lens[b] tokens (at most max_new tokens each): codes [num_blocks][num_heads]
- * [2][D] int8 (16-byte aligned), upper then lower bound of the keys per channel in
+ * seq_lens[b] tokens (at most max_new tokens each and, unless it is 0, max_total in
+ * all; the bounds size the grid): codes [num_blocks][num_heads][2][D] int8 (16-byte aligned), upper then lower bound of the keys per channel in
  * units of scales [num_blocks][num_heads], a power of two (infinite, with codes
  * of zero, for a page with a non-finite key). D is 64, 128 or 256. */
 typedef struct ZsPageBounds {
@@ -347,7 +347,7 @@ typedef struct ZsPageBounds {
     float* scales;
     unsigned* err;
     ZsPagePool k_pool;
-    int B, width, max_new, reserved;
+    int B, width, max_new, max_total;
 } ZsPageBounds;
 int zs_page_bounds(const ZsPageBounds* args);
 

@@ -324,6 +324,18 @@ def test_paged_attention(lens, hq, hkv, D, page, dtype, layout):
     assert again.shape == (len(lens), 1, hq, D) and torch.equal(again.squeeze(1), out)      # bit for bit
 
 
+def test_no_sequences():
+    z = zs()
+    c = Cache([40], 2, 64, 16, BF, "heads", 1)
+    q, lens = torch.zeros(0, 4, 64, device=DEV, dtype=BF), c.lens[:0]
+    assert z.paged_attention(q, c.k, c.v, c.table[:0], lens).shape == (0, 4, 64)
+    codes = torch.zeros(c.k.shape[0], 2, 2, 64, dtype=torch.int8, device=DEV)
+    scales = torch.zeros(c.k.shape[0], 2, device=DEV)
+    z.page_bounds(c.k, c.table[:0], lens, lens, codes, scales, 5)
+    out, pages, counts = z.sparse_attention(q, c.k, c.v, codes, scales, c.table[:0], lens, 4)
+    assert out.shape == (0, 4, 64) and pages.shape == (0, 2, 4) and counts.shape == (0, 2)
+
+
 def test_paged_attention_large_scores_and_scale():
     """Scores of some hundreds: the running maximum moves, all but a few weights vanish."""
     c = Cache([700, 90], 2, 128, 64, BF, "heads", 5, k_scale=4.0)
@@ -467,7 +479,8 @@ def test_page_bounds(page, hkv, D, dtype, layout):
     codes = torch.full((n, hkv, 2, D), 99, dtype=torch.int8, device=DEV)
     scales = torch.full((n, hkv), -3.0, device=DEV)
     err = torch.zeros(1, dtype=torch.int32, device=DEV)
-    zs().page_bounds(k, c.table, i32(before), c.lens, codes, scales, max(a - b for a, b in zip(after, before)), err)
+    zs().page_bounds(k, c.table, i32(before), c.lens, codes, scales, max(a - b for a, b in zip(after, before)),
+                     err=err)
     done = set()
     for i, (a, z) in enumerate(zip(before, after)):
         done |= {int(c.table[i, p]) for p in range(a // page, z // page)}
@@ -479,6 +492,27 @@ def test_page_bounds(page, hkv, D, dtype, layout):
         else:
             assert bool((codes[blk] == 99).all() and (scales[blk] == -3).all())
     assert err.item() == 0
+
+
+@pytest.mark.parametrize("B,prompts,page", [(3, {1: 700}, 16), (70, {0: 333, 69: 90}, 32), (300, {7: 5000}, 64),
+                                            (1, {0: 129}, 128)])
+def test_page_bounds_of_a_few_prompts_among_many_sequences(B, prompts, page):
+    """The same bounds whether the tokens in all are bounded or not."""
+    rng = np.random.default_rng(B)
+    before = rng.integers(0, 3 * page, B)
+    after = before + 1
+    for b, n in prompts.items():
+        after[b] = before[b] + n
+    c = Cache(after, 2, 64, page, BF, "heads", seed=B)
+    n = c.k.shape[0]
+    got = []
+    for total in (None, int((after - before).sum())):
+        codes = torch.full((n, 2, 2, 64), 99, dtype=torch.int8, device=DEV)
+        scales = torch.full((n, 2), -3.0, device=DEV)
+        zs().page_bounds(c.k, c.table, i32(before), c.lens, codes, scales, max(prompts.values()), total)
+        got.append((codes, scales))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    assert int((got[0][1][:, 0] > 0).sum()) == int((after // page - before // page).sum())
 
 
 def select_ref(q, codes, scales, table, lens, page, top, sinks, local):

@@ -473,7 +473,11 @@ PyObject* page_bounds(PyObject* const* a) {
     p.seq_lens = vec<int>(a[3], B, at::kInt, "seq_lens", index);
     const Bounds b = bounds_buffers(a[4], a[5], p.k_pool.num_blocks, p.k_pool.num_heads, dim, index);
     need(most >= 0 && most <= INT32_MAX, "max_new must be from 0 to 2**31 - 1");
-    p.err = err_word(a[7], index);
+    const int64_t total = given(a[7]) ? integer(a[7]) : 0;
+    need(total >= 0 && total <= INT32_MAX, "max_total must be from 0 to 2**31 - 1");
+    if (given(a[7]) && total == 0) Py_RETURN_NONE;
+    p.max_total = static_cast<int>(total);
+    p.err = err_word(a[8], index);
     OnDevice on(index);
     p.stream = current_stream(index);
     p.block_table = table.data;
@@ -589,7 +593,7 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 #define ZS_ENTRY(name, n) \
     {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<name, n>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {ZS_ENTRY(plan_step, 9),    ZS_ENTRY(rope_write, 12),  ZS_ENTRY(paged_attention, 11),
-                         ZS_ENTRY(page_bounds, 8),  ZS_ENTRY(select_pages, 10), ZS_ENTRY(sparse_attention, 13),
+                         ZS_ENTRY(page_bounds, 9),  ZS_ENTRY(select_pages, 10), ZS_ENTRY(sparse_attention, 13),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_paged_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -49,27 +49,35 @@ struct PlanArgs {
     unsigned* err;
 };
 
-// Exclusive prefix of v over the block's threads; *total gets the block's sum.
-// `part` is this scan's own kPlanWarps entries of shared memory.
-__device__ __forceinline__ long long block_scan(long long v, long long* part, long long* total) {
+// Exclusive prefixes of N values over the block's threads, their sums in total.
+// `part` is this scan's own N * kPlanWarps entries of shared memory.
+template <int N>
+__device__ __forceinline__ void block_scan(long long (&v)[N], long long* part, long long (&total)[N]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long inc = v;
+    long long inc[N];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(~0u, inc, o);
-        if (lane >= o) inc += u;
+    for (int i = 0; i < N; ++i) {
+        inc[i] = v[i];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(~0u, inc[i], o);
+            if (lane >= o) inc[i] += u;
+        }
+        if (lane == 31) part[i * kPlanWarps + warp] = inc[i];
     }
-    if (lane == 31) part[warp] = inc;
     __syncthreads();
-    long long w = lane < kPlanWarps ? part[lane] : 0;
 #pragma unroll
-    for (int o = 1; o < kPlanWarps; o <<= 1) {
-        const long long u = __shfl_up_sync(~0u, w, o);
-        if (lane >= o) w += u;
+    for (int i = 0; i < N; ++i) {
+        long long w = lane < kPlanWarps ? part[i * kPlanWarps + lane] : 0;
+#pragma unroll
+        for (int o = 1; o < kPlanWarps; o <<= 1) {
+            const long long u = __shfl_up_sync(~0u, w, o);
+            if (lane >= o) w += u;
+        }
+        const long long before = __shfl_sync(~0u, w, warp ? warp - 1 : 0);
+        total[i] = __shfl_sync(~0u, w, kPlanWarps - 1);
+        v[i] = inc[i] - v[i] + (warp ? before : 0);
     }
-    const long long before = __shfl_sync(~0u, w, warp ? warp - 1 : 0);
-    *total = __shfl_sync(~0u, w, kPlanWarps - 1);
-    return inc - v + (warp ? before : 0);
 }
 
 // Largest r in [0, n) with pre[r] <= x (pre ascending, pre[0] == 0).
@@ -84,63 +92,69 @@ __device__ __forceinline__ int owner(const int* pre, int n, int x) {
 
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     extern __shared__ int plan_smem[];
-    __shared__ long long parts[4][kPlanWarps];
+    __shared__ long long parts[4 * kPlanWarps];
     __shared__ int s_taken;            // pages taken by the step
-    if (threadIdx.x == 0) s_taken = 0;
-    int* cu = plan_smem;               // [R + 1] admitted tokens before request r
-    int* need0 = cu + a.R + 1;         // [R] pages taken before request r
-    int* back0 = need0 + a.R + 1;      // [R + 1] pages given back before request r
     const int R = a.R, sh = a.page_shift, P1 = (1 << sh) - 1;
+    int* cu = plan_smem;               // [R + 1] admitted tokens before request r
+    int* back0 = cu + R + 1;           // [R + 1] pages given back before request r
+    int* need0 = back0 + R + 1;        // [R] pages taken before request r
+    int* lens = need0 + R;             // [R] lengths before the step
+    int* fresh = lens + R;             // [R] tokens asked for, negative: ended
+    const int count_in = *a.count;
+    const int len_cap = (int)min((long long)a.width << sh, (long long)INT_MAX - P1);
+    for (int r = threadIdx.x; r < R; r += kPlanThreads) {
+        lens[r] = max(0, min(a.lens[r], len_cap));
+        fresh[r] = a.fresh[r];
+    }
+    if (threadIdx.x == 0) s_taken = 0;
+    __syncthreads();
     const int per = (R + kPlanThreads - 1) / kPlanThreads;
     const int r0 = min(R, (int)threadIdx.x * per), r1 = min(R, r0 + per);
-    const int len_cap = (int)min((long long)a.width << sh, (long long)INT_MAX - P1);
-
-    auto length = [&](int r) { return max(0, min(a.lens[r], len_cap)); };
     // 1. pages given back, tokens asked for
-    long long back_sum = 0, want_sum = 0;
+    long long first_sums[2] = {0, 0}, first_totals[2];
     for (int r = r0; r < r1; ++r) {
-        const int f = a.fresh[r];
-        if (f < 0) back_sum += (length(r) + P1) >> sh;
-        else want_sum += f;
+        if (fresh[r] < 0) first_sums[0] += (lens[r] + P1) >> sh;
+        else first_sums[1] += fresh[r];
     }
-    long long back_total, want_total, need_total, got_total;
-    long long back = block_scan(back_sum, parts[0], &back_total);
-    long long want = block_scan(want_sum, parts[1], &want_total);
-    const int count0 = max(0, min(*a.count, a.capacity));
+    block_scan(first_sums, parts, first_totals);
+    long long back = first_sums[0];
+    const long long want = first_sums[1], back_total = first_totals[0];
+    const int count0 = max(0, min(count_in, a.capacity));
     const long long have = min((long long)count0 + back_total, (long long)a.capacity);
     // 2. pages needed by the requests that fit the step and the table
     auto pages_needed = [&](int r, long long want_end) -> int {
-        const int f = a.fresh[r], len = length(r);
+        const int f = fresh[r], len = lens[r];
         const long long pages = ((long long)len + max(f, 0) + P1) >> sh;
         if (f < 0 || want_end > a.max_tokens || pages > a.width) return -1;
         return (int)(pages - ((len + P1) >> sh));
     };
-    long long need_sum = 0;
+    long long need[1] = {0}, need_total[1];
     long long w = want;
     for (int r = r0; r < r1; ++r) {
-        w += max(a.fresh[r], 0);
-        need_sum += max(pages_needed(r, w), 0);
+        w += max(fresh[r], 0);
+        need[0] += max(pages_needed(r, w), 0);
     }
-    long long need = block_scan(need_sum, parts[2], &need_total);
+    block_scan(need, parts + 2 * kPlanWarps, need_total);
     // 3. admitted tokens
-    long long got_sum = 0;
+    long long got_sum[1] = {0}, got_total[1];
     w = want;
-    long long n = need;
+    long long n = need[0];
     for (int r = r0; r < r1; ++r) {
-        const int f = a.fresh[r];
+        const int f = fresh[r];
         w += max(f, 0);
         const int p = pages_needed(r, w);
         n += max(p, 0);
-        if (p == 0 || (p > 0 && n <= have)) got_sum += f;
+        if (p == 0 || (p > 0 && n <= have)) got_sum[0] += f;
     }
-    long long got = block_scan(got_sum, parts[3], &got_total);
+    block_scan(got_sum, parts + 3 * kPlanWarps, got_total);
+    long long got = got_sum[0];
     w = want;
-    n = need;
+    n = need[0];
     const bool first = blockIdx.x == 0;
     bool any_refused = false;
     int end = 0;
     for (int r = r0; r < r1; ++r) {
-        const int f = a.fresh[r], len = length(r);
+        const int f = fresh[r], len = lens[r];
         w += max(f, 0);
         const int p = pages_needed(r, w);
         const bool ok = p == 0 || (p > 0 && n + p <= have);
@@ -163,7 +177,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     // admitted request's do.
     if (end) atomicMax(&s_taken, end);
     if (threadIdx.x == 0) {
-        cu[R] = (int)got_total;
+        cu[R] = (int)got_total[0];
         back0[R] = (int)back_total;
     }
     if (first && any_refused) set_err(a.err, kErrPagedFull);
@@ -189,7 +203,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     // new table entries
     for (int j = gid; j < used; j += gsize) {
         const int r = owner(need0, R, j);
-        const int col = ((length(r) + P1) >> sh) + (j - need0[r]);
+        const int col = ((lens[r] + P1) >> sh) + (j - need0[r]);
         a.table[(long long)r * a.table_stride + col] = free_page((int)have - 1 - j);
     }
     // tokens
@@ -199,7 +213,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
         int r = -1, pos = 0;
         if (t < tokens) {
             r = owner(cu, R, t);
-            const int len = length(r);
+            const int len = lens[r];
             pos = len + (t - cu[r]);
             const int col = pos >> sh, old = (len + P1) >> sh;
             const int blk = col < old ? a.table[(long long)r * a.table_stride + col]
@@ -232,8 +246,8 @@ extern "C" int zs_plan_step(const ZsPlanStep* p) {
                p->free_blocks, p->free_count, p->out_lens, p->out_count, p->out_cu,
                reinterpret_cast<long long*>(p->slots), p->token_seq, p->positions, p->refused, p->err};
     while ((1 << a.page_shift) < page_size) ++a.page_shift;
-    const size_t smem = 3 * sizeof(int) * ((size_t)R + 1);
-    if (smem > 48 * 1024) {
+    const size_t smem = sizeof(int) * (5 * (size_t)R + 2);
+    if (smem > 40 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
     }

@@ -33,7 +33,8 @@ struct BoundsArgs {
     PoolView kp;
     const int* table;
     long long table_stride;
-    int B, width, per_seq;
+    int B, width;
+    int per_seq;       // tasks a sequence, or 0: tasks are the complete pages in order
     const int* before;
     const int* lens;
     int8_t* codes;     // [num_blocks][heads][2][D]
@@ -65,14 +66,44 @@ __global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const Bound
     const int lane = threadIdx.x & 31;
     const long long warp = (long long)blockIdx.x * (kBoundsThreads / 32) + (threadIdx.x >> 5);
     const int h = (int)(warp % a.kp.heads);
-    const long long bj = warp / a.kp.heads;
-    const int b = (int)(bj / a.per_seq), j = (int)(bj % a.per_seq);
-    if (b >= a.B) return;
+    const long long task = warp / a.kp.heads;
     const int sh = a.kp.page_shift;
-    const int before = max(a.before[b], 0);
-    const int last = min(a.lens[b] >> sh, a.width);
-    const int p = (before >> sh) + j;        // pages [before / P, len / P) became complete
-    if (p >= last) return;
+    // pages [before / P, len / P) of a sequence became complete
+    auto range = [&](int b, int& first) {
+        first = max(a.before[b], 0) >> sh;
+        return max(0, min(a.lens[b] >> sh, a.width) - first);
+    };
+    int b, p;
+    if (a.per_seq) {                         // a rectangle of tasks
+        b = (int)(task / a.per_seq);
+        p = (int)(task % a.per_seq);
+        if (b >= a.B) return;
+        int first;
+        if (p >= range(b, first)) return;
+        p += first;
+    } else {                                 // the complete pages in order: found by a prefix over the sequences
+        const int per = (a.B + 31) / 32;
+        long long mine = 0;
+        int first;
+        for (int i = 0; i < per; ++i)
+            if (lane * per + i < a.B) mine += range(lane * per + i, first);
+        long long inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(~0u, inc, o);
+            if (lane >= o) inc += u;
+        }
+        const unsigned past = __ballot_sync(~0u, inc > task);
+        if (!past) return;
+        const int owner = __ffs(past) - 1;
+        long long left = task - __shfl_sync(~0u, inc - mine, owner);
+        for (b = owner * per;; ++b) {
+            const int n = range(b, first);
+            if (left < n) break;
+            left -= n;
+        }
+        p = first + (int)left;
+    }
     const int blk = a.table[b * a.table_stride + p];
     if (blk < 0 || blk >= a.kp.num_blocks) {
         if (lane == 0) set_err(a.err, kErrPagedIndex);
@@ -463,7 +494,7 @@ extern "C" int zs_page_bounds(const ZsPageBounds* p) {
     using namespace zs;
     BoundsArgs a{};
     if (!p || !make_pool(&p->k_pool, &a.kp) || p->B < 0 || p->width <= 0 || p->table_stride < p->width ||
-        p->max_new < 0)
+        p->max_new < 0 || p->max_total < 0)
         return cudaErrorInvalidValue;
     if (a.kp.dim != 64 && a.kp.dim != 128 && a.kp.dim != 256) return cudaErrorInvalidValue;
     if (p->B == 0 || p->max_new == 0) return cudaSuccess;
@@ -474,15 +505,24 @@ extern "C" int zs_page_bounds(const ZsPageBounds* p) {
     a.table_stride = p->table_stride;
     a.B = B;
     a.width = p->width;
-    // max_new tokens complete at most this many pages of a sequence
-    a.per_seq = (int)std::min<long long>(p->width, ((long long)p->max_new + (1 << a.kp.page_shift) - 1) >>
-                                                       a.kp.page_shift);
+    // max_new tokens complete at most this many pages of a sequence; max_total
+    // tokens in all at most one a sequence more than their pages. The second
+    // bound is the smaller one where a few of many sequences got a prompt: then
+    // each warp looks its page up.
+    const int page = 1 << a.kp.page_shift;
+    const long long per_seq = std::min<long long>(p->width, ((long long)p->max_new + page - 1) / page);
+    long long tasks = per_seq * B;
+    a.per_seq = (int)per_seq;
+    if (p->max_total > 0 && p->max_total / page + B < tasks / 2) {
+        tasks = p->max_total / page + B;
+        a.per_seq = 0;
+    }
     a.before = p->lens_before;
     a.lens = p->seq_lens;
     a.codes = p->codes;
     a.scales = p->scales;
     a.err = p->err;
-    const long long warps = (long long)B * a.per_seq * a.kp.heads;
+    const long long warps = tasks * a.kp.heads;
     const long long grid = (warps + kBoundsThreads / 32 - 1) / (kBoundsThreads / 32);
     if (grid > INT32_MAX) return cudaErrorInvalidValue;
     cudaStream_t s = (cudaStream_t)p->stream;

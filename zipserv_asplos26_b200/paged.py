@@ -117,11 +117,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 # ------------------------------------------------------------------ sparse
 def page_bounds(k_pages: torch.Tensor, block_table: torch.Tensor, lens_before: torch.Tensor, seq_lens: torch.Tensor,
                 page_codes: torch.Tensor, page_scales: torch.Tensor, max_new: int,
-                err: Optional[torch.Tensor] = None) -> None:
+                max_total: Optional[int] = None, err: Optional[torch.Tensor] = None) -> None:
     """Bounds of the pages that sequences completed between lens_before and
-    seq_lens (at most max_new tokens each), written to page_codes int8
-    [num_blocks, Hkv, 2, D] (upper, lower) and page_scales fp32 [num_blocks, Hkv]."""
-    (_native or _load()).page_bounds(k_pages, block_table, lens_before, seq_lens, page_codes, page_scales, max_new, err)
+    seq_lens, written to page_codes int8 [num_blocks, Hkv, 2, D] (upper, lower)
+    and page_scales fp32 [num_blocks, Hkv]. At most max_new tokens are new in a
+    sequence, and at most max_total in all sequences where it is given."""
+    (_native or _load()).page_bounds(k_pages, block_table, lens_before, seq_lens, page_codes, page_scales, max_new,
+                                     max_total, err)
 
 
 def select_pages(q: torch.Tensor, page_codes: torch.Tensor, page_scales: torch.Tensor, block_table: torch.Tensor,
@@ -215,8 +217,9 @@ class PagedKVCache:
         q = rope_write(q, k, v, plan.positions if positions is None else positions, cos_sin, plan.slots, self.k,
                        self.v, sections, interleaved, None, self.err)
         if self.codes is not None:
-            page_bounds(self.k, self.block_table, self.lens_before, self.seqlens, self.codes, self.scales,
-                        plan.slots.numel(), self.err)
+            n = plan.slots.numel()
+            page_bounds(self.k, self.block_table, self.lens_before, self.seqlens, self.codes, self.scales, n, n,
+                        self.err)
         return q
 
     def attention(self, q: torch.Tensor, softmax_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
