@@ -196,33 +196,35 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
         const int r = owner(back0, R, b);
         return a.table[(long long)r * a.table_stride + (b - back0[r])];
     };
-    const int gid = blockIdx.x * kPlanThreads + threadIdx.x, gsize = gridDim.x * kPlanThreads;
-    // give pages back (the free list has room for every page of the pool)
-    const int nback = (int)(have - count0);
-    for (int i = gid; i < nback; i += gsize) a.free_list[count0 + i] = free_page(count0 + i);
-    // new table entries
-    for (int j = gid; j < used; j += gsize) {
-        const int r = owner(need0, R, j);
-        const int col = ((lens[r] + P1) >> sh) + (j - need0[r]);
-        a.table[(long long)r * a.table_stride + col] = free_page((int)have - 1 - j);
-    }
-    // tokens
-    const int tokens = cu[R];
-    for (int t = gid; t < a.max_tokens; t += gsize) {
-        long long slot = -1;
-        int r = -1, pos = 0;
-        if (t < tokens) {
-            r = owner(cu, R, t);
-            const int len = lens[r];
-            pos = len + (t - cu[r]);
-            const int col = pos >> sh, old = (len + P1) >> sh;
-            const int blk = col < old ? a.table[(long long)r * a.table_stride + col]
-                                      : free_page((int)have - 1 - (need0[r] + col - old));
-            slot = ((long long)blk << sh) + (pos & P1);
+    // One index space for the pages given back (the free list has room for every
+    // page of the pool), the new table entries and the tokens, so that their
+    // lookups are in flight together.
+    const int nback = (int)(have - count0), tokens = cu[R];
+    const long long items = (long long)nback + used + a.max_tokens;
+    for (long long i = blockIdx.x * kPlanThreads + threadIdx.x; i < items; i += gridDim.x * kPlanThreads) {
+        if (i < nback) {
+            a.free_list[count0 + i] = free_page(count0 + (int)i);
+        } else if (i < nback + (long long)used) {
+            const int j = (int)(i - nback), r = owner(need0, R, j);
+            const int col = ((lens[r] + P1) >> sh) + (j - need0[r]);
+            a.table[(long long)r * a.table_stride + col] = free_page((int)have - 1 - j);
+        } else {
+            const int t = (int)(i - nback - used);
+            long long slot = -1;
+            int r = -1, pos = 0;
+            if (t < tokens) {
+                r = owner(cu, R, t);
+                const int len = lens[r];
+                pos = len + (t - cu[r]);
+                const int col = pos >> sh, old = (len + P1) >> sh;
+                const int blk = col < old ? a.table[(long long)r * a.table_stride + col]
+                                          : free_page((int)have - 1 - (need0[r] + col - old));
+                slot = ((long long)blk << sh) + (pos & P1);
+            }
+            a.slots[t] = slot;
+            a.token_seq[t] = r;
+            a.positions[t] = pos;
         }
-        a.slots[t] = slot;
-        a.token_seq[t] = r;
-        a.positions[t] = pos;
     }
 }
 
@@ -251,7 +253,9 @@ extern "C" int zs_plan_step(const ZsPlanStep* p) {
         const cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
     }
-    const int grid = std::max(1, std::min(148, (max_tokens + kPlanThreads - 1) / kPlanThreads));
+    // a thread a token, with some more for pages
+    const long long items = max_tokens + ((long long)max_tokens >> a.page_shift) + 2ll * R;
+    const int grid = (int)std::min(148ll, (items + kPlanThreads - 1) / kPlanThreads);
     plan_kernel<<<grid, kPlanThreads, smem, (cudaStream_t)p->stream>>>(a);
     return cudaGetLastError();
 }

@@ -150,22 +150,24 @@ def sparse_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
 
 # ------------------------------------------------------------------- cache
 class PagedKVCache:
-    """Buffers of an uncompressed paged cache for up to max_batch sequences of up
-    to max_blocks_per_seq pages, and a step's calls on them:
+    """Buffers of an uncompressed paged cache of num_layers layers for up to
+    max_batch sequences of up to max_blocks_per_seq pages, and a step's calls on
+    them (one plan a step, the others a layer):
 
-        plan = cache.step(new_lens, max_tokens)      # tokens of each row; -1: ended
-        q = cache.write(q, k, v, cos_sin, plan)      # rotary, then into the pages
-        o = cache.attention(q_last)                  # one new token per row
-        o = cache.sparse_attention(q_last, 64)       # over 64 pages per KV head
+        plan = cache.step(new_lens, max_tokens)          # tokens of each row; -1: ended
+        q = cache.write(q, k, v, cos_sin, plan, layer)   # rotary, then into the pages
+        o = cache.attention(q_last, layer)               # one new token per row
+        o = cache.sparse_attention(q_last, 64, layer)    # over 64 pages per KV head
 
     All state (tables, lengths, the free list) is on the GPU in fixed buffers, so
     a step can be captured in a CUDA graph and replayed. layout "heads" keeps
-    each head's rows of a page together, "tokens" each token's heads."""
+    each head's rows of a page together, "tokens" each token's heads. bounds
+    keeps the pages' 8-bit bounds for sparse_attention."""
 
     def __init__(self, num_blocks: int, max_batch: int, max_blocks_per_seq: int, num_kv_heads: int,
                  head_dim: int = 128, page_size: int = 64, dtype: torch.dtype = torch.bfloat16, layout: str = "heads",
-                 bounds: bool = True, device="cuda"):
-        if min(num_blocks, max_batch, max_blocks_per_seq, num_kv_heads) <= 0:
+                 bounds: bool = True, num_layers: int = 1, device="cuda"):
+        if min(num_blocks, max_batch, max_blocks_per_seq, num_kv_heads, num_layers) <= 0:
             raise ValueError("sizes must be positive")
         if layout not in ("heads", "tokens"):
             raise ValueError(f"unknown layout {layout!r}")
@@ -173,18 +175,18 @@ class PagedKVCache:
             raise ValueError("pages hold bf16 or fp16 heads of dim 64 or 128")
         if not 16 <= page_size <= 256 or page_size & (page_size - 1):
             raise ValueError("page_size must be a power of two from 16 to 256")
-        self.device = torch.device(device)
         self.Hkv, self.D, self.page_size, self.max_batch = num_kv_heads, head_dim, page_size, max_batch
 
         def pool():
             if layout == "heads":
                 return torch.zeros(num_blocks, num_kv_heads, page_size, head_dim, dtype=dtype,
-                                   device=self.device).transpose(1, 2)
-            return torch.zeros(num_blocks, page_size, num_kv_heads, head_dim, dtype=dtype, device=self.device)
+                                   device=device).transpose(1, 2)
+            return torch.zeros(num_blocks, page_size, num_kv_heads, head_dim, dtype=dtype, device=device)
 
+        self.k = [pool() for _ in range(num_layers)]
+        self.v = [pool() for _ in range(num_layers)]
+        self.device = self.k[0].device
         i32 = dict(dtype=torch.int32, device=self.device)
-        self.k, self.v = pool(), pool()
-        self.device = self.k.device
         self.block_table = torch.full((max_batch, max_blocks_per_seq), -1, **i32)
         self.seqlens = torch.zeros(max_batch, **i32)
         self.lens_before = torch.zeros(max_batch, **i32)
@@ -194,8 +196,10 @@ class PagedKVCache:
         self.err = torch.zeros(1, **i32)
         self.codes = self.scales = None
         if bounds:
-            self.codes = torch.zeros(num_blocks, num_kv_heads, 2, head_dim, dtype=torch.int8, device=self.device)
-            self.scales = torch.zeros(num_blocks, num_kv_heads, dtype=torch.float32, device=self.device)
+            self.codes = [torch.zeros(num_blocks, num_kv_heads, 2, head_dim, dtype=torch.int8, device=self.device)
+                          for _ in range(num_layers)]
+            self.scales = [torch.zeros(num_blocks, num_kv_heads, dtype=torch.float32, device=self.device)
+                           for _ in range(num_layers)]
 
     def step(self, new_lens: torch.Tensor, max_tokens: int) -> StepPlan:
         """Admit new_lens (int32 [max_batch]; negative: the row has ended) tokens
@@ -210,33 +214,34 @@ class PagedKVCache:
                          self.page_size, max_tokens, out, self.err)
 
     def write(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos_sin: torch.Tensor, plan: StepPlan,
-              positions: Optional[torch.Tensor] = None, sections: Optional[Sequence[int]] = None,
+              layer: int = 0, positions: Optional[torch.Tensor] = None, sections: Optional[Sequence[int]] = None,
               interleaved: bool = False) -> torch.Tensor:
         """rope_write of the step's tokens (positions default to the plan's), then
         the bounds of the pages that it completed."""
-        q = rope_write(q, k, v, plan.positions if positions is None else positions, cos_sin, plan.slots, self.k,
-                       self.v, sections, interleaved, None, self.err)
+        q = rope_write(q, k, v, plan.positions if positions is None else positions, cos_sin, plan.slots,
+                       self.k[layer], self.v[layer], sections, interleaved, None, self.err)
         if self.codes is not None:
             n = plan.slots.numel()
-            page_bounds(self.k, self.block_table, self.lens_before, self.seqlens, self.codes, self.scales, n, n,
-                        self.err)
+            page_bounds(self.k[layer], self.block_table, self.lens_before, self.seqlens, self.codes[layer],
+                        self.scales[layer], n, n, self.err)
         return q
 
-    def attention(self, q: torch.Tensor, softmax_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
-                  lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def attention(self, q: torch.Tensor, layer: int = 0, softmax_scale: Optional[float] = None,
+                  out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of q [B, Hq, D] over rows 0 .. B-1."""
         B = q.shape[0]
-        return paged_attention(q, self.k, self.v, self.block_table[:B], self.seqlens[:B], softmax_scale, None, None,
-                               out, lse, self.err)
+        return paged_attention(q, self.k[layer], self.v[layer], self.block_table[:B], self.seqlens[:B], softmax_scale,
+                               None, None, out, lse, self.err)
 
-    def sparse_attention(self, q: torch.Tensor, top_pages: int, sink_pages: int = 1, local_pages: int = 1,
-                         softmax_scale: Optional[float] = None):
+    def sparse_attention(self, q: torch.Tensor, top_pages: int, layer: int = 0, sink_pages: int = 1,
+                         local_pages: int = 1, softmax_scale: Optional[float] = None):
         """Attention of q [B, Hq, D] over top_pages chosen pages of rows 0 .. B-1: (out, pages, counts)."""
         if self.codes is None:
             raise RuntimeError("the cache was made without bounds")
         B = q.shape[0]
-        return sparse_attention(q, self.k, self.v, self.codes, self.scales, self.block_table[:B], self.seqlens[:B],
-                                top_pages, sink_pages, local_pages, softmax_scale, None, self.err)
+        return sparse_attention(q, self.k[layer], self.v[layer], self.codes[layer], self.scales[layer],
+                                self.block_table[:B], self.seqlens[:B], top_pages, sink_pages, local_pages,
+                                softmax_scale, None, self.err)
 
     def check_errors(self) -> int:
         """Error bits recorded by the kernels (synchronises)."""
