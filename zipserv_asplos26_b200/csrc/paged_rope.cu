@@ -17,9 +17,9 @@
 namespace zs {
 namespace {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 64;
 constexpr int kRopeMaxAxes = 4;
-constexpr int kRopeBatch = 2;       // heads whose loads are in flight together
+constexpr int kRopeBatch = 4;       // passes whose loads are in flight together
 
 struct RopeArgs {
     const uint16_t* q;

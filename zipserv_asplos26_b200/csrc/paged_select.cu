@@ -26,7 +26,7 @@ namespace {
 // One warp reduces one page of one KV head: a lane holds 8 channels of every
 // (32 / (D / 8))-th token, running maximum and minimum as packed 16-bit pairs
 // (exact), 16-byte loads. Bound by HBM: the keys are read once.
-constexpr int kBoundsThreads = 128;
+constexpr int kBoundsThreads = 32;
 constexpr int kBoundsBatch = 8;
 
 struct BoundsArgs {
@@ -60,7 +60,7 @@ __device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b, __half) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kBoundsThreads) page_bounds_kernel(const BoundsArgs a) {
+__global__ void __launch_bounds__(kBoundsThreads, 32) page_bounds_kernel(const BoundsArgs a) {
     constexpr int kLanes = D / 8;            // lanes a token
     constexpr int kRows = 32 / kLanes;       // tokens a pass
     const int lane = threadIdx.x & 31;
