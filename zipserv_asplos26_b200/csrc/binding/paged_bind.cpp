@@ -205,6 +205,8 @@ void call(int (*f)(const A*), const A& args, const char* name) {
 
 // ------------------------------------------------------------------ plan
 PyObject* plan_step(PyObject* const* a) {
+    PyTypeObject* type = reinterpret_cast<PyTypeObject*>(a[9]);      // StepPlan
+    if (!PyType_Check(a[9]) || !PyType_IsSubtype(type, &PyTuple_Type)) refuse("plan_step needs its tuple class");
     const at::Tensor& lens = cuda_tensor(a[1], "seq_lens");
     const int index = static_cast<int>(lens.get_device());
     const int64_t R = lens.numel(), page = integer(a[5]), room = integer(a[6]);
@@ -265,7 +267,7 @@ PyObject* plan_step(PyObject* const* a) {
     p.positions = ptr<int>(out[5]);
     p.refused = ptr<uint8_t>(out[6]);
     call(zs_plan_step, p, "zs_plan_step");
-    PyObject* r = PyTuple_New(7);
+    PyObject* r = type->tp_alloc(type, 7);           // a named tuple without a call of its class
     if (!r) throw PyRaised{};
     for (int i = 0; i < 7; ++i) PyTuple_SET_ITEM(r, i, THPVariable_Wrap(std::move(out[i])));
     return r;
@@ -592,7 +594,7 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 #define ZS_ENTRY(name, n) \
     {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<name, n>)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {ZS_ENTRY(plan_step, 9),    ZS_ENTRY(rope_write, 12),  ZS_ENTRY(paged_attention, 11),
+PyMethodDef methods[] = {ZS_ENTRY(plan_step, 10),    ZS_ENTRY(rope_write, 12),  ZS_ENTRY(paged_attention, 11),
                          ZS_ENTRY(page_bounds, 9),  ZS_ENTRY(select_pages, 10), ZS_ENTRY(sparse_attention, 13),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_paged_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

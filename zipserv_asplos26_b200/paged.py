@@ -73,9 +73,8 @@ def plan_step(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch
     enough pages are free; otherwise it keeps its state and is marked refused.
     block_table and free_blocks (a stack, its first free_count[0] entries) are
     updated in place; the new lengths and count are returned."""
-    r = (_native or _load()).plan_step(block_table, seq_lens, new_lens, free_blocks, free_count, page_size,
-                                       max_tokens, out, err)
-    return r if r is out else StepPlan._make(r)
+    return (_native or _load()).plan_step(block_table, seq_lens, new_lens, free_blocks, free_count, page_size,
+                                          max_tokens, out, err, StepPlan)
 
 
 # ----------------------------------------------------------- rotary + write
