@@ -309,8 +309,11 @@ int zs_rope_write(const ZsRopeWrite* args);
  * pages ([B][Hkv][top] distinct logical pages) and counts ([B][Hkv]) only the
  * tokens of the listed pages count. A sequence with nothing to attend gets zeros.
  * lse (nullable, [B][Hq]) receives log sum exp(softmax_scale q.k), -inf where
- * nothing counts. ws: 16-byte aligned workspace of
- * zs_paged_attention_workspace_bytes. */
+ * nothing counts. max_seqlen: a bound on seq_lens where the host has one closer
+ * than the table's width (0: none); it chooses between two kernels and no result
+ * depends on it. ws: 16-byte aligned workspace of ws_bytes, at least what
+ * zs_paged_attention_workspace returns for the same arguments (0: none is read);
+ * zs_paged_attention_workspace_bytes is enough for every call of these sizes. */
 typedef struct ZsPagedAttention {
     void* stream;
     const uint16_t* q;
@@ -327,8 +330,9 @@ typedef struct ZsPagedAttention {
     ZsPagePool k_pool, v_pool;
     int B, Hq, width, top;
     float softmax_scale;
-    int reserved;
+    int max_seqlen;
 } ZsPagedAttention;
+size_t zs_paged_attention_workspace(const ZsPagedAttention* args);
 size_t zs_paged_attention_workspace_bytes(int B, int Hq, int Hkv, int D);
 int zs_paged_attention(const ZsPagedAttention* args);
 

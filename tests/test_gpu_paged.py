@@ -322,6 +322,17 @@ def test_paged_attention(lens, hq, hkv, D, page, dtype, layout):
     assert torch.allclose(lse.double().cpu(), ref_lse, rtol=1e-6, atol=ATT)
     again = zs().paged_attention(q.unsqueeze(1), c.k, c.v, c.table, c.lens)
     assert again.shape == (len(lens), 1, hq, D) and torch.equal(again.squeeze(1), out)      # bit for bit
+    # a wide table: the same in runs of chunks, the way of long sequences
+    wide = torch.nn.functional.pad(c.table, (0, 8192 - c.table.shape[1]), value=-1)
+    out = zs().paged_attention(q, c.k, c.v, wide, c.lens, lse=lse.fill_(5.0), err=err)
+    assert close(out, ref, vmax, dtype)
+    assert bool((out[c.lens == 0] == 0).all()) and err.item() == 0
+    assert torch.allclose(lse.double().cpu(), ref_lse, rtol=1e-6, atol=ATT)
+    assert torch.equal(zs().paged_attention(q, c.k, c.v, wide, c.lens), out)
+    # no result depends on the bound, a wrong one included
+    for most in (max(lens), 1):
+        out = zs().paged_attention(q, c.k, c.v, wide, c.lens, max_seqlen=most)
+        assert close(out, ref, vmax, dtype)
 
 
 def test_no_sequences():
@@ -609,6 +620,12 @@ def test_sparse_attention(lens, hq, hkv, D, page, top, dtype, layout):
 
     ref, _, vmax = attend_ref(q, c.dense, 1 / math.sqrt(D), rows)
     assert close(out, ref, vmax, dtype)
+    # the same list with room for many more pages: in runs of chunks
+    wide = torch.nn.functional.pad(pages, (0, 4096 - top), value=-1)
+    lse = torch.empty(len(lens), hq, device=DEV)
+    out = zs().paged_attention(q, c.k, c.v, c.table, c.lens, pages=wide, counts=counts, lse=lse)
+    assert close(out, ref, vmax, dtype)
+    assert bool(((lse == -math.inf) == (c.lens == 0).unsqueeze(1)).all())
 
 
 def test_listed_pages_out_of_range_are_skipped():
@@ -616,10 +633,11 @@ def test_listed_pages_out_of_range_are_skipped():
     c = Cache([100, 40], 1, 64, 16, BF, "heads", 8)
     q = torch.randn(2, 2, 64, device=DEV).to(BF)
     pages, counts = i32([[[6, -1, 2, 500]], [[7, 3, 1, 0]]]), i32([[4], [2]])
-    out = zs().paged_attention(q, c.k, c.v, c.table, c.lens, pages=pages, counts=counts)
     ref, _, vmax = attend_ref(q, c.dense, 0.125,
                               lambda b, h: [] if b else list(range(32, 48)) + list(range(96, 100)))
-    assert close(out, ref, vmax, BF) and bool((out[1] == 0).all())
+    for p in (pages, torch.nn.functional.pad(pages, (0, 4092), value=3)):
+        out = zs().paged_attention(q, c.k, c.v, c.table, c.lens, pages=p, counts=counts)
+        assert close(out, ref, vmax, BF) and bool((out[1] == 0).all())
 
 
 # ----------------------------------------------------------------- the cache
@@ -716,7 +734,8 @@ def test_refusals_on_the_gpu():
                 dict(v_pages=c.v.half()), dict(block_table=c.table.long()), dict(block_table=c.table[:0]),
                 dict(seq_lens=c.lens.long()), dict(seq_lens=c.lens.cpu()), dict(softmax_scale=float("nan")),
                 dict(pages=i32([[[0], [0]]])), dict(out=torch.empty(1, 4, 32, device=DEV, dtype=BF)),
-                dict(lse=torch.empty(1, 3, device=DEV))):
+                dict(lse=torch.empty(1, 3, device=DEV)),
+                dict(max_seqlen=-1)):
         args = dict(q=q, k_pages=c.k, v_pages=c.v, block_table=c.table, seq_lens=c.lens)
         args.update(bad)
         with pytest.raises(ValueError):

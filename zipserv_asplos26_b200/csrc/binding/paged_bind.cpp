@@ -11,6 +11,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -374,7 +375,8 @@ PyObject* rope_write(PyObject* const* a) {
 // ------------------------------------------------------------- attention
 // The attention proper; q3 is checked, `out` may be undefined. Returns out as [B, Hq, D].
 at::Tensor attend(const Pools& pools, const at::Tensor& q3, const Table& table, const int* lens, const int* pages,
-                  const int* counts, int64_t top, PyObject* scale_o, PyObject* out_o, PyObject* lse_o, unsigned* err) {
+                  const int* counts, int64_t top, PyObject* scale_o, PyObject* out_o, PyObject* lse_o, PyObject* most_o,
+                  unsigned* err) {
     const int index = pools.index;
     const int64_t dim = pools.k.head_dim, B = q3.size(0), hq = q3.size(-2);
     need(static_cast<int64_t>(table.width) * pools.k.page_size <= INT32_MAX,
@@ -391,10 +393,12 @@ at::Tensor attend(const Pools& pools, const at::Tensor& q3, const Table& table, 
         out = fresh(q3.sizes(), pools.type, index);
     }
     ZsPagedAttention p{};
+    if (given(most_o)) {
+        const int64_t most = integer(most_o);
+        need(most >= 0, "max_seqlen must not be negative");
+        p.max_seqlen = static_cast<int>(std::min<int64_t>(most, INT32_MAX));
+    }
     p.lse = given(lse_o) ? vec<float>(lse_o, B * hq, at::kFloat, "lse", index) : nullptr;
-    p.ws_bytes = zs_paged_attention_workspace_bytes(static_cast<int>(B), static_cast<int>(hq), pools.k.num_heads,
-                                                    static_cast<int>(dim));
-    const at::Tensor ws = fresh({static_cast<int64_t>(p.ws_bytes)}, at::kByte, index);
     p.stream = current_stream(index);
     p.q = ptr<uint16_t>(q3);
     p.block_table = table.data;
@@ -402,7 +406,6 @@ at::Tensor attend(const Pools& pools, const at::Tensor& q3, const Table& table, 
     p.seq_lens = lens;
     p.pages = pages;
     p.counts = counts;
-    p.ws = ptr(ws);
     p.out = ptr<uint16_t>(out);
     p.err = err;
     p.k_pool = pools.k;
@@ -412,6 +415,11 @@ at::Tensor attend(const Pools& pools, const at::Tensor& q3, const Table& table, 
     p.width = table.width;
     p.top = static_cast<int>(top);
     p.softmax_scale = static_cast<float>(scale);
+    at::Tensor ws;
+    if ((p.ws_bytes = zs_paged_attention_workspace(&p)) > 0) {
+        ws = fresh({static_cast<int64_t>(p.ws_bytes)}, at::kByte, index);
+        p.ws = ptr(ws);
+    }
     call(zs_paged_attention, p, "zs_paged_attention");
     return out;
 }
@@ -441,7 +449,7 @@ PyObject* paged_attention(PyObject* const* a) {
         pages = vec<int>(a[6], B * hkv * top, at::kInt, "pages", index);
         counts = vec<int>(a[7], B * hkv, at::kInt, "counts", index);
     }
-    at::Tensor out = attend(pools, q3, table, lens, pages, counts, top, a[5], a[8], a[9], err_word(a[10], index));
+    at::Tensor out = attend(pools, q3, table, lens, pages, counts, top, a[5], a[8], a[9], a[10], err_word(a[11], index));
     return THPVariable_Wrap(std::move(out));
 }
 
@@ -567,7 +575,7 @@ PyObject* sparse_attention(PyObject* const* a) {
     need(top > 0 && top <= INT32_MAX / pools.k.page_size, "top_pages must be positive, and cover less than 2**31 tokens");
     Choice c = choose(q3, b, nb, hkv, table, lens, pools.k.page_size, top, integer(a[8]), integer(a[9]), err, index);
     at::Tensor out = attend(pools, q3, table, lens, ptr<int>(c.pages), ptr<int>(c.counts), top, a[10], a[11], Py_None,
-                            err);
+                            Py_None, err);
     return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(c.pages)),
                          THPVariable_Wrap(std::move(c.counts)));
 }
@@ -594,7 +602,7 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 #define ZS_ENTRY(name, n) \
     {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<name, n>)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {ZS_ENTRY(plan_step, 10),    ZS_ENTRY(rope_write, 12),  ZS_ENTRY(paged_attention, 11),
+PyMethodDef methods[] = {ZS_ENTRY(plan_step, 10),    ZS_ENTRY(rope_write, 12),  ZS_ENTRY(paged_attention, 12),
                          ZS_ENTRY(page_bounds, 9),  ZS_ENTRY(select_pages, 10), ZS_ENTRY(sparse_attention, 13),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_paged_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

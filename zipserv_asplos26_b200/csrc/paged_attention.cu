@@ -46,6 +46,7 @@ struct PaArgs {
     const int* pages;         // nullable: [B][Hkv][top]
     const int* counts;        // with pages: [B][Hkv]
     int B, Hq, Hkv, G, tiles, width, top;
+    int max_len;              // host's bound on the lengths, 0: none (chooses the way, no result depends on it)
     float scale2;             // softmax scale * log2(e)
     uint16_t* out;            // [B][Hq][D]
     float* lse;               // nullable: [B][Hq]
@@ -110,6 +111,18 @@ constexpr float kPBias = 0.f;
 template <>
 constexpr float kPBias<__half> = 15.f;
 
+__device__ __forceinline__ float2 ld_dsmem_f2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+
+// log sum exp of a row from its base-2 maximum and sum.
+template <typename T>
+__device__ __forceinline__ float log_sum(float m, float l) {
+    return l == 0.f ? -INFINITY : (m + log2f(l) - kPBias<T>) / kLog2e;
+}
+
 // Chunks of entry e: a sequence (whole cache) or a (sequence, KV head) with a page list.
 template <bool kListed>
 __device__ __forceinline__ int entry_chunks(const PaArgs& a, int e) {
@@ -132,9 +145,175 @@ template <int D>
 struct PaCfg {
     static constexpr int kRowBytes = D * 2;
     static constexpr int kTile = kPaChunk * kRowBytes;             // one K or V chunk
-    static constexpr int kStages = D <= 64 ? 6 : 3;
+    // CTAs an SM: rows of 128 bytes take more steps for the same bytes, so D = 64
+    // wants more warps (B=32 T=4129: 2 of 6 stages 51.9 us, 3 of 4 stages 48.8)
+    static constexpr int kCtas = D <= 64 ? 3 : 2;
+    static constexpr int kStages = D <= 64 ? 4 : 3;
+    // CTAs for long units, see launch_paged
+    static constexpr int kLongCtas = D <= 64 ? 148 * kCtas : 256;
     static constexpr int kRing = kStages * 2 * kTile;              // a warp's ring
     static constexpr int kSmem = kPaWarps * kRing;
+};
+
+// ---- a warp's work on a unit, shared by both kernels
+
+// The block and the number of valid tokens of chunk `ch` of an entry (lim 0: none).
+template <bool kListed>
+__device__ __forceinline__ void look_chunk(const PaArgs& a, int e, int b, int ch, int len, int& id, int& lim) {
+    const int cps = a.kp.page_shift - 4;                               // log2 chunks a page
+    int p = ch >> cps;
+    if (kListed) p = a.pages[(long long)e * a.top + p];
+    const int t0 = ((p << cps) + (ch & ((1 << cps) - 1))) * kPaChunk;
+    id = lim = 0;
+    if (p < 0 || p >= a.width || t0 >= len) return;
+    const int blk = a.table[b * a.table_stride + p];
+    if (blk < 0 || blk >= a.kp.num_blocks) {
+        set_err(a.err, kErrPagedIndex);
+        return;
+    }
+    id = blk;
+    lim = min(kPaChunk, len - t0);
+}
+
+// Starts the copies of one chunk (its rows past `lim` are zeros).
+template <int D>
+__device__ __forceinline__ void copy_chunk(const PaArgs& a, uint32_t dst, int blk, int ch, int h, int lim,
+                                           uint64_t policy) {
+    using C = PaCfg<D>;
+    constexpr int kPieces = D / 8;                 // 16-byte pieces a row
+    const int lane = threadIdx.x & 31;
+    const int row0 = (ch & ((1 << (a.kp.page_shift - 4)) - 1)) * kPaChunk;
+    const uint16_t* ks =
+        static_cast<const uint16_t*>(a.kp.data) + h * a.kp.s_head + blk * a.kp.s_block + row0 * a.kp.s_token;
+    const uint16_t* vs =
+        static_cast<const uint16_t*>(a.vp.data) + h * a.vp.s_head + blk * a.vp.s_block + row0 * a.vp.s_token;
+#pragma unroll
+    for (int i = 0; i < kPaChunk * kPieces / 32; ++i) {
+        const int x = i * 32 + lane, r = x / kPieces, pc = x % kPieces;
+        const uint32_t to = dst + r * C::kRowBytes + ((pc ^ (r & 7)) * 16);
+        cp16(to, ks + r * a.kp.s_token + pc * 8, r < lim, policy);
+        cp16(to + C::kTile, vs + r * a.vp.s_token + pc * 8, r < lim, policy);
+    }
+}
+
+// What a warp holds of a unit: q as product fragments, running maximum (base 2),
+// sum and output; lane rows lane / 4 and lane / 4 + 8.
+template <typename T, int D>
+struct PaState {
+    uint32_t qf[D / 16][4];
+    float o[D / 8][4], m[2], l[2];
+
+    __device__ __forceinline__ void start(const uint16_t* q, int rows) {
+        const int lane = threadIdx.x & 31, r = lane >> 2, cc = (lane & 3) * 2;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = r + (i & 1) * 8, col = ks * 16 + (i >> 1) * 8 + cc;
+                qf[ks][i] = row < rows ? *reinterpret_cast<const uint32_t*>(q + (long long)row * D + col) : 0u;
+            }
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
+    }
+
+    // One chunk: keys at kt, values behind them.
+    __device__ __forceinline__ void attend(uint32_t kt, int lim, float scale2) {
+        using C = PaCfg<D>;
+        constexpr int kKs = D / 16;
+        const int lane = threadIdx.x & 31;
+        const uint32_t vt = kt + C::kTile;
+        // S = Q K^T: 16 heads x 16 tokens
+        float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        {
+            const int r = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+            const uint32_t row = kt + r * C::kRowBytes;
+#pragma unroll
+            for (int ks = 0; ks < kKs; ++ks) {
+                uint32_t f[4];
+                ldsm4(f, row + (((ks * 2 + half) ^ (r & 7)) * 16));
+                mma16816(sc[0], qf[ks], f[0], f[1], T());
+                mma16816(sc[1], qf[ks], f[2], f[3], T());
+            }
+        }
+        // running maximum and sum
+        const int t = (lane & 3) * 2;
+        float p[2][4];
+        bool grew = false;
+        float keep[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float x = j * 8 + t + i < lim ? sc[j][r * 2 + i] * scale2 : -INFINITY;
+                    p[j][r * 2 + i] = x;
+                    mx = fmaxf(mx, x);
+                }
+            mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+            const float mn = fmaxf(m[r], mx);
+            grew |= mn > m[r];
+            const float ref = mn == -INFINITY ? 0.f : mn;
+            keep[r] = exp2f(m[r] - ref);
+            m[r] = mn;
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float x = exp2f(p[j][r * 2 + i] - ref + kPBias<T>);
+                    p[j][r * 2 + i] = x;
+                    sum += x;
+                }
+            l[r] = l[r] * keep[r] + sum;
+        }
+        if (__any_sync(~0u, grew)) {
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                o[i][0] *= keep[0];
+                o[i][1] *= keep[0];
+                o[i][2] *= keep[1];
+                o[i][3] *= keep[1];
+            }
+        }
+        // O += P V, P in two 16-bit parts
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = p[i >> 1][(i & 1) * 2], y = p[i >> 1][(i & 1) * 2 + 1];
+            hi[i] = pack2<T>(x, y);
+            const float2 back = unpack2<T>(hi[i]);
+            lo[i] = pack2<T>(x - back.x, y - back.y);
+        }
+        {
+            const int r = lane & 15, half = lane >> 4;
+            const uint32_t row = vt + r * C::kRowBytes;
+#pragma unroll
+            for (int ks = 0; ks < kKs; ++ks) {
+                uint32_t f[4];
+                ldsm4t(f, row + (((ks * 2 + half) ^ (r & 7)) * 16));
+                mma16816(o[ks * 2], hi, f[0], f[1], T());
+                mma16816(o[ks * 2 + 1], hi, f[2], f[3], T());
+                mma16816(o[ks * 2], lo, f[0], f[1], T());
+                mma16816(o[ks * 2 + 1], lo, f[2], f[3], T());
+            }
+        }
+    }
+
+    // The sums of the four lanes of a row.
+    __device__ __forceinline__ void finish() {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(~0u, l[r], 1);
+            l[r] += __shfl_xor_sync(~0u, l[r], 2);
+        }
+    }
 };
 
 // Where a warp is in the sequence of all chunks: chunk `ch` of the n chunks of
@@ -154,10 +333,8 @@ __device__ __forceinline__ void next_unit(const PaArgs& a, int per_entry, PaCurs
 }
 
 template <typename T, int D, bool kListed>
-__global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const PaArgs a) {
+__global__ void __launch_bounds__(kPaThreads, PaCfg<D>::kCtas) paged_attn_kernel(const PaArgs a) {
     using C = PaCfg<D>;
-    constexpr int kPieces = D / 8;                 // 16-byte pieces a row
-    constexpr int kKs = D / 16;
     extern __shared__ __align__(1024) uint8_t pa_smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t ring = smem_u32(pa_smem) + warp * C::kRing;
@@ -223,7 +400,6 @@ __global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const PaArgs 
     // ---- copies: batches of up to 32 chunks of one unit, a lane holding the block
     // and the number of valid tokens of one chunk; the next batch is looked up
     // while the present one is copied
-    const int cps = a.kp.page_shift - 4;                               // log2 chunks a page
     const int table_len = (int)min((long long)a.width << a.kp.page_shift, (long long)INT_MAX);
     struct Batch {
         int ids, lims, count, h, ch;
@@ -238,20 +414,7 @@ __global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const PaArgs 
         if (t.count <= 0) return;
         if (lane < t.count) {
             const int b = kListed ? at.e / a.Hkv : at.e;
-            const int ch = at.ch + lane;
-            int p = ch >> cps;
-            if (kListed) p = a.pages[(long long)at.e * a.top + p];
-            const int t0 = ((p << cps) + (ch & ((1 << cps) - 1))) * kPaChunk;
-            const int len = min(a.lens[b], table_len);
-            if (p >= 0 && p < a.width && t0 < len) {
-                t.ids = a.table[b * a.table_stride + p];
-                t.lims = min(kPaChunk, len - t0);
-                if (t.ids < 0 || t.ids >= a.kp.num_blocks) {
-                    set_err(a.err, kErrPagedIndex);
-                    t.ids = 0;
-                    t.lims = 0;
-                }
-            }
+            look_chunk<kListed>(a, at.e, b, at.ch + lane, min(a.lens[b], table_len), t.ids, t.lims);
         }
         looked += t.count;
         at.ch += t.count;
@@ -270,20 +433,8 @@ __global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const PaArgs 
             }
             const int blk = __shfl_sync(~0u, now.ids, in_batch);
             lim = __shfl_sync(~0u, now.lims, in_batch);
-            const int row0 = ((now.ch + in_batch) & ((1 << cps) - 1)) * kPaChunk;
+            copy_chunk<D>(a, ring + (s % C::kStages) * 2 * C::kTile, blk, now.ch + in_batch, now.h, lim, policy);
             ++in_batch;
-            const uint16_t* ks = static_cast<const uint16_t*>(a.kp.data) + now.h * a.kp.s_head + blk * a.kp.s_block +
-                                 row0 * a.kp.s_token;
-            const uint16_t* vs = static_cast<const uint16_t*>(a.vp.data) + now.h * a.vp.s_head + blk * a.vp.s_block +
-                                 row0 * a.vp.s_token;
-            const uint32_t dst = ring + (s % C::kStages) * 2 * C::kTile;
-#pragma unroll
-            for (int i = 0; i < kPaChunk * kPieces / 32; ++i) {
-                const int x = i * 32 + lane, r = x / kPieces, pc = x % kPieces;
-                const uint32_t to = dst + r * C::kRowBytes + ((pc ^ (r & 7)) * 16);
-                cp16(to, ks + r * a.kp.s_token + pc * 8, r < lim, policy);
-                cp16(to + C::kTile, vs + r * a.vp.s_token + pc * 8, r < lim, policy);
-            }
         }
         cp_commit();
         return lim;
@@ -304,25 +455,8 @@ __global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const PaArgs 
         const int g0 = tile * kPaRows, rows = min(kPaRows, a.G - g0);
         if (first == 0 && lane == 0) a.plan[1 + (b * a.Hkv + h) * a.tiles + tile] = u_lo;
         const long long head0 = (long long)b * a.Hq + (long long)h * a.G + g0;
-        uint32_t qf[kKs][4];
-        {
-            const uint16_t* q = a.q + head0 * D;
-            const int r = lane >> 2, cc = (lane & 3) * 2;
-#pragma unroll
-            for (int ks = 0; ks < kKs; ++ks)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = r + (i & 1) * 8, col = ks * 16 + (i >> 1) * 8 + cc;
-                    qf[ks][i] = row < rows ? *reinterpret_cast<const uint32_t*>(q + (long long)row * D + col) : 0u;
-                }
-        }
-        float o[D / 8][4];
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-
+        PaState<T, D> st;
+        st.start(a.q + head0 * D, rows);
         for (const int end = s + count; s < end; ++s) {
             cp_wait<C::kStages - 2>();
             __syncwarp();
@@ -330,112 +464,32 @@ __global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const PaArgs 
 #pragma unroll
             for (int i = 0; i + 1 < C::kStages; ++i) lim_at[i] = lim_at[i + 1];
             lim_at[C::kStages - 2] = produce(s + C::kStages - 1);
-            const uint32_t kt = ring + (s % C::kStages) * 2 * C::kTile, vt = kt + C::kTile;
-            // S = Q K^T: 16 heads x 16 tokens
-            float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-            {
-                const int r = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
-                const uint32_t row = kt + r * C::kRowBytes;
-#pragma unroll
-                for (int ks = 0; ks < kKs; ++ks) {
-                    uint32_t f[4];
-                    ldsm4(f, row + (((ks * 2 + half) ^ (r & 7)) * 16));
-                    mma16816(sc[0], qf[ks], f[0], f[1], T());
-                    mma16816(sc[1], qf[ks], f[2], f[3], T());
-                }
-            }
-            // running maximum and sum
-            const int t = (lane & 3) * 2;
-            float p[2][4];
-            bool grew = false;
-            float keep[2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                float mx = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float x = j * 8 + t + i < lim ? sc[j][r * 2 + i] * a.scale2 : -INFINITY;
-                        p[j][r * 2 + i] = x;
-                        mx = fmaxf(mx, x);
-                    }
-                mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
-                const float mn = fmaxf(m[r], mx);
-                grew |= mn > m[r];
-                const float ref = mn == -INFINITY ? 0.f : mn;
-                keep[r] = exp2f(m[r] - ref);
-                m[r] = mn;
-                float sum = 0.f;
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float x = exp2f(p[j][r * 2 + i] - ref + kPBias<T>);
-                        p[j][r * 2 + i] = x;
-                        sum += x;
-                    }
-                l[r] = l[r] * keep[r] + sum;
-            }
-            if (__any_sync(~0u, grew)) {
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    o[i][0] *= keep[0];
-                    o[i][1] *= keep[0];
-                    o[i][2] *= keep[1];
-                    o[i][3] *= keep[1];
-                }
-            }
-            // O += P V, P in two 16-bit parts
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = p[i >> 1][(i & 1) * 2], y = p[i >> 1][(i & 1) * 2 + 1];
-                hi[i] = pack2<T>(x, y);
-                const float2 back = unpack2<T>(hi[i]);
-                lo[i] = pack2<T>(x - back.x, y - back.y);
-            }
-            {
-                const int r = lane & 15, half = lane >> 4;
-                const uint32_t row = vt + r * C::kRowBytes;
-#pragma unroll
-                for (int ks = 0; ks < kKs; ++ks) {
-                    uint32_t f[4];
-                    ldsm4t(f, row + (((ks * 2 + half) ^ (r & 7)) * 16));
-                    mma16816(o[ks * 2], hi, f[0], f[1], T());
-                    mma16816(o[ks * 2 + 1], hi, f[2], f[3], T());
-                    mma16816(o[ks * 2], lo, f[0], f[1], T());
-                    mma16816(o[ks * 2 + 1], lo, f[2], f[3], T());
-                }
-            }
+            st.attend(ring + (s % C::kStages) * 2 * C::kTile, lim, a.scale2);
             __syncwarp();
         }
         // ---- out, or to the workspace where the run cuts the unit
         const bool whole = first == 0 && count == cur.n;
         const long long slot = 2ll * id + (s == count ? 0 : 1);       // the run's first part, or its last
         const int d0 = (lane & 3) * 2;
+        st.finish();
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            l[r] += __shfl_xor_sync(~0u, l[r], 1);
-            l[r] += __shfl_xor_sync(~0u, l[r], 2);
             const int row = (lane >> 2) + r * 8;
             if (row >= rows) continue;
             if (whole) {
-                const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+                const float inv = st.l[r] == 0.f ? 0.f : 1.f / st.l[r];
                 uint16_t* out = a.out + (head0 + row) * D + d0;
 #pragma unroll
                 for (int i = 0; i < D / 8; ++i)
-                    *reinterpret_cast<uint32_t*>(out + i * 8) = pack2<T>(o[i][r * 2] * inv, o[i][r * 2 + 1] * inv);
-                if (a.lse && d0 == 0)
-                    a.lse[head0 + row] = l[r] == 0.f ? -INFINITY : (m[r] + log2f(l[r]) - kPBias<T>) / kLog2e;
+                    *reinterpret_cast<uint32_t*>(out + i * 8) = pack2<T>(st.o[i][r * 2] * inv, st.o[i][r * 2 + 1] * inv);
+                if (a.lse && d0 == 0) a.lse[head0 + row] = log_sum<T>(st.m[r], st.l[r]);
             } else {
                 float* po = a.part_o + (slot * a.prow + row) * D + d0;
 #pragma unroll
                 for (int i = 0; i < D / 8; ++i)
-                    *reinterpret_cast<float2*>(po + i * 8) = make_float2(o[i][r * 2], o[i][r * 2 + 1]);
+                    *reinterpret_cast<float2*>(po + i * 8) = make_float2(st.o[i][r * 2], st.o[i][r * 2 + 1]);
                 if (d0 == 0)
-                    *reinterpret_cast<float2*>(a.part_ml + (slot * a.prow + row) * 2) = make_float2(m[r], l[r]);
+                    *reinterpret_cast<float2*>(a.part_ml + (slot * a.prow + row) * 2) = make_float2(st.m[r], st.l[r]);
             }
         }
         if (s == steps) break;
@@ -443,6 +497,132 @@ __global__ void __launch_bounds__(kPaThreads, 2) paged_attn_kernel(const PaArgs 
         next_unit<kListed>(a, per_entry, cur);
     }
     cp_wait<0>();
+}
+
+// ---- Each unit by a fixed number W of warps, 1 to 16: no prefix over the
+// lengths, no workspace and no second kernel. Warp w of the unit's W takes chunks
+// [n w / W, n (w + 1) / W) of the unit's n, leaves (m, l, O) in its own shared
+// memory, and after a cluster barrier the unit's threads join the W pieces
+// through distributed shared memory, in order. With W below 4 a CTA has several
+// units, from 4 on a cluster of W / 4 CTAs has one.
+template <typename T, int D, bool kListed>
+__global__ void __launch_bounds__(kPaThreads, PaCfg<D>::kCtas) paged_attn_units_kernel(const PaArgs a, int W) {
+    using C = PaCfg<D>;
+    extern __shared__ __align__(1024) uint8_t pa_smem[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t ring = smem_u32(pa_smem) + warp * C::kRing;
+    const long long warp_id = (long long)blockIdx.x * kPaWarps + warp;
+    const int unit = (int)(warp_id / W), w = (int)(warp_id % W);
+    const int units = a.B * a.Hkv * a.tiles;
+    const bool on = unit < units;          // the last CTA may have fewer
+    const int e = on ? (kListed ? unit / a.tiles : unit / (a.Hkv * a.tiles)) : 0;
+    const int b = kListed ? e / a.Hkv : e, h = kListed ? e % a.Hkv : unit / a.tiles % a.Hkv;
+    const int g0 = unit % a.tiles * kPaRows, rows = on ? min(kPaRows, a.G - g0) : 0;
+    const long long head0 = (long long)b * a.Hq + (long long)h * a.G + g0;
+    const uint64_t policy = evict_first_policy();
+    grid_dep_launch();
+    grid_dep_wait();
+    const int table_len = (int)min((long long)a.width << a.kp.page_shift, (long long)INT_MAX);
+    const int len = min(a.lens[b], table_len), n = on ? entry_chunks<kListed>(a, e) : 0;
+    const int first = (int)((long long)n * w / W), steps = (int)((long long)n * (w + 1) / W) - first;
+    PaState<T, D> st;
+    int ids = 0, lims = 0;         // of 32 chunks, a lane each
+    auto produce = [&](int s) {
+        int lim = 0;
+        if (s < steps) {
+            if ((s & 31) == 0) {
+                ids = lims = 0;
+                if (s + lane < steps) look_chunk<kListed>(a, e, b, first + s + lane, len, ids, lims);
+            }
+            lim = __shfl_sync(~0u, lims, s & 31);
+            copy_chunk<D>(a, ring + (s % C::kStages) * 2 * C::kTile, __shfl_sync(~0u, ids, s & 31), first + s, h, lim,
+                          policy);
+        }
+        cp_commit();
+        return lim;
+    };
+    int lim_at[C::kStages];
+#pragma unroll
+    for (int s = 0; s < C::kStages - 1; ++s) lim_at[s] = produce(s);
+    st.start(a.q + head0 * D, rows);
+    for (int s = 0; s < steps; ++s) {
+        cp_wait<C::kStages - 2>();
+        __syncwarp();
+        const int lim = lim_at[0];
+#pragma unroll
+        for (int i = 0; i + 1 < C::kStages; ++i) lim_at[i] = lim_at[i + 1];
+        lim_at[C::kStages - 2] = produce(s + C::kStages - 1);
+        st.attend(ring + (s % C::kStages) * 2 * C::kTile, lim, a.scale2);
+        __syncwarp();
+    }
+    cp_wait<0>();
+    __syncwarp();
+    st.finish();
+    // the warp's piece, over its ring: [16][D] outputs, [16][2] maxima and sums
+    static_assert(C::kRing >= kPaRows * (D + 2) * 4, "a warp's piece fits its ring");
+    float* po = reinterpret_cast<float*>(pa_smem + warp * C::kRing);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int row = (lane >> 2) + r * 8, d0 = (lane & 3) * 2;
+        if (row >= rows) continue;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+            *reinterpret_cast<float2*>(po + row * D + i * 8 + d0) = make_float2(st.o[i][r * 2], st.o[i][r * 2 + 1]);
+        if (d0 == 0) *reinterpret_cast<float2*>(po + kPaRows * D + row * 2) = make_float2(st.m[r], st.l[r]);
+    }
+    // One warp a unit needs no barrier, several of a CTA the CTA's, more the cluster's
+    // (its second one keeps a CTA's shared memory until its peers have read it).
+    if (W == 1) __syncwarp();
+    else if (W <= kPaWarps) __syncthreads();
+    else cluster_sync();
+    // four channels a thread
+    const uint32_t base = smem_u32(pa_smem);
+    const int v0 = W < kPaWarps ? warp / W * W : 0;               // the unit's first warp in its (first) CTA
+    const int in_cta = min(W, kPaWarps);
+    for (int x = w * 32 + lane; x < rows * (D / 4); x += W * 32) {
+        const int row = x / (D / 4), d4 = x % (D / 4) * 4;
+        float m = -INFINITY, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int r = 0; r < W; r += kPaWarps) {
+            const uint32_t peer = W <= kPaWarps ? base : mapa_shared(base, r / kPaWarps);
+            float2 ml[kPaWarps];
+            float4 o[kPaWarps];
+#pragma unroll
+            for (int v = 0; v < kPaWarps; ++v) {
+                ml[v] = make_float2(-INFINITY, 0.f);
+                o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (v < in_cta) {
+                    const uint32_t piece = peer + (v0 + v) * C::kRing;
+                    ml[v] = ld_dsmem_f2(piece + (kPaRows * D + row * 2) * 4);
+                    o[v] = ld_dsmem_f4(piece + (row * D + d4) * 4);
+                }
+            }
+            float mn = m;
+#pragma unroll
+            for (int v = 0; v < kPaWarps; ++v) mn = fmaxf(mn, ml[v].x);
+            const float ref = mn == -INFINITY ? 0.f : mn, f0 = exp2f(m - ref);
+            l *= f0;
+            acc.x *= f0;
+            acc.y *= f0;
+            acc.z *= f0;
+            acc.w *= f0;
+#pragma unroll
+            for (int v = 0; v < kPaWarps; ++v) {
+                const float f = exp2f(ml[v].x - ref);
+                l += ml[v].y * f;
+                acc.x += o[v].x * f;
+                acc.y += o[v].y * f;
+                acc.z += o[v].z * f;
+                acc.w += o[v].w * f;
+            }
+            m = mn;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        *reinterpret_cast<uint2*>(a.out + (head0 + row) * D + d4) =
+            make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+        if (a.lse && d4 == 0) a.lse[head0 + row] = log_sum<T>(m, l);
+    }
+    if (W > kPaWarps) cluster_sync();
 }
 
 // Joins the pieces of the units that the runs cut and writes zeros where nothing
@@ -538,13 +718,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PaArg
     uint32_t* out = reinterpret_cast<uint32_t*>(a.out + (long long)head * D + lane * kVec);
 #pragma unroll
     for (int j = 0; j < kVec; j += 2) out[j / 2] = pack2<T>(acc[j] * inv, acc[j + 1] * inv);
-    if (a.lse && lane == 0) a.lse[head] = l == 0.f ? -INFINITY : (m + log2f(l) - kPBias<T>) / kLog2e;
+    if (a.lse && lane == 0) a.lse[head] = log_sum<T>(m, l);
 }
 
-constexpr int kPaMaxCtas = 148 * 2;      // the workspace's bound on the grid
+// The workspace's bound on the run kernel's grid.
+inline int pa_max_ctas(int D) { return 148 * (D <= 64 ? PaCfg<64>::kCtas : PaCfg<128>::kCtas); }
 
 size_t plan_bytes(long long units) { return ((size_t)(1 + units) * 8 + 255) / 256 * 256; }
-size_t ml_bytes(int prow) { return (size_t)2 * kPaMaxCtas * kPaWarps * prow * 2 * 4; }
+size_t ml_bytes(int prow, int D) { return (size_t)2 * pa_max_ctas(D) * kPaWarps * prow * 2 * 4; }
 
 // The attention kernel's grid: the CTAs that the GPU holds at once (looked up once per device).
 template <typename T, int D, bool kListed>
@@ -563,16 +744,74 @@ cudaError_t resident_ctas(int* ctas) {
     e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return e;
     if (per < 1) return cudaErrorInvalidConfiguration;
-    *ctas = std::min(per * sms, kPaMaxCtas);
+    *ctas = std::min(per * sms, pa_max_ctas(D));
     cached[dev].store(*ctas, std::memory_order_release);
     return cudaSuccess;
 }
 
+// Warps a unit for paged_attn_units_kernel, or 0 where runs of chunks are the
+// better way. Fixed shares have no second kernel (some 5 us less: B=32 T=200 12.6
+// us in runs, 8.4 so; 64 x 300 20.3 and 16.1; B=1 T=97 6.5 and 4.7), but the
+// longest unit's share is the time (16 sequences of 0..2048: 18.9 in runs, 21.3
+// so at 17 chunks a warp; 64 of 0..1000: 28.6 and 34.6 at 36). So they serve
+// units that are bounded to 16 chunks a warp (a page list's units are alike: 64;
+// 8 x 64 pages: 42.5 in runs, 37.9 so), or to 5 where they leave SMs idle (B=1
+// T=4096, 17 chunks a warp: 9.8 in runs, 15.9 so). W is what fills the GPU, at
+// most a portable cluster's half: clusters of 8 and 16 CTAs were slower in all.
+constexpr int kPaMaxUnitWarps = 16;
+constexpr int kPaLongUnit = 128;       // chunks
+
+// A bound on a unit's chunks: of the page list, the table or the caller's.
+inline long long unit_chunks(const PaArgs& a, bool listed) {
+    const long long pages = ((long long)(listed ? a.top : a.width)) << (a.kp.page_shift - 4);
+    return a.max_len > 0 && !listed ? std::min(pages, ((long long)a.max_len + kPaChunk - 1) / kPaChunk) : pages;
+}
+
+inline int unit_warps(const PaArgs& a, bool listed) {
+    const long long units = (long long)a.B * a.Hkv * a.tiles, chunks = unit_chunks(a, listed);
+    int W = 1;
+    while (W < kPaMaxUnitWarps && units * W * 2 <= 148 * 8 && W < chunks) W *= 2;
+    const long long steps = (chunks + W - 1) / W;
+    const long long most = units * W < 148 * 4 ? 5 : listed ? 64 : 16;
+    return steps <= most && units * W <= INT32_MAX ? W : 0;
+}
+
+template <typename T, int D, bool kListed>
+cudaError_t launch_units(const PaArgs& a, int W, cudaStream_t s) {
+    const auto kernel = paged_attn_units_kernel<T, D, kListed>;
+    static std::atomic<unsigned long long> ready{0};      // a bit a device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PaCfg<D>::kSmem);
+        if (e != cudaSuccess) return e;
+        ready.fetch_or(1ull << dev, std::memory_order_release);
+    }
+    const long long warps = (long long)a.B * a.Hkv * a.tiles * W;
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[2];
+    pdl_config(&cfg, attr, dim3((unsigned)((warps + kPaWarps - 1) / kPaWarps)), dim3(kPaThreads), PaCfg<D>::kSmem, s);
+    if (W > kPaWarps) {
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = W / kPaWarps;
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.numAttrs = 2;
+    }
+    return cudaLaunchKernelEx(&cfg, kernel, a, W);
+}
+
 template <typename T, int D, bool kListed>
 cudaError_t launch_paged(const PaArgs& a, cudaStream_t s) {
+    if (const int W = unit_warps(a, kListed)) return launch_units<T, D, kListed>(a, W, s);
     int ctas = 0;
     cudaError_t e = resident_ctas<T, D, kListed>(&ctas);
     if (e != cudaSuccess) return e;
+    // On long units fewer warps read faster: at D = 128 1024 of the 1184 that fit
+    // took 85.3 us for 90.4 at B=32 T=4129, 86.0 for 91.2 at B=1 T=131105; short
+    // ones want all (64 sequences of up to 1000 tokens: 28.6 us, 30.3 with 1024).
+    if (unit_chunks(a, kListed) >= kPaLongUnit) ctas = std::min(ctas, PaCfg<D>::kLongCtas);
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr;
     pdl_config(&cfg, &attr, dim3(ctas), dim3(kPaThreads), PaCfg<D>::kSmem, s);
@@ -601,45 +840,69 @@ extern "C" size_t zs_paged_attention_workspace_bytes(int B, int Hq, int Hkv, int
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0) return 0;
     const long long tiles = (Hq / Hkv + kPaRows - 1) / kPaRows;
     const int prow = std::min(Hq / Hkv, kPaRows);
-    return plan_bytes((long long)B * Hkv * tiles) + ml_bytes(prow) + (size_t)2 * kPaMaxCtas * kPaWarps * prow * D * 4;
+    return plan_bytes((long long)B * Hkv * tiles) + ml_bytes(prow, D) + (size_t)2 * pa_max_ctas(D) * kPaWarps * prow * D * 4;
+}
+
+namespace zs {
+namespace {
+
+// The checked arguments of a call, but for its workspace.
+bool attention_args(const ZsPagedAttention* p, PaArgs* a) {
+    if (!p || !make_pool(&p->k_pool, &a->kp) || !make_pool(&p->v_pool, &a->vp) || !same_pools(p->k_pool, p->v_pool))
+        return false;
+    const int B = p->B, Hq = p->Hq, Hkv = a->kp.heads, D = a->kp.dim, top = p->top;
+    if (B < 0 || Hq <= 0 || Hq % Hkv || p->width <= 0 || p->table_stride < p->width ||
+        !std::isfinite(p->softmax_scale) || (D != 64 && D != 128))
+        return false;
+    if ((long long)B * Hq > INT32_MAX || (long long)p->width << a->kp.page_shift > INT32_MAX) return false;
+    if (B && (!p->q || !p->block_table || !p->seq_lens || !p->out || !aligned16p(p->q) || !aligned16p(p->out)))
+        return false;
+    if (!p->pages != !p->counts || (p->pages && (top <= 0 || (long long)top << a->kp.page_shift > INT32_MAX)))
+        return false;
+    a->G = Hq / Hkv;
+    a->tiles = (a->G + kPaRows - 1) / kPaRows;
+    a->prow = std::min(a->G, kPaRows);
+    a->q = p->q;
+    a->table = p->block_table;
+    a->table_stride = p->table_stride;
+    a->lens = p->seq_lens;
+    a->pages = p->pages;
+    a->counts = p->counts;
+    a->B = B; a->Hq = Hq; a->Hkv = Hkv; a->width = p->width; a->top = top;
+    a->max_len = std::max(p->max_seqlen, 0);
+    a->scale2 = p->softmax_scale * kLog2e;
+    a->out = p->out;
+    a->lse = p->lse;
+    a->err = p->err;
+    return true;
+}
+
+}  // namespace
+}  // namespace zs
+
+extern "C" size_t zs_paged_attention_workspace(const ZsPagedAttention* p) {
+    using namespace zs;
+    PaArgs a{};
+    if (!attention_args(p, &a) || a.B == 0 || unit_warps(a, a.pages != nullptr)) return 0;
+    return zs_paged_attention_workspace_bytes(a.B, a.Hq, a.Hkv, a.kp.dim);
 }
 
 extern "C" int zs_paged_attention(const ZsPagedAttention* p) {
     using namespace zs;
     PaArgs a{};
-    if (!p || !make_pool(&p->k_pool, &a.kp) || !make_pool(&p->v_pool, &a.vp) || !same_pools(p->k_pool, p->v_pool))
-        return cudaErrorInvalidValue;
-    const int B = p->B, Hq = p->Hq, Hkv = a.kp.heads, D = a.kp.dim, top = p->top;
-    if (B < 0 || Hq <= 0 || Hq % Hkv || p->width <= 0 || p->table_stride < p->width ||
-        !std::isfinite(p->softmax_scale))
-        return cudaErrorInvalidValue;
-    if (B == 0) return cudaSuccess;
-    a.G = Hq / Hkv;
-    a.tiles = (a.G + kPaRows - 1) / kPaRows;
-    if ((long long)B * Hq > INT32_MAX || (long long)p->width << a.kp.page_shift > INT32_MAX) return cudaErrorInvalidValue;
-    if (!p->q || !p->block_table || !p->seq_lens || !p->out || !p->ws || !aligned16p(p->q) || !aligned16p(p->out) ||
-        !aligned16p(p->ws) || p->ws_bytes < zs_paged_attention_workspace_bytes(B, Hq, Hkv, D))
-        return cudaErrorInvalidValue;
-    if (!p->pages != !p->counts || (p->pages && (top <= 0 || (long long)top << a.kp.page_shift > INT32_MAX)))
-        return cudaErrorInvalidValue;
-    a.q = p->q;
-    a.table = p->block_table;
-    a.table_stride = p->table_stride;
-    a.lens = p->seq_lens;
-    a.pages = p->pages;
-    a.counts = p->counts;
-    a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.width = p->width; a.top = top;
-    a.prow = std::min(a.G, kPaRows);
-    a.scale2 = p->softmax_scale * kLog2e;
-    a.out = p->out;
-    a.lse = p->lse;
-    uint8_t* ws = static_cast<uint8_t*>(p->ws);
-    a.plan = reinterpret_cast<long long*>(ws);
-    ws += plan_bytes((long long)B * Hkv * a.tiles);
-    a.part_ml = reinterpret_cast<float*>(ws);
-    ws += ml_bytes(a.prow);
-    a.part_o = reinterpret_cast<float*>(ws);
-    a.err = p->err;
+    if (!attention_args(p, &a)) return cudaErrorInvalidValue;
+    if (a.B == 0) return cudaSuccess;
+    if (!unit_warps(a, a.pages != nullptr)) {
+        if (!p->ws || !aligned16p(p->ws) ||
+            p->ws_bytes < zs_paged_attention_workspace_bytes(a.B, a.Hq, a.Hkv, a.kp.dim))
+            return cudaErrorInvalidValue;
+        uint8_t* ws = static_cast<uint8_t*>(p->ws);
+        a.plan = reinterpret_cast<long long*>(ws);
+        ws += plan_bytes((long long)a.B * a.Hkv * a.tiles);
+        a.part_ml = reinterpret_cast<float*>(ws);
+        ws += ml_bytes(a.prow, a.kp.dim);
+        a.part_o = reinterpret_cast<float*>(ws);
+    }
     cudaStream_t s = (cudaStream_t)p->stream;
     if (p->k_pool.dtype == ZS_BF16)
         return a.pages ? dispatch_dim<__nv_bfloat16, true>(a, s) : dispatch_dim<__nv_bfloat16, false>(a, s);

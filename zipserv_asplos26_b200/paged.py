@@ -100,16 +100,18 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                     seq_lens: torch.Tensor, softmax_scale: Optional[float] = None,
                     pages: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
                     out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
-                    err: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    max_seqlen: Optional[int] = None, err: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one new token per sequence, q [B, Hq, D] (or [B, 1, Hq, D]),
     over the first seq_lens[b] tokens of its pages; D is 64 or 128.
 
     With pages (int32 [B, Hkv, top], distinct logical pages) and counts (int32
     [B, Hkv]) only the listed pages' tokens count. A sequence with nothing to
     attend gets zeros. lse (optional, fp32 [B, Hq]) receives the log of the sum
-    of exponentials of the scaled scores."""
+    of exponentials of the scaled scores. max_seqlen is a bound on seq_lens that
+    the host may have (else the table's width is one); only the choice of the
+    kernel depends on it: short sequences want a close one."""
     o = (_native or _load()).paged_attention(q, k_pages, v_pages, block_table, seq_lens, softmax_scale, pages, counts,
-                                             out, lse, err)
+                                             out, lse, max_seqlen, err)
     return o if q.dim() == 3 and out is None else o.view(q.shape)
 
 
@@ -226,11 +228,12 @@ class PagedKVCache:
         return q
 
     def attention(self, q: torch.Tensor, layer: int = 0, softmax_scale: Optional[float] = None,
-                  out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """Attention of q [B, Hq, D] over rows 0 .. B-1."""
+                  out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                  max_seqlen: Optional[int] = None) -> torch.Tensor:
+        """Attention of q [B, Hq, D] over rows 0 .. B-1 (max_seqlen: see paged_attention)."""
         B = q.shape[0]
         return paged_attention(q, self.k[layer], self.v[layer], self.block_table[:B], self.seqlens[:B], softmax_scale,
-                               None, None, out, lse, self.err)
+                               None, None, out, lse, max_seqlen, self.err)
 
     def sparse_attention(self, q: torch.Tensor, top_pages: int, layer: int = 0, sink_pages: int = 1,
                          local_pages: int = 1, softmax_scale: Optional[float] = None):
