@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectA
     constexpr int kGroups = D <= 128 ? 4 : 2;        // of them a warp pass, loads in flight together
     extern __shared__ uint4 select_smem[];
     __shared__ __align__(16) uint32_t s_hist[kSelectBins];
-    __shared__ uint32_t s_part[2][kSelectWarps], s_pick[3], s_lo, s_hi, s_most;
+    __shared__ uint32_t s_part[2][kSelectWarps], s_pick[3], s_lo, s_hi;
     const int unit = blockIdx.x / cluster, rank = blockIdx.x % cluster;
     const int b = unit / a.Hkv, h = unit % a.Hkv;
     const int G = a.Hq / a.Hkv, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -268,7 +268,13 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectA
     grid_dep_launch();
     grid_dep_wait();
     const uint32_t* q = reinterpret_cast<const uint32_t*>(a.q + ((long long)b * a.Hq + (long long)h * G) * D);
-    const uint32_t q0 = tid < G * D / 2 ? q[tid] : 0;              // beside the length
+    // q's largest magnitude, by every warp for itself, beside the length
+    uint32_t most = 0;
+#pragma unroll 4
+    for (int i = lane; i < G * D / 2; i += 32) {
+        const float2 f = unpack2<T>(q[i]);
+        most = max(most, max(__float_as_uint(f.x) & 0x7FFFFFFFu, __float_as_uint(f.y) & 0x7FFFFFFFu));
+    }
     const int len = max(0, min(a.lens[b], (int)min((long long)a.width << sh, (long long)INT_MAX)));
     const int n = (int)(((long long)len + (1 << sh) - 1) >> sh);
     int* out = a.pages + (long long)unit * a.top;
@@ -289,28 +295,20 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectA
     int blk = lane < pass && p0 + lane < p_end ? row[p0 + lane] : -1;
     int8_t* q8 = reinterpret_cast<int8_t*>(select_smem);              // [G][2 D]: positive part, negative part
     uint32_t* keys = reinterpret_cast<uint32_t*>(select_smem + G * kPieces);
-    // q to whole numbers
+    // No CTA writes into the first one's shared memory before that one has set this
+    // up: waited for before the scores.
     if (tid == 0) {
-        s_most = 0;
         s_lo = 0xFFFFFFFFu;
         s_hi = 0;
     }
-    __syncthreads();
-    // no CTA writes into the first one's shared memory before that one has set it up
+    if (tid < 3) keys[n + tid] = 0;                  // up to a multiple of four; no page's key is 0
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    uint32_t most = 0;
-    for (int i = tid; i < G * D / 2; i += kSelectThreads) {
-        const float2 f = unpack2<T>(i == tid ? q0 : q[i]);
-        most = max(most, max(__float_as_uint(f.x) & 0x7FFFFFFFu, __float_as_uint(f.y) & 0x7FFFFFFFu));
-    }
+    // q to whole numbers
     most = __reduce_max_sync(~0u, most);
-    if (lane == 0 && most) atomicMax(&s_most, most);
-    __syncthreads();
-    most = s_most;
     const float step = __uint_as_float(most & 0x7F800000u) * 0.015625f;
     const bool live = most < 0x7F800000u && step > 0.f;
     for (int i = tid; i < G * D / 2; i += kSelectThreads) {
-        const float2 f = unpack2<T>(i == tid ? q0 : q[i]);
+        const float2 f = unpack2<T>(q[i]);
         const int x = live ? max(-127, min(127, (int)rintf(f.x / step))) : 0;
         const int y = live ? max(-127, min(127, (int)rintf(f.y / step))) : 0;
         char2* at = reinterpret_cast<char2*>(q8 + (i / (D / 2)) * 2 * D + i % (D / 2) * 2);
@@ -400,30 +398,39 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectA
     if (rank) return;
     lo = s_lo;
     hi = s_hi;
+    const uint4* keys4 = reinterpret_cast<const uint4*>(keys);
+    const int n4 = (n + 3) / 4;
     // top < n and the forced pages are sinks + local <= top, all different, so
     // at least one page is scored and `want` of the scored ones are chosen
     uint32_t want = (uint32_t)(a.top - a.sinks - a.local);
     while (want && lo != hi) {
         const int shift = max(0, 22 - __clz(hi - lo));          // (hi - lo) >> shift is below 1024
-        for (int i = tid; i < kSelectBins; i += kSelectThreads) s_hist[i] = 0;
+        static_assert(kSelectBins == 4 * kSelectThreads, "four bins a thread");
+        reinterpret_cast<uint4*>(s_hist)[tid] = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        for (int i = tid; i < n; i += kSelectThreads) {
-            const uint32_t k = keys[i];
+        auto count = [&](uint32_t k) {
             if (k >= lo && k <= hi) atomicAdd(&s_hist[(k - lo) >> shift], 1u);
+        };
+        for (int i = tid; i < n4; i += kSelectThreads) {
+            const uint4 k = keys4[i];
+            count(k.x);
+            count(k.y);
+            count(k.z);
+            count(k.w);
         }
         __syncthreads();
         // thread t looks at four bins, from kSelectBins - 1 - 4 t down
         const uint4 bins = reinterpret_cast<const uint4*>(s_hist)[kSelectThreads - 1 - tid];
         uint32_t above = select_scan(bins.x + bins.y + bins.z + bins.w, s_part[0]);
-        const uint32_t count[4] = {bins.w, bins.z, bins.y, bins.x};
+        const uint32_t held[4] = {bins.w, bins.z, bins.y, bins.x};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (above < want && above + count[i] >= want) {
+            if (above < want && above + held[i] >= want) {
                 s_pick[0] = kSelectBins - 1 - 4 * tid - i;
                 s_pick[1] = want - above;
-                s_pick[2] = count[i];
+                s_pick[2] = held[i];
             }
-            above += count[i];
+            above += held[i];
         }
         __syncthreads();
         const uint32_t from = lo + (s_pick[0] << shift);
@@ -439,27 +446,35 @@ __global__ void __launch_bounds__(kSelectThreads, 2) select_kernel(const SelectA
     }
     // keys above lo are in; of its equals the first `want` pages
     if (a.top == a.sinks + a.local) lo = 0xFFFFFFFEu;
-    const int per = (n + kSelectThreads - 1) / kSelectThreads;
-    const int i0 = min(n, tid * per), i1 = min(n, i0 + per);
+    const int per = (n4 + kSelectThreads - 1) / kSelectThreads;
+    const int i0 = min(n4, tid * per), i1 = min(n4, i0 + per);
     uint32_t above = 0, equal = 0;
     for (int i = i0; i < i1; ++i) {
-        above += keys[i] > lo;
-        equal += keys[i] == lo;
+        const uint4 k = keys4[i];
+        above += (k.x > lo) + (k.y > lo) + (k.z > lo) + (k.w > lo);
+        equal += (k.x == lo) + (k.y == lo) + (k.z == lo) + (k.w == lo);
     }
     const uint32_t before = select_scan(above << 16 | equal, s_part[1]);
     uint32_t at_above = before >> 16, at_equal = before & 0xFFFFu;
-    for (int i = i0; i < i1; ++i) {
-        const bool gt = keys[i] > lo, eq = keys[i] == lo;
+    auto emit = [&](uint32_t k, int i) {
+        const bool gt = k > lo, eq = k == lo;
         if (gt || (eq && at_equal < want)) out[at_above + min(at_equal, want)] = i;
         at_above += gt;
         at_equal += eq;
+    };
+    for (int i = i0; i < i1; ++i) {
+        const uint4 k = keys4[i];
+        emit(k.x, 4 * i);
+        emit(k.y, 4 * i + 1);
+        emit(k.z, 4 * i + 2);
+        emit(k.w, 4 * i + 3);
     }
 }
 
 template <typename T>
 cudaError_t launch_select(const SelectArgs& a, int D, cudaStream_t s) {
     const int G = a.Hq / a.Hkv;
-    const size_t smem = (size_t)G * 2 * D + sizeof(uint32_t) * (size_t)a.width;
+    const size_t smem = (size_t)G * 2 * D + sizeof(uint32_t) * ((size_t)a.width + 3);
     // CTAs a (sequence, KV head): as many as the GPU holds at once (two an SM), while
     // each still has 32 pages for a part of its 16 warps
     int cluster = 1;
