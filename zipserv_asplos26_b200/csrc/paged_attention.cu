@@ -8,20 +8,30 @@
 //
 // Bound by HBM: each K and V row is read once for all the query heads that share
 // it. The work is cut into chunks of 16 tokens of a unit (sequence, KV head, tile
-// of up to 16 query heads); all chunks in order are dealt to the CTAs in equal
-// runs, found by a prefix sum over the lengths in the kernel, so ragged batches
-// and single long sequences load every SM alike and no length is needed on the
-// host. A run that ends inside a unit leaves its (m, l, O) in a workspace and a
-// second kernel joins a unit's pieces in order.
+// of up to 16 query heads), a warp's step, and dealt in one of two ways, chosen by
+// sizes that the host has (unit_warps):
+//   * paged_attn_kernel: all chunks in order go to the warps of the GPU in equal
+//     runs, found by a prefix sum over the lengths in the kernel, so ragged
+//     batches and single long sequences load every SM alike and no length is
+//     needed on the host. A run that ends inside a unit leaves its (m, l, O) in a
+//     workspace, and paged_join_kernel joins a unit's pieces in order.
+//   * paged_attn_units_kernel: a fixed number of warps a unit, joined through
+//     distributed shared memory in the same kernel: short units and page lists.
+// Sums are always in the same order: a result does not change from run to run.
 //
-// Inside a CTA each warp works on every fourth chunk by itself: it copies its
-// chunk's K and V rows with 16-byte cp.async into its own ring (rows past the
-// length are zero-filled and never read), so there is no barrier in the loop.
-// S = Q K^T and O += P V are m16n8k16 products: the rows are query heads, of
-// which a decode step has 1 to 16 a KV head, far below a tcgen05 tile's 128, and
-// the tensor work is a third of the memory time even with rows unused.
+// A warp copies its chunk's K and V rows with 16-byte cp.async into a ring of its
+// own, two chunks ahead (rows past the length are zero-filled and never read), so
+// there is no barrier in the loop and copies run on while a unit ends and the next
+// begins. S = Q K^T and O += P V are m16n8k16 products: the rows are query heads,
+// of which a decode step has 1 to 16 a KV head, far below a tcgen05 tile's 128;
+// the tensor pipe is busy 27% of the time with P in two parts and 12 rows unused.
 // P is fed as a 16-bit high part plus its 16-bit remainder, so that rounding P
 // adds nothing to the output's own rounding.
+//
+// Measured (bf16, 32 query and 8 KV heads of 128, pages of 64, us and GB/s of keys
+// and values): B=32 T=4129 84.8, 6.39 TB/s; B=1 T=131105 86.8, 6.18 TB/s; 61
+// sequences of 0..16417 with 64 query heads 308, 6.70 TB/s; B=1 T=97 4.5. A plain
+// copy does 6.56 TB/s. DRAM reads are the algorithm's bytes (541.5 MB of 541).
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -103,6 +113,13 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Transposes an 8 x 8 matrix of 16-bit values held a row a quad of lanes.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
 // P is computed as 2^(s - m + bias): for fp16 the bias keeps probabilities down
 // to 2^-39 of the largest above fp16's smallest step (long tails of a long cache
 // would vanish otherwise); bf16 has fp32's exponents.
@@ -142,16 +159,22 @@ __device__ __forceinline__ long long warp_prefix(long long v) {
 }
 
 template <int D>
-struct PaCfg {
+struct PaTile {
     static constexpr int kRowBytes = D * 2;
     static constexpr int kTile = kPaChunk * kRowBytes;             // one K or V chunk
-    // CTAs an SM: rows of 128 bytes take more steps for the same bytes, so D = 64
-    // wants more warps (B=32 T=4129: 2 of 6 stages 51.9 us, 3 of 4 stages 48.8)
-    static constexpr int kCtas = D <= 64 ? 3 : 2;
-    static constexpr int kStages = D <= 64 ? 4 : 3;
-    // CTAs for long units, see launch_paged
-    static constexpr int kLongCtas = D <= 64 ? 148 * kCtas : 256;
-    static constexpr int kRing = kStages * 2 * kTile;              // a warp's ring
+};
+
+// CTAs an SM and chunks of a warp's ring. What counts is how much is on its way:
+// some 96 KB an SM read fastest where the products leave the time (the form for 8
+// heads), from more warps rather than deeper rings. B=32 T=4129 in a long run under
+// the power cap: 12 warps of 2 chunks 87.3 us, 8 of 3 91.4; D = 64: 16 of 2 90.9,
+// 16 of 3 95.0, 12 of 4 95.6. The form for 16 heads holds twice the registers: 8
+// warps at D = 128 (94.6 us with 16 heads a KV head), 12 at 64.
+template <int D, bool kNarrow>
+struct PaCfg : PaTile<D> {
+    static constexpr int kCtas = kNarrow ? (D <= 64 ? 4 : 3) : (D <= 64 ? 3 : 2);
+    static constexpr int kStages = kNarrow ? 2 : (D <= 64 ? 4 : 3);
+    static constexpr int kRing = kStages * 2 * PaTile<D>::kTile;   // bytes of a warp's ring
     static constexpr int kSmem = kPaWarps * kRing;
 };
 
@@ -163,9 +186,10 @@ __device__ __forceinline__ void look_chunk(const PaArgs& a, int e, int b, int ch
     const int cps = a.kp.page_shift - 4;                               // log2 chunks a page
     int p = ch >> cps;
     if (kListed) p = a.pages[(long long)e * a.top + p];
-    const int t0 = ((p << cps) + (ch & ((1 << cps) - 1))) * kPaChunk;
     id = lim = 0;
-    if (p < 0 || p >= a.width || t0 >= len) return;
+    if (p < 0 || p >= a.width) return;
+    const int t0 = ((p << cps) + (ch & ((1 << cps) - 1))) * kPaChunk;
+    if (t0 >= len) return;
     const int blk = a.table[b * a.table_stride + p];
     if (blk < 0 || blk >= a.kp.num_blocks) {
         set_err(a.err, kErrPagedIndex);
@@ -179,7 +203,7 @@ __device__ __forceinline__ void look_chunk(const PaArgs& a, int e, int b, int ch
 template <int D>
 __device__ __forceinline__ void copy_chunk(const PaArgs& a, uint32_t dst, int blk, int ch, int h, int lim,
                                            uint64_t policy) {
-    using C = PaCfg<D>;
+    using C = PaTile<D>;
     constexpr int kPieces = D / 8;                 // 16-byte pieces a row
     const int lane = threadIdx.x & 31;
     const int row0 = (ch & ((1 << (a.kp.page_shift - 4)) - 1)) * kPaChunk;
@@ -197,11 +221,18 @@ __device__ __forceinline__ void copy_chunk(const PaArgs& a, uint32_t dst, int bl
 }
 
 // What a warp holds of a unit: q as product fragments, running maximum (base 2),
-// sum and output; lane rows lane / 4 and lane / 4 + 8.
+// sum and output. Two forms: 16 heads as the rows of S and O (here; a lane has rows
+// lane / 4 and lane / 4 + 8), or up to 8 heads as the columns of S^T and O^T.
 template <typename T, int D>
-struct PaState {
+struct PaWide {
     uint32_t qf[D / 16][4];
     float o[D / 8][4], m[2], l[2];
+    struct Scores {
+        float v[2][4];
+    };
+    struct Weights {
+        uint32_t hi[4], lo[4];
+    };
 
     __device__ __forceinline__ void start(const uint16_t* q, int rows) {
         const int lane = threadIdx.x & 31, r = lane >> 2, cc = (lane & 3) * 2;
@@ -220,27 +251,28 @@ struct PaState {
         l[0] = l[1] = 0.f;
     }
 
-    // One chunk: keys at kt, values behind them.
-    __device__ __forceinline__ void attend(uint32_t kt, int lim, float scale2) {
-        using C = PaCfg<D>;
-        constexpr int kKs = D / 16;
-        const int lane = threadIdx.x & 31;
-        const uint32_t vt = kt + C::kTile;
-        // S = Q K^T: 16 heads x 16 tokens
-        float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        {
-            const int r = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
-            const uint32_t row = kt + r * C::kRowBytes;
+    // S = Q K^T of a chunk's keys at kt: 16 heads x 16 tokens.
+    __device__ __forceinline__ void scores(uint32_t kt, Scores& s) {
+        auto& sc = s.v;
+        const int lane = threadIdx.x & 31, r = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+        const uint32_t row = kt + r * PaTile<D>::kRowBytes;
 #pragma unroll
-            for (int ks = 0; ks < kKs; ++ks) {
-                uint32_t f[4];
-                ldsm4(f, row + (((ks * 2 + half) ^ (r & 7)) * 16));
-                mma16816(sc[0], qf[ks], f[0], f[1], T());
-                mma16816(sc[1], qf[ks], f[2], f[3], T());
-            }
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[j][i] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            uint32_t f[4];
+            ldsm4(f, row + (((ks * 2 + half) ^ (r & 7)) * 16));
+            mma16816(sc[0], qf[ks], f[0], f[1], T());
+            mma16816(sc[1], qf[ks], f[2], f[3], T());
         }
-        // running maximum and sum
-        const int t = (lane & 3) * 2;
+    }
+
+    // Running maximum and sum; P = 2^(S - m) as fragments of two 16-bit parts.
+    __device__ __forceinline__ void weigh(const Scores& s, int lim, float scale2, Weights& w) {
+        const auto& sc = s.v;
+        const int t = (threadIdx.x & 3) * 2;
         float p[2][4];
         bool grew = false;
         float keep[2];
@@ -282,37 +314,251 @@ struct PaState {
                 o[i][3] *= keep[1];
             }
         }
-        // O += P V, P in two 16-bit parts
-        uint32_t hi[4], lo[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float x = p[i >> 1][(i & 1) * 2], y = p[i >> 1][(i & 1) * 2 + 1];
-            hi[i] = pack2<T>(x, y);
-            const float2 back = unpack2<T>(hi[i]);
-            lo[i] = pack2<T>(x - back.x, y - back.y);
-        }
-        {
-            const int r = lane & 15, half = lane >> 4;
-            const uint32_t row = vt + r * C::kRowBytes;
-#pragma unroll
-            for (int ks = 0; ks < kKs; ++ks) {
-                uint32_t f[4];
-                ldsm4t(f, row + (((ks * 2 + half) ^ (r & 7)) * 16));
-                mma16816(o[ks * 2], hi, f[0], f[1], T());
-                mma16816(o[ks * 2 + 1], hi, f[2], f[3], T());
-                mma16816(o[ks * 2], lo, f[0], f[1], T());
-                mma16816(o[ks * 2 + 1], lo, f[2], f[3], T());
-            }
+            w.hi[i] = pack2<T>(x, y);
+            const float2 back = unpack2<T>(w.hi[i]);
+            w.lo[i] = pack2<T>(x - back.x, y - back.y);
         }
     }
 
-    // The sums of the four lanes of a row.
+    // O += P V of a chunk's values at vt.
+    __device__ __forceinline__ void add(uint32_t vt, const Weights& w) {
+        const int lane = threadIdx.x & 31, r = lane & 15, half = lane >> 4;
+        const uint32_t row = vt + r * PaTile<D>::kRowBytes;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            uint32_t f[4];
+            ldsm4t(f, row + (((ks * 2 + half) ^ (r & 7)) * 16));
+            mma16816(o[ks * 2], w.hi, f[0], f[1], T());
+            mma16816(o[ks * 2 + 1], w.hi, f[2], f[3], T());
+            mma16816(o[ks * 2], w.lo, f[0], f[1], T());
+            mma16816(o[ks * 2 + 1], w.lo, f[2], f[3], T());
+        }
+    }
+
+    // The sums of a row's four lanes.
     __device__ __forceinline__ void finish() {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             l[r] += __shfl_xor_sync(~0u, l[r], 1);
             l[r] += __shfl_xor_sync(~0u, l[r], 2);
         }
+    }
+    // The finished rows, to the output [rows][D].
+    __device__ __forceinline__ void write(uint16_t* out, float* lse, int rows) const {
+        const int lane = threadIdx.x & 31, d0 = (lane & 3) * 2;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int row = (lane >> 2) + r * 8;
+            if (row >= rows) continue;
+            const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+                *reinterpret_cast<uint32_t*>(out + row * D + i * 8 + d0) = pack2<T>(o[i][r * 2] * inv, o[i][r * 2 + 1] * inv);
+            if (lse && d0 == 0) lse[row] = log_sum<T>(m[r], l[r]);
+        }
+    }
+    // A piece: unnormalised rows [rows][D], and [rows][2] maxima and sums.
+    __device__ __forceinline__ void park(float* po, float* ml, int rows) const {
+        const int lane = threadIdx.x & 31, d0 = (lane & 3) * 2;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int row = (lane >> 2) + r * 8;
+            if (row >= rows) continue;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+                *reinterpret_cast<float2*>(po + row * D + i * 8 + d0) = make_float2(o[i][r * 2], o[i][r * 2 + 1]);
+            if (d0 == 0) *reinterpret_cast<float2*>(ml + row * 2) = make_float2(m[r], l[r]);
+        }
+    }
+};
+
+// Up to 8 heads: the keys are the rows of S^T = K Q^T (16 tokens x 8 heads) and the
+// channels those of O^T += V^T P^T, half the products and half the exponentials of
+// the form above. A lane has heads 2 (lane % 4) and the next, of S^T tokens lane / 4
+// and lane / 4 + 8, of O^T channels likewise; P^T gets its fragment by transposing
+// 8 x 8 blocks in registers.
+template <typename T, int D>
+struct PaNarrow {
+    uint32_t qf[D / 16][2];
+    float o[D / 16][4], m[2], l[2];
+    struct Scores {
+        float v[4];
+    };
+    struct Weights {
+        uint32_t hi[2], lo[2];
+    };
+
+    __device__ __forceinline__ void start(const uint16_t* q, int rows) {
+        const int lane = threadIdx.x & 31, head = lane >> 2, cc = (lane & 3) * 2;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                qf[ks][i] = head < rows ? *reinterpret_cast<const uint32_t*>(q + head * D + ks * 16 + i * 8 + cc) : 0u;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
+    }
+
+    __device__ __forceinline__ void scores(uint32_t kt, Scores& s) {
+        const int lane = threadIdx.x & 31, r = lane & 15, half = lane >> 4;
+        const uint32_t row = kt + r * PaTile<D>::kRowBytes;
+        // two sums: the products of a chain wait for one another
+        float odd[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s.v[i] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            uint32_t f[4];
+            ldsm4(f, row + (((ks * 2 + half) ^ (r & 7)) * 16));
+            mma16816(ks & 1 ? odd : s.v, f, qf[ks][0], qf[ks][1], T());
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s.v[i] += odd[i];
+    }
+
+    __device__ __forceinline__ void weigh(const Scores& s, int lim, float scale2, Weights& w) {
+        const int t = (threadIdx.x & 31) >> 2;
+        float p[4], keep[2];
+        bool grew = false;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {               // head
+            const float x = t < lim ? s.v[j] * scale2 : -INFINITY;
+            const float y = t + 8 < lim ? s.v[2 + j] * scale2 : -INFINITY;
+            float mx = fmaxf(x, y);
+#pragma unroll
+            for (int k = 4; k < 32; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, k));
+            const float mn = fmaxf(m[j], mx);
+            grew |= mn > m[j];
+            const float ref = mn == -INFINITY ? 0.f : mn;
+            keep[j] = exp2f(m[j] - ref);
+            m[j] = mn;
+            p[j] = exp2f(x - ref + kPBias<T>);
+            p[2 + j] = exp2f(y - ref + kPBias<T>);
+            l[j] = l[j] * keep[j] + (p[j] + p[2 + j]);
+        }
+        if (__any_sync(~0u, grew)) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                o[i][0] *= keep[0];
+                o[i][1] *= keep[1];
+                o[i][2] *= keep[0];
+                o[i][3] *= keep[1];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t hi = pack2<T>(p[2 * i], p[2 * i + 1]);
+            const float2 back = unpack2<T>(hi);
+            w.hi[i] = transpose8(hi);
+            w.lo[i] = transpose8(pack2<T>(p[2 * i] - back.x, p[2 * i + 1] - back.y));
+        }
+    }
+
+    __device__ __forceinline__ void add(uint32_t vt, const Weights& w) {
+        const int lane = threadIdx.x & 31, r = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+        const uint32_t row = vt + r * PaTile<D>::kRowBytes;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            uint32_t f[4];
+            ldsm4t(f, row + (((i * 2 + half) ^ (r & 7)) * 16));
+            mma16816(o[i], f, w.hi[0], w.hi[1], T());
+            mma16816(o[i], f, w.lo[0], w.lo[1], T());
+        }
+    }
+
+    __device__ __forceinline__ void finish() {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int k = 4; k < 32; k <<= 1) l[j] += __shfl_xor_sync(~0u, l[j], k);
+    }
+    __device__ __forceinline__ void write(uint16_t* out, float* lse, int rows) const {
+        const int lane = threadIdx.x & 31, d0 = lane >> 2;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int row = (lane & 3) * 2 + j;
+            if (row >= rows) continue;
+            const float inv = l[j] == 0.f ? 0.f : 1.f / l[j];
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                const uint32_t v = pack2<T>(o[i][j] * inv, o[i][2 + j] * inv);
+                out[row * D + i * 16 + d0] = (uint16_t)v;
+                out[row * D + i * 16 + 8 + d0] = (uint16_t)(v >> 16);
+            }
+            if (lse && d0 == 0) lse[row] = log_sum<T>(m[j], l[j]);
+        }
+    }
+    __device__ __forceinline__ void park(float* po, float* ml, int rows) const {
+        const int lane = threadIdx.x & 31, d0 = lane >> 2;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int row = (lane & 3) * 2 + j;
+            if (row >= rows) continue;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                po[row * D + i * 16 + d0] = o[i][j];
+                po[row * D + i * 16 + 8 + d0] = o[i][2 + j];
+            }
+            if (d0 == 0) *reinterpret_cast<float2*>(ml + row * 2) = make_float2(m[j], l[j]);
+        }
+    }
+};
+
+template <typename T, int D, bool kNarrow>
+struct PaStateOf {
+    using type = PaWide<T, D>;
+};
+template <typename T, int D>
+struct PaStateOf<T, D, true> {
+    using type = PaNarrow<T, D>;
+};
+
+// A warp's ring: kStages - 1 chunks are on their way while one is worked on.
+// find(blk, ch, h, s) gives the place of the chunk of step s and returns its number
+// of valid tokens. (Keys and values apart, each slot filled again as soon as it is
+// used, kept 2 1/2 chunks on their way and was 3% slower.)
+template <int D, bool kNarrow>
+struct PaRing {
+    using C = PaCfg<D, kNarrow>;
+    uint32_t base;
+    uint64_t policy;
+    int steps;
+    int lims[C::kStages - 1];      // of the chunks on their way, oldest first
+
+    __device__ __forceinline__ uint32_t slot(int s) const { return base + (s % C::kStages) * 2 * C::kTile; }
+    template <typename Find>
+    __device__ __forceinline__ void ask(const PaArgs& a, int s, Find&& find) {
+        int lim = 0;
+        if (s < steps) {
+            int blk, ch, h;
+            lim = find(blk, ch, h, s);
+            copy_chunk<D>(a, slot(s), blk, ch, h, lim, policy);
+        }
+        cp_commit();
+#pragma unroll
+        for (int i = 0; i + 2 < C::kStages; ++i) lims[i] = lims[i + 1];
+        lims[C::kStages - 2] = lim;
+    }
+    // Step s of a unit.
+    template <typename State, typename Find>
+    __device__ __forceinline__ void step(const PaArgs& a, int s, State& st, Find&& find) {
+        typename State::Scores sc;
+        typename State::Weights w;
+        cp_wait<C::kStages - 2>();
+        __syncwarp();
+        const int lim = lims[0];
+        ask(a, s + C::kStages - 1, find);
+        st.scores(slot(s), sc);
+        st.weigh(sc, lim, a.scale2, w);
+        st.add(slot(s) + C::kTile, w);
+        __syncwarp();
     }
 };
 
@@ -332,16 +578,13 @@ __device__ __forceinline__ void next_unit(const PaArgs& a, int per_entry, PaCurs
     while (c.n == 0);
 }
 
-template <typename T, int D, bool kListed>
-__global__ void __launch_bounds__(kPaThreads, PaCfg<D>::kCtas) paged_attn_kernel(const PaArgs a) {
-    using C = PaCfg<D>;
+template <typename T, int D, bool kListed, bool kNarrow>
+__global__ void __launch_bounds__(kPaThreads, PaCfg<D, kNarrow>::kCtas) paged_attn_kernel(const PaArgs a) {
+    using C = PaCfg<D, kNarrow>;
     extern __shared__ __align__(1024) uint8_t pa_smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t ring = smem_u32(pa_smem) + warp * C::kRing;
     grid_dep_launch();
     grid_dep_wait();
-
-    const uint64_t policy = evict_first_policy();
 
     // ---- each warp's run of chunks
     const int entries = kListed ? a.B * a.Hkv : a.B;
@@ -422,28 +665,26 @@ __global__ void __launch_bounds__(kPaThreads, PaCfg<D>::kCtas) paged_attn_kernel
     };
     look(now);
     int in_batch = 0;
-    // starts the copies of step s; returns its number of valid tokens
-    auto produce = [&](int s) {
-        int lim = 0;
-        if (s < steps) {
-            if (in_batch == now.count) {
-                now = next;
-                in_batch = 0;
-                look(next);
-            }
-            const int blk = __shfl_sync(~0u, now.ids, in_batch);
-            lim = __shfl_sync(~0u, now.lims, in_batch);
-            copy_chunk<D>(a, ring + (s % C::kStages) * 2 * C::kTile, blk, now.ch + in_batch, now.h, lim, policy);
-            ++in_batch;
+    auto find = [&](int& blk, int& ch, int& h, int) {
+        if (in_batch == now.count) {
+            now = next;
+            in_batch = 0;
+            look(next);
         }
-        cp_commit();
-        return lim;
+        blk = __shfl_sync(~0u, now.ids, in_batch);
+        ch = now.ch + in_batch;
+        h = now.h;
+        return __shfl_sync(~0u, now.lims, in_batch++);
     };
-    int lim_at[C::kStages];        // of the steps in flight, oldest first
-    lim_at[0] = produce(0);        // on its way while the next batch is looked up
-    look(next);
+    PaRing<D, kNarrow> ring;
+    ring.base = smem_u32(pa_smem) + warp * C::kRing;
+    ring.policy = evict_first_policy();
+    ring.steps = steps;
 #pragma unroll
-    for (int s = 1; s < C::kStages - 1; ++s) lim_at[s] = produce(s);
+    for (int s = 0; s < C::kStages - 1; ++s) {
+        ring.ask(a, s, find);
+        if (s == 0) look(next);    // the first chunk is on its way while the next batch is looked up
+    }
 
     int s = 0;
     while (true) {
@@ -455,43 +696,15 @@ __global__ void __launch_bounds__(kPaThreads, PaCfg<D>::kCtas) paged_attn_kernel
         const int g0 = tile * kPaRows, rows = min(kPaRows, a.G - g0);
         if (first == 0 && lane == 0) a.plan[1 + (b * a.Hkv + h) * a.tiles + tile] = u_lo;
         const long long head0 = (long long)b * a.Hq + (long long)h * a.G + g0;
-        PaState<T, D> st;
+        typename PaStateOf<T, D, kNarrow>::type st;
         st.start(a.q + head0 * D, rows);
-        for (const int end = s + count; s < end; ++s) {
-            cp_wait<C::kStages - 2>();
-            __syncwarp();
-            const int lim = lim_at[0];
-#pragma unroll
-            for (int i = 0; i + 1 < C::kStages; ++i) lim_at[i] = lim_at[i + 1];
-            lim_at[C::kStages - 2] = produce(s + C::kStages - 1);
-            st.attend(ring + (s % C::kStages) * 2 * C::kTile, lim, a.scale2);
-            __syncwarp();
-        }
+        for (const int end = s + count; s < end; ++s) ring.step(a, s, st, find);
         // ---- out, or to the workspace where the run cuts the unit
         const bool whole = first == 0 && count == cur.n;
         const long long slot = 2ll * id + (s == count ? 0 : 1);       // the run's first part, or its last
-        const int d0 = (lane & 3) * 2;
         st.finish();
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int row = (lane >> 2) + r * 8;
-            if (row >= rows) continue;
-            if (whole) {
-                const float inv = st.l[r] == 0.f ? 0.f : 1.f / st.l[r];
-                uint16_t* out = a.out + (head0 + row) * D + d0;
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i)
-                    *reinterpret_cast<uint32_t*>(out + i * 8) = pack2<T>(st.o[i][r * 2] * inv, st.o[i][r * 2 + 1] * inv);
-                if (a.lse && d0 == 0) a.lse[head0 + row] = log_sum<T>(st.m[r], st.l[r]);
-            } else {
-                float* po = a.part_o + (slot * a.prow + row) * D + d0;
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i)
-                    *reinterpret_cast<float2*>(po + i * 8) = make_float2(st.o[i][r * 2], st.o[i][r * 2 + 1]);
-                if (d0 == 0)
-                    *reinterpret_cast<float2*>(a.part_ml + (slot * a.prow + row) * 2) = make_float2(st.m[r], st.l[r]);
-            }
-        }
+        if (whole) st.write(a.out + head0 * D, a.lse ? a.lse + head0 : nullptr, rows);
+        else st.park(a.part_o + slot * a.prow * D, a.part_ml + slot * a.prow * 2, rows);
         if (s == steps) break;
         u_lo += cur.n;
         next_unit<kListed>(a, per_entry, cur);
@@ -505,12 +718,11 @@ __global__ void __launch_bounds__(kPaThreads, PaCfg<D>::kCtas) paged_attn_kernel
 // memory, and after a cluster barrier the unit's threads join the W pieces
 // through distributed shared memory, in order. With W below 4 a CTA has several
 // units, from 4 on a cluster of W / 4 CTAs has one.
-template <typename T, int D, bool kListed>
-__global__ void __launch_bounds__(kPaThreads, PaCfg<D>::kCtas) paged_attn_units_kernel(const PaArgs a, int W) {
-    using C = PaCfg<D>;
+template <typename T, int D, bool kListed, bool kNarrow>
+__global__ void __launch_bounds__(kPaThreads, PaCfg<D, kNarrow>::kCtas) paged_attn_units_kernel(const PaArgs a, int W) {
+    using C = PaCfg<D, kNarrow>;
     extern __shared__ __align__(1024) uint8_t pa_smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t ring = smem_u32(pa_smem) + warp * C::kRing;
     const long long warp_id = (long long)blockIdx.x * kPaWarps + warp;
     const int unit = (int)(warp_id / W), w = (int)(warp_id % W);
     const int units = a.B * a.Hkv * a.tiles;
@@ -519,57 +731,38 @@ __global__ void __launch_bounds__(kPaThreads, PaCfg<D>::kCtas) paged_attn_units_
     const int b = kListed ? e / a.Hkv : e, h = kListed ? e % a.Hkv : unit / a.tiles % a.Hkv;
     const int g0 = unit % a.tiles * kPaRows, rows = on ? min(kPaRows, a.G - g0) : 0;
     const long long head0 = (long long)b * a.Hq + (long long)h * a.G + g0;
-    const uint64_t policy = evict_first_policy();
     grid_dep_launch();
     grid_dep_wait();
     const int table_len = (int)min((long long)a.width << a.kp.page_shift, (long long)INT_MAX);
     const int len = min(a.lens[b], table_len), n = on ? entry_chunks<kListed>(a, e) : 0;
     const int first = (int)((long long)n * w / W), steps = (int)((long long)n * (w + 1) / W) - first;
-    PaState<T, D> st;
+    typename PaStateOf<T, D, kNarrow>::type st;
     int ids = 0, lims = 0;         // of 32 chunks, a lane each
-    auto produce = [&](int s) {
-        int lim = 0;
-        if (s < steps) {
-            if ((s & 31) == 0) {
-                ids = lims = 0;
-                if (s + lane < steps) look_chunk<kListed>(a, e, b, first + s + lane, len, ids, lims);
-            }
-            lim = __shfl_sync(~0u, lims, s & 31);
-            copy_chunk<D>(a, ring + (s % C::kStages) * 2 * C::kTile, __shfl_sync(~0u, ids, s & 31), first + s, h, lim,
-                          policy);
+    auto find = [&](int& blk, int& ch, int& head, int s) {
+        if ((s & 31) == 0) {
+            ids = lims = 0;
+            if (s + lane < steps) look_chunk<kListed>(a, e, b, first + s + lane, len, ids, lims);
         }
-        cp_commit();
-        return lim;
+        blk = __shfl_sync(~0u, ids, s & 31);
+        ch = first + s;
+        head = h;
+        return __shfl_sync(~0u, lims, s & 31);
     };
-    int lim_at[C::kStages];
+    PaRing<D, kNarrow> ring;
+    ring.base = smem_u32(pa_smem) + warp * C::kRing;
+    ring.policy = evict_first_policy();
+    ring.steps = steps;
 #pragma unroll
-    for (int s = 0; s < C::kStages - 1; ++s) lim_at[s] = produce(s);
+    for (int s = 0; s < C::kStages - 1; ++s) ring.ask(a, s, find);
     st.start(a.q + head0 * D, rows);
-    for (int s = 0; s < steps; ++s) {
-        cp_wait<C::kStages - 2>();
-        __syncwarp();
-        const int lim = lim_at[0];
-#pragma unroll
-        for (int i = 0; i + 1 < C::kStages; ++i) lim_at[i] = lim_at[i + 1];
-        lim_at[C::kStages - 2] = produce(s + C::kStages - 1);
-        st.attend(ring + (s % C::kStages) * 2 * C::kTile, lim, a.scale2);
-        __syncwarp();
-    }
+    for (int s = 0; s < steps; ++s) ring.step(a, s, st, find);
     cp_wait<0>();
     __syncwarp();
     st.finish();
     // the warp's piece, over its ring: [16][D] outputs, [16][2] maxima and sums
     static_assert(C::kRing >= kPaRows * (D + 2) * 4, "a warp's piece fits its ring");
     float* po = reinterpret_cast<float*>(pa_smem + warp * C::kRing);
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const int row = (lane >> 2) + r * 8, d0 = (lane & 3) * 2;
-        if (row >= rows) continue;
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-            *reinterpret_cast<float2*>(po + row * D + i * 8 + d0) = make_float2(st.o[i][r * 2], st.o[i][r * 2 + 1]);
-        if (d0 == 0) *reinterpret_cast<float2*>(po + kPaRows * D + row * 2) = make_float2(st.m[r], st.l[r]);
-    }
+    st.park(po, po + kPaRows * D, rows);
     // One warp a unit needs no barrier, several of a CTA the CTA's, more the cluster's
     // (its second one keeps a CTA's shared memory until its peers have read it).
     if (W == 1) __syncwarp();
@@ -630,7 +823,8 @@ __global__ void __launch_bounds__(kPaThreads, PaCfg<D>::kCtas) paged_attn_units_
 // pieces are read in batches, weights and outputs together. A warp takes a query
 // head, D / 32 channels a lane; with few heads (long sequences: up to a piece a
 // warp of the attention kernel) the warps of a CTA share a head's pieces and add
-// their sums in order.
+// their sums in order. With its launch it costs 3 (B=1 T=97) to 5 us (B=1
+// T=131105, 148 pieces a unit; 10 us when the pieces were read one by one).
 constexpr int kJoinWarps = 16;
 constexpr int kJoinShare = 148;        // heads joined by a CTA each
 constexpr int kJoinBatch = 8;
@@ -721,45 +915,50 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PaArg
     if (a.lse && lane == 0) a.lse[head] = log_sum<T>(m, l);
 }
 
-// The workspace's bound on the run kernel's grid.
-inline int pa_max_ctas(int D) { return 148 * (D <= 64 ? PaCfg<64>::kCtas : PaCfg<128>::kCtas); }
+// CTAs of the run kernel, at most.
+inline int pa_max_ctas(int D, int G) {
+    if (G <= 8) return 148 * (D <= 64 ? PaCfg<64, true>::kCtas : PaCfg<128, true>::kCtas);
+    return 148 * (D <= 64 ? PaCfg<64, false>::kCtas : PaCfg<128, false>::kCtas);
+}
 
 size_t plan_bytes(long long units) { return ((size_t)(1 + units) * 8 + 255) / 256 * 256; }
-size_t ml_bytes(int prow, int D) { return (size_t)2 * pa_max_ctas(D) * kPaWarps * prow * 2 * 4; }
+// G is bounded by prow where it matters (both are above 8, or equal)
+size_t ml_bytes(int prow, int D) { return (size_t)2 * pa_max_ctas(D, prow) * kPaWarps * prow * 2 * 4; }
 
 // The attention kernel's grid: the CTAs that the GPU holds at once (looked up once per device).
-template <typename T, int D, bool kListed>
+template <typename T, int D, bool kListed, bool kNarrow>
 cudaError_t resident_ctas(int* ctas) {
     static std::atomic<int> cached[64];
-    const auto kernel = paged_attn_kernel<T, D, kListed>;
+    const auto kernel = paged_attn_kernel<T, D, kListed, kNarrow>;
     int dev = 0, per = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     if ((*ctas = cached[dev].load(std::memory_order_acquire)) > 0) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PaCfg<D>::kSmem);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PaCfg<D, kNarrow>::kSmem);
     if (e != cudaSuccess) return e;
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, kPaThreads, PaCfg<D>::kSmem);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, kPaThreads, PaCfg<D, kNarrow>::kSmem);
     if (e != cudaSuccess) return e;
     e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return e;
     if (per < 1) return cudaErrorInvalidConfiguration;
-    *ctas = std::min(per * sms, pa_max_ctas(D));
+    *ctas = std::min(per * sms, pa_max_ctas(D, kNarrow ? 8 : 16));
     cached[dev].store(*ctas, std::memory_order_release);
     return cudaSuccess;
 }
 
 // Warps a unit for paged_attn_units_kernel, or 0 where runs of chunks are the
-// better way. Fixed shares have no second kernel (some 5 us less: B=32 T=200 12.6
-// us in runs, 8.4 so; 64 x 300 20.3 and 16.1; B=1 T=97 6.5 and 4.7), but the
-// longest unit's share is the time (16 sequences of 0..2048: 18.9 in runs, 21.3
-// so at 17 chunks a warp; 64 of 0..1000: 28.6 and 34.6 at 36). So they serve
-// units that are bounded to 16 chunks a warp (a page list's units are alike: 64;
-// 8 x 64 pages: 42.5 in runs, 37.9 so), or to 5 where they leave SMs idle (B=1
-// T=4096, 17 chunks a warp: 9.8 in runs, 15.9 so). W is what fills the GPU, at
-// most a portable cluster's half: clusters of 8 and 16 CTAs were slower in all.
+// better way. Fixed shares have no second kernel (us in runs and so: B=1 T=97 7.5
+// and 4.9, 16 sequences of 300 11.1 and 8.7, 512 of 100..200 59.3 and 54.0), but
+// the longest unit's share is the time where one wave of warps holds all units (64
+// of 0..1000: 26.4 and 34.6 at 36 chunks a warp; 16 of 2048: 27.1 and 28.5 at 17).
+// So they serve units that are bounded to 16 chunks a warp, to 64 for page lists,
+// whose units are alike (8 x 64 pages: 43.5 and 39.3), or to 5 where they leave SMs
+// idle (B=1 T=4096: 9.6 and 15.6). W fills the GPU once, with two chunks a warp or
+// more; units of unlike lengths in more waves want shares of some 12 chunks (128
+// of 0..600: 41.1 us with one warp each, 28.7 with four, 31.4 in runs). Clusters of
+// more than 4 CTAs were slower in all of these.
 constexpr int kPaMaxUnitWarps = 16;
-constexpr int kPaLongUnit = 128;       // chunks
 
 // A bound on a unit's chunks: of the page list, the table or the caller's.
 inline long long unit_chunks(const PaArgs& a, bool listed) {
@@ -769,30 +968,32 @@ inline long long unit_chunks(const PaArgs& a, bool listed) {
 
 inline int unit_warps(const PaArgs& a, bool listed) {
     const long long units = (long long)a.B * a.Hkv * a.tiles, chunks = unit_chunks(a, listed);
+    const long long resident = (long long)pa_max_ctas(a.kp.dim, a.G) * kPaWarps;
     int W = 1;
-    while (W < kPaMaxUnitWarps && units * W * 2 <= 148 * 8 && W < chunks) W *= 2;
+    while (W < kPaMaxUnitWarps && units * W * 2 <= resident && W * 4 <= chunks) W *= 2;
+    while (!listed && W < kPaWarps && W * 12 < chunks) W *= 2;
     const long long steps = (chunks + W - 1) / W;
     const long long most = units * W < 148 * 4 ? 5 : listed ? 64 : 16;
     return steps <= most && units * W <= INT32_MAX ? W : 0;
 }
 
-template <typename T, int D, bool kListed>
+template <typename T, int D, bool kListed, bool kNarrow>
 cudaError_t launch_units(const PaArgs& a, int W, cudaStream_t s) {
-    const auto kernel = paged_attn_units_kernel<T, D, kListed>;
+    const auto kernel = paged_attn_units_kernel<T, D, kListed, kNarrow>;
     static std::atomic<unsigned long long> ready{0};      // a bit a device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PaCfg<D>::kSmem);
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PaCfg<D, kNarrow>::kSmem);
         if (e != cudaSuccess) return e;
         ready.fetch_or(1ull << dev, std::memory_order_release);
     }
     const long long warps = (long long)a.B * a.Hkv * a.tiles * W;
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr[2];
-    pdl_config(&cfg, attr, dim3((unsigned)((warps + kPaWarps - 1) / kPaWarps)), dim3(kPaThreads), PaCfg<D>::kSmem, s);
+    pdl_config(&cfg, attr, dim3((unsigned)((warps + kPaWarps - 1) / kPaWarps)), dim3(kPaThreads), PaCfg<D, kNarrow>::kSmem, s);
     if (W > kPaWarps) {
         attr[1].id = cudaLaunchAttributeClusterDimension;
         attr[1].val.clusterDim.x = W / kPaWarps;
@@ -802,20 +1003,16 @@ cudaError_t launch_units(const PaArgs& a, int W, cudaStream_t s) {
     return cudaLaunchKernelEx(&cfg, kernel, a, W);
 }
 
-template <typename T, int D, bool kListed>
+template <typename T, int D, bool kListed, bool kNarrow>
 cudaError_t launch_paged(const PaArgs& a, cudaStream_t s) {
-    if (const int W = unit_warps(a, kListed)) return launch_units<T, D, kListed>(a, W, s);
+    if (const int W = unit_warps(a, kListed)) return launch_units<T, D, kListed, kNarrow>(a, W, s);
     int ctas = 0;
-    cudaError_t e = resident_ctas<T, D, kListed>(&ctas);
+    cudaError_t e = resident_ctas<T, D, kListed, kNarrow>(&ctas);
     if (e != cudaSuccess) return e;
-    // On long units fewer warps read faster: at D = 128 1024 of the 1184 that fit
-    // took 85.3 us for 90.4 at B=32 T=4129, 86.0 for 91.2 at B=1 T=131105; short
-    // ones want all (64 sequences of up to 1000 tokens: 28.6 us, 30.3 with 1024).
-    if (unit_chunks(a, kListed) >= kPaLongUnit) ctas = std::min(ctas, PaCfg<D>::kLongCtas);
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr;
-    pdl_config(&cfg, &attr, dim3(ctas), dim3(kPaThreads), PaCfg<D>::kSmem, s);
-    e = cudaLaunchKernelEx(&cfg, paged_attn_kernel<T, D, kListed>, a);
+    pdl_config(&cfg, &attr, dim3(ctas), dim3(kPaThreads), PaCfg<D, kNarrow>::kSmem, s);
+    e = cudaLaunchKernelEx(&cfg, paged_attn_kernel<T, D, kListed, kNarrow>, a);
     if (e != cudaSuccess) return e;
     // a head a CTA while there are SMs for it, else a head a warp in small CTAs
     const int heads = a.B * a.Hq, share = heads <= kJoinShare ? 1 : 0;
@@ -826,8 +1023,8 @@ cudaError_t launch_paged(const PaArgs& a, cudaStream_t s) {
 template <typename T, bool kListed>
 cudaError_t dispatch_dim(const PaArgs& a, cudaStream_t s) {
     switch (a.kp.dim) {
-        case 64: return launch_paged<T, 64, kListed>(a, s);
-        case 128: return launch_paged<T, 128, kListed>(a, s);
+        case 64: return a.G <= 8 ? launch_paged<T, 64, kListed, true>(a, s) : launch_paged<T, 64, kListed, false>(a, s);
+        case 128: return a.G <= 8 ? launch_paged<T, 128, kListed, true>(a, s) : launch_paged<T, 128, kListed, false>(a, s);
     }
     return cudaErrorInvalidValue;
 }
@@ -840,7 +1037,7 @@ extern "C" size_t zs_paged_attention_workspace_bytes(int B, int Hq, int Hkv, int
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0) return 0;
     const long long tiles = (Hq / Hkv + kPaRows - 1) / kPaRows;
     const int prow = std::min(Hq / Hkv, kPaRows);
-    return plan_bytes((long long)B * Hkv * tiles) + ml_bytes(prow, D) + (size_t)2 * pa_max_ctas(D) * kPaWarps * prow * D * 4;
+    return plan_bytes((long long)B * Hkv * tiles) + ml_bytes(prow, D) + (size_t)2 * pa_max_ctas(D, prow) * kPaWarps * prow * D * 4;
 }
 
 namespace zs {

@@ -9,7 +9,11 @@
 //
 // Bound by HBM: q, k, v are read once and written once. A lane owns 16 channels
 // of a head (two 16-byte accesses, eight pairs), so its eight cosines and sines
-// stay in registers while its warp walks the token's heads.
+// stay in registers while its warp walks the token's heads, four passes of loads
+// ahead of their stores, both marked as read and written once. CTAs of two warps:
+// an SM takes on a new token as soon as one is done (256 threads 68.7 us, 64
+// threads 64.8 for 16411 tokens of 32 + 2 x 8 heads of 128, 412 MB, 6.36 TB/s; a
+// plain copy does 6.56). 32 tokens take 2.7 us, the launch and two dependent reads.
 #include <algorithm>
 
 #include "paged.cuh"

@@ -25,7 +25,9 @@ namespace {
 // ------------------------------------------------------------------ bounds
 // One warp reduces one page of one KV head: a lane holds 8 channels of every
 // (32 / (D / 8))-th token, running maximum and minimum as packed 16-bit pairs
-// (exact), 16-byte loads. Bound by HBM: the keys are read once.
+// (exact), 16-byte loads in full batches of eight. Bound by HBM: the keys are read
+// once. A warp a CTA, so that an SM takes new pages a warp at a time: 12 thousand
+// pages and heads of 16 KB (207 MB) in 33.4 us, 6.2 TB/s (35.7 with four warps).
 constexpr int kBoundsThreads = 32;
 constexpr int kBoundsBatch = 8;
 
@@ -183,8 +185,12 @@ __global__ void __launch_bounds__(kBoundsThreads, 32) page_bounds_kernel(const B
 // memory; that one finds the K-th largest key by histograms over the range of the
 // keys (1024 bins of it, then of the bin that holds the K-th, until a bin ends at
 // the K-th or is one key wide) and writes the chosen pages in ascending order,
-// ties to the lowest page. Scoring is bound by HBM (2 D + 4 bytes a page and
-// head), choosing by the latency of some ten barriers.
+// ties to the lowest page. Scores are 8-bit matrix products (16 heads x 32 codes x
+// 8 pages): a loop of 4-way dot products over the heads took 14 thousand cycles
+// where the products take 7.5, which is what the codes take to arrive. Bound by
+// HBM while scoring (2 D + 4 bytes a page and head), then by the latency of some
+// ten barriers: 64 of up to 2049 pages for 64 (sequence, head) pairs, 26 MB, 12 us
+// (4 of them the bytes); 48 of 513 pages for 8 pairs 5.7 us.
 constexpr int kSelectThreads = 256;
 constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kSelectMaxPages = 32768;
@@ -476,7 +482,7 @@ cudaError_t launch_select(const SelectArgs& a, int D, cudaStream_t s) {
     const int G = a.Hq / a.Hkv;
     const size_t smem = (size_t)G * 2 * D + sizeof(uint32_t) * ((size_t)a.width + 3);
     // CTAs a (sequence, KV head): as many as the GPU holds at once (two an SM), while
-    // each still has 32 pages for a part of its 16 warps
+    // each still has 64 pages for its eight warps
     int cluster = 1;
     while (cluster < kSelectMaxCluster && (long long)a.B * a.Hkv * cluster * 2 <= 296 && a.width / (2 * cluster) >= 64) cluster *= 2;
     if ((long long)a.B * a.Hkv * cluster > INT32_MAX) return cudaErrorInvalidValue;
