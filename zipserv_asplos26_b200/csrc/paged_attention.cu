@@ -604,7 +604,9 @@ __global__ void __launch_bounds__(kPaThreads, PaCfg<D, kNarrow>::kCtas) paged_at
     const long long inc = warp_prefix(mine);
     const long long total = __shfl_sync(~0u, inc, 31) * per_entry;
     const int warps = gridDim.x * kPaWarps;
-    const long long run = max(div_nonneg(total + warps - 1, warps), 1ll);
+    // two chunks or more: pieces of one would double what is joined (48 pages for 8
+    // pairs 17.5 us, 16.3 so)
+    const long long run = max(div_nonneg(total + warps - 1, warps), 2ll);
     if (blockIdx.x == 0 && tid == 0) a.plan[0] = run;
     // neighbouring runs go to different CTAs, so that few chunks spread over the SMs
     const int id = warp * (int)gridDim.x + (int)blockIdx.x;
