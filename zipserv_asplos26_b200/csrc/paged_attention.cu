@@ -19,19 +19,19 @@
 //     distributed shared memory in the same kernel: short units and page lists.
 // Sums are always in the same order: a result does not change from run to run.
 //
-// A warp copies its chunk's K and V rows with 16-byte cp.async into a ring of its
-// own, two chunks ahead (rows past the length are zero-filled and never read), so
-// there is no barrier in the loop and copies run on while a unit ends and the next
-// begins. S = Q K^T and O += P V are m16n8k16 products: the rows are query heads,
-// of which a decode step has 1 to 16 a KV head, far below a tcgen05 tile's 128;
-// the tensor pipe is busy 27% of the time with P in two parts and 12 rows unused.
-// P is fed as a 16-bit high part plus its 16-bit remainder, so that rounding P
-// adds nothing to the output's own rounding.
+// A warp copies its chunks' K and V rows with 16-byte cp.async into a ring of its
+// own, ahead of the chunk it works on (rows past the length are zero-filled and
+// never read), so there is no barrier in the loop and copies run on while a unit
+// ends and the next begins. The products are m16n8k16 ones: a decode step has 1 to
+// 16 query heads a KV head, far below a tcgen05 tile's 128 rows. Up to 8 heads they
+// are the columns (PaNarrow), up to 16 the rows (PaWide); the tensor pipe is busy
+// 14% of the time with 4 heads. P is fed as a 16-bit high part plus its 16-bit
+// remainder, so that rounding P adds nothing to the output's own rounding.
 //
-// Measured (bf16, 32 query and 8 KV heads of 128, pages of 64, us and GB/s of keys
-// and values): B=32 T=4129 84.8, 6.39 TB/s; B=1 T=131105 86.8, 6.18 TB/s; 61
-// sequences of 0..16417 with 64 query heads 308, 6.70 TB/s; B=1 T=97 4.5. A plain
-// copy does 6.56 TB/s. DRAM reads are the algorithm's bytes (541.5 MB of 541).
+// Measured in long runs, at the power cap that they reach (bf16, 32 query and 8 KV
+// heads of 128, pages of 64): B=32 T=4129 86.5 us, 6.26 TB/s; B=1 T=131105 87, 6.2;
+// 61 sequences of 0..16417 (fp16, 64 query heads, pages of 16) 314, 6.6; B=1 T=97
+// 4.7. A plain copy does 6.56 TB/s. DRAM reads are the algorithm's bytes (541.5 MB).
 #include <algorithm>
 #include <atomic>
 #include <cmath>
