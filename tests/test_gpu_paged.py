@@ -302,6 +302,8 @@ BF, HF = torch.bfloat16, torch.float16
     ([63, 64, 65, 129, 1], 32, 8, 128, 64, BF, "heads"),
     ([300], 7, 1, 128, 32, BF, "tokens"),                               # seven heads a KV head
     ([511, 2, 300], 16, 1, 64, 128, HF, "heads"),                       # a full tile of heads
+    ([100, 2049], 16, 2, 128, 64, HF, "heads"),                         # eight heads: as columns
+    ([100, 2049], 9, 1, 128, 64, BF, "tokens"),                         # nine: as rows
     ([260, 33], 40, 2, 128, 256, BF, "heads"),                          # twenty heads: two tiles
     ([77, 1000], 64, 1, 64, 16, HF, "tokens"),                          # four tiles
     ([9001], 32, 8, 128, 64, BF, "heads"),                              # one long: split over its length
