@@ -169,11 +169,12 @@ struct PaTile {
 // heads), from more warps rather than deeper rings. B=32 T=4129 in a long run under
 // the power cap: 12 warps of 2 chunks 87.3 us, 8 of 3 91.4; D = 64: 16 of 2 90.9,
 // 16 of 3 95.0, 12 of 4 95.6. The form for 16 heads holds twice the registers: 8
-// warps at D = 128 (94.6 us with 16 heads a KV head), 12 at 64.
+// warps of 2 chunks at D = 128 (90.0 us with 16 heads a KV head, 93.0 with 3), 12 of
+// 3 at 64.
 template <int D, bool kNarrow>
 struct PaCfg : PaTile<D> {
     static constexpr int kCtas = kNarrow ? (D <= 64 ? 4 : 3) : (D <= 64 ? 3 : 2);
-    static constexpr int kStages = kNarrow ? 2 : (D <= 64 ? 4 : 3);
+    static constexpr int kStages = !kNarrow && D <= 64 ? 3 : 2;
     static constexpr int kRing = kStages * 2 * PaTile<D>::kTile;   // bytes of a warp's ring
     static constexpr int kSmem = kPaWarps * kRing;
 };
