@@ -642,6 +642,42 @@ def test_listed_pages_out_of_range_are_skipped():
         assert close(out, ref, vmax, BF) and bool((out[1] == 0).all())
 
 
+# --------------------------------------------------------------- the C ABI
+def test_paged_attention_from_c():
+    """The argument struct filled by a foreign caller; a workspace that is too small is refused."""
+    import ctypes as C
+
+    from test_paged_args import STRUCTS
+    from zipserv_asplos26_b200._lib import lib
+    L = lib()
+    f, need = L.zs_paged_attention, L.zs_paged_attention_workspace
+    f.argtypes, f.restype, need.argtypes, need.restype = [C.c_char_p], C.c_int, [C.c_char_p], C.c_size_t
+    pack = STRUCTS["ZsPagedAttention"].pack
+    for lens, wants in (([100, 33], False), ([40000], True)):
+        c = Cache(lens, 2, 128, 64, BF, "heads", seed=31)
+        q = torch.randn(len(lens), 8, 128, device=DEV).to(BF)
+        want = zs().paged_attention(q, c.k, c.v, c.table, c.lens)
+        out = torch.full_like(q, 7.0)
+        pools = [x for t in (c.k, c.v) for x in (t.data_ptr(), *t.stride()[:3], *t.shape, 0)]
+
+        def args(ws, n):
+            return pack(torch.cuda.current_stream().cuda_stream, q.data_ptr(), c.table.data_ptr(), c.table.stride(0),
+                        c.lens.data_ptr(), 0, 0, ws, n, out.data_ptr(), 0, 0, *pools, len(lens), 8, c.table.shape[1],
+                        0, 128 ** -0.5, 0)
+
+        n = need(args(0, 0))
+        assert (n > 0) == wants
+        if n:
+            ws = torch.empty(n, dtype=torch.uint8, device=DEV)
+            assert f(args(ws.data_ptr(), n - 1)) == 1 and f(args(0, n)) == 1
+            torch.cuda.synchronize()
+            assert bool((out == 7).all())
+            assert f(args(ws.data_ptr(), n)) == 0
+        else:
+            assert f(args(0, 0)) == 0
+        assert torch.equal(out, want)
+
+
 # ----------------------------------------------------------------- the cache
 def test_cache_steps_in_a_graph():
     """Prompts, then decode steps replayed from one CUDA graph, one request ending
