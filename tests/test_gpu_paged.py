@@ -128,6 +128,25 @@ def test_plan_step_large_asks_are_refused():
     assert p.cu_tokens.tolist() == [0, 0, 0, 0] and p.free_count.item() == 2
 
 
+def test_plan_step_lengths_end_below_31_bits():
+    """A table of more than 2**31 tokens: a request grows up to the last whole page below that, and not past it."""
+    page, width = 256, (1 << 23) + 4
+    start = (1 << 31) - 300
+    table = torch.zeros(2, width, dtype=torch.int32, device=DEV)
+    table[0, start // page] = 7
+    for new, refused in ((44, False), (45, True), (600, True)):
+        err = torch.zeros(1, dtype=torch.int32, device=DEV)
+        p = zs().plan_step(table, i32([start, 0]), i32([new, 1]), i32(np.arange(64)), i32([64]), page, 1024, err=err)
+        assert p.refused.tolist() == [refused, False]
+        assert p.seq_lens.tolist() == [start + (0 if refused else new), 1]
+        assert p.free_count.item() == 63 and err.item() == (4 if refused else 0)
+        n = p.cu_tokens[-1].item()
+        assert n == (1 if refused else new + 1)
+        if not refused:
+            assert p.positions[:new].tolist() == list(range(start, start + new))
+            assert p.slots[:new].tolist() == [7 * page + x % page for x in range(start, start + new)]
+
+
 def test_plan_step_free_list_overflow_is_flagged():
     """A free list that claims more entries than its buffer holds stays in bounds."""
     table, free = i32([[0, 1], [2, 3]]), i32([9, 8, 7])

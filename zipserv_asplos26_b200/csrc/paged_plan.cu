@@ -104,6 +104,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     int* lens = need0 + R;             // [R] lengths before the step
     int* fresh = lens + R;             // [R] tokens asked for, negative: ended
     const int count_in = *a.count;
+    // what a row of the table holds, and a position can be
     const int len_cap = (int)min((long long)a.width << sh, (long long)INT_MAX - P1);
     for (int r = threadIdx.x; r < R; r += kPlanThreads) {
         lens[r] = max(0, min(a.lens[r], len_cap));
@@ -127,9 +128,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     // 2. pages needed by the requests that fit the step and the table
     auto pages_needed = [&](int r, long long want_end) -> int {
         const int f = fresh[r], len = lens[r];
-        const long long pages = ((long long)len + max(f, 0) + P1) >> sh;
-        if (f < 0 || want_end > a.max_tokens || pages > a.width) return -1;
-        return (int)(pages - ((len + P1) >> sh));
+        const long long end = (long long)len + max(f, 0);
+        if (f < 0 || want_end > a.max_tokens || end > len_cap) return -1;
+        return (int)(((end + P1) >> sh) - ((len + P1) >> sh));
     };
     long long need[1] = {0}, need_total[1];
     long long w = want;
