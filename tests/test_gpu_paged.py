@@ -649,6 +649,32 @@ def test_sparse_attention(lens, hq, hkv, D, page, top, dtype, layout):
     assert bool(((lse == -math.inf) == (c.lens == 0).unsqueeze(1)).all())
 
 
+def test_calls_of_different_sizes_from_two_threads():
+    """The shared memory that a call needs goes by its sizes; another thread's call must not take it away."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    def select(width):
+        torch.manual_seed(width)
+        codes = torch.randint(-127, 128, (64, 1, 2, 64), dtype=torch.int8, device=DEV)
+        scales = torch.ones(64, 1, device=DEV)
+        table = torch.randint(0, 64, (1, width), dtype=torch.int32, device=DEV)
+        q = torch.randn(1, 4, 64, dtype=torch.bfloat16, device=DEV)
+        args = (q, codes, scales, table, i32([width * 16]), 16, 32)
+        first = zs().select_pages(*args)[0].clone()
+        same = [torch.equal(zs().select_pages(*args)[0], first) for _ in range(200)]
+        return all(same)
+
+    def plan(R):
+        for _ in range(200):
+            p = zs().plan_step(torch.zeros(R, 1, dtype=torch.int32, device=DEV), i32([0] * R), i32([1] * R),
+                               i32(np.arange(R)), i32([R]), 16, 16)
+        return p.cu_tokens[-1].item() == 16
+
+    for f, sizes in ((select, (12000, 32768)), (plan, (3000, 8192))):
+        with ThreadPoolExecutor(2) as pool:
+            assert all(pool.map(f, sizes))
+
+
 def test_listed_pages_out_of_range_are_skipped():
     """Entries of a caller's page list that name no page of the sequence count nothing."""
     c = Cache([100, 40], 1, 64, 16, BF, "heads", 8)

@@ -253,8 +253,9 @@ extern "C" int zs_plan_step(const ZsPlanStep* p) {
                reinterpret_cast<long long*>(p->slots), p->token_seq, p->positions, p->refused, p->err};
     while ((1 << a.page_shift) < page_size) ++a.page_shift;
     const size_t smem = sizeof(int) * (5 * (size_t)R + 2);
-    if (smem > 40 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (smem > 40 * 1024) {    // the same limit every time: threads may call with different sizes
+        const cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (int)sizeof(int) * (5 * kPlanMaxRequests + 2));
         if (e != cudaSuccess) return e;
     }
     // a thread a token, with some more for pages

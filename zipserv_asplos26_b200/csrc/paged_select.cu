@@ -487,8 +487,9 @@ cudaError_t launch_select(const SelectArgs& a, int D, cudaStream_t s) {
     while (cluster < kSelectMaxCluster && (long long)a.B * a.Hkv * cluster * 2 <= 296 && a.width / (2 * cluster) >= 64) cluster *= 2;
     if ((long long)a.B * a.Hkv * cluster > INT32_MAX) return cudaErrorInvalidValue;
     auto go = [&](auto kernel) -> cudaError_t {
-        if (smem > 40 * 1024) {
-            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (smem > 40 * 1024) {    // the same limit every time: threads may call with different sizes
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                       kSelectMaxGroup * 2 * D + 4 * (kSelectMaxPages + 3));
             if (e != cudaSuccess) return e;
         }
         cudaLaunchConfig_t cfg;
