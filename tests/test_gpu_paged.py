@@ -848,6 +848,8 @@ def test_refusals_on_the_gpu():
     p = z.plan_step(table, lens, lens, free, one, 16, 6)
     with pytest.raises(ValueError):
         z.plan_step(table, p.seq_lens, lens, free, one, 16, 6, out=p)          # lengths in place
+    with pytest.raises(ValueError):
+        z.plan_step(table, lens, p.seq_lens, free, one, 16, 6, out=p)          # over what is asked for
     cs = torch.zeros(5, 64, device=DEV)
     k = torch.zeros(1, 2, 64, device=DEV, dtype=BF)
     slot = torch.zeros(1, dtype=torch.int64, device=DEV)

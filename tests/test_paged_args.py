@@ -91,6 +91,18 @@ def test_null_and_bad_arguments_are_refused(zlib):
                                                           0, 4, 8, 0)) == 0          # no sequences: nothing to do
 
 
+def test_plan_outputs_are_other_buffers(zlib):
+    """Every thread block reads lengths, asks and count, so none of them may be written."""
+    a = 1 << 20
+    names = ("table", "seq_lens", "new_lens", "free_blocks", "free_count", "out_lens", "out_count")
+    for same in (("out_lens", "seq_lens"), ("out_lens", "new_lens"), ("out_count", "free_count")):
+        at = {n: a + 4096 * i for i, n in enumerate(names)}
+        at[same[0]] = at[same[1]]
+        args = STRUCTS["ZsPlanStep"].pack(0, at["table"], 4, at["seq_lens"], at["new_lens"], at["free_blocks"],
+                                          at["free_count"], at["out_lens"], at["out_count"], *[2 * a] * 5, 0, 1, 4, 8, 16, 8, 0)
+        assert _fn(zlib, "zs_plan_step")(args) == 1, same
+
+
 def test_workspace_bytes(zlib):
     f = _fn(zlib, "zs_paged_attention_workspace_bytes", [C.c_int] * 4, C.c_size_t)
     assert f(0, 32, 8, 128) == 0 and f(1, 30, 8, 128) == 0

@@ -243,7 +243,7 @@ PyObject* plan_step(PyObject* const* a) {
         p.token_seq = vec<int>(item(4), room, at::kInt, "out.token_seq", index);
         p.positions = vec<int>(item(5), room, at::kInt, "out.positions", index);
         p.refused = vec<uint8_t>(item(6), R, at::kBool, "out.refused", index);
-        need(p.out_lens != p.seq_lens && p.out_count != p.free_count,
+        need(p.out_lens != p.seq_lens && p.out_lens != p.new_lens && p.out_count != p.free_count,
              "out.seq_lens and out.free_count must be other buffers than the inputs");
         call(zs_plan_step, p, "zs_plan_step");
         Py_INCREF(a[7]);

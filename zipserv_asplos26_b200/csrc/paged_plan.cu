@@ -247,7 +247,8 @@ extern "C" int zs_plan_step(const ZsPlanStep* p) {
         !p->out_count || !p->out_cu || !p->refused || (max_tokens && (!p->slots || !p->token_seq || !p->positions)))
         return cudaErrorInvalidValue;
     // every CTA repeats the prefix sums from these; the outputs are other buffers
-    if (p->out_lens == p->seq_lens || p->out_count == p->free_count) return cudaErrorInvalidValue;
+    if (p->out_lens == p->seq_lens || p->out_lens == p->new_lens || p->out_count == p->free_count)
+        return cudaErrorInvalidValue;
     PlanArgs a{p->block_table, p->table_stride, R, p->width, 0, max_tokens, p->capacity, p->seq_lens, p->new_lens,
                p->free_blocks, p->free_count, p->out_lens, p->out_count, p->out_cu,
                reinterpret_cast<long long*>(p->slots), p->token_seq, p->positions, p->refused, p->err};
