@@ -687,6 +687,19 @@ def test_listed_pages_out_of_range_are_skipped():
         assert close(out, ref, vmax, BF) and bool((out[1] == 0).all())
 
 
+@pytest.mark.parametrize("page, flagged", ((-1, 2), (8, 2), (500, 2), (7, 0)))
+def test_listed_pages_outside_the_table_are_flagged(page, flagged):
+    """A page past the length but inside the table counts nothing and is no error."""
+    c = Cache([100, 40], 1, 64, 16, BF, "heads", 8)
+    table = c.table[:, :8]
+    q = torch.randn(2, 2, 64, device=DEV).to(BF)
+    for top in (4, 4096):
+        err = torch.zeros(1, dtype=torch.int32, device=DEV)
+        pages = torch.full((2, 1, top), page, dtype=torch.int32, device=DEV)
+        out = zs().paged_attention(q, c.k, c.v, table, c.lens, pages=pages, counts=i32([[1], [1]]), err=err)
+        assert bool((out == 0).all()) and err.item() == flagged
+
+
 # --------------------------------------------------------------- the C ABI
 def test_paged_attention_from_c():
     """The argument struct filled by a foreign caller; a workspace that is too small is refused."""

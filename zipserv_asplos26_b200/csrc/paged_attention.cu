@@ -188,7 +188,10 @@ __device__ __forceinline__ void look_chunk(const PaArgs& a, int e, int b, int ch
     int p = ch >> cps;
     if (kListed) p = a.pages[(long long)e * a.top + p];
     id = lim = 0;
-    if (p < 0 || p >= a.width) return;
+    if (p < 0 || p >= a.width) {
+        set_err(a.err, kErrPagedIndex);
+        return;
+    }
     const int t0 = ((p << cps) + (ch & ((1 << cps) - 1))) * kPaChunk;
     if (t0 >= len) return;
     const int blk = a.table[b * a.table_stride + p];
