@@ -253,13 +253,16 @@ typedef struct ZsPagePool {
  * back at its end in order of request and page, then taken from its end. In
  * request order, a request is admitted when the tokens asked for up to and
  * including it are at most max_tokens (<= 2^30), its pages fit the table's width,
- * and the pages needed up to and including it are free; one that is not admitted
- * keeps its state, is marked in `refused` and sets bit 4 in *err. Outputs:
+ * and the pages needed up to and including it are free (what a refused request asks
+ * for counts too, pages only where its tokens and length fit); one that is not
+ * admitted keeps its state, is marked in `refused` and sets bit 4 in *err. Outputs:
  * out_lens [R], *out_count, out_cu [R + 1] (prefix sums of the admitted tokens),
  * refused [R], and for each of max_tokens tokens its slot (block * page_size +
  * row), request and position (-1, -1 and 0 past the last). block_table and
  * free_blocks are updated in place; seq_lens and free_count are not (out_lens
- * and out_count are other buffers), so a repeated call gives the same result. */
+ * and out_count are other buffers than any input), so a repeated call gives the
+ * same result. Lengths are at most what a row of the table holds, below 2^31: one
+ * that comes in longer counts as that. */
 typedef struct ZsPlanStep {
     void* stream;
     int* block_table;
@@ -286,8 +289,9 @@ int zs_plan_step(const ZsPlanStep* args);
  * channels turn, in pairs (j, j + rot / 2) or (2j, 2j + 1) when interleaved, pair
  * j by row positions[axis * pos_axis + n] of cos_sin [table_rows][rot] fp32 (rot
  * / 2 cosines, then rot / 2 sines), axis the one of the `axes` (1..4) sections
- * (sum rot / 2) that j falls in. Slots of -1 are skipped; the slots of one call
- * are distinct. D is a multiple of 16, up to 512. */
+ * (sum rot / 2) that j falls in (a row out of range counts as 0 and sets bit 2 in
+ * *err). Slots of -1 are skipped; the slots of one call are distinct. D is a
+ * multiple of 16, up to 512. */
 typedef struct ZsRopeWrite {
     void* stream;
     const uint16_t *q, *k, *v;
@@ -310,8 +314,9 @@ int zs_rope_write(const ZsRopeWrite* args);
  * tokens of the listed pages count. A sequence with nothing to attend gets zeros.
  * lse (nullable, [B][Hq]) receives log sum exp(softmax_scale q.k), -inf where
  * nothing counts. max_seqlen: a bound on seq_lens where the host has one closer
- * than the table's width (0: none); it chooses between two kernels and no result
- * depends on it. ws: 16-byte aligned workspace of ws_bytes, at least what
+ * than the table's width (0: none); it chooses between two kernels, whose results
+ * differ by the order of fp32 sums. Lengths count up to the table's width. ws:
+ * 16-byte aligned workspace of ws_bytes, at least what
  * zs_paged_attention_workspace returns for the same arguments (0: none is read);
  * zs_paged_attention_workspace_bytes is enough for every call of these sizes. */
 typedef struct ZsPagedAttention {
@@ -338,9 +343,10 @@ int zs_paged_attention(const ZsPagedAttention* args);
 
 /* Bounds of the pages that sequences completed between lens_before[b] and
  * seq_lens[b] tokens (at most max_new tokens each and, unless it is 0, max_total in
- * all; the bounds size the grid): codes [num_blocks][num_heads][2][D] int8 (16-byte aligned), upper then lower bound of the keys per channel in
- * units of scales [num_blocks][num_heads], a power of two (infinite, with codes
- * of zero, for a page with a non-finite key). D is 64, 128 or 256. */
+ * all; the bounds size the grid): codes [num_blocks][num_heads][2][D] int8 (16-byte
+ * aligned), upper then lower bound of the keys per channel in units of scales
+ * [num_blocks][num_heads], a power of two (infinite, with codes of zero, for a page
+ * with a non-finite key). D is 64, 128 or 256. */
 typedef struct ZsPageBounds {
     void* stream;
     const int* block_table;

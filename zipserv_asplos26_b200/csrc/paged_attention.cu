@@ -17,7 +17,8 @@
 //     workspace, and paged_join_kernel joins a unit's pieces in order.
 //   * paged_attn_units_kernel: a fixed number of warps a unit, joined through
 //     distributed shared memory in the same kernel: short units and page lists.
-// Sums are always in the same order: a result does not change from run to run.
+// Sums are always in the same order for the same sizes on the host and the same
+// lengths: a result does not change from run to run.
 //
 // A warp copies its chunks' K and V rows with 16-byte cp.async into a ring of its
 // own, ahead of the chunk it works on (rows past the length are zero-filled and
@@ -56,7 +57,7 @@ struct PaArgs {
     const int* pages;         // nullable: [B][Hkv][top]
     const int* counts;        // with pages: [B][Hkv]
     int B, Hq, Hkv, G, tiles, width, top;
-    int max_len;              // host's bound on the lengths, 0: none (chooses the way, no result depends on it)
+    int max_len;              // host's bound on the lengths, 0: none (chooses the way, and so the order of sums)
     float scale2;             // softmax scale * log2(e)
     uint16_t* out;            // [B][Hq][D]
     float* lse;               // nullable: [B][Hq]

@@ -19,8 +19,8 @@ bf16 or fp16, its last axis contiguous and the others of any strides that are
 multiples of 8 elements: `torch.empty(blocks, heads, page, dim).transpose(1, 2)`
 keeps each head's rows of a page together. Every call runs on the current
 stream of its tensors' device and synchronises nothing. `err` (optional, int32[1])
-collects error bits: 2 = an index was out of range and skipped, 4 = a request
-was refused by plan_step.
+collects error bits: 2 = an index was out of range (skipped; a position: taken as
+0), 4 = a request was refused by plan_step.
 """
 from __future__ import annotations
 
@@ -69,8 +69,9 @@ def plan_step(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch
 
     Request r has seq_lens[r] tokens and gets new_lens[r] more (negative: it has
     ended and its pages return to the free list). A request is admitted, in
-    order, when its tokens fit max_tokens, its pages fit the table's width and
-    enough pages are free; otherwise it keeps its state and is marked refused.
+    order, when the tokens asked for up to it fit max_tokens, its pages fit the
+    table's width and the pages needed up to it are free; otherwise it keeps its
+    state and is marked refused.
     block_table and free_blocks (a stack, its first free_count[0] entries) are
     updated in place; the new lengths and count are returned."""
     return (_native or _load()).plan_step(block_table, seq_lens, new_lens, free_blocks, free_count, page_size,
@@ -109,7 +110,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     attend gets zeros. lse (optional, fp32 [B, Hq]) receives the log of the sum
     of exponentials of the scaled scores. max_seqlen is a bound on seq_lens that
     the host may have (else the table's width is one); only the choice of the
-    kernel depends on it: short sequences want a close one."""
+    kernel, and with it the order of sums, depends on it: short sequences want a
+    close one. Lengths count up to the table's width."""
     o = (_native or _load()).paged_attention(q, k_pages, v_pages, block_table, seq_lens, softmax_scale, pages, counts,
                                              out, lse, max_seqlen, err)
     return o if q.dim() == 3 and out is None else o.view(q.shape)
