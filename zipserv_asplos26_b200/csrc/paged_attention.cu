@@ -27,7 +27,10 @@
 // 16 query heads a KV head, far below a tcgen05 tile's 128 rows. Up to 8 heads they
 // are the columns (PaNarrow), up to 16 the rows (PaWide); the tensor pipe is busy
 // 14% of the time with 4 heads. P is fed as a 16-bit high part plus its 16-bit
-// remainder, so that rounding P adds nothing to the output's own rounding.
+// remainder (at most 2^-16 of a bf16 weight is left out, 2^-22 of an fp16 one), so that
+// rounding P adds nothing to the output's own rounding. An infinite value would meet a
+// remainder of zero or of the other sign there and give NaN: outputs that are not finite
+// are looked at again (odd_values).
 //
 // Measured in long runs, at the power cap that they reach (bf16, 32 query and 8 KV
 // heads of 128, pages of 64): B=32 T=4129 86.5 us, 6.26 TB/s; B=1 T=131105 87, 6.2;
@@ -36,6 +39,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -225,6 +229,49 @@ __device__ __forceinline__ void copy_chunk(const PaArgs& a, uint32_t dst, int bl
     }
 }
 
+// A weight of a finite score is positive, however small, so an output channel whose
+// values include an infinity is that infinity, and NaN only where they include both
+// signs or a NaN. The products cannot tell (0 * inf is NaN, and the remainder of a
+// weight may be zero or negative), so where a finished output is not finite although
+// the sum of its weights is a number, the unit's values are read once more. Returns
+// for each of the kCount channels from c0 on three bits: an infinity is there, a
+// negative one, a NaN. Nothing of this runs while outputs are finite; to see that they
+// are costs 0.05 us of 4.0 at B=1 T=97 and nothing in long runs.
+template <typename T, int kCount, bool kListed>
+__device__ __forceinline__ uint32_t odd_values(const PaArgs& a, int e, int b, int h, int n, int c0) {
+    constexpr uint32_t kInf = std::is_same<T, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;
+    const int len = min(a.lens[b], (int)min((long long)a.width << a.kp.page_shift, (long long)INT_MAX));
+    const uint16_t* base = static_cast<const uint16_t*>(a.vp.data) + h * a.vp.s_head + c0;
+    uint32_t seen = 0;
+#pragma unroll 1
+    for (int ch = 0; ch < n; ++ch) {
+        int blk, lim;
+        look_chunk<kListed>(a, e, b, ch, len, blk, lim);
+        const int row0 = (ch & ((1 << (a.kp.page_shift - 4)) - 1)) * kPaChunk;
+        const uint16_t* v = base + blk * a.vp.s_block + row0 * a.vp.s_token;
+#pragma unroll 4
+        for (int r = 0; r < kPaChunk; ++r) {
+            if (r >= lim) break;
+            uint32_t w[2] = {0u, 0u};
+            if constexpr (kCount == 4) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(v + r * a.vp.s_token);
+            else w[0] = *reinterpret_cast<const uint32_t*>(v + r * a.vp.s_token);
+#pragma unroll
+            for (int j = 0; j < kCount; ++j) {
+                const uint32_t x = w[j / 2] >> (j % 2 * 16) & 0xFFFFu, mag = x & 0x7FFFu;
+                seen |= (mag > kInf ? 4u : mag < kInf ? 0u : x >> 15 ? 2u : 1u) << (3 * j);
+            }
+        }
+    }
+    return seen;
+}
+// The output of the j-th of these channels; o where nothing odd is among its values.
+__device__ __forceinline__ float odd_output(uint32_t seen, int j, float o) {
+    const uint32_t f = seen >> (3 * j) & 7u;
+    return f == 1 ? INFINITY : f == 2 ? -INFINITY : f ? NAN : o;
+}
+// Whether an output is not finite although the sum of its weights, l, is a number.
+__device__ __forceinline__ bool is_odd(float sum_of_zeros, float l) { return isnan(sum_of_zeros) && !isnan(l); }
+
 // What a warp holds of a unit: q as product fragments, running maximum (base 2),
 // sum and output. Two forms: 16 heads as the rows of S and O (here; a lane has rows
 // lane / 4 and lane / 4 + 8), or up to 8 heads as the columns of S^T and O^T.
@@ -350,6 +397,29 @@ struct PaWide {
             l[r] += __shfl_xor_sync(~0u, l[r], 1);
             l[r] += __shfl_xor_sync(~0u, l[r], 2);
         }
+    }
+    // Whether any lane's output is odd, and the odd ones from what each lane saw of D / 32 channels.
+    __device__ __forceinline__ bool odd() const {
+        float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};       // short chains
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+            x[i % 2 * 2] += o[i][0] * 0.f;
+            x[i % 2 * 2 + 1] += o[i][1] * 0.f;
+            y[i % 2 * 2] += o[i][2] * 0.f;
+            y[i % 2 * 2 + 1] += o[i][3] * 0.f;
+        }
+        return __any_sync(~0u, is_odd((x[0] + x[1]) + (x[2] + x[3]), l[0]) || is_odd((y[0] + y[1]) + (y[2] + y[3]), l[1]));
+    }
+    __device__ __forceinline__ void mend(uint32_t seen) {
+        const int d0 = (threadIdx.x & 3) * 2;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = i * 8 + d0 + (j & 1);
+                const float x = odd_output(__shfl_sync(~0u, seen, c / (D / 32)), c % (D / 32), o[i][j]);
+                if (!isnan(l[j >> 1])) o[i][j] = x;
+            }
     }
     // The finished rows, to the output [rows][D].
     __device__ __forceinline__ void write(uint16_t* out, float* lse, int rows) const {
@@ -483,6 +553,28 @@ struct PaNarrow {
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int k = 4; k < 32; k <<= 1) l[j] += __shfl_xor_sync(~0u, l[j], k);
+    }
+    __device__ __forceinline__ bool odd() const {
+        float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            x[i % 2 * 2] += o[i][0] * 0.f;
+            x[i % 2 * 2 + 1] += o[i][2] * 0.f;
+            y[i % 2 * 2] += o[i][1] * 0.f;
+            y[i % 2 * 2 + 1] += o[i][3] * 0.f;
+        }
+        return __any_sync(~0u, is_odd((x[0] + x[1]) + (x[2] + x[3]), l[0]) || is_odd((y[0] + y[1]) + (y[2] + y[3]), l[1]));
+    }
+    __device__ __forceinline__ void mend(uint32_t seen) {
+        const int d0 = (threadIdx.x & 31) >> 2;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = i * 16 + (j >> 1) * 8 + d0;
+                const float x = odd_output(__shfl_sync(~0u, seen, c / (D / 32)), c % (D / 32), o[i][j]);
+                if (!isnan(l[j & 1])) o[i][j] = x;
+            }
     }
     __device__ __forceinline__ void write(uint16_t* out, float* lse, int rows) const {
         const int lane = threadIdx.x & 31, d0 = lane >> 2;
@@ -710,8 +802,11 @@ __global__ void __launch_bounds__(kPaThreads, PaCfg<D, kNarrow>::kCtas) paged_at
         const bool whole = first == 0 && count == cur.n;
         const long long slot = 2ll * id + (s == count ? 0 : 1);       // the run's first part, or its last
         st.finish();
-        if (whole) st.write(a.out + head0 * D, a.lse ? a.lse + head0 : nullptr, rows);
-        else st.park(a.part_o + slot * a.prow * D, a.part_ml + slot * a.prow * 2, rows);
+        if (whole) {
+            if (__builtin_expect(st.odd(), false))
+                st.mend(odd_values<T, D / 32, kListed>(a, cur.e, b, h, cur.n, lane * (D / 32)));
+            st.write(a.out + head0 * D, a.lse ? a.lse + head0 : nullptr, rows);
+        } else st.park(a.part_o + slot * a.prow * D, a.part_ml + slot * a.prow * 2, rows);
         if (s == steps) break;
         u_lo += cur.n;
         next_unit<kListed>(a, per_entry, cur);
@@ -817,6 +912,13 @@ __global__ void __launch_bounds__(kPaThreads, PaCfg<D, kNarrow>::kCtas) paged_at
             }
             m = mn;
         }
+        if (__builtin_expect(is_odd((acc.x * 0.f + acc.y * 0.f) + (acc.z * 0.f + acc.w * 0.f), l), false)) {
+            const uint32_t seen = odd_values<T, 4, kListed>(a, e, b, h, n, d4);
+            acc.x = odd_output(seen, 0, acc.x);
+            acc.y = odd_output(seen, 1, acc.y);
+            acc.z = odd_output(seen, 2, acc.z);
+            acc.w = odd_output(seen, 3, acc.w);
+        }
         const float inv = l == 0.f ? 0.f : 1.f / l;
         *reinterpret_cast<uint2*>(a.out + (head0 + row) * D + d4) =
             make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
@@ -914,6 +1016,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PaArg
 #pragma unroll
             for (int j = 0; j < kVec; ++j) acc[j] += s_acc[w][lane * kVec + j] * f;
         }
+    }
+    float zeros = 0.f;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) zeros += acc[j] * 0.f;
+    if (__builtin_expect(is_odd(zeros, l), false)) {
+        const uint32_t seen = odd_values<T, kVec, kListed>(a, kListed ? b * a.Hkv + h : b, b, h, n, lane * kVec);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) acc[j] = odd_output(seen, j, acc[j]);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     uint32_t* out = reinterpret_cast<uint32_t*>(a.out + (long long)head * D + lane * kVec);
