@@ -105,12 +105,15 @@ def run(steps=48, top=0, prompts=(33, 120, 7), seed=0, page=16):
     tokens = first.clone()                                     # static input of the graph: row r's last token
     ones = torch.ones(rows, dtype=torch.int32, device="cuda")
 
-    def decode(layer, q, cache):
-        # every row has one token, in order of rows
-        return cache.sparse_attention(q, top, layer)[0] if top else cache.attention(q, layer)
-
     def step():
         plan = cache.step(ones, rows)
+        own = cache.token_rows(plan)                           # each token attends its own row
+
+        def decode(layer, q, cache):
+            if top:
+                return cache.sparse_attention(q, top, layer, rows=own)[0]
+            return cache.attention(q, layer, rows=own)
+
         return model.forward(tokens, plan, cache, decode)
 
     state = [cache.seqlens, cache.free_count, cache.block_table, cache.free_blocks]

@@ -152,15 +152,26 @@ def sparse_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
 
 
 # ------------------------------------------------------------------- cache
+class TokenRows(NamedTuple):
+    """What each token of a plan attends: the pages of its row, up to itself."""
+    block_table: torch.Tensor   # int32 [tokens, max_blocks_per_seq]
+    seq_lens: torch.Tensor      # int32 [tokens], 0 past the plan's last token
+
+
 class PagedKVCache:
     """Buffers of an uncompressed paged cache of num_layers layers for up to
     max_batch sequences of up to max_blocks_per_seq pages, and a step's calls on
-    them (one plan a step, the others a layer):
+    them (a plan and its rows a step, the others a layer):
 
-        plan = cache.step(new_lens, max_tokens)          # tokens of each row; -1: ended
-        q = cache.write(q, k, v, cos_sin, plan, layer)   # rotary, then into the pages
-        o = cache.attention(q_last, layer)               # one new token per row
-        o = cache.sparse_attention(q_last, 64, layer)    # over 64 pages per KV head
+        plan = cache.step(new_lens, max_tokens)            # tokens of each row; -1: ended
+        rows = cache.token_rows(plan)                      # what each token attends
+        q = cache.write(q, k, v, cos_sin, plan, layer)     # rotary, then into the pages
+        o = cache.attention(q, layer, rows=rows)           # output of each token
+        o = cache.sparse_attention(q, 64, layer, rows=rows)[0]   # over 64 pages per KV head
+
+    A plan holds the admitted tokens one after another, so its i-th token belongs
+    to row plan.token_seq[i], not to row i: without `rows` the attention calls
+    take one query per row instead, in order of rows.
 
     All state (tables, lengths, the free list) is on the GPU in fixed buffers, so
     a step can be captured in a CUDA graph and replayed. layout "heads" keeps
@@ -229,23 +240,37 @@ class PagedKVCache:
                         self.scales[layer], n, n, self.err)
         return q
 
+    def token_rows(self, plan: StepPlan) -> TokenRows:
+        """The rows that the tokens of the last step's plan attend (causal: a token
+        sees its row up to itself). For decode steps and short pieces of prompts:
+        a row of the table is copied for each token, and attention reads a
+        sequence's pages once for each of its tokens."""
+        table = self.block_table.index_select(0, plan.token_seq.clamp(min=0))
+        return TokenRows(table, (plan.positions + 1).masked_fill_(plan.token_seq < 0, 0))
+
+    def _rows(self, q, rows):
+        return rows if rows is not None else (self.block_table[:q.shape[0]], self.seqlens[:q.shape[0]])
+
     def attention(self, q: torch.Tensor, layer: int = 0, softmax_scale: Optional[float] = None,
                   out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
-                  max_seqlen: Optional[int] = None) -> torch.Tensor:
-        """Attention of q [B, Hq, D] over rows 0 .. B-1 (max_seqlen: see paged_attention)."""
-        B = q.shape[0]
-        return paged_attention(q, self.k[layer], self.v[layer], self.block_table[:B], self.seqlens[:B], softmax_scale,
-                               None, None, out, lse, max_seqlen, self.err)
+                  max_seqlen: Optional[int] = None, rows: Optional[TokenRows] = None) -> torch.Tensor:
+        """Attention of q [N, Hq, D], the plan's tokens with rows=token_rows(plan);
+        without rows q is one query per row, of rows 0 .. N-1 (max_seqlen: see
+        paged_attention)."""
+        table, lens = self._rows(q, rows)
+        return paged_attention(q, self.k[layer], self.v[layer], table, lens, softmax_scale, None, None, out, lse,
+                               max_seqlen, self.err)
 
     def sparse_attention(self, q: torch.Tensor, top_pages: int, layer: int = 0, sink_pages: int = 1,
-                         local_pages: int = 1, softmax_scale: Optional[float] = None):
-        """Attention of q [B, Hq, D] over top_pages chosen pages of rows 0 .. B-1: (out, pages, counts)."""
+                         local_pages: int = 1, softmax_scale: Optional[float] = None,
+                         rows: Optional[TokenRows] = None):
+        """Attention of q over top_pages chosen pages per KV head (q and rows as for
+        attention): (out, pages, counts)."""
         if self.codes is None:
             raise RuntimeError("the cache was made without bounds")
-        B = q.shape[0]
-        return sparse_attention(q, self.k[layer], self.v[layer], self.codes[layer], self.scales[layer],
-                                self.block_table[:B], self.seqlens[:B], top_pages, sink_pages, local_pages,
-                                softmax_scale, None, self.err)
+        table, lens = self._rows(q, rows)
+        return sparse_attention(q, self.k[layer], self.v[layer], self.codes[layer], self.scales[layer], table, lens,
+                                top_pages, sink_pages, local_pages, softmax_scale, None, self.err)
 
     def check_errors(self) -> int:
         """Error bits recorded by the kernels (synchronises)."""
