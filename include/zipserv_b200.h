@@ -285,13 +285,14 @@ int zs_plan_step(const ZsPlanStep* args);
 
 /* Rotary positions on q and k, and k and v to their slots. q is [N][Hq][D], k
  * and v [N][Hkv][D] with token and head strides in elements (multiples of 8);
- * q_out [N][Hq][D] contiguous (may be q). The first `rot` (a multiple of 16)
- * channels turn, in pairs (j, j + rot / 2) or (2j, 2j + 1) when interleaved, pair
- * j by row positions[axis * pos_axis + n] of cos_sin [table_rows][rot] fp32 (rot
- * / 2 cosines, then rot / 2 sines), axis the one of the `axes` (1..4) sections
- * (sum rot / 2) that j falls in (a row out of range counts as 0 and sets bit 2 in
- * *err). Slots of -1 are skipped; the slots of one call are distinct. D is a
- * multiple of 16, up to 512. */
+ * q_out [N][Hq][D] is contiguous: q itself where that is contiguous too, else
+ * apart from q, k and v, which is checked; none of the four lies in the pools. The
+ * first `rot` (a multiple of 16) channels turn, in pairs (j, j + rot / 2) or (2j,
+ * 2j + 1) when interleaved, pair j by row positions[axis * pos_axis + n] of cos_sin
+ * [table_rows][rot] fp32 (rot / 2 cosines, then rot / 2 sines), axis the one of the
+ * `axes` (1..4) sections (sum rot / 2) that j falls in (a row out of range counts
+ * as 0 and sets bit 2 in *err). Slots of -1 are skipped; the slots of one call are
+ * distinct. D is a multiple of 16, up to 512. */
 typedef struct ZsRopeWrite {
     void* stream;
     const uint16_t *q, *k, *v;

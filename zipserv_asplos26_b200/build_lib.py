@@ -81,7 +81,7 @@ def build(verbose: bool = False) -> str:
 
 def _build_binding(verbose: bool) -> str:
     src = os.path.join(CSRC, "binding", "paged_bind.cpp")
-    if not _stale(BINDING, [src, LIB, os.path.join(INCLUDE, "zipserv_b200.h")]):
+    if not _stale(BINDING, [src, LIB, os.path.join(INCLUDE, "zipserv_b200.h"), os.path.join(CSRC, "rows_meet.h")]):
         return BINDING
     import sysconfig
 

@@ -15,6 +15,7 @@
 #include <cmath>
 #include <string>
 
+#include "../rows_meet.h"
 #include "zipserv_b200.h"
 
 namespace {
@@ -340,6 +341,9 @@ PyObject* rope_write(PyObject* const* a) {
         need(out.sizes() == q.sizes() && out.scalar_type() == pools.type && out.is_cuda() &&
                  out.get_device() == index && out.is_contiguous() && aligned16(out),
              "q_out must be contiguous, aligned and of q's shape and type");
+        need(zs::q_out_is_apart(out.data_ptr(), N, q.size(1), k.size(1), dim, q.data_ptr(), q.stride(0), q.stride(1),
+                                k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1)),
+             "q_out must be a contiguous q itself, or apart from q, k and v");
     } else {
         out = fresh({N, q.size(1), dim}, pools.type, index);
     }

@@ -17,6 +17,7 @@
 #include <algorithm>
 
 #include "paged.cuh"
+#include "rows_meet.h"
 
 namespace zs {
 namespace {
@@ -206,6 +207,9 @@ extern "C" int zs_rope_write(const ZsRopeWrite* p) {
     if (end != rot / 2) return cudaErrorInvalidValue;
     if (!aligned16p(p->q) || !aligned16p(p->k) || !aligned16p(p->v) || !aligned16p(p->q_out) ||
         !aligned16p(p->cos_sin) || ((p->q_tok | p->q_head | p->k_tok | p->k_head | p->v_tok | p->v_head) % 8))
+        return cudaErrorInvalidValue;
+    if (!q_out_is_apart(p->q_out, N, Hq, Hkv, D, p->q, p->q_tok, p->q_head, p->k, p->k_tok, p->k_head, p->v, p->v_tok,
+                        p->v_head))
         return cudaErrorInvalidValue;
     a.q = p->q; a.k = p->k; a.v = p->v; a.q_out = p->q_out;
     a.q_tok = p->q_tok; a.q_head = p->q_head; a.k_tok = p->k_tok; a.k_head = p->k_head;

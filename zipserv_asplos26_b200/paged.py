@@ -91,7 +91,8 @@ def rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: tor
     or (2j, 2j + 1) when interleaved. positions is int32 [N], or [A, N] with one
     row per axis and `sections` (sum rot / 2) saying how many pairs follow each
     axis in turn. Slots (int64, distinct) of -1 are skipped. q, k and v may be
-    slices of one projection."""
+    slices of one projection. q_out (contiguous) may be q itself where q is
+    contiguous, and else lies apart from q, k and v."""
     return (_native or _load()).rope_write(q, k, v, positions, cos_sin, slots, k_pages, v_pages, sections,
                                            interleaved, q_out, err)
 
