@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_write_kernel(const RopeArgs
     const long long slot = a.slots[n];
     const long long cap = (long long)a.kp.num_blocks << a.kp.page_shift;
     const bool live = slot >= 0 && slot < cap;
-    if (slot >= cap && lane == 0) set_err(a.err, kErrPagedIndex);
+    if ((slot < -1 || slot >= cap) && lane == 0) set_err(a.err, kErrPagedIndex);     // -1: padding
     const long long blk = slot >> a.kp.page_shift, row = slot & ((1 << a.kp.page_shift) - 1);
     if (!on) return;
     uint16_t* kdst = static_cast<uint16_t*>(a.kp.data) + blk * a.kp.s_block + row * a.kp.s_token;
