@@ -237,8 +237,9 @@ int zs_decode_attention_paged(void* stream, const uint16_t* d_q, const ZsKvPool*
  * (strides in elements, multiples of 8; base 16-byte aligned), so a page may hold
  * its heads or its tokens outermost. Logical page p of sequence b is block
  * block_table[b * table_stride + p], p < width. Kernels check every index that
- * they read from a table, a list or the slots against the pool; a bad one is
- * skipped and sets bit 2 in *err (nullable). Pointers are device memory. */
+ * they read from a table, a list or the slots against the pool (zs_plan_step, which
+ * is given no pool, that it is not negative); a bad one is skipped and sets bit 2 in
+ * *err (nullable). Pointers are device memory. */
 enum { ZS_BF16 = 0, ZS_FP16 = 1 };
 typedef struct ZsPagePool {
     void* data;
@@ -262,7 +263,9 @@ typedef struct ZsPagePool {
  * free_blocks are updated in place; seq_lens and free_count are not (out_lens
  * and out_count are other buffers than any input), so a repeated call gives the
  * same result. Lengths are at most what a row of the table holds, below 2^31: one
- * that comes in longer counts as that. */
+ * that comes in longer counts as that. A *free_count outside 0 .. capacity counts as
+ * the nearest of these, and a page below 0 in a table or the free list gives its
+ * tokens slot -1; both set bit 2 in *err, as does a free list that runs over. */
 typedef struct ZsPlanStep {
     void* stream;
     int* block_table;

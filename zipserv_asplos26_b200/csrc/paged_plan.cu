@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     if (first && threadIdx.x == 0) {
         a.out_cu[R] = cu[R];
         *a.out_count = (int)have - used;
-        if (back_total + count0 > a.capacity) set_err(a.err, kErrPagedIndex);
+        if (count_in != count0 || back_total + count0 > a.capacity) set_err(a.err, kErrPagedIndex);
     }
 
     // the page at position x of the free list once the ended requests' pages are on it
@@ -202,16 +202,23 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
     };
     // One index space for the pages given back (the free list has room for every
     // page of the pool), the new table entries and the tokens, so that their
-    // lookups are in flight together.
+    // lookups are in flight together. The pool's size is not known here: a page
+    // below 0 (one that a table or the free list does not have) is flagged, and its
+    // tokens get no slot; the rotary write flags slots past the pool.
     const int nback = (int)(have - count0), tokens = cu[R];
     const long long items = (long long)nback + used + a.max_tokens;
+    bool bad = false;
     for (long long i = blockIdx.x * kPlanThreads + threadIdx.x; i < items; i += gridDim.x * kPlanThreads) {
         if (i < nback) {
-            a.free_list[count0 + i] = free_page(count0 + (int)i);
+            const int blk = free_page(count0 + (int)i);
+            bad |= blk < 0;
+            a.free_list[count0 + i] = blk;
         } else if (i < nback + (long long)used) {
             const int j = (int)(i - nback), r = owner(need0, R, j);
             const int col = ((lens[r] + P1) >> sh) + (j - need0[r]);
-            a.table[(long long)r * a.table_stride + col] = free_page((int)have - 1 - j);
+            const int blk = free_page((int)have - 1 - j);
+            bad |= blk < 0;
+            a.table[(long long)r * a.table_stride + col] = blk;
         } else {
             const int t = (int)(i - nback - used);
             long long slot = -1;
@@ -223,13 +230,15 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
                 const int col = pos >> sh, old = (len + P1) >> sh;
                 const int blk = col < old ? a.table[(long long)r * a.table_stride + col]
                                           : free_page((int)have - 1 - (need0[r] + col - old));
-                slot = ((long long)blk << sh) + (pos & P1);
+                bad |= blk < 0;
+                slot = blk < 0 ? -1 : ((long long)blk << sh) + (pos & P1);
             }
             a.slots[t] = slot;
             a.token_seq[t] = r;
             a.positions[t] = pos;
         }
     }
+    if (bad) set_err(a.err, kErrPagedIndex);
 }
 
 }  // namespace
