@@ -12,6 +12,9 @@ import concurrent.futures as cf
 import glob
 import os
 import subprocess
+import sysconfig
+
+import torch
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -20,7 +23,6 @@ INCLUDE = os.path.join(ROOT, "include")
 LIBDIR = os.path.join(PKG, "lib")
 OBJDIR = os.path.join(LIBDIR, "obj")
 LIB = os.path.join(LIBDIR, "libzipserv_b200.so")
-BINDING = os.path.join(LIBDIR, "_paged_native.so")
 CUDA = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA, "bin", "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -28,6 +30,15 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fopenmp",
                      "--expt-relaxed-constexpr", "-Xptxas", "-v,-warn-spills", f"-I{INCLUDE}", f"-I{CSRC}"]
 CXX_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-fopenmp", f"-I{INCLUDE}", f"-I{CSRC}", f"-I{CUDA}/include"]
+
+
+def binding_path(torch_version: str, suffix: str) -> str:
+    """The binding's file for one torch and one Python (its extension suffix): it
+    depends on the ABI of both, so another one's is never loaded."""
+    return os.path.join(LIBDIR, f"_paged_native.torch{torch_version}{suffix}")
+
+
+BINDING = binding_path(torch.__version__, sysconfig.get_config_var("EXT_SUFFIX"))
 
 
 def _headers():
@@ -83,9 +94,6 @@ def _build_binding(verbose: bool) -> str:
     src = os.path.join(CSRC, "binding", "paged_bind.cpp")
     if not _stale(BINDING, [src, LIB, os.path.join(INCLUDE, "zipserv_b200.h"), os.path.join(CSRC, "rows_meet.h")]):
         return BINDING
-    import sysconfig
-
-    import torch
     tdir = os.path.dirname(torch.__file__)
     tmp = BINDING + ".tmp"
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
