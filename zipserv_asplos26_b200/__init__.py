@@ -12,8 +12,8 @@ from .attention import (compress_kv, decode_attention, decode_attention_dense, f
 __all__ += ["compress_kv", "decode_attention", "decode_attention_dense", "flash_attn_with_kvcache", "pad_kv_by_kv_head",
             "pad_kv_token_major"]
 from . import store  # noqa: E402,F401  (save / load of compressed matrices)
-from .paged import (PagedKVCache, StepPlan, page_bounds, paged_attention, plan_step, rope_write,  # noqa: E402,F401
-                    select_pages, sparse_attention)
+from .paged import (PagedKVCache, StepPlan, TokenRows, page_bounds, paged_attention, plan_step,  # noqa: E402,F401
+                    rope_write, select_pages, sparse_attention)
 
-__all__ += ["PagedKVCache", "StepPlan", "page_bounds", "paged_attention", "plan_step", "rope_write", "select_pages",
+__all__ += ["PagedKVCache", "StepPlan", "TokenRows", "page_bounds", "paged_attention", "plan_step", "rope_write", "select_pages",
             "sparse_attention"]
