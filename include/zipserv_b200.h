@@ -315,8 +315,9 @@ int zs_rope_write(const ZsRopeWrite* args);
  * q[b][i] . K^T) V over the first seq_lens[b] tokens of the cache, KV head i /
  * (Hq / Hkv); D is 64 or 128; q and out are [B][Hq][D], 16-byte aligned. With
  * pages ([B][Hkv][top] distinct logical pages) and counts ([B][Hkv]) only the
- * tokens of the listed pages count. A sequence with nothing to attend gets zeros; a
- * channel with an infinite value is that infinity, with both signs or a NaN it is NaN.
+ * tokens of the listed pages count. A score of -inf weighs nothing, and a query with
+ * nothing to attend gets zeros; a channel with an infinite value is that infinity, with
+ * both signs or a NaN it is NaN.
  * lse (nullable, [B][Hq]) receives log sum exp(softmax_scale q.k), -inf where
  * nothing counts. max_seqlen: a bound on seq_lens where the host has one closer
  * than the table's width (0: none); it chooses between two kernels, whose results

@@ -118,3 +118,22 @@ def test_an_infinite_value_under_a_vanishing_weight(dtype, hq, at):
     ref, vmax = reference(q, c.dense, 300.0)
     assert int(ref.isinf().sum()) == hq
     both_ways(q, c, ref, vmax, dtype, softmax_scale=300.0)
+
+
+@pytest.mark.parametrize("T", [1, 20, 300])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_scores_of_minus_infinity_weigh_nothing(T, dtype):
+    """A key with an infinity: no weight where the score is -inf, and zeros where every score is."""
+    c = Cache([T, T + 3], 1, 64, 16, dtype, "heads", 8)
+    q = torch.randn(2, 2, 64, device=DEV).to(dtype)
+    q[..., 4] = 1.0
+    lost = range(T) if T < 300 else range(100, 220)
+    for t in lost:
+        c.k[int(c.table[0, t // 16]), t % 16, 0, 4] = -INF
+    keep = torch.tensor([t for t in range(T) if t not in lost], device=DEV, dtype=torch.long)
+    dense = [(c.dense[0][0][keep], c.dense[0][1][keep]), c.dense[1]]
+    ref, vmax = reference(q, dense, 0.125)
+    both_ways(q, c, ref, vmax, dtype)
+    lse = torch.zeros(2, 2, device=DEV)
+    zs().paged_attention(q, c.k, c.v, c.table, c.lens, lse=lse)
+    assert bool((lse[0] == -INF).all()) == (T < 300) and bool(lse[1].isfinite().all())
