@@ -369,7 +369,7 @@ int zs_page_bounds(const ZsPageBounds* args);
 
 /* Choice of up to `top` pages per (sequence, KV head) for sparse attention: the
  * first `sinks` pages, the last `local` (>= 1) and the best of the others by the
- * bound max_g sum_d max(q_gd up_d, q_gd lo_d) * scale, q in whole numbers, ties
+ * score max_g sum_d max(q_gd up_d, q_gd lo_d) * scale, q in whole numbers, ties
  * to the lowest page. pages [B][Hkv][top]: ascending, -1 past counts [B][Hkv].
  * width <= 32768, Hq / Hkv <= 128, top >= sinks + local; D is 64, 128 or 256. */
 typedef struct ZsSelectPages {

@@ -6,10 +6,12 @@
 // i / (Hq / Hkv), m = max s_t; zero where nothing is attended. One pass: every
 // warp keeps a running maximum, sum and unnormalised output in fp32 registers.
 //
-// Bound by HBM: each K and V row is read once for all the query heads that share
+// Bound by HBM: each K and V row is read once for every 16 query heads that share
 // it. The work is cut into chunks of 16 tokens of a unit (sequence, KV head, tile
 // of up to 16 query heads), a warp's step, and dealt in one of two ways, chosen by
-// sizes that the host has (unit_warps):
+// sizes that the host has (unit_warps). Tiles do not share their reads: 64 sequences
+// of 8193 with one KV head take 51 us for 16 query heads, 82 for 32 and 163 for 64
+// (their keys and values once: 41).
 //   * paged_attn_kernel: all chunks in order go to the warps of the GPU in equal
 //     runs, found by a prefix sum over the lengths in the kernel, so ragged
 //     batches and single long sequences load every SM alike and no length is
@@ -33,9 +35,9 @@
 // are looked at again (odd_values).
 //
 // Measured in long runs, at the power cap that they reach (bf16, 32 query and 8 KV
-// heads of 128, pages of 64): B=32 T=4129 86.5 us, 6.26 TB/s; B=1 T=131105 87, 6.2;
-// 61 sequences of 0..16417 (fp16, 64 query heads, pages of 16) 314, 6.6; B=1 T=97
-// 4.7. A plain copy does 6.56 TB/s. DRAM reads are the algorithm's bytes (541.5 MB).
+// heads of 128, pages of 64): B=32 T=4129 87.5 us, 6.19 TB/s; B=1 T=131105 89, 6.0;
+// 61 sequences of 0..16417 (fp16, 64 query heads, pages of 16) 319, 6.5; B=1 T=97
+// 4.8. A plain copy does 6.56 TB/s. DRAM reads are the algorithm's bytes (541.5 MB).
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -932,8 +934,8 @@ __global__ void __launch_bounds__(kPaThreads, PaCfg<D, kNarrow>::kCtas) paged_at
 // pieces are read in batches, weights and outputs together. A warp takes a query
 // head, D / 32 channels a lane; with few heads (long sequences: up to a piece a
 // warp of the attention kernel) the warps of a CTA share a head's pieces and add
-// their sums in order. With its launch it costs 3 (B=1 T=97) to 5 us (B=1
-// T=131105, 148 pieces a unit; 10 us when the pieces were read one by one).
+// their sums in order. It costs some 6 us of 87 at B=1 T=131105, where a unit is cut
+// into 222 pieces (runs of 37 of its 8195 chunks).
 constexpr int kJoinWarps = 16;
 constexpr int kJoinShare = 148;        // heads joined by a CTA each
 constexpr int kJoinBatch = 8;

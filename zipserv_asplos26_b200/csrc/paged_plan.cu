@@ -21,7 +21,7 @@
 // formula and not in the table, and a taken page that was given back in the
 // same step is found in the ended request's row and not in the free list.
 //
-// Measured: 3 requests 3.3 us, 256 requests with 16 thousand tokens 5.2, 37
+// Measured: 3 requests 3.4 us, 256 requests with 16 thousand tokens 5.3, 37
 // prompts of 131 thousand tokens in all 4.9, of which an empty launch is some 2.
 #include <algorithm>
 

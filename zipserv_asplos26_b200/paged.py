@@ -135,7 +135,8 @@ def select_pages(q: torch.Tensor, page_codes: torch.Tensor, page_scales: torch.T
                  err: Optional[torch.Tensor] = None):
     """Up to top_pages pages per (sequence, KV head): the first sink_pages, the
     last local_pages (the newest, possibly incomplete, among them) and the best
-    of the others by the bound of q . k over the page's keys. Returns pages
+    of the others by a score: the largest q . k that the page's bounds allow, of q
+    rounded to 8 bits (so keys near the clamp of the codes may pass it). Returns pages
     (int32 [B, Hkv, top_pages], ascending, -1 past the count) and counts."""
     return (_native or _load()).select_pages(q, page_codes, page_scales, block_table, seq_lens, page_size, top_pages,
                                              sink_pages, local_pages, err)
