@@ -235,18 +235,21 @@ __device__ __forceinline__ void copy_chunk(const PaArgs& a, uint32_t dst, int bl
 // values include an infinity is that infinity, and NaN only where they include both
 // signs or a NaN. The products cannot tell (0 * inf is NaN, and the remainder of a
 // weight may be zero or negative), so where a finished output is not finite although
-// the sum of its weights is a number, the unit's values are read once more. Returns
-// for each of the kCount channels from c0 on three bits: an infinity is there, a
-// negative one, a NaN. Nothing of this runs while outputs are finite; to see that they
-// are costs 0.05 us of 4.0 at B=1 T=97 and nothing in long runs.
+// the sum of its weights is a number, the values of its pieces that are not finite are
+// read once more, here `count` chunks from `first` on. Adds to `seen`, for each of the
+// kCount channels from c0 on, three bits: an infinity is there, a negative one, a NaN.
+// Nothing of this runs while outputs are finite; to see that they are costs 0.1 us of
+// 4.0 at B=1 T=97 and nothing in long runs. One infinity among B=32 T=4129: 160 us
+// (finite 83), B=1 T=131105: 209 (83); with all of a unit read again it was 520 and
+// 14186.
 template <typename T, int kCount, bool kListed>
-__device__ __forceinline__ uint32_t odd_values(const PaArgs& a, int e, int b, int h, int n, int c0) {
+__device__ __forceinline__ void odd_values(const PaArgs& a, int e, int b, int h, int first, int count, int c0,
+                                           uint32_t& seen) {
     constexpr uint32_t kInf = std::is_same<T, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;
     const int len = min(a.lens[b], (int)min((long long)a.width << a.kp.page_shift, (long long)INT_MAX));
     const uint16_t* base = static_cast<const uint16_t*>(a.vp.data) + h * a.vp.s_head + c0;
-    uint32_t seen = 0;
 #pragma unroll 1
-    for (int ch = 0; ch < n; ++ch) {
+    for (int ch = first; ch < first + count; ++ch) {
         int blk, lim;
         look_chunk<kListed>(a, e, b, ch, len, blk, lim);
         const int row0 = (ch & ((1 << (a.kp.page_shift - 4)) - 1)) * kPaChunk;
@@ -264,7 +267,18 @@ __device__ __forceinline__ uint32_t odd_values(const PaArgs& a, int e, int b, in
             }
         }
     }
-    return seen;
+}
+// Whether nothing more can change the outputs of the channels whose bits 3 j are in `odd`.
+__device__ __forceinline__ bool odd_decided(uint32_t seen, uint32_t odd) {
+    return ((seen >> 2 | (seen & seen >> 1)) & odd) == odd;
+}
+// Bits 3 j of the channels j that are not finite.
+template <int kCount>
+__device__ __forceinline__ uint32_t odd_channels(const float (&o)[kCount]) {
+    uint32_t f = 0;
+#pragma unroll
+    for (int j = 0; j < kCount; ++j) f |= (isfinite(o[j]) ? 0u : 1u) << (3 * j);
+    return f;
 }
 // The output of the j-th of these channels; o where nothing odd is among its values.
 __device__ __forceinline__ float odd_output(uint32_t seen, int j, float o) {
@@ -805,8 +819,11 @@ __global__ void __launch_bounds__(kPaThreads, PaCfg<D, kNarrow>::kCtas) paged_at
         const long long slot = 2ll * id + (s == count ? 0 : 1);       // the run's first part, or its last
         st.finish();
         if (whole) {
-            if (__builtin_expect(st.odd(), false))
-                st.mend(odd_values<T, D / 32, kListed>(a, cur.e, b, h, cur.n, lane * (D / 32)));
+            if (__builtin_expect(st.odd(), false)) {
+                uint32_t seen = 0;
+                odd_values<T, D / 32, kListed>(a, cur.e, b, h, 0, cur.n, lane * (D / 32), seen);
+                st.mend(seen);
+            }
             st.write(a.out + head0 * D, a.lse ? a.lse + head0 : nullptr, rows);
         } else st.park(a.part_o + slot * a.prow * D, a.part_ml + slot * a.prow * 2, rows);
         if (s == steps) break;
@@ -915,7 +932,14 @@ __global__ void __launch_bounds__(kPaThreads, PaCfg<D, kNarrow>::kCtas) paged_at
             m = mn;
         }
         if (__builtin_expect(is_odd((acc.x * 0.f + acc.y * 0.f) + (acc.z * 0.f + acc.w * 0.f), l), false)) {
-            const uint32_t seen = odd_values<T, 4, kListed>(a, e, b, h, n, d4);
+            const uint32_t odd = odd_channels<4>({acc.x, acc.y, acc.z, acc.w});
+            uint32_t seen = 0;
+            for (int v = 0; v < W && !odd_decided(seen, odd); ++v) {
+                const uint32_t peer = W <= kPaWarps ? base : mapa_shared(base, v / kPaWarps);
+                const float4 o = ld_dsmem_f4(peer + (v0 + v % kPaWarps) * C::kRing + (row * D + d4) * 4);
+                const int c = (int)((long long)n * v / W), end = (int)((long long)n * (v + 1) / W);
+                if (odd_channels<4>({o.x, o.y, o.z, o.w})) odd_values<T, 4, kListed>(a, e, b, h, c, end - c, d4, seen);
+            }
             acc.x = odd_output(seen, 0, acc.x);
             acc.y = odd_output(seen, 1, acc.y);
             acc.z = odd_output(seen, 2, acc.z);
@@ -1023,7 +1047,19 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PaArg
 #pragma unroll
     for (int j = 0; j < kVec; ++j) zeros += acc[j] * 0.f;
     if (__builtin_expect(is_odd(zeros, l), false)) {
-        const uint32_t seen = odd_values<T, kVec, kListed>(a, kListed ? b * a.Hkv + h : b, b, h, n, lane * kVec);
+        const uint32_t odd = odd_channels<kVec>(acc);
+        const int w0 = (int)div_nonneg(lo, run), w1 = (int)div_nonneg(lo + n - 1, run);
+        uint32_t seen = 0;
+        for (int w = w0; w <= w1 && !odd_decided(seen, odd); ++w) {
+            const long long s = (2ll * w + (w == w0 && lo != w0 * run ? 1 : 0)) * a.prow + row;
+            float o[kVec];
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) o[j] = a.part_o[s * D + lane * kVec + j];
+            const long long c = max(w * run, lo), end = min((w + 1) * run, lo + n);
+            if (odd_channels<kVec>(o))
+                odd_values<T, kVec, kListed>(a, kListed ? b * a.Hkv + h : b, b, h, (int)(c - lo), (int)(end - c),
+                                             lane * kVec, seen);
+        }
 #pragma unroll
         for (int j = 0; j < kVec; ++j) acc[j] = odd_output(seen, j, acc[j]);
     }
