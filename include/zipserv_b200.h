@@ -387,6 +387,79 @@ typedef struct ZsSelectPages {
 } ZsSelectPages;
 int zs_select_pages(const ZsSelectPages* args);
 
+/* ---- 4-bit paged KV cache ------------------------------------------------
+ * A row (a token's keys or values of one KV head, head_dim channels, 64 or 128) in
+ * groups of `group` (32 or 64) channels: codes, 4 bits a channel, channel 2i in the low
+ * half of byte i; params, bf16: the groups' scales, then their centres. A channel stands
+ * for c + s (u - 8), with s = bf16((max - min) / 15), c = bf16(min + 8 s) and u =
+ * clamp(rint((x - c) / s) + 8, 0, 15) in fp32. A group whose scale is below 2^-126 has
+ * s = 0, c = bf16(min) and codes of 8; one with a value that is not finite, or whose
+ * max - min is not, c = NaN: it reads back as NaN. Row (block, token, head) starts at
+ * codes + block * codes_block + ... (bytes, multiples of 16) and params + block *
+ * params_block + ... (elements, multiples of 2 head_dim / group); both are 16-byte
+ * aligned; pages as in ZsPagePool. */
+typedef struct ZsInt4Pool {
+    uint8_t* codes;
+    uint16_t* params;
+    int64_t codes_block, codes_token, codes_head, params_block, params_token, params_head;
+    int num_blocks, page_size, num_heads, head_dim, group, reserved;
+} ZsInt4Pool;
+
+/* zs_rope_write into a 4-bit cache: q_out as there; k, turned in fp32, and v are
+ * quantised as they are written. */
+typedef struct ZsRopeWriteInt4 {
+    void* stream;
+    const uint16_t *q, *k, *v;
+    int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
+    uint16_t* q_out;
+    const int* positions;
+    int64_t pos_axis;
+    const float* cos_sin;
+    const int64_t* slots;
+    unsigned* err;
+    ZsInt4Pool k_pool, v_pool;
+    int N, Hq, axes, sections[4], table_rows, rot, interleaved;
+    int dtype;                      /* of q, k and v: ZS_BF16 or ZS_FP16 */
+} ZsRopeWriteInt4;
+int zs_rope_write_int4(const ZsRopeWriteInt4* args);
+
+/* Rows of a 4-bit cache by slot: k_out and v_out [N][num_heads][head_dim], contiguous and
+ * 16-byte aligned, what the codes stand for rounded to dtype. Slots of -1 give zeros;
+ * others out of range too, and set bit 2 in *err. A slot may be listed more than once. */
+typedef struct ZsReadInt4 {
+    void* stream;
+    const int64_t* slots;
+    uint16_t *k_out, *v_out;
+    unsigned* err;
+    ZsInt4Pool k_pool, v_pool;
+    int N, dtype;
+} ZsReadInt4;
+int zs_read_int4(const ZsReadInt4* args);
+
+/* zs_paged_attention over a 4-bit cache: keys and values are what the codes stand for,
+ * before any rounding to 16 bits; magnitudes of q, and of s times a weight, count below
+ * 2^63. dtype is q's and out's. The other arguments, and the workspace, are as there. */
+typedef struct ZsPagedAttentionInt4 {
+    void* stream;
+    const uint16_t* q;
+    const int* block_table;
+    int64_t table_stride;
+    const int* seq_lens;
+    const int* pages;
+    const int* counts;
+    void* ws;
+    size_t ws_bytes;
+    uint16_t* out;
+    float* lse;
+    unsigned* err;
+    ZsInt4Pool k_pool, v_pool;
+    int B, Hq, width, top;
+    float softmax_scale;
+    int max_seqlen, dtype;
+} ZsPagedAttentionInt4;
+size_t zs_paged_attention_int4_workspace(const ZsPagedAttentionInt4* args);
+int zs_paged_attention_int4(const ZsPagedAttentionInt4* args);
+
 /* ---- On-disk TCA-TBE container (file format version 1) -------------------
  * No counterpart in the reference, which keeps no serialised compressed form
  * (its benchmarks re-encode the dense checkpoint at start-up,

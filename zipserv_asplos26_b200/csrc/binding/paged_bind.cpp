@@ -288,17 +288,23 @@ at::Tensor rows(PyObject* o, int64_t n, int64_t dim, at::ScalarType type, const 
     return aligned16(c) ? c : c.clone();
 }
 
-PyObject* rope_write(PyObject* const* a) {
-    const Pools pools = page_pools(a[6], a[7]);
-    const int index = pools.index;
-    const int64_t dim = pools.k.head_dim;
+// The arguments of a rotary write, a[0 .. 11] of rope_write, into pools on device `index`
+// of hkv heads of dim channels: fills p but for its pools. `type` is q's, k's and v's.
+struct Turned {
+    at::Tensor q, k, v, out;           // keeps copies and the output alive
+};
+
+template <class P>
+Turned rope_args(PyObject* const* a, P& p, int64_t hkv, int64_t dim, at::ScalarType type, int index) {
     const at::Tensor& q0 = tensor(a[0], "q");
     need(q0.dim() == 3 && q0.size(0) <= INT32_MAX, "q must be [N, Hq, D]");
     const int64_t N = q0.size(0);
-    OnDevice on(index);
-    const at::Tensor q = rows(a[0], N, dim, pools.type, "q", index), k = rows(a[1], N, dim, pools.type, "k", index),
-                     v = rows(a[2], N, dim, pools.type, "v", index);
-    need(k.size(1) == pools.k.num_heads && v.size(1) == pools.k.num_heads, "k and v must have the cache's heads");
+    Turned t;
+    t.q = rows(a[0], N, dim, type, "q", index);
+    t.k = rows(a[1], N, dim, type, "k", index);
+    t.v = rows(a[2], N, dim, type, "v", index);
+    const at::Tensor &q = t.q, &k = t.k, &v = t.v;
+    need(k.size(1) == hkv && v.size(1) == hkv, "k and v must have the cache's heads");
     const at::Tensor& cs = tensor(a[4], "cos_sin");
     need(cs.scalar_type() == at::kFloat && cs.dim() == 2 && cs.is_cuda() && cs.get_device() == index &&
              cs.is_contiguous() && cs.size(0) > 0 && cs.size(0) <= INT32_MAX && aligned16(cs),
@@ -312,7 +318,6 @@ PyObject* rope_write(PyObject* const* a) {
              (pos.dim() == 1 || pos.dim() == 2) && pos.size(-1) == N && (N <= 1 || pos.stride(-1) == 1) && axes >= 1 &&
              axes <= 4,
          "positions must be int32 [N] or [axes, N] with contiguous rows and 1 to 4 axes");
-    ZsRopeWrite p{};
     const char* bad_sections = "sections must give each axis its share of the rot / 2 pairs";
     if (given(a[8])) {
         PyObject* seq = PySequence_Fast(a[8], bad_sections);
@@ -335,17 +340,17 @@ PyObject* rope_write(PyObject* const* a) {
     p.slots = vec<int64_t>(a[5], N, at::kLong, "slots", index);
     p.err = err_word(a[11], index);
     p.interleaved = truth(a[9]);
-    at::Tensor out;
+    at::Tensor& out = t.out;
     if (given(a[10])) {
         out = tensor(a[10], "q_out");
-        need(out.sizes() == q.sizes() && out.scalar_type() == pools.type && out.is_cuda() &&
+        need(out.sizes() == q.sizes() && out.scalar_type() == type && out.is_cuda() &&
                  out.get_device() == index && out.is_contiguous() && aligned16(out),
              "q_out must be contiguous, aligned and of q's shape and type");
         need(zs::q_out_is_apart(out.data_ptr(), N, q.size(1), k.size(1), dim, q.data_ptr(), q.stride(0), q.stride(1),
                                 k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1)),
              "q_out must be a contiguous q itself, or apart from q, k and v");
     } else {
-        out = fresh({N, q.size(1), dim}, pools.type, index);
+        out = fresh({N, q.size(1), dim}, type, index);
     }
     p.stream = current_stream(index);
     p.q = ptr<uint16_t>(q);
@@ -361,42 +366,67 @@ PyObject* rope_write(PyObject* const* a) {
     p.positions = ptr<int>(pos);
     p.pos_axis = axes > 1 ? pos.stride(0) : 0;
     p.cos_sin = ptr<float>(cs);
-    p.k_pool = pools.k;
-    p.v_pool = pools.v;
     p.N = static_cast<int>(N);
     p.Hq = static_cast<int>(q.size(1));
     p.axes = static_cast<int>(axes);
     p.table_rows = static_cast<int>(cs.size(0));
     p.rot = static_cast<int>(rot);
-    call(zs_rope_write, p, "zs_rope_write");
-    if (given(a[10])) {
-        Py_INCREF(a[10]);
-        return a[10];
+    return t;
+}
+
+// q_out as given, or the fresh output.
+PyObject* turned_q(PyObject* q_out, Turned& t) {
+    if (given(q_out)) {
+        Py_INCREF(q_out);
+        return q_out;
     }
-    return THPVariable_Wrap(std::move(out));
+    return THPVariable_Wrap(std::move(t.out));
+}
+
+PyObject* rope_write(PyObject* const* a) {
+    const Pools pools = page_pools(a[6], a[7]);
+    OnDevice on(pools.index);
+    ZsRopeWrite p{};
+    Turned t = rope_args(a, p, pools.k.num_heads, pools.k.head_dim, pools.type, pools.index);
+    p.k_pool = pools.k;
+    p.v_pool = pools.v;
+    call(zs_rope_write, p, "zs_rope_write");
+    return turned_q(a[10], t);
 }
 
 // ------------------------------------------------------------- attention
-// The attention proper; q3 is checked, `out` may be undefined. Returns out as [B, Hq, D].
-at::Tensor attend(const Pools& pools, const at::Tensor& q3, const Table& table, const int* lens, const int* pages,
-                  const int* counts, int64_t top, PyObject* scale_o, PyObject* out_o, PyObject* lse_o, PyObject* most_o,
-                  unsigned* err) {
-    const int index = pools.index;
-    const int64_t dim = pools.k.head_dim, B = q3.size(0), hq = q3.size(-2);
-    need(static_cast<int64_t>(table.width) * pools.k.page_size <= INT32_MAX,
+// The attention proper: fills p, but for its pools and dtype, from q3 (checked) and the
+// rest, and calls it. Returns out as [B, Hq, D].
+struct Attended {
+    const at::Tensor& q3;
+    at::ScalarType type;
+    int index;
+    int64_t page_size;
+    Table table;
+    const int *lens, *pages, *counts;
+    int64_t top;
+    unsigned* err;
+};
+
+template <class P>
+at::Tensor attend(P& p, const Attended& x, PyObject* scale_o, PyObject* out_o, PyObject* lse_o, PyObject* most_o,
+                  size_t (*workspace)(const P*), int (*f)(const P*), const char* name) {
+    const int index = x.index;
+    const at::Tensor& q3 = x.q3;
+    const int64_t dim = q3.size(-1), B = q3.size(0), hq = q3.size(-2);
+    need(static_cast<int64_t>(x.table.width) * x.page_size <= INT32_MAX,
          "block_table covers more than 2**31 - 1 tokens");
     const double scale = given(scale_o) ? number(scale_o) : 1.0 / std::sqrt(static_cast<double>(dim));
     need(std::isfinite(static_cast<float>(scale)), "softmax_scale must be finite");
     at::Tensor out;
     if (given(out_o)) {
         out = tensor(out_o, "out");
-        need(out.numel() == q3.numel() && out.scalar_type() == pools.type && out.is_cuda() &&
+        need(out.numel() == q3.numel() && out.scalar_type() == x.type && out.is_cuda() &&
                  out.get_device() == index && out.is_contiguous() && aligned16(out),
              "out must be contiguous, aligned and of q's shape and type");
     } else {
-        out = fresh(q3.sizes(), pools.type, index);
+        out = fresh(q3.sizes(), x.type, index);
     }
-    ZsPagedAttention p{};
     if (given(most_o)) {
         const int64_t most = integer(most_o);
         need(most >= 0, "max_seqlen must not be negative");
@@ -405,27 +435,50 @@ at::Tensor attend(const Pools& pools, const at::Tensor& q3, const Table& table, 
     p.lse = given(lse_o) ? vec<float>(lse_o, B * hq, at::kFloat, "lse", index) : nullptr;
     p.stream = current_stream(index);
     p.q = ptr<uint16_t>(q3);
-    p.block_table = table.data;
-    p.table_stride = table.stride;
-    p.seq_lens = lens;
-    p.pages = pages;
-    p.counts = counts;
+    p.block_table = x.table.data;
+    p.table_stride = x.table.stride;
+    p.seq_lens = x.lens;
+    p.pages = x.pages;
+    p.counts = x.counts;
     p.out = ptr<uint16_t>(out);
-    p.err = err;
-    p.k_pool = pools.k;
-    p.v_pool = pools.v;
+    p.err = x.err;
     p.B = static_cast<int>(B);
     p.Hq = static_cast<int>(hq);
-    p.width = table.width;
-    p.top = static_cast<int>(top);
+    p.width = x.table.width;
+    p.top = static_cast<int>(x.top);
     p.softmax_scale = static_cast<float>(scale);
     at::Tensor ws;
-    if ((p.ws_bytes = zs_paged_attention_workspace(&p)) > 0) {
+    if ((p.ws_bytes = workspace(&p)) > 0) {
         ws = fresh({static_cast<int64_t>(p.ws_bytes)}, at::kByte, index);
         p.ws = ptr(ws);
     }
-    call(zs_paged_attention, p, "zs_paged_attention");
+    call(f, p, name);
     return out;
+}
+
+at::Tensor attend16(const Pools& pools, const at::Tensor& q3, const Table& table, const int* lens, const int* pages,
+                    const int* counts, int64_t top, PyObject* scale_o, PyObject* out_o, PyObject* lse_o,
+                    PyObject* most_o, unsigned* err) {
+    ZsPagedAttention p{};
+    p.k_pool = pools.k;
+    p.v_pool = pools.v;
+    return attend(p, Attended{q3, pools.type, pools.index, pools.k.page_size, table, lens, pages, counts, top, err},
+                  scale_o, out_o, lse_o, most_o, zs_paged_attention_workspace, zs_paged_attention, "zs_paged_attention");
+}
+
+// The page lists of a call: pages [B, Hkv, top] and counts, or neither.
+struct Lists {
+    const int *pages, *counts;
+    int64_t top;
+};
+
+Lists page_lists(PyObject* pages_o, PyObject* counts_o, int64_t B, int64_t hkv, int64_t page_size, int index) {
+    need(given(pages_o) == given(counts_o), "pages and counts go together");
+    if (!given(pages_o)) return {nullptr, nullptr, 0};
+    const at::Tensor& t = tensor(pages_o, "pages");
+    need(t.dim() == 3 && t.size(2) > 0 && t.size(2) * page_size <= INT32_MAX, "pages must be int32 [B, Hkv, top]");
+    return {vec<int>(pages_o, B * hkv * t.size(2), at::kInt, "pages", index),
+            vec<int>(counts_o, B * hkv, at::kInt, "counts", index), t.size(2)};
 }
 
 void check_attention_dim(const Pools& pools) {
@@ -442,18 +495,9 @@ PyObject* paged_attention(PyObject* const* a) {
     const int64_t B = q3.size(0);
     const Table table = block_table(a[3], B, index);
     const int* lens = vec<int>(a[4], B, at::kInt, "seq_lens", index);
-    need(given(a[6]) == given(a[7]), "pages and counts go together");
-    const int *pages = nullptr, *counts = nullptr;
-    int64_t top = 0;
-    if (given(a[6])) {
-        const at::Tensor& t = tensor(a[6], "pages");
-        need(t.dim() == 3 && t.size(2) > 0 && t.size(2) * pools.k.page_size <= INT32_MAX,
-             "pages must be int32 [B, Hkv, top]");
-        top = t.size(2);
-        pages = vec<int>(a[6], B * hkv * top, at::kInt, "pages", index);
-        counts = vec<int>(a[7], B * hkv, at::kInt, "counts", index);
-    }
-    at::Tensor out = attend(pools, q3, table, lens, pages, counts, top, a[5], a[8], a[9], a[10], err_word(a[11], index));
+    const Lists l = page_lists(a[6], a[7], B, hkv, pools.k.page_size, index);
+    at::Tensor out = attend16(pools, q3, table, lens, l.pages, l.counts, l.top, a[5], a[8], a[9], a[10],
+                              err_word(a[11], index));
     return THPVariable_Wrap(std::move(out));
 }
 
@@ -578,10 +622,138 @@ PyObject* sparse_attention(PyObject* const* a) {
     const int64_t top = integer(a[7]);
     need(top > 0 && top <= INT32_MAX / pools.k.page_size, "top_pages must be positive, and cover less than 2**31 tokens");
     Choice c = choose(q3, b, nb, hkv, table, lens, pools.k.page_size, top, integer(a[8]), integer(a[9]), err, index);
-    at::Tensor out = attend(pools, q3, table, lens, ptr<int>(c.pages), ptr<int>(c.counts), top, a[10], a[11], Py_None,
-                            Py_None, err);
+    at::Tensor out = attend16(pools, q3, table, lens, ptr<int>(c.pages), ptr<int>(c.counts), top, a[10], a[11], Py_None,
+                              Py_None, err);
     return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(c.pages)),
                          THPVariable_Wrap(std::move(c.counts)));
+}
+
+// ------------------------------------------------------------ 4-bit cache
+// codes uint8 [num_blocks, page_size, heads, dim / 2] and params bf16 [num_blocks,
+// page_size, heads, 2, dim / group] of one pool.
+ZsInt4Pool int4_pool(PyObject* codes_o, PyObject* params_o, const char* name) {
+    const std::string n(name);
+    const at::Tensor &c = cuda_tensor(codes_o, (n + ".codes").c_str()), &t = cuda_tensor(params_o, (n + ".params").c_str());
+    if (c.scalar_type() != at::kByte || c.dim() != 4 || t.scalar_type() != at::kBFloat16 || t.dim() != 5 ||
+        t.get_device() != c.get_device())
+        refuse(n + " must be uint8 codes [num_blocks, page_size, heads, dim / 2] and bfloat16 params [num_blocks, "
+                   "page_size, heads, 2, dim / group] on one CUDA device");
+    check_page_size(c.size(1));
+    const int64_t dim = c.size(3) * 2, groups = t.size(4);
+    need(dim == 64 || dim == 128, "head dim must be 64 or 128");
+    need(groups > 0 && (groups * 32 == dim || groups * 64 == dim), "params must have a scale and a centre for every 32 or 64 channels");
+    if (c.numel() == 0 || c.size(0) > INT32_MAX || c.size(2) > INT32_MAX) refuse(n + " must not be empty");
+    if (t.size(0) != c.size(0) || t.size(1) != c.size(1) || t.size(2) != c.size(2) || t.size(3) != 2)
+        refuse(n + ": codes and params must agree in blocks, page size and heads");
+    if (c.stride(3) != 1 || (c.stride(0) | c.stride(1) | c.stride(2)) % 16 || !aligned16(c) ||
+        (t.stride(4) != 1 && groups > 1) || t.stride(3) != groups ||
+        (t.stride(0) | t.stride(1) | t.stride(2)) % (2 * groups) || !aligned16(t))
+        refuse(n + ": rows must be contiguous and aligned (codes to 16 bytes, params to a row's)");
+    return {ptr<uint8_t>(c), ptr<uint16_t>(t), c.stride(0), c.stride(1), c.stride(2), t.stride(0), t.stride(1),
+            t.stride(2), static_cast<int>(c.size(0)), static_cast<int>(c.size(1)), static_cast<int>(c.size(2)),
+            static_cast<int>(dim), static_cast<int>(dim / groups), 0};
+}
+
+struct Int4Pools {
+    ZsInt4Pool k, v;
+    int index;
+};
+
+// k and v, each (codes, params).
+Int4Pools int4_pools(PyObject* ko, PyObject* vo) {
+    need(PyTuple_Check(ko) && PyTuple_GET_SIZE(ko) == 2 && PyTuple_Check(vo) && PyTuple_GET_SIZE(vo) == 2,
+         "k_pages and v_pages must be Int4Pages");
+    Int4Pools p{int4_pool(PyTuple_GET_ITEM(ko, 0), PyTuple_GET_ITEM(ko, 1), "k_pages"),
+                int4_pool(PyTuple_GET_ITEM(vo, 0), PyTuple_GET_ITEM(vo, 1), "v_pages"),
+                static_cast<int>(THPVariable_Unpack(PyTuple_GET_ITEM(ko, 0)).get_device())};
+    need(p.k.num_blocks == p.v.num_blocks && p.k.page_size == p.v.page_size && p.k.num_heads == p.v.num_heads &&
+             p.k.head_dim == p.v.head_dim && p.k.group == p.v.group &&
+             THPVariable_Unpack(PyTuple_GET_ITEM(vo, 0)).get_device() == p.index,
+         "k_pages and v_pages must agree in shape and device");
+    return p;
+}
+
+at::ScalarType half_type(const at::Tensor& t, const char* name) {
+    if (dtype_code(t.scalar_type()) < 0) refuse(std::string(name) + " must be bf16 or fp16");
+    return t.scalar_type();
+}
+
+PyObject* rope_write_int4(PyObject* const* a) {
+    const Int4Pools pools = int4_pools(a[6], a[7]);
+    const at::ScalarType type = half_type(tensor(a[0], "q"), "q");
+    OnDevice on(pools.index);
+    ZsRopeWriteInt4 p{};
+    Turned t = rope_args(a, p, pools.k.num_heads, pools.k.head_dim, type, pools.index);
+    p.k_pool = pools.k;
+    p.v_pool = pools.v;
+    p.dtype = dtype_code(type);
+    call(zs_rope_write_int4, p, "zs_rope_write_int4");
+    return turned_q(a[10], t);
+}
+
+// k_pages, v_pages, slots, dtype as one of ZS_BF16 and ZS_FP16, out (None or a pair), err.
+PyObject* read_int4(PyObject* const* a) {
+    const Int4Pools pools = int4_pools(a[0], a[1]);
+    const int index = pools.index;
+    const int64_t dtype = integer(a[3]);
+    need(dtype == ZS_BF16 || dtype == ZS_FP16, "dtype must be bfloat16 or float16");
+    const at::ScalarType type = dtype == ZS_BF16 ? at::kBFloat16 : at::kHalf;
+    const at::Tensor& slots = tensor(a[2], "slots");
+    const int64_t N = slots.numel();
+    need(slots.dim() == 1 && N <= INT32_MAX, "slots must be int64 [N]");
+    ZsReadInt4 p{};
+    p.slots = vec<int64_t>(a[2], N, at::kLong, "slots", index);
+    p.err = err_word(a[5], index);
+    OnDevice on(index);
+    at::Tensor out[2];
+    for (int i = 0; i < 2; ++i) {
+        if (given(a[4])) {
+            need(PyTuple_Check(a[4]) && PyTuple_GET_SIZE(a[4]) == 2, "out must be a pair of tensors");
+            out[i] = tensor(PyTuple_GET_ITEM(a[4], i), "out");
+            need(out[i].dim() == 3 && out[i].size(0) == N && out[i].size(1) == pools.k.num_heads &&
+                     out[i].size(2) == pools.k.head_dim && out[i].scalar_type() == type && out[i].is_cuda() &&
+                     out[i].get_device() == index && out[i].is_contiguous() && aligned16(out[i]),
+                 "out must be two contiguous, aligned tensors [N, heads, dim] of dtype on the cache's device");
+        } else {
+            out[i] = fresh({N, pools.k.num_heads, pools.k.head_dim}, type, index);
+        }
+    }
+    p.k_out = ptr<uint16_t>(out[0]);
+    p.v_out = ptr<uint16_t>(out[1]);
+    p.stream = current_stream(index);
+    p.k_pool = pools.k;
+    p.v_pool = pools.v;
+    p.N = static_cast<int>(N);
+    p.dtype = static_cast<int>(dtype);
+    call(zs_read_int4, p, "zs_read_int4");
+    if (given(a[4])) {
+        Py_INCREF(a[4]);
+        return a[4];
+    }
+    return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(out[0])), THPVariable_Wrap(std::move(out[1])));
+}
+
+PyObject* paged_attention_int4(PyObject* const* a) {
+    const Int4Pools pools = int4_pools(a[1], a[2]);
+    const int index = pools.index;
+    const int64_t hkv = pools.k.num_heads;
+    const at::Tensor& q = tensor(a[0], "q");
+    const at::ScalarType type = half_type(q, "q");
+    OnDevice on(index);
+    const at::Tensor q3 = query(q, hkv, pools.k.head_dim, type, index);
+    const int64_t B = q3.size(0);
+    const Table table = block_table(a[3], B, index);
+    const int* lens = vec<int>(a[4], B, at::kInt, "seq_lens", index);
+    const Lists l = page_lists(a[6], a[7], B, hkv, pools.k.page_size, index);
+    ZsPagedAttentionInt4 p{};
+    p.k_pool = pools.k;
+    p.v_pool = pools.v;
+    p.dtype = dtype_code(type);
+    at::Tensor out = attend(p, Attended{q3, type, index, pools.k.page_size, table, lens, l.pages, l.counts, l.top,
+                                        err_word(a[11], index)},
+                            a[5], a[8], a[9], a[10], zs_paged_attention_int4_workspace, zs_paged_attention_int4,
+                            "zs_paged_attention_int4");
+    return THPVariable_Wrap(std::move(out));
 }
 
 // No C++ exception leaves a C entry: refusals are ValueErrors, the rest RuntimeErrors.
@@ -608,6 +780,7 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
     {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<name, n>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {ZS_ENTRY(plan_step, 10),    ZS_ENTRY(rope_write, 12),  ZS_ENTRY(paged_attention, 12),
                          ZS_ENTRY(page_bounds, 9),  ZS_ENTRY(select_pages, 10), ZS_ENTRY(sparse_attention, 13),
+                         ZS_ENTRY(rope_write_int4, 12), ZS_ENTRY(read_int4, 6), ZS_ENTRY(paged_attention_int4, 12),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_paged_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

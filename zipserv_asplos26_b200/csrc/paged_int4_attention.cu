@@ -1,0 +1,83 @@
+// Entry points of attention over a 4-bit paged KV cache: checks, the workspace and the
+// choice of the kernel (paged_int4_attention.cuh).
+#include "paged_int4_attention.cuh"
+
+namespace zs {
+namespace {
+
+inline int q4_max_ctas(int D, int G) {
+    if (G <= 8) return 148 * (D == 64 ? Q4Cfg<64, 1>::kCtas : Q4Cfg<128, 1>::kCtas);
+    return 148 * (D == 64 ? Q4Cfg<64, 2>::kCtas : Q4Cfg<128, 2>::kCtas);
+}
+
+// The checked arguments of a call, but for its workspace.
+bool int4_attention_args(const ZsPagedAttentionInt4* p, Q4Args* a, int* groups) {
+    Int4View k, v;
+    if (!p || !make_int4_pool(&p->k_pool, &k) || !make_int4_pool(&p->v_pool, &v) || !same_int4_pools(p->k_pool, p->v_pool))
+        return false;
+    const int B = p->B, Hq = p->Hq, Hkv = k.heads, top = p->top;
+    if (B < 0 || Hq <= 0 || Hq % Hkv || p->width <= 0 || p->table_stride < p->width || !std::isfinite(p->softmax_scale) ||
+        (p->dtype != ZS_BF16 && p->dtype != ZS_FP16))
+        return false;
+    if ((long long)B * Hq > INT32_MAX || (long long)p->width << k.page_shift > INT32_MAX) return false;
+    if (B && (!p->q || !p->block_table || !p->seq_lens || !p->out || !aligned16p(p->q) || !aligned16p(p->out)))
+        return false;
+    if (!p->pages != !p->counts || (p->pages && (top <= 0 || (long long)top << k.page_shift > INT32_MAX))) return false;
+    a->kp = {k.codes, k.c_block, k.c_token, k.c_head, k.num_blocks, k.page_shift, k.heads, k.dim};
+    a->vp = {v.codes, v.c_block, v.c_token, v.c_head, v.num_blocks, v.page_shift, v.heads, v.dim};
+    a->kpar = k.params;
+    a->kpar_block = k.p_block; a->kpar_token = k.p_token; a->kpar_head = k.p_head;
+    a->vpar = v.params;
+    a->vpar_block = v.p_block; a->vpar_token = v.p_token; a->vpar_head = v.p_head;
+    *groups = k.groups;
+    a->G = Hq / Hkv;
+    a->tiles = (a->G + kPaRows - 1) / kPaRows;
+    a->prow = std::min(a->G, kPaRows);
+    a->q = p->q;
+    a->table = p->block_table;
+    a->table_stride = p->table_stride;
+    a->lens = p->seq_lens;
+    a->pages = p->pages;
+    a->counts = p->counts;
+    a->B = B; a->Hq = Hq; a->Hkv = Hkv; a->width = p->width; a->top = top;
+    a->max_len = std::max(p->max_seqlen, 0);
+    a->scale2 = p->softmax_scale * kLog2e;
+    a->out = p->out;
+    a->lse = p->lse;
+    a->err = p->err;
+    return true;
+}
+
+size_t int4_workspace(const Q4Args& a) {
+    return run_workspace_bytes((long long)a.B * a.Hkv * a.tiles, q4_max_ctas(a.kp.dim, a.G), a.prow, a.kp.dim);
+}
+
+}  // namespace
+}  // namespace zs
+
+extern "C" size_t zs_paged_attention_int4_workspace(const ZsPagedAttentionInt4* p) {
+    using namespace zs;
+    Q4Args a{};
+    int groups;
+    if (!int4_attention_args(p, &a, &groups) || a.B == 0 ||
+        unit_warps(a, a.pages != nullptr, q4_max_ctas(a.kp.dim, a.G)))
+        return 0;
+    return int4_workspace(a);
+}
+
+extern "C" int zs_paged_attention_int4(const ZsPagedAttentionInt4* p) {
+    using namespace zs;
+    Q4Args a{};
+    int groups;
+    if (!int4_attention_args(p, &a, &groups)) return cudaErrorInvalidValue;
+    if (a.B == 0) return cudaSuccess;
+    const int max_ctas = q4_max_ctas(a.kp.dim, a.G), W = unit_warps(a, a.pages != nullptr, max_ctas);
+    if (!W) {
+        if (!p->ws || !aligned16p(p->ws) || p->ws_bytes < int4_workspace(a)) return cudaErrorInvalidValue;
+        lay_workspace(&a, p->ws, max_ctas);
+    }
+    cudaStream_t s = (cudaStream_t)p->stream;
+    if (p->dtype == ZS_BF16)
+        return a.pages ? int4_attention_bf16_listed(a, groups, W, s) : int4_attention_bf16(a, groups, W, s);
+    return a.pages ? int4_attention_fp16_listed(a, groups, W, s) : int4_attention_fp16(a, groups, W, s);
+}

@@ -1,0 +1,10 @@
+// Attention over a 4-bit cache, fp16 queries over lists of pages (paged_int4_attention.cuh).
+#include "paged_int4_attention.cuh"
+
+namespace zs {
+
+cudaError_t int4_attention_fp16_listed(const Q4Args& a, int groups, int W, cudaStream_t s) {
+    return launch_int4<__half, true>(a, groups, W, s);
+}
+
+}  // namespace zs

@@ -12,12 +12,16 @@ a table on the host, so a step can be captured in a CUDA graph:
 * page_bounds, select_pages, sparse_attention
                     8-bit bounds of complete pages, the choice of pages by
                     those bounds, attention over the chosen pages
+* rope_write_int4, read_int4, paged_attention_int4
+                    the write, its reverse and attention for pages held in 4
+                    bits (Int4Pages)
 * PagedKVCache      the buffers, and the calls above on them
 
 A page pool is a tensor of logical shape [num_blocks, page_size, heads, dim],
 bf16 or fp16, its last axis contiguous and the others of any strides that are
 multiples of 8 elements: `torch.empty(blocks, heads, page, dim).transpose(1, 2)`
-keeps each head's rows of a page together. Every call runs on the current
+keeps each head's rows of a page together. A 4-bit pool is an Int4Pages, in either
+order too. Every call runs on the current
 stream of its tensors' device and synchronises nothing. `err` (optional, int32[1])
 collects error bits: 2 = an index was out of range (skipped; a position: taken as
 0), 4 = a request was refused by plan_step.
@@ -153,6 +157,76 @@ def sparse_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     return (o if q.dim() == 3 and out is None else o.view(q.shape)), pages, counts
 
 
+# ------------------------------------------------------------- 4-bit pages
+class Int4Pages(NamedTuple):
+    """A pool of pages in 4 bits. Channels come in groups of 32 or 64 of a token's row of one
+    head (dim 64 or 128); a channel stands for c + s (u - 8), u its 4-bit code, s and c its
+    group's scale and centre:
+
+        s = bf16((max - min) / 15), c = bf16(min + 8 s), u = clamp(rint((x - c) / s) + 8, 0, 15)
+
+    in fp32, so it is off by s / 2 at most, or (15 s + |c|) / 256 more at the group's ends.
+    4.5 bits a value with groups of 64, 5 with 32. A group whose scale is below 2**-126 has
+    s = 0, c = bf16(min) and codes of 8; one with a value that is not finite (or whose
+    max - min is not) reads back as NaN.
+
+    Both tensors have contiguous rows and any strides otherwise (codes: multiples of 16;
+    params: of a row's size)."""
+    codes: torch.Tensor     # uint8 [num_blocks, page_size, heads, dim / 2], channel 2i in the low half of byte i
+    params: torch.Tensor    # bfloat16 [num_blocks, page_size, heads, 2, dim / group]: scales, then centres
+
+
+def int4_pages(num_blocks: int, page_size: int, num_heads: int, head_dim: int, group: int = 64,
+               layout: str = "heads", device="cuda") -> Int4Pages:
+    """A pool whose rows read back as zeros; layout "heads" keeps each head's rows of a page
+    together, "tokens" each token's heads."""
+    if min(num_blocks, num_heads) <= 0:
+        raise ValueError("sizes must be positive")
+    if layout not in ("heads", "tokens"):
+        raise ValueError(f"unknown layout {layout!r}")
+    if head_dim not in (64, 128) or group not in (32, 64):
+        raise ValueError("4-bit pages hold heads of dim 64 or 128 in groups of 32 or 64")
+    if not 16 <= page_size <= 256 or page_size & (page_size - 1):
+        raise ValueError("page_size must be a power of two from 16 to 256")
+    at = (num_blocks, num_heads, page_size) if layout == "heads" else (num_blocks, page_size, num_heads)
+    codes = torch.full((*at, head_dim // 2), 0x88, dtype=torch.uint8, device=device)
+    params = torch.zeros(*at, 2, head_dim // group, dtype=torch.bfloat16, device=device)
+    return Int4Pages(codes.transpose(1, 2), params.transpose(1, 2)) if layout == "heads" else Int4Pages(codes, params)
+
+
+def rope_write_int4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+                    slots: torch.Tensor, k_pages: Int4Pages, v_pages: Int4Pages,
+                    sections: Optional[Sequence[int]] = None, interleaved: bool = False,
+                    q_out: Optional[torch.Tensor] = None, err: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """rope_write into a 4-bit cache: k, turned in fp32, and v are quantised as they are
+    written; returns the turned q. The arguments are rope_write's but for the pools; q, k
+    and v are bf16 or fp16, whatever was written before."""
+    return (_native or _load()).rope_write_int4(q, k, v, positions, cos_sin, slots, k_pages, v_pages, sections,
+                                                interleaved, q_out, err)
+
+
+def read_int4(k_pages: Int4Pages, v_pages: Int4Pages, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
+              out=None, err: Optional[torch.Tensor] = None):
+    """Rows of a 4-bit cache by slot (int64 [N], block * page_size + row): (k, v), each
+    [N, heads, dim] of dtype (bf16 or fp16), what the codes stand for rounded once. A slot of
+    -1 gives zeros. out (optional) is a pair of contiguous tensors to write to."""
+    kind = {torch.bfloat16: 0, torch.float16: 1}.get(dtype, -1)
+    return (_native or _load()).read_int4(k_pages, v_pages, slots, kind, out, err)
+
+
+def paged_attention_int4(q: torch.Tensor, k_pages: Int4Pages, v_pages: Int4Pages, block_table: torch.Tensor,
+                         seq_lens: torch.Tensor, softmax_scale: Optional[float] = None,
+                         pages: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
+                         out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                         max_seqlen: Optional[int] = None, err: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_attention over a 4-bit cache, q bf16 or fp16 (below 2**63 in magnitude). Keys and
+    values are what the codes stand for, not rounded to q's type in between. The arguments are
+    paged_attention's but for the pools."""
+    o = (_native or _load()).paged_attention_int4(q, k_pages, v_pages, block_table, seq_lens, softmax_scale, pages,
+                                                  counts, out, lse, max_seqlen, err)
+    return o if q.dim() == 3 and out is None else o.view(q.shape)
+
+
 # ------------------------------------------------------------------- cache
 class TokenRows(NamedTuple):
     """What each token of a plan attends: the pages of its row, up to itself."""
@@ -178,11 +252,15 @@ class PagedKVCache:
     All state (tables, lengths, the free list) is on the GPU in fixed buffers, so
     a step can be captured in a CUDA graph and replayed. layout "heads" keeps
     each head's rows of a page together, "tokens" each token's heads. bounds
-    keeps the pages' 8-bit bounds for sparse_attention."""
+    keeps the pages' 8-bit bounds for sparse_attention (default: where bits is 16).
+
+    bits 4 holds the pages as Int4Pages (groups of `group` channels) in 28% of the room
+    (31% with groups of 32): write quantises, attention reads the codes, and read gives
+    rows back in dtype. Such a cache keeps no bounds."""
 
     def __init__(self, num_blocks: int, max_batch: int, max_blocks_per_seq: int, num_kv_heads: int,
                  head_dim: int = 128, page_size: int = 64, dtype: torch.dtype = torch.bfloat16, layout: str = "heads",
-                 bounds: bool = True, num_layers: int = 1, device="cuda"):
+                 bounds: Optional[bool] = None, num_layers: int = 1, device="cuda", bits: int = 16, group: int = 64):
         if min(num_blocks, max_batch, max_blocks_per_seq, num_kv_heads, num_layers) <= 0:
             raise ValueError("sizes must be positive")
         if layout not in ("heads", "tokens"):
@@ -191,9 +269,17 @@ class PagedKVCache:
             raise ValueError("pages hold bf16 or fp16 heads of dim 64 or 128")
         if not 16 <= page_size <= 256 or page_size & (page_size - 1):
             raise ValueError("page_size must be a power of two from 16 to 256")
+        if bits not in (4, 16):
+            raise ValueError("pages hold 4 or 16 bits a value")
+        if bits == 4 and bounds:
+            raise ValueError("a 4-bit cache keeps no bounds")
+        bounds = bits == 16 if bounds is None else bounds
         self.Hkv, self.D, self.page_size, self.max_batch = num_kv_heads, head_dim, page_size, max_batch
+        self.bits, self.dtype = bits, dtype
 
         def pool():
+            if bits == 4:
+                return int4_pages(num_blocks, page_size, num_kv_heads, head_dim, group, layout, device)
             if layout == "heads":
                 return torch.zeros(num_blocks, num_kv_heads, page_size, head_dim, dtype=dtype,
                                    device=device).transpose(1, 2)
@@ -201,7 +287,7 @@ class PagedKVCache:
 
         self.k = [pool() for _ in range(num_layers)]
         self.v = [pool() for _ in range(num_layers)]
-        self.device = self.k[0].device
+        self.device = (self.k[0].codes if bits == 4 else self.k[0]).device
         i32 = dict(dtype=torch.int32, device=self.device)
         self.block_table = torch.full((max_batch, max_blocks_per_seq), -1, **i32)
         self.seqlens = torch.zeros(max_batch, **i32)
@@ -234,13 +320,24 @@ class PagedKVCache:
               interleaved: bool = False) -> torch.Tensor:
         """rope_write of the step's tokens (positions default to the plan's), then
         the bounds of the pages that it completed."""
-        q = rope_write(q, k, v, plan.positions if positions is None else positions, cos_sin, plan.slots,
-                       self.k[layer], self.v[layer], sections, interleaved, None, self.err)
+        put = rope_write_int4 if self.bits == 4 else rope_write
+        q = put(q, k, v, plan.positions if positions is None else positions, cos_sin, plan.slots, self.k[layer],
+                self.v[layer], sections, interleaved, None, self.err)
         if self.codes is not None:
             n = plan.slots.numel()
             page_bounds(self.k[layer], self.block_table, self.lens_before, self.seqlens, self.codes[layer],
                         self.scales[layer], n, n, self.err)
         return q
+
+    def read(self, slots: torch.Tensor, layer: int = 0):
+        """The rows of a layer at slots (int64 [N]; -1: zeros), such as a plan's: (k, v), each
+        [N, heads, dim] of the cache's dtype."""
+        if self.bits == 4:
+            return read_int4(self.k[layer], self.v[layer], slots, self.dtype, None, self.err)
+        at = slots.clamp(min=0)
+        block, row = at // self.page_size, at % self.page_size
+        dead = (slots < 0).view(-1, 1, 1)
+        return self.k[layer][block, row].masked_fill_(dead, 0), self.v[layer][block, row].masked_fill_(dead, 0)
 
     def token_rows(self, plan: StepPlan) -> TokenRows:
         """The rows that the tokens of the last step's plan attend (causal: a token
@@ -260,8 +357,9 @@ class PagedKVCache:
         without rows q is one query per row, of rows 0 .. N-1 (max_seqlen: see
         paged_attention)."""
         table, lens = self._rows(q, rows)
-        return paged_attention(q, self.k[layer], self.v[layer], table, lens, softmax_scale, None, None, out, lse,
-                               max_seqlen, self.err)
+        attend = paged_attention_int4 if self.bits == 4 else paged_attention
+        return attend(q, self.k[layer], self.v[layer], table, lens, softmax_scale, None, None, out, lse, max_seqlen,
+                      self.err)
 
     def sparse_attention(self, q: torch.Tensor, top_pages: int, layer: int = 0, sink_pages: int = 1,
                          local_pages: int = 1, softmax_scale: Optional[float] = None,
