@@ -57,11 +57,14 @@ def attention_error(q, k, v, kparams, scale, longest):
     """A bound on what attention in fp32 over 4-bit pages is off before the output is rounded,
     relative to max |v|. Scores in base 2: sums of dim + 8 terms, none of which, nor a partial
     sum, passes (15 s + |c|) sum |q|, each addition losing 2^-23 (tensor cores cut). Both sums of
-    the softmax get it. Weights: parts in bf16 and its remainder (2^-16), the exponential (2^-22);
-    sums over the tokens in steps of 8 or more, of terms up to 3 max |v| (|c| + 8 s)."""
+    the softmax get it. Weights: in two bf16 parts (2^-16) and the exponential (2^-22) for the
+    centres; times the scale, in fp16 for the codes, half a step or 2^-11 for bf16 queries (and
+    its remainder, then 2^-22, for fp16 ones), of s |u - 8| = |v - c|, at most 2 max |v|; sums
+    over the tokens in steps of 8 or more, of terms up to 3 max |v| (|c| + 8 s)."""
     if k.numel() == 0:
         return 0.0
     s, c = kparams.double().unbind(-2)
     most = float((15 * s + c.abs()).nan_to_num(0.0).max()) * float(q.double().abs().sum(-1).max())
     d = q.shape[-1]
-    return 2 * (d + 8) * 2.0 ** -23 * most * abs(scale) + 3 * 2.0 ** -16 + (longest / 8 + 16) * 3 * 2.0 ** -23
+    part = 2.0 ** -10 if q.dtype == BF else 0.0
+    return 2 * (d + 8) * 2.0 ** -23 * most * abs(scale) + 3 * 2.0 ** -16 + part + (longest / 8 + 16) * 3 * 2.0 ** -23

@@ -489,7 +489,7 @@ struct PaRing {
         int lim = 0;
         if (s < steps) {
             int blk, ch, h;
-            lim = find(blk, ch, h, s);
+            lim = find(blk, ch, h, s, 0);
             copy_chunk<D>(a, slot(s), blk, ch, h, lim, policy);
         }
         cp_commit();
@@ -518,7 +518,7 @@ template <typename T_, int D_, bool kListed_>
 struct PaBase {
     using T = T_;
     using Args = PaArgs;
-    static constexpr int D = D_;
+    static constexpr int D = D_, kParts = 1;
     static constexpr bool kListed = kListed_, kOdd = true;
     static constexpr float kBias = kPBias<T>;
     template <int kCount>
@@ -532,6 +532,7 @@ struct PaForm : PaBase<T, D, kListed>, PaCfg<D, kNarrow> {
     using Joined = PaBase<T, D, kListed>;
     using State = typename PaStateOf<T, D, kNarrow>::type;
     using Ring = PaRing<D, kNarrow>;
+    __device__ __forceinline__ static void start(State& st, const PaArgs&, const uint16_t* q, int rows) { st.start(q, rows); }
 };
 
 // CTAs of the run kernel, at most.
@@ -605,7 +606,7 @@ bool attention_args(const ZsPagedAttention* p, PaArgs* a) {
 extern "C" size_t zs_paged_attention_workspace(const ZsPagedAttention* p) {
     using namespace zs;
     PaArgs a{};
-    if (!attention_args(p, &a) || a.B == 0 || unit_warps(a, a.pages != nullptr, pa_max_ctas(a.kp.dim, a.G))) return 0;
+    if (!attention_args(p, &a) || a.B == 0 || unit_warps(a, a.pages != nullptr, pa_max_ctas(a.kp.dim, a.G), 1)) return 0;
     return zs_paged_attention_workspace_bytes(a.B, a.Hq, a.Hkv, a.kp.dim);
 }
 
@@ -614,7 +615,7 @@ extern "C" int zs_paged_attention(const ZsPagedAttention* p) {
     PaArgs a{};
     if (!attention_args(p, &a)) return cudaErrorInvalidValue;
     if (a.B == 0) return cudaSuccess;
-    const int max_ctas = pa_max_ctas(a.kp.dim, a.G), W = unit_warps(a, a.pages != nullptr, max_ctas);
+    const int max_ctas = pa_max_ctas(a.kp.dim, a.G), W = unit_warps(a, a.pages != nullptr, max_ctas, 1);
     if (!W) {
         if (!p->ws || !aligned16p(p->ws) ||
             p->ws_bytes < zs_paged_attention_workspace_bytes(a.B, a.Hq, a.Hkv, a.kp.dim))

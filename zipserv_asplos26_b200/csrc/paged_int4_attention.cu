@@ -25,10 +25,20 @@ bool int4_attention_args(const ZsPagedAttentionInt4* p, Q4Args* a, int* groups) 
     if (!p->pages != !p->counts || (p->pages && (top <= 0 || (long long)top << k.page_shift > INT32_MAX))) return false;
     a->kp = {k.codes, k.c_block, k.c_token, k.c_head, k.num_blocks, k.page_shift, k.heads, k.dim};
     a->vp = {v.codes, v.c_block, v.c_token, v.c_head, v.num_blocks, v.page_shift, v.heads, v.dim};
-    a->kpar = k.params;
-    a->kpar_block = k.p_block; a->kpar_token = k.p_token; a->kpar_head = k.p_head;
-    a->vpar = v.params;
-    a->vpar_block = v.p_block; a->vpar_token = v.p_token; a->vpar_head = v.p_head;
+    auto places = [](Q4Places* x, const void* base, long long block, long long token, long long head) {
+        x->base = static_cast<const uint8_t*>(base);
+        x->block = (uint32_t)block;
+        x->token = (uint32_t)token;
+        x->head = (uint32_t)head;
+        return block <= UINT32_MAX && token <= UINT32_MAX && head <= UINT32_MAX;
+    };
+    if (!places(&a->kcode, k.codes, k.c_block, k.c_token, k.c_head) ||
+        !places(&a->vcode, v.codes, v.c_block, v.c_token, v.c_head) ||
+        !places(&a->kpar, k.params, 2 * k.p_block, 2 * k.p_token, 2 * k.p_head) ||
+        !places(&a->vpar, v.params, 2 * v.p_block, 2 * v.p_token, 2 * v.p_head))
+        return false;
+    const uint32_t row = k.dim / 2, par = 4 * k.groups;
+    a->packed = k.page_shift > 4 && a->kcode.token == row && a->vcode.token == row && a->kpar.token == par && a->vpar.token == par;
     *groups = k.groups;
     a->G = Hq / Hkv;
     a->tiles = (a->G + kPaRows - 1) / kPaRows;
@@ -60,7 +70,7 @@ extern "C" size_t zs_paged_attention_int4_workspace(const ZsPagedAttentionInt4* 
     Q4Args a{};
     int groups;
     if (!int4_attention_args(p, &a, &groups) || a.B == 0 ||
-        unit_warps(a, a.pages != nullptr, q4_max_ctas(a.kp.dim, a.G)))
+        unit_warps(a, a.pages != nullptr, q4_max_ctas(a.kp.dim, a.G), kQ4Parts))
         return 0;
     return int4_workspace(a);
 }
@@ -71,7 +81,7 @@ extern "C" int zs_paged_attention_int4(const ZsPagedAttentionInt4* p) {
     int groups;
     if (!int4_attention_args(p, &a, &groups)) return cudaErrorInvalidValue;
     if (a.B == 0) return cudaSuccess;
-    const int max_ctas = q4_max_ctas(a.kp.dim, a.G), W = unit_warps(a, a.pages != nullptr, max_ctas);
+    const int max_ctas = q4_max_ctas(a.kp.dim, a.G), W = unit_warps(a, a.pages != nullptr, max_ctas, kQ4Parts);
     if (!W) {
         if (!p->ws || !aligned16p(p->ws) || p->ws_bytes < int4_workspace(a)) return cudaErrorInvalidValue;
         lay_workspace(&a, p->ws, max_ctas);

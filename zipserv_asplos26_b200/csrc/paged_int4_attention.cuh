@@ -10,20 +10,24 @@
 // they are, and scales and centres are applied to sums:
 //   * Four bits anywhere in the low eight of a 16-bit float are a whole number times its
 //     smallest step (2^-133 for bf16, 2^-24 for fp16), exact in a product: one AND makes
-//     two operands, with one shift for every four. What sits four bits up counts 16-fold
-//     and has sums of its own.
+//     two operands, with one shift for every four. What sits four bits up counts 16-fold,
+//     and meets a q of a sixteenth (scores) or has sums of its own (outputs).
 //   * Scores: sum_g s_g (q_g . u_g) + sum_g (c_g - 8 s_g) sum(q_g). The second part is a
 //     product too, of the row of parameters with q's sums (in three bf16 parts, 24 bits).
-//     Keys are the rows (16 tokens), heads the columns, 8 or twice 8.
-//   * Outputs: sum_t (p_t s_t) (u_t - 8) + sum_t p_t c_t. The codes are centred by a
-//     bf16x2 add, exact: sums of codes from 0 to 15 would be far larger than the outputs
-//     that are left of them, and a tensor core's sums lose low bits. p s, and p for the
-//     centres, are fed as a bf16 high part plus its bf16 remainder (2^-16 is left out).
-// q (bf16) and p s are scaled by 2^64 on the way in, so that neither they nor the
-// products leave fp32's range; powers of two are exact.
+//     Keys are the rows (16 tokens), heads the columns, 8 or twice 8. q is scaled by a
+//     power of two (bf16: 2^64; fp16: to its type's top), which loses nothing that counts.
+//   * Outputs: sum_t (p_t s_t) (u_t - 8) + sum_t p_t c_t. p s goes in as fp16, scaled by a
+//     power of two that follows the largest scale of the group so far, so that it has all
+//     11 bits from there down to 2^-26 of it and vanishes below 2^-37. For bf16 outputs
+//     that is all: 2^-11 of a weight is an eighth of the output's own rounding. For fp16
+//     ones its remainder follows as a second part. The centres meet p in two bf16 parts.
+//     The codes are centred afterwards, every 128 tokens (64 for fp16): sums of codes from
+//     0 to 15 would in the end be far larger than the outputs that are left of them, and a
+//     tensor core's sums lose low bits. (Centring each code before its product took 32
+//     instructions of some 350 for every 16 tokens.)
 //
-// The maximum that exponents refer to follows the scores only where one passes it by 8
-// or more (base 2), so that most chunks need no maximum over their lanes.
+// The maximum that exponents refer to follows the scores only where one passes it by 2
+// or more (base 2), so that most steps need no maximum over their lanes.
 #pragma once
 
 #include "paged_int4.cuh"
@@ -31,16 +35,20 @@
 
 namespace zs {
 
-struct Q4Args : PaArgs {          // kp and vp: the codes, strides in bytes
-    const uint16_t* kpar;
-    const uint16_t* vpar;
-    long long kpar_block, kpar_token, kpar_head, vpar_block, vpar_token, vpar_head;
+// Rows by place: strides in bytes, below 2^32, so that an address is a few multiply-adds.
+struct Q4Places {
+    const uint8_t* base;
+    uint32_t block, token, head;
+};
+struct Q4Args : PaArgs {          // kp and vp: the codes (for page size, blocks and heads)
+    Q4Places kcode, vcode, kpar, vpar;
+    int packed;                   // rows of a page's head follow one another, 32 or more of them
 };
 
 namespace {
 
-constexpr float kTwo64 = 18446744073709551616.f;
-constexpr float kTwo24 = 16777216.f;
+constexpr int kQ4Parts = 2;     // a step takes 32 tokens: see Q4Ring
+constexpr int kNoTop = -100, kMostTop = 100;        // of scales that count: 2^-100 to 2^100
 constexpr uint32_t kLowCodes = 0x000F000Fu, kHighCodes = 0x00F000F0u;
 
 template <int D>
@@ -48,7 +56,7 @@ struct Q4Tile {
     static constexpr int kRow = D / 2;                       // bytes of a row's codes
     static constexpr int kCodes = kPaChunk * kRow;
     static constexpr int kParams = kPaChunk * 16;            // a row's parameters in 16 bytes
-    static constexpr int kTile = kCodes + kParams;           // one K or V chunk
+    static constexpr int kTile = kCodes + kParams;           // keys or values of a part
     // the 16-byte piece of a row in shared memory: eight rows' pieces fill all banks
     __device__ __forceinline__ static int place(int r, int piece) {
         return r * kRow + (piece ^ (D == 128 ? (r >> 1) & 3 : (r >> 2) & 1)) * 16;
@@ -57,29 +65,25 @@ struct Q4Tile {
 
 template <int D, int NT>
 struct Q4Cfg {
-    static constexpr int kCtas = NT == 1 ? 4 : 3;
-    static constexpr int kStages = 4;
-    static constexpr int kChunkBytes = 2 * Q4Tile<D>::kTile;
+    static constexpr int kCtas = NT == 1 ? 3 : 2;
+    static constexpr int kStages = 3;
+    static constexpr int kPartBytes = 2 * Q4Tile<D>::kTile;
+    static constexpr int kChunkBytes = kQ4Parts * kPartBytes;
     static constexpr int kPiece = kPaRows * (D + 2) * 4;     // a warp's piece in the units kernel
     static constexpr int kRing = kStages * kChunkBytes > kPiece ? kStages * kChunkBytes : kPiece;
     static constexpr int kSmem = kPaWarps * kRing;
 };
 
-__device__ __forceinline__ void ldsm2(uint32_t (&r)[2], uint32_t a) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(a) : "memory");
-}
-__device__ __forceinline__ void ldsm2t(uint32_t (&r)[2], uint32_t a) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];"
-                 : "=r"(r[0]), "=r"(r[1])
-                 : "r"(a)
-                 : "memory");
-}
 __device__ __forceinline__ float exp2_fast(float x) {        // 2 ulp; below 2^-126 it is zero
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Bytes bytes (4, 8 or 16) of parameters.
+__device__ __forceinline__ void cp16_all(uint32_t dst, const void* src, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy)
+                 : "memory");
+}
+// kBytes bytes (4, 8 or 16) of parameters.
 template <int kBytes>
 __device__ __forceinline__ void cp_params(uint32_t dst, const void* src, bool on, uint64_t policy) {
     if constexpr (kBytes == 16)
@@ -91,21 +95,57 @@ __device__ __forceinline__ void cp_params(uint32_t dst, const void* src, bool on
                      "n"(kBytes), "r"(on ? kBytes : 0), "l"(policy)
                      : "memory");
 }
-// The kN scales (bf16) at the start of a row of parameters, in fp32.
+// The kN scales (bf16) at the start of a row of parameters: two a word, and one of them in fp32.
 template <int kN>
-__device__ __forceinline__ void ld_scales(float (&s)[kN], uint32_t at) {
-    uint32_t w[2];
+__device__ __forceinline__ void ld_scales(uint32_t (&w)[(kN + 1) / 2], uint32_t at) {
     if constexpr (kN == 4)
         asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
-    else
+    else if constexpr (kN == 2)
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
-#pragma unroll
-    for (int g = 0; g < kN; ++g) s[g] = g & 1 ? __uint_as_float(w[g / 2] & 0xFFFF0000u) : bf16_bits_to_float(w[g / 2]);
+    else {
+        uint16_t x;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(at) : "memory");
+        w[0] = x;
+    }
 }
-__device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
+template <int kN>
+__device__ __forceinline__ float scale_of(const uint32_t (&w)[(kN + 1) / 2], int g) {
+    return g & 1 ? __uint_as_float(w[g / 2] & 0xFFFF0000u) : bf16_bits_to_float(w[g / 2]);
 }
+// The larger of each of two bf16 numbers that are not negative.
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// mma16816, free to move among other work, and from sums of a column's own.
+__device__ __forceinline__ void product(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+        "%2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void product(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+        "%2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void first_product(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
+                                              float c1, __nv_bfloat16) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, "
+        "%10, %11};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void first_product(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0,
+                                              float c1, __half) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, "
+        "%10, %11};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }   // e from -126 to 127
 
 // What a warp holds of a unit of up to NT x 8 heads. A lane has heads 2 (lane % 4) and
 // the next of each eight; of scores, tokens lane / 4 and lane / 4 + 8; of outputs the
@@ -114,59 +154,93 @@ template <typename T, int D, int NG, int NT>
 struct Q4State {
     static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     static constexpr int kBlocks = D / 32, kPer = kBlocks / NG;      // 32 channels: a 16-byte piece of a row
+    static constexpr int kTerms = kBf16 ? 1 : 2;                     // fp16 parts of p s
+    static constexpr int kSettle = kBf16 ? 4 : 2;                    // steps after which codes are centred
     using Bf = __nv_bfloat16;
-    uint32_t qf[NT][kBlocks][2][2];    // q of the even, odd channels
-    uint32_t zf[NT][3];                // of what meets the parameters: -8 sum(q_g), sum(q_g), in three parts
+    uint32_t qf[NT][kBlocks][2][2];    // q of the even, odd channels (these a sixteenth)
+    uint32_t zf[NT][3];                // of what meets the parameters: -8 sum(q_g), sum(q_g), times scale2, in three parts
+    float unit[NT][2];                 // of the sums over codes, with scale2
     float o[NT][kBlocks][2][4];        // sums of the even, odd channels
     float z[NT][4];                    // sums of p times the parameters
-    float m[NT][2], l[NT][2];
+    float m[NT][2], l[NT][2];          // largest score, sum of weights
+    float less[NT][2], most[NT][2];    // scores count from ref = m + top - 13 = -less; at most `most` from there
+    int top;                           // scales of values are below 2^top, weights times them below 2^15
+    int owed;                          // steps whose codes are still to be centred
 
-    struct Weights {
-        float p[NT][4];
-    };
+    using Four = float[NT][4];         // of a lane's tokens of a part and heads
 
-    __device__ __forceinline__ void start(const uint16_t* q, int rows) {
+    __device__ __forceinline__ void start(const uint16_t* q, int rows, float scale2) {
         const int lane = threadIdx.x & 31;
+        top = kNoTop;
+        owed = 0;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int head = nt * 8 + (lane >> 2);
-            float sum[NG];
+            uint32_t w[kBlocks][4];
+            float sum[NG], peak = 0.f;
 #pragma unroll
             for (int g = 0; g < NG; ++g) sum[g] = 0.f;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
                 uint4 x = make_uint4(0u, 0u, 0u, 0u);
                 if (head < rows) x = *reinterpret_cast<const uint4*>(q + (long long)head * D + b * 32 + (lane & 3) * 8);
-                uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                w[b][0] = x.x;
+                w[b][1] = x.y;
+                w[b][2] = x.z;
+                w[b][3] = x.w;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float2 f = unpack2<T>(w[i]);
+                    const float2 f = unpack2<T>(w[b][i]);
                     sum[b / kPer] += f.x + f.y;
-                    if constexpr (kBf16) w[i] = pack2<T>(f.x * kTwo64, f.y * kTwo64);
+                    peak = fmaxf(peak, fmaxf(fabsf(f.x), fabsf(f.y)));
+                }
+            }
+            // bf16: 2^64; fp16: the head's largest below 2^15 (even channels) and 2^11 (odd ones)
+            int e = 64;
+            if constexpr (!kBf16) {
+                peak = fmaxf(peak, __shfl_xor_sync(~0u, peak, 1));
+                peak = fmaxf(peak, __shfl_xor_sync(~0u, peak, 2));
+                e = 14 - ((__float_as_int(peak) >> 23) - 127);
+                e = min(e, 60);                          // a head of zeros
+                if (e < -1) e = 0;                       // a head with infinities or NaN
+            }
+            const float even = power_of_two(e), odd = power_of_two(e - 4);
+            // codes in steps of 2^-133 or 2^-24; of the lane's heads
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int ej = __shfl_sync(~0u, e, ((lane & 3) * 2 + j) * 4);
+                unit[nt][j] = kBf16 ? scale2 * power_of_two(69) : scale2 * power_of_two(24 - ej);
+            }
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {            // channels 2i (even) and 2i + 1 (odd)
+                    const float2 f = unpack2<T>(w[b][i]);
+                    w[b][i] = pack2<T>(f.x * even, f.y * odd);
                 }
                 // codes of channels i and i + 4 lie 16 bits apart
-                qf[nt][b][0][0] = __byte_perm(w[0], w[2], 0x5410);
-                qf[nt][b][0][1] = __byte_perm(w[1], w[3], 0x5410);
-                qf[nt][b][1][0] = __byte_perm(w[0], w[2], 0x7632);
-                qf[nt][b][1][1] = __byte_perm(w[1], w[3], 0x7632);
+                qf[nt][b][0][0] = __byte_perm(w[b][0], w[b][2], 0x5410);
+                qf[nt][b][0][1] = __byte_perm(w[b][1], w[b][3], 0x5410);
+                qf[nt][b][1][0] = __byte_perm(w[b][0], w[b][2], 0x7632);
+                qf[nt][b][1][1] = __byte_perm(w[b][1], w[b][3], 0x7632);
             }
-            float e[2] = {0.f, 0.f};                 // of parameters 2 (lane % 4) and the next
+            float y[2] = {0.f, 0.f};                     // of parameters 2 (lane % 4) and the next
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 sum[g] += __shfl_xor_sync(~0u, sum[g], 1);
                 sum[g] += __shfl_xor_sync(~0u, sum[g], 2);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    if ((lane & 3) * 2 + i == g) e[i] = -8.f * sum[g];
-                    if ((lane & 3) * 2 + i == NG + g) e[i] = sum[g];
+                    if ((lane & 3) * 2 + i == g) y[i] = -8.f * (sum[g] * scale2);
+                    if ((lane & 3) * 2 + i == NG + g) y[i] = sum[g] * scale2;
                 }
             }
 #pragma unroll
             for (int i = 0; i < 3; ++i) {
-                zf[nt][i] = pack2<Bf>(e[0], e[1]);
+                zf[nt][i] = pack2<Bf>(y[0], y[1]);
                 const float2 back = unpack2<Bf>(zf[nt][i]);
-                e[0] -= back.x;
-                e[1] -= back.y;
+                y[0] -= back.x;
+                y[1] -= back.y;
             }
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b)
@@ -175,28 +249,36 @@ struct Q4State {
 #pragma unroll
             for (int i = 0; i < 4; ++i) z[nt][i] = 0.f;
             m[nt][0] = m[nt][1] = -INFINITY;
+            less[nt][0] = less[nt][1] = 0.f;
+            most[nt][0] = most[nt][1] = -INFINITY;
             l[nt][0] = l[nt][1] = 0.f;
         }
     }
 
-    // Scores (times scale2) of the chunk whose keys are at kt.
-    __device__ __forceinline__ void scores(uint32_t kt, float scale2, float (&x)[NT][4]) {
+    // The scales of a part's keys or values, at `at`: of a lane's two tokens.
+    using Scales = uint32_t[2][(NG + 1) / 2];
+    __device__ __forceinline__ void look(uint32_t at, Scales& v) {
+        const uint32_t par = at + Q4Tile<D>::kCodes + ((threadIdx.x & 31) >> 2) * 16;
+        ld_scales<NG>(v[0], par);
+        ld_scales<NG>(v[1], par + 8 * 16);
+    }
+
+    // Scores (times scale2, from ref on) of the part whose keys are at kt.
+    __device__ __forceinline__ void scores(uint32_t kt, Four& x) {
         const int lane = threadIdx.x & 31, r = lane & 15, half = lane >> 4;
         const uint32_t par = kt + Q4Tile<D>::kCodes;
-        float sc[2][NG], c[NT][4], s[NT][4];
-        ld_scales<NG>(sc[0], par + (lane >> 2) * 16);
-        ld_scales<NG>(sc[1], par + ((lane >> 2) + 8) * 16);
-        uint32_t pr[2];
-        ldsm2(pr, par + r * 16);
-        const uint32_t a2[4] = {pr[0], pr[1], pr[0], pr[1]}, a1[4] = {pr[0], pr[1], 0u, 0u};
+        float c[NT][4], s[NT][4];
+        Scales sc;
+        look(kt, sc);
+        // the rows of parameters twice over: what they meet is in the two halves of the depth
+        uint32_t pr[4];
+        ldsm4(pr, par + r * 16);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[nt][i] = c[nt][i] = 0.f;
-            mma16816(c[nt], a2, zf[nt][0], zf[nt][1], Bf());
-            mma16816(c[nt], a1, zf[nt][2], 0u, Bf());
+            first_product(c[nt], pr, zf[nt][0], zf[nt][1], less[nt][0], less[nt][1], Bf());
+            product(c[nt], pr, zf[nt][2], 0u, Bf());
         }
-        float e[NT][2][4];
+        float e[NT][4];
 #pragma unroll
         for (int b2 = 0; b2 < kBlocks / 2; ++b2) {
             uint32_t f[4];
@@ -209,101 +291,131 @@ struct Q4State {
                 const uint32_t hi[4] = {u & kHighCodes, w & kHighCodes, u8 & kHighCodes, w8 & kHighCodes};
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    if (b % kPer == 0) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) e[nt][0][j] = e[nt][1][j] = 0.f;
-                    }
-                    mma16816(e[nt][0], lo, qf[nt][b][0][0], qf[nt][b][0][1], T());
-                    mma16816(e[nt][1], hi, qf[nt][b][1][0], qf[nt][b][1][1], T());
+                    if (b % kPer == 0) first_product(e[nt], lo, qf[nt][b][0][0], qf[nt][b][0][1], 0.f, 0.f, T());
+                    else product(e[nt], lo, qf[nt][b][0][0], qf[nt][b][0][1], T());
+                    product(e[nt], hi, qf[nt][b][1][0], qf[nt][b][1][1], T());
                     if (b % kPer == kPer - 1) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) s[nt][j] += sc[j >> 1][g] * (e[nt][0][j] + e[nt][1][j] * 0.0625f);
+                        for (int j = 0; j < 4; ++j) {
+                            const float k = scale_of<NG>(sc[j >> 1], g);
+                            s[nt][j] = g ? s[nt][j] + k * e[nt][j] : k * e[nt][j];
+                        }
                     }
                 }
             }
         }
-        // codes in steps of 2^-133 against q times 2^64, or in steps of 2^-24
-        const float unit = kBf16 ? scale2 * (kTwo64 * 32.f) : scale2 * kTwo24;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[nt][i] = s[nt][i] * unit + c[nt][i] * scale2;
+            for (int i = 0; i < 4; ++i) x[nt][i] = s[nt][i] * unit[nt][i & 1] + c[nt][i];
     }
 
-    // Weights 2^(x - m) of a chunk's first `lim` tokens.
-    __device__ __forceinline__ void weigh(float (&x)[NT][4], int lim, Weights& w) {
+    // From scores x - ref to weights 2^(x - ref), of the first lim[i] tokens of each part, whose
+    // values have the scales v.
+    __device__ __forceinline__ void weigh(Four (&x)[kQ4Parts], const int (&lim)[kQ4Parts], const Scales (&v)[kQ4Parts]) {
         const int t = (threadIdx.x & 31) >> 2;
-        bool up = false;
+        uint32_t big = 0u;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int i = 0; i < kQ4Parts; ++i)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (t + (i >> 1) * 8 >= lim) x[nt][i] = -INFINITY;
-                up |= x[nt][i] > m[nt][i & 1] + 8.f;
+            for (int w = 0; w < (NG + 1) / 2; ++w) big = max2(big, max2(v[i][0][w], v[i][1][w]));
+        const uint32_t room = (uint32_t)(((top + 127) << 7) - 1) * 0x10001u;       // the largest bf16 below 2^top
+        bool up = max2(big, room) != room;
+#pragma unroll
+        for (int i = 0; i < kQ4Parts; ++i) {
+            if (lim[i] < kPaChunk) {                   // the same for the warp: a unit's last part
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (t + (j >> 1) * 8 >= lim[i]) x[i][nt][j] = -INFINITY;
             }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) up |= x[i][nt][j] > most[nt][j & 1];
+        }
         if (__any_sync(~0u, up)) {
+#pragma unroll
+            for (int k = 4; k < 32; k <<= 1) big = max2(big, __shfl_xor_sync(~0u, big, k));
+            top = min(max((int)(max(big & 0xFFFFu, big >> 16) >> 7) - 126, top), kMostTop);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    float mx = fmaxf(x[nt][j], x[nt][2 + j]);
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < kQ4Parts; ++i) mx = fmaxf(mx, fmaxf(x[i][nt][j], x[i][nt][2 + j]));
 #pragma unroll
                     for (int k = 4; k < 32; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, k));
-                    const float mn = fmaxf(m[nt][j], mx);
-                    const float keep = exp2_fast(m[nt][j] - (mn == -INFINITY ? 0.f : mn));
-                    m[nt][j] = mn;
-                    l[nt][j] *= keep;
-                    z[nt][j] *= keep;
+                    m[nt][j] = fmaxf(m[nt][j], mx - less[nt][j]);
+                    const bool none = m[nt][j] == -INFINITY;
+                    const float now = (none ? 0.f : m[nt][j]) + (float)(top - 13);
+                    const float by = -less[nt][j] - now, keep = exp2_fast(by);
+                    less[nt][j] = -now;
+                    most[nt][j] = none ? -INFINITY : (float)(15 - top);
 #pragma unroll
-                    for (int b = 0; b < kBlocks; ++b)
+                    for (int i = 0; i < kQ4Parts; ++i) {
+                        x[i][nt][j] += by;
+                        x[i][nt][2 + j] += by;
+                    }
+                    if (l[nt][j] != 0.f) {             // else nothing is held
+                        l[nt][j] *= keep;
+                        z[nt][j] *= keep;
 #pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            o[nt][b][y][j] *= keep;
-                            o[nt][b][y][2 + j] *= keep;
-                        }
+                        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                o[nt][b][y][j] *= keep;
+                                o[nt][b][y][2 + j] *= keep;
+                            }
+                    }
                 }
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const float ref = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
-                w.p[nt][j] = exp2_fast(x[nt][j] - ref);
-                w.p[nt][2 + j] = exp2_fast(x[nt][2 + j] - ref);
-                l[nt][j] += w.p[nt][j] + w.p[nt][2 + j];
+            for (int i = 0; i < kQ4Parts; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    x[i][nt][j] = exp2_fast(x[i][nt][j]);
+                    x[i][nt][2 + j] = exp2_fast(x[i][nt][2 + j]);
+                    l[nt][j] += x[i][nt][j] + x[i][nt][2 + j];
+                }
+    }
+
+    // Four weights (a lane's tokens and heads) as fragments of kParts 16-bit parts.
+    template <typename P, int kParts>
+    __device__ __forceinline__ static void split(float a, float b, float c, float d, uint32_t (&f)[kParts][2]) {
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+            const uint32_t x = pack2<P>(a, b), y = pack2<P>(c, d);
+            f[i][0] = transpose8(x);
+            f[i][1] = transpose8(y);
+            if (i + 1 < kParts) {
+                const float2 xb = unpack2<P>(x), yb = unpack2<P>(y);
+                a -= xb.x;
+                b -= xb.y;
+                c -= yb.x;
+                d -= yb.y;
             }
+        }
     }
 
-    // Four weights (a lane's tokens and heads) as the fragments of their two parts.
-    struct Parts {
-        uint32_t hi[2], lo[2];
-    };
-    __device__ __forceinline__ static void split(float a, float b, float c, float d, Parts& f) {
-        const uint32_t x = pack2<Bf>(a, b), y = pack2<Bf>(c, d);
-        const float2 xb = unpack2<Bf>(x), yb = unpack2<Bf>(y);
-        f.hi[0] = transpose8(x);
-        f.hi[1] = transpose8(y);
-        f.lo[0] = transpose8(pack2<Bf>(a - xb.x, b - xb.y));
-        f.lo[1] = transpose8(pack2<Bf>(c - yb.x, d - yb.y));
-    }
-
-    // Adds the chunk whose values are at vt.
-    __device__ __forceinline__ void add(uint32_t vt, const Weights& w) {
+    // Adds the part whose values are at vt, of scales sc, by weights w.
+    __device__ __forceinline__ void add(uint32_t vt, const Four& w, const Scales& sc) {
         const int lane = threadIdx.x & 31, r = lane & 15, half = lane >> 4;
-        const uint32_t par = vt + Q4Tile<D>::kCodes;
-        float sc[2][NG];
-        ld_scales<NG>(sc[0], par + (lane >> 2) * 16);
-        ld_scales<NG>(sc[1], par + ((lane >> 2) + 8) * 16);
-        uint32_t pr[2];
-        ldsm2t(pr, par + r * 16);
-        const uint32_t a0[4] = {pr[0], 0u, pr[1], 0u};
-        Parts f[NT];
+        // the rows of parameters as columns, twice over: rows 8 to 15 of z are not looked at
+        uint32_t pr[4];
+        ldsm4t(pr, vt + Q4Tile<D>::kCodes + ((lane & 7) + half * 8) * 16);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            split(w.p[nt][0], w.p[nt][1], w.p[nt][2], w.p[nt][3], f[nt]);
-            mma16816(z[nt], a0, f[nt].hi[0], f[nt].hi[1], Bf());
-            mma16816(z[nt], a0, f[nt].lo[0], f[nt].lo[1], Bf());
+            uint32_t f[2][2];
+            split<Bf>(w[nt][0], w[nt][1], w[nt][2], w[nt][3], f);
+            product(z[nt], pr, f[0][0], f[0][1], Bf());
+            product(z[nt], pr, f[1][0], f[1][1], Bf());
         }
+        uint32_t f[NT][kTerms][2];
 #pragma unroll
         for (int b2 = 0; b2 < kBlocks / 2; ++b2) {
             uint32_t v[4];
@@ -312,32 +424,55 @@ struct Q4State {
             for (int i = 0; i < 2; ++i) {
                 const int b = b2 * 2 + i, g = b / kPer;
                 if (b % kPer == 0) {
-                    const float s0 = sc[0][g] * kTwo64, s1 = sc[1][g] * kTwo64;
+                    const float s0 = scale_of<NG>(sc[0], g), s1 = scale_of<NG>(sc[1], g);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
-                        split(w.p[nt][0] * s0, w.p[nt][1] * s0, w.p[nt][2] * s1, w.p[nt][3] * s1, f[nt]);
+                        split<__half>(w[nt][0] * s0, w[nt][1] * s0, w[nt][2] * s1, w[nt][3] * s1, f[nt]);
                 }
                 const uint32_t t[4] = {v[i * 2], v[i * 2] >> 8, v[i * 2 + 1], v[i * 2 + 1] >> 8};
                 uint32_t lo[4], hi[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    lo[j] = add_bf16x2(t[j] & kLowCodes, 0x80088008u);       // - 8 steps
-                    hi[j] = add_bf16x2(t[j] & kHighCodes, 0x80808080u);      // - 128 steps
+                    lo[j] = t[j] & kLowCodes;
+                    hi[j] = t[j] & kHighCodes;
                 }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    mma16816(o[nt][b][0], lo, f[nt].hi[0], f[nt].hi[1], Bf());
-                    mma16816(o[nt][b][1], hi, f[nt].hi[0], f[nt].hi[1], Bf());
-                    mma16816(o[nt][b][0], lo, f[nt].lo[0], f[nt].lo[1], Bf());
-                    mma16816(o[nt][b][1], hi, f[nt].lo[0], f[nt].lo[1], Bf());
-                }
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int x = 0; x < kTerms; ++x) {
+                        product(o[nt][b][0], lo, f[nt][x][0], f[nt][x][1], __half());
+                        product(o[nt][b][1], hi, f[nt][x][0], f[nt][x][1], __half());
+                    }
             }
         }
+    }
+
+    // Centres the codes of the last steps: takes 8 sum(p s) off the sums over them.
+    __device__ __forceinline__ void settle() {
+        const int lane = threadIdx.x & 31;
+        owed = 0;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) {
+                    const float ps = __shfl_sync(~0u, z[nt][j], b / kPer * 4 + (lane & 3));
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const float by = y ? -power_of_two(7 - 24) : -power_of_two(3 - 24);
+                        o[nt][b][y][j] = fmaf(ps, by, o[nt][b][y][j]);
+                        o[nt][b][y][2 + j] = fmaf(ps, by, o[nt][b][y][2 + j]);
+                    }
+                }
+                if (lane >> 2 < NG) z[nt][j] = 0.f;
+            }
     }
 
     // The sums of a head's eight lanes, and the outputs (unnormalised) from the sums.
     __device__ __forceinline__ void finish() {
         const int lane = threadIdx.x & 31;
+        settle();
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -349,9 +484,9 @@ struct Q4State {
                     const float c = __shfl_sync(~0u, z[nt][j], (NG + b / kPer) * 4 + (lane & 3));
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
-                        const float unit = kTwo64 * (y ? 2.f : 32.f);
-                        o[nt][b][y][j] = o[nt][b][y][j] * unit + c;
-                        o[nt][b][y][2 + j] = o[nt][b][y][2 + j] * unit + c;
+                        const float by = y ? power_of_two(20) : power_of_two(24);
+                        o[nt][b][y][j] = o[nt][b][y][j] * by + c;
+                        o[nt][b][y][2 + j] = o[nt][b][y][2 + j] * by + c;
                     }
                 }
             }
@@ -372,7 +507,7 @@ struct Q4State {
                     *reinterpret_cast<uint2*>(out + row * D + b * 32 + (lane >> 2) * 4) =
                         make_uint2(pack2<T>(o[nt][b][0][j] * inv, o[nt][b][1][j] * inv),
                                    pack2<T>(o[nt][b][0][2 + j] * inv, o[nt][b][1][2 + j] * inv));
-                if (lse && lane < 4) lse[row] = log_sum(m[nt][j], l[nt][j], 0.f);
+                if (lse && lane < 4) lse[row] = log_sum(-less[nt][j], l[nt][j], 0.f);
             }
     }
     // A piece: unnormalised rows [rows][D], and [rows][2] maxima and sums.
@@ -388,85 +523,151 @@ struct Q4State {
                 for (int b = 0; b < kBlocks; ++b)
                     *reinterpret_cast<float4*>(po + row * D + b * 32 + (lane >> 2) * 4) =
                         make_float4(o[nt][b][0][j], o[nt][b][1][j], o[nt][b][0][2 + j], o[nt][b][1][2 + j]);
-                if (lane < 4) *reinterpret_cast<float2*>(ml + row * 2) = make_float2(m[nt][j], l[nt][j]);
+                if (lane < 4) *reinterpret_cast<float2*>(ml + row * 2) = make_float2(-less[nt][j], l[nt][j]);
             }
     }
 };
 
-// A warp's ring: kStages - 1 chunks are on their way while one is worked on.
+// A warp's ring: kStages - 1 chunks are on their way while one is worked on. A chunk is
+// two parts of 16 tokens: their sums do not wait for one another, and what a step costs
+// beside the products is shared.
 template <int D, int NG, int NT>
 struct Q4Ring {
     using C = Q4Cfg<D, NT>;
     using Tile = Q4Tile<D>;
+    static constexpr int kPieces = D / 32;             // 16-byte pieces a row
+    static constexpr int kEach = kPaChunk * kPieces / 32;      // of K, and of V, a lane and part
     uint32_t base;
     uint64_t policy;
-    int steps;
-    int lims[C::kStages - 1];      // of the chunks on their way, oldest first
+    int steps, head;
+    const uint8_t *kfrom, *vfrom, *pfrom;              // a lane's places in the present head's rows
+    int lims[C::kStages - 1][kQ4Parts];                // of the chunks on their way, oldest first
 
     __device__ __forceinline__ void start(uint32_t at, int n) {
         base = at;
         policy = evict_first_policy();
         steps = n;
+        head = -1;
         // rows of parameters shorter than 16 bytes end in zeros
         if constexpr (NG < 4) {
             const int lane = threadIdx.x & 31;
 #pragma unroll
-            for (int s = 0; s < C::kStages; ++s)
+            for (int s = 0; s < C::kStages * kQ4Parts; ++s)
                 asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(
-                                 slot(s) + (lane >> 4) * Tile::kTile + Tile::kCodes + (lane & 15) * 16),
+                                 base + s * C::kPartBytes + (lane >> 4) * Tile::kTile + Tile::kCodes + (lane & 15) * 16),
                              "r"(0)
                              : "memory");
             __syncwarp();
         }
     }
     __device__ __forceinline__ uint32_t slot(int s) const { return base + (s % C::kStages) * C::kChunkBytes; }
-    __device__ __forceinline__ void copy(const Q4Args& a, uint32_t dst, int blk, int ch, int h, int lim) {
-        constexpr int kPieces = D / 32;                // 16-byte pieces a row
-        const int lane = threadIdx.x & 31;
-        const int row0 = (ch & ((1 << (a.kp.page_shift - 4)) - 1)) * kPaChunk;
-        const uint8_t* ks = static_cast<const uint8_t*>(a.kp.data) + h * a.kp.s_head + blk * a.kp.s_block + row0 * a.kp.s_token;
-        const uint8_t* vs = static_cast<const uint8_t*>(a.vp.data) + h * a.vp.s_head + blk * a.vp.s_block + row0 * a.vp.s_token;
-#pragma unroll
-        for (int i = 0; i < kPaChunk * kPieces / 32; ++i) {
-            const int x = i * 32 + lane, r = x / kPieces, pc = x % kPieces;
-            const uint32_t to = dst + Tile::place(r, pc);
-            cp16(to, ks + r * a.kp.s_token + pc * 16, r < lim, policy);
-            cp16(to + Tile::kTile, vs + r * a.vp.s_token + pc * 16, r < lim, policy);
-        }
+    __device__ __forceinline__ static const uint8_t* at(const uint8_t* p, uint32_t n, uint32_t stride) {
+        return p + (uint64_t)n * stride;
+    }
+    // To the present head's rows, where it is another one (the same for the warp).
+    __device__ __forceinline__ void turn_to(const Q4Args& a, int h) {
+        if (h == head) return;
+        head = h;
+        const int lane = threadIdx.x & 31, r0 = lane / kPieces, pc = lane % kPieces;
+        kfrom = at(at(a.kcode.base, h, a.kcode.head), r0, a.kcode.token) + pc * 16;
+        vfrom = at(at(a.vcode.base, h, a.vcode.head), r0, a.vcode.token) + pc * 16;
         // a row of parameters a lane, the keys' first
-        const int r = lane & 15;
-        const bool v = lane >> 4;
-        const uint16_t* src = v ? a.vpar + h * a.vpar_head + blk * a.vpar_block + (row0 + r) * a.vpar_token
-                                : a.kpar + h * a.kpar_head + blk * a.kpar_block + (row0 + r) * a.kpar_token;
-        cp_params<4 * NG>(dst + (v ? Tile::kTile : 0) + Tile::kCodes + r * 16, src, r < lim, policy);
+        if (lane < 16) pfrom = at(at(a.kpar.base, h, a.kpar.head), lane, a.kpar.token);
+        else pfrom = at(at(a.vpar.base, h, a.vpar.head), lane - 16, a.vpar.token);
+    }
+    static constexpr int kStep = 32 / kPieces;                 // rows that a warp's 16-byte pieces make
+    // 16 rows (the first `lim` of them, zeros behind) to dst; steps: bytes between the rows of a lane's pieces.
+    __device__ __forceinline__ void copy_part(uint32_t dst, const uint8_t* ks, const uint8_t* vs, const uint8_t* ps,
+                                              uint64_t kstep, uint64_t vstep, int lim) {
+        const int lane = threadIdx.x & 31, r0 = lane / kPieces;
+        const uint32_t to = dst + Tile::place(r0, lane % kPieces);
+        const uint32_t par = dst + (lane >> 4) * Tile::kTile + Tile::kCodes + (lane & 15) * 16;
+        if (lim == kPaChunk) {                                 // the same for the warp
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {                  // 8 or 16 rows on, a piece's place is as many rows on
+                cp16_all(to + i * kStep * Tile::kRow, ks + i * kstep, policy);
+                cp16_all(to + i * kStep * Tile::kRow + Tile::kTile, vs + i * vstep, policy);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                cp16(to + i * kStep * Tile::kRow, ks + i * kstep, r0 + i * kStep < lim, policy);
+                cp16(to + i * kStep * Tile::kRow + Tile::kTile, vs + i * vstep, r0 + i * kStep < lim, policy);
+            }
+        }
+        cp_params<4 * NG>(par, ps, (lane & 15) < lim, policy);
+    }
+    // The parts of a chunk: the second one's rows follow the first one's in pages of 32 tokens or more.
+    __device__ __forceinline__ void copy(const Q4Args& a, uint32_t dst, const int (&blk)[kQ4Parts], int ch,
+                                         const int (&lim)[kQ4Parts]) {
+        const bool key = (threadIdx.x & 31) < 16;
+        const uint32_t p_block = key ? a.kpar.block : a.vpar.block, p_token = key ? a.kpar.token : a.vpar.token;
+        const uint32_t row0 = (ch & ((1 << (a.kp.page_shift - 4)) - 1)) * kPaChunk;
+        const uint8_t* ks = at(at(kfrom, blk[0], a.kcode.block), row0, a.kcode.token);
+        const uint8_t* vs = at(at(vfrom, blk[0], a.vcode.block), row0, a.vcode.token);
+        const uint8_t* ps = at(at(pfrom, blk[0], p_block), row0, p_token);
+        if (a.packed && lim[kQ4Parts - 1] == kPaChunk) {       // whole chunks whose rows follow one another
+#pragma unroll
+            for (int j = 0; j < kQ4Parts; ++j)
+                copy_part(dst + j * C::kPartBytes, ks + j * kPaChunk * Tile::kRow, vs + j * kPaChunk * Tile::kRow,
+                          ps + j * kPaChunk * 4 * NG, kStep * Tile::kRow, kStep * Tile::kRow, kPaChunk);
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < kQ4Parts; ++j) {
+            if (j > 0) {
+                const uint32_t row = a.kp.page_shift > 4 ? row0 + j * kPaChunk : 0u;
+                ks = at(at(kfrom, blk[j], a.kcode.block), row, a.kcode.token);
+                vs = at(at(vfrom, blk[j], a.vcode.block), row, a.vcode.token);
+                ps = at(at(pfrom, blk[j], p_block), row, p_token);
+            }
+            copy_part(dst + j * C::kPartBytes, ks, vs, ps, (uint64_t)kStep * a.kcode.token, (uint64_t)kStep * a.vcode.token,
+                      lim[j]);
+        }
     }
     template <typename Find>
     __device__ __forceinline__ void ask(const Q4Args& a, int s, Find&& find) {
-        int lim = 0;
+        int lim[kQ4Parts] = {};
         if (s < steps) {
-            int blk, ch, h;
-            lim = find(blk, ch, h, s);
-            copy(a, slot(s), blk, ch, h, lim);
-        }
-        cp_commit();
+            int blk[kQ4Parts], ch0 = 0;
 #pragma unroll
-        for (int i = 0; i + 2 < C::kStages; ++i) lims[i] = lims[i + 1];
-        lims[C::kStages - 2] = lim;
+            for (int j = 0; j < kQ4Parts; ++j) {
+                int ch, h;
+                lim[j] = find(blk[j], ch, h, s, j);
+                if (j == 0) {
+                    ch0 = ch;
+                    turn_to(a, h);
+                }
+            }
+            copy(a, slot(s), blk, ch0, lim);
+        }
+#pragma unroll
+        for (int i = 0; i + 2 < C::kStages; ++i)
+#pragma unroll
+            for (int j = 0; j < kQ4Parts; ++j) lims[i][j] = lims[i + 1][j];
+#pragma unroll
+        for (int j = 0; j < kQ4Parts; ++j) lims[C::kStages - 2][j] = lim[j];
+        cp_commit();
     }
     // Step s of a unit.
     template <typename State, typename Find>
     __device__ __forceinline__ void step(const Q4Args& a, int s, State& st, Find&& find) {
-        typename State::Weights w;
         cp_wait<C::kStages - 2>();
         __syncwarp();
-        const int lim = lims[0];
+        int lim[kQ4Parts];
+#pragma unroll
+        for (int j = 0; j < kQ4Parts; ++j) lim[j] = lims[0][j];
         ask(a, s + C::kStages - 1, find);
-        {
-            decltype(w.p) x;
-            st.scores(slot(s), a.scale2, x);
-            st.weigh(x, lim, w);
-        }
-        st.add(slot(s) + Tile::kTile, w);
+        typename State::Four x[kQ4Parts];
+#pragma unroll
+        for (int j = 0; j < kQ4Parts; ++j) st.scores(slot(s) + j * C::kPartBytes, x[j]);
+        typename State::Scales v[kQ4Parts];
+#pragma unroll
+        for (int j = 0; j < kQ4Parts; ++j) st.look(slot(s) + j * C::kPartBytes + Tile::kTile, v[j]);
+        st.weigh(x, lim, v);
+#pragma unroll
+        for (int j = 0; j < kQ4Parts; ++j) st.add(slot(s) + j * C::kPartBytes + Tile::kTile, x[j], v[j]);
+        if (++st.owed == State::kSettle) st.settle();
         __syncwarp();
     }
 };
@@ -475,7 +676,7 @@ template <typename T_, int D_, bool kListed_>
 struct Q4Base {
     using T = T_;
     using Args = Q4Args;
-    static constexpr int D = D_;
+    static constexpr int D = D_, kParts = kQ4Parts;
     static constexpr bool kListed = kListed_, kOdd = false;
     static constexpr float kBias = 0.f;
 };
@@ -484,6 +685,9 @@ struct Q4Form : Q4Base<T, D, kListed>, Q4Cfg<D, NT> {
     using Joined = Q4Base<T, D, kListed>;
     using State = Q4State<T, D, NG, NT>;
     using Ring = Q4Ring<D, NG, NT>;
+    __device__ __forceinline__ static void start(State& st, const Q4Args& a, const uint16_t* q, int rows) {
+        st.start(q, rows, a.scale2);
+    }
 };
 
 template <typename T, int D, int NG, bool kListed>

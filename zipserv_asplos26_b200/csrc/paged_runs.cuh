@@ -1,9 +1,9 @@
 // How paged attention is dealt to the GPU and joined, whatever the cache holds
 // (paged_attention.cu: 16-bit keys and values; paged_int4_attention.cuh: 4-bit ones).
 //
-// The work is cut into chunks of 16 tokens of a unit (sequence, KV head, tile of up to
-// 16 query heads), a warp's step, and dealt in one of two ways, chosen by sizes that
-// the host has (unit_warps):
+// The work is cut into chunks, a warp's step: one or two parts of 16 tokens of a unit
+// (sequence, KV head, tile of up to 16 query heads). They are dealt in one of two ways,
+// chosen by sizes that the host has (unit_warps):
 //   * paged_attn_kernel: all chunks in order go to the warps of the GPU in equal
 //     runs, found by a prefix sum over the lengths in the kernel, so ragged
 //     batches and single long sequences load every SM alike and no length is
@@ -16,11 +16,11 @@
 // those of 16-bit keys and values.
 //
 // A form F says what a warp does: T (of q and the output), D, kListed (page lists),
-// Args (PaArgs or more), kCtas, kStages, kRing, kSmem, Ring (start, ask, step), State
-// (what a warp holds of a unit: start, finish, write, park), kBias (of its
-// exponentials), kOdd (whether infinite values are looked at again, by odd_values and
-// State's odd and mend) and Joined (a form of the same T, D, kListed and odd_values:
-// the one that the join is built for).
+// kParts (of a chunk), Args (PaArgs or more), kCtas, kStages, kRing, kSmem, Ring (start,
+// ask, step), State (what a warp holds of a unit: finish, write, park), start (of a
+// State), kBias (of its exponentials), kOdd (whether infinite values are looked at again,
+// by odd_values and State's odd and mend) and Joined (a form of the same T, D, kListed,
+// kParts and odd_values: the one that the join is built for).
 #pragma once
 
 #include <algorithm>
@@ -57,7 +57,7 @@ namespace {
 
 constexpr int kPaWarps = 4;
 constexpr int kPaThreads = kPaWarps * 32;
-constexpr int kPaChunk = 16;       // tokens a warp step; pages are multiples of it
+constexpr int kPaChunk = 16;       // tokens of a chunk's part; pages are multiples of it
 constexpr int kPaRows = 16;        // query heads a unit
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -125,12 +125,17 @@ __device__ __forceinline__ float log_sum(float m, float l, float bias) {
     return l == 0.f ? -INFINITY : (m + log2f(l) - bias) / kLog2e;
 }
 
-// Chunks of entry e: a sequence (whole cache) or a (sequence, KV head) with a page list.
+// Parts of 16 tokens, and chunks, of entry e: a sequence (whole cache) or a (sequence, KV
+// head) with a page list.
 template <bool kListed>
-__device__ __forceinline__ int entry_chunks(const PaArgs& a, int e) {
+__device__ __forceinline__ int entry_parts(const PaArgs& a, int e) {
     if (kListed) return max(0, min(a.counts[e], a.top)) << (a.kp.page_shift - 4);
     const int cap = (int)min((long long)a.width << a.kp.page_shift, (long long)INT_MAX - 15);
     return (max(0, min(a.lens[e], cap)) + kPaChunk - 1) / kPaChunk;
+}
+template <class F>
+__device__ __forceinline__ int entry_chunks(const PaArgs& a, int e) {
+    return (entry_parts<F::kListed>(a, e) + F::kParts - 1) / F::kParts;
 }
 
 // Inclusive prefix over the warp's lanes.
@@ -143,7 +148,7 @@ __device__ __forceinline__ long long warp_prefix(long long v) {
     return v;
 }
 
-// The block and the number of valid tokens of chunk `ch` of an entry (lim 0: none).
+// The block and the number of valid tokens of part `ch` of an entry (lim 0: none).
 template <bool kListed>
 __device__ __forceinline__ void look_chunk(const PaArgs& a, int e, int b, int ch, int len, int& id, int& lim) {
     const int cps = a.kp.page_shift - 4;                               // log2 chunks a page
@@ -194,12 +199,12 @@ struct PaCursor {
 };
 
 // To the next unit that has chunks (there is one: the caller has chunks left).
-template <bool kListed>
+template <class F>
 __device__ __forceinline__ void next_unit(const PaArgs& a, int per_entry, PaCursor& c) {
     c.ch = 0;
     if (++c.in_e < per_entry) return;
     c.in_e = 0;
-    do c.n = entry_chunks<kListed>(a, ++c.e);
+    do c.n = entry_chunks<F>(a, ++c.e);
     while (c.n == 0);
 }
 
@@ -225,7 +230,7 @@ __global__ void __launch_bounds__(kPaThreads, F::kCtas) paged_attn_kernel(const 
 #pragma unroll 4
     for (int i = 0; i < per; ++i) {
         const int e = lane * per + i;
-        n1 = e < entries ? entry_chunks<kListed>(a, e) : 0;
+        n1 = e < entries ? entry_chunks<F>(a, e) : 0;
         mine += n1;
     }
     const long long inc = warp_prefix(mine);
@@ -246,7 +251,7 @@ __global__ void __launch_bounds__(kPaThreads, F::kCtas) paged_attn_kernel(const 
     if (per > 1) {
         for (;; entry += 32) {
             const int e = entry + lane;
-            const int ne = e < min(entries, (owner + 1) * per) ? entry_chunks<kListed>(a, e) : 0;
+            const int ne = e < min(entries, (owner + 1) * per) ? entry_chunks<F>(a, e) : 0;
             const long long ie = warp_prefix((long long)ne);
             const unsigned past = __ballot_sync(~0u, (lo + ie) * per_entry > c_begin);
             if (past) {
@@ -269,39 +274,41 @@ __global__ void __launch_bounds__(kPaThreads, F::kCtas) paged_attn_kernel(const 
     PaCursor cur = at;             // of the products
     long long u_lo = c_begin - at.ch;
 
-    // ---- copies: batches of up to 32 chunks of one unit, a lane holding the block
-    // and the number of valid tokens of one chunk; the next batch is looked up
+    // ---- copies: batches of chunks of one unit, up to 32 parts, a lane holding the
+    // block and the number of valid tokens of one part; the next batch is looked up
     // while the present one is copied
+    constexpr int kParts = F::kParts;
     const int table_len = (int)min((long long)a.width << a.kp.page_shift, (long long)INT_MAX);
     struct Batch {
         int ids, lims, count, h, ch;
     } now, next;
     int looked = 0;                // chunks looked up
     auto look = [&](Batch& t) {
-        t.count = min(32, min(at.n - at.ch, steps - looked));
+        t.count = min(32 / kParts, min(at.n - at.ch, steps - looked));
         t.ids = 0;
         t.lims = 0;
         t.ch = at.ch;
         t.h = kListed ? at.e % a.Hkv : at.in_e / a.tiles;
         if (t.count <= 0) return;
-        if (lane < t.count) {
+        if (lane < t.count * kParts && (kParts == 1 || at.ch * kParts + lane < entry_parts<kListed>(a, at.e))) {
             const int b = kListed ? at.e / a.Hkv : at.e;
-            look_chunk<kListed>(a, at.e, b, at.ch + lane, min(a.lens[b], table_len), t.ids, t.lims);
+            look_chunk<kListed>(a, at.e, b, at.ch * kParts + lane, min(a.lens[b], table_len), t.ids, t.lims);
         }
         looked += t.count;
         at.ch += t.count;
-        if (at.ch == at.n && looked < steps) next_unit<kListed>(a, per_entry, at);
+        if (at.ch == at.n && looked < steps) next_unit<F>(a, per_entry, at);
     };
     look(now);
     int in_batch = 0;
-    auto find = [&](int& blk, int& ch, int& h, int) {
-        if (in_batch == now.count) {
+    // part `part` of the next chunk (parts in order, from 0)
+    auto find = [&](int& blk, int& ch, int& h, int, int part) {
+        if (part == 0 && in_batch == now.count * kParts) {
             now = next;
             in_batch = 0;
             look(next);
         }
         blk = __shfl_sync(~0u, now.ids, in_batch);
-        ch = now.ch + in_batch;
+        ch = now.ch * kParts + in_batch;
         h = now.h;
         return __shfl_sync(~0u, now.lims, in_batch++);
     };
@@ -324,7 +331,7 @@ __global__ void __launch_bounds__(kPaThreads, F::kCtas) paged_attn_kernel(const 
         if (first == 0 && lane == 0) a.plan[1 + (b * a.Hkv + h) * a.tiles + tile] = u_lo;
         const long long head0 = (long long)b * a.Hq + (long long)h * a.G + g0;
         typename F::State st;
-        st.start(a.q + head0 * D, rows);
+        F::start(st, a, a.q + head0 * D, rows);
         for (const int end = s + count; s < end; ++s) ring.step(a, s, st, find);
         // ---- out, or to the workspace where the run cuts the unit
         const bool whole = first == 0 && count == cur.n;
@@ -342,7 +349,7 @@ __global__ void __launch_bounds__(kPaThreads, F::kCtas) paged_attn_kernel(const 
         } else st.park(a.part_o + slot * a.prow * D, a.part_ml + slot * a.prow * 2, rows);
         if (s == steps) break;
         u_lo += cur.n;
-        next_unit<kListed>(a, per_entry, cur);
+        next_unit<F>(a, per_entry, cur);
     }
     cp_wait<0>();
 }
@@ -371,25 +378,29 @@ __global__ void __launch_bounds__(kPaThreads, F::kCtas) paged_attn_units_kernel(
     grid_dep_launch();
     grid_dep_wait();
     const int table_len = (int)min((long long)a.width << a.kp.page_shift, (long long)INT_MAX);
-    const int len = min(a.lens[b], table_len), n = on ? entry_chunks<kListed>(a, e) : 0;
+    const int len = min(a.lens[b], table_len), n = on ? entry_chunks<F>(a, e) : 0;
     const int first = (int)((long long)n * w / W), steps = (int)((long long)n * (w + 1) / W) - first;
     typename F::State st;
-    int ids = 0, lims = 0;         // of 32 chunks, a lane each
-    auto find = [&](int& blk, int& ch, int& head, int s) {
-        if ((s & 31) == 0) {
+    int ids = 0, lims = 0;         // of 32 parts, a lane each
+    constexpr int kParts = F::kParts;
+    const int parts = kParts > 1 && on ? entry_parts<kListed>(a, e) : 0;
+    auto find = [&](int& blk, int& ch, int& head, int s, int part) {
+        const int x = s * kParts + part;                       // part of the warp's share
+        if ((x & 31) == 0) {
             ids = lims = 0;
-            if (s + lane < steps) look_chunk<kListed>(a, e, b, first + s + lane, len, ids, lims);
+            const int y = first * kParts + x + lane;
+            if (x + lane < steps * kParts && (kParts == 1 || y < parts)) look_chunk<kListed>(a, e, b, y, len, ids, lims);
         }
-        blk = __shfl_sync(~0u, ids, s & 31);
-        ch = first + s;
+        blk = __shfl_sync(~0u, ids, x & 31);
+        ch = first * kParts + x;
         head = h;
-        return __shfl_sync(~0u, lims, s & 31);
+        return __shfl_sync(~0u, lims, x & 31);
     };
     typename F::Ring ring;
     ring.start(smem_u32(pa_smem) + warp * F::kRing, steps);
 #pragma unroll
     for (int s = 0; s < F::kStages - 1; ++s) ring.ask(a, s, find);
-    st.start(a.q + head0 * D, rows);
+    F::start(st, a, a.q + head0 * D, rows);
     for (int s = 0; s < steps; ++s) ring.step(a, s, st, find);
     cp_wait<0>();
     __syncwarp();
@@ -494,7 +505,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const typen
     const int tile = g / kPaRows, row = g % kPaRows;
     grid_dep_wait();
     const long long run = a.plan[0], lo = a.plan[1 + (b * a.Hkv + h) * a.tiles + tile];
-    const int n = entry_chunks<kListed>(a, kListed ? b * a.Hkv + h : b);
+    const int n = entry_chunks<F>(a, kListed ? b * a.Hkv + h : b);
     float m = -INFINITY, l = 0.f, acc[kVec];
 #pragma unroll
     for (int j = 0; j < kVec; ++j) acc[j] = 0.f;
@@ -641,14 +652,14 @@ cudaError_t resident_ctas(int* ctas) {
 // more than 4 CTAs were slower in all of these.
 constexpr int kPaMaxUnitWarps = 16;
 
-// A bound on a unit's chunks: of the page list, the table or the caller's.
-inline long long unit_chunks(const PaArgs& a, bool listed) {
+// A bound on a unit's parts: of the page list, the table or the caller's.
+inline long long unit_parts(const PaArgs& a, bool listed) {
     const long long pages = ((long long)(listed ? a.top : a.width)) << (a.kp.page_shift - 4);
     return a.max_len > 0 && !listed ? std::min(pages, ((long long)a.max_len + kPaChunk - 1) / kPaChunk) : pages;
 }
 
-inline int unit_warps(const PaArgs& a, bool listed, int max_ctas) {
-    const long long units = (long long)a.B * a.Hkv * a.tiles, chunks = unit_chunks(a, listed);
+inline int unit_warps(const PaArgs& a, bool listed, int max_ctas, int parts) {
+    const long long units = (long long)a.B * a.Hkv * a.tiles, chunks = (unit_parts(a, listed) + parts - 1) / parts;
     const long long resident = (long long)max_ctas * kPaWarps;
     int W = 1;
     while (W < kPaMaxUnitWarps && units * W * 2 <= resident && W * 4 <= chunks) W *= 2;
