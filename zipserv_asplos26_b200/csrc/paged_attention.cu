@@ -478,7 +478,7 @@ struct PaRing {
     int steps;
     int lims[C::kStages - 1];      // of the chunks on their way, oldest first
 
-    __device__ __forceinline__ void start(uint32_t at, int n) {
+    __device__ __forceinline__ void start(const PaArgs&, uint32_t at, int n) {
         base = at;
         policy = evict_first_policy();
         steps = n;
@@ -519,7 +519,7 @@ struct PaBase {
     using T = T_;
     using Args = PaArgs;
     static constexpr int D = D_, kParts = 1;
-    static constexpr bool kListed = kListed_, kOdd = true;
+    static constexpr bool kListed = kListed_, kOdd = true, kGrouped = false;
     static constexpr float kBias = kPBias<T>;
     template <int kCount>
     __device__ __forceinline__ static void odd_values(const PaArgs& a, int e, int b, int h, int first, int count, int c0,
@@ -541,15 +541,20 @@ inline int pa_max_ctas(int D, int G) {
     return 148 * (D <= 64 ? PaCfg<64, false>::kCtas : PaCfg<128, false>::kCtas);
 }
 
+template <class F>
+cudaError_t launch_form(const PaArgs& a, int W, cudaStream_t s) {
+    return launch_paged<F, F>(a, W, s);
+}
+
 template <typename T, bool kListed>
 cudaError_t dispatch_dim(const PaArgs& a, int W, cudaStream_t s) {
     switch (a.kp.dim) {
         case 64:
-            return a.G <= 8 ? launch_paged<PaForm<T, 64, kListed, true>>(a, W, s)
-                            : launch_paged<PaForm<T, 64, kListed, false>>(a, W, s);
+            return a.G <= 8 ? launch_form<PaForm<T, 64, kListed, true>>(a, W, s)
+                            : launch_form<PaForm<T, 64, kListed, false>>(a, W, s);
         case 128:
-            return a.G <= 8 ? launch_paged<PaForm<T, 128, kListed, true>>(a, W, s)
-                            : launch_paged<PaForm<T, 128, kListed, false>>(a, W, s);
+            return a.G <= 8 ? launch_form<PaForm<T, 128, kListed, true>>(a, W, s)
+                            : launch_form<PaForm<T, 128, kListed, false>>(a, W, s);
     }
     return cudaErrorInvalidValue;
 }

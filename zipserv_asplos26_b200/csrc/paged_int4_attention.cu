@@ -5,9 +5,17 @@
 namespace zs {
 namespace {
 
+// CTAs of the run kernel, at most.
 inline int q4_max_ctas(int D, int G) {
-    if (G <= 8) return 148 * (D == 64 ? Q4Cfg<64, 1>::kCtas : Q4Cfg<128, 1>::kCtas);
-    return 148 * (D == 64 ? Q4Cfg<64, 2>::kCtas : Q4Cfg<128, 2>::kCtas);
+    if (G <= 8) return 148 * (D == 64 ? Q4Cfg<64, 1, false>::kCtas : Q4Cfg<128, 1, false>::kCtas);
+    return 148 * (D == 64 ? Q4Cfg<64, 2, false>::kCtas : Q4Cfg<128, 2, false>::kCtas);
+}
+// Warps a unit, or 0 for runs.
+inline int q4_unit_warps(const Q4Args& a) {
+    using One = Q4Cfg<128, 1, true>;
+    using Two = Q4Cfg<128, 2, true>;
+    static_assert(One::kParts == 2 && Two::kParts == 2, "units' chunks are two parts");
+    return unit_warps(a, a.pages != nullptr, 148 * (a.G <= 8 ? One::kCtas : Two::kCtas), 2);
 }
 
 // The checked arguments of a call, but for its workspace.
@@ -38,7 +46,7 @@ bool int4_attention_args(const ZsPagedAttentionInt4* p, Q4Args* a, int* groups) 
         !places(&a->vpar, v.params, 2 * v.p_block, 2 * v.p_token, 2 * v.p_head))
         return false;
     const uint32_t row = k.dim / 2, par = 4 * k.groups;
-    a->packed = k.page_shift > 4 && a->kcode.token == row && a->vcode.token == row && a->kpar.token == par && a->vpar.token == par;
+    a->packed = a->kcode.token == row && a->vcode.token == row && a->kpar.token == par && a->vpar.token == par;
     *groups = k.groups;
     a->G = Hq / Hkv;
     a->tiles = (a->G + kPaRows - 1) / kPaRows;
@@ -47,6 +55,7 @@ bool int4_attention_args(const ZsPagedAttentionInt4* p, Q4Args* a, int* groups) 
     a->table = p->block_table;
     a->table_stride = p->table_stride;
     a->lens = p->seq_lens;
+    a->group = !a->packed && !p->pages && Hkv * a->tiles % kPaWarps == 0 ? kPaWarps : 1;
     a->pages = p->pages;
     a->counts = p->counts;
     a->B = B; a->Hq = Hq; a->Hkv = Hkv; a->width = p->width; a->top = top;
@@ -70,7 +79,7 @@ extern "C" size_t zs_paged_attention_int4_workspace(const ZsPagedAttentionInt4* 
     Q4Args a{};
     int groups;
     if (!int4_attention_args(p, &a, &groups) || a.B == 0 ||
-        unit_warps(a, a.pages != nullptr, q4_max_ctas(a.kp.dim, a.G), kQ4Parts))
+        q4_unit_warps(a))
         return 0;
     return int4_workspace(a);
 }
@@ -81,7 +90,7 @@ extern "C" int zs_paged_attention_int4(const ZsPagedAttentionInt4* p) {
     int groups;
     if (!int4_attention_args(p, &a, &groups)) return cudaErrorInvalidValue;
     if (a.B == 0) return cudaSuccess;
-    const int max_ctas = q4_max_ctas(a.kp.dim, a.G), W = unit_warps(a, a.pages != nullptr, max_ctas, kQ4Parts);
+    const int max_ctas = q4_max_ctas(a.kp.dim, a.G), W = q4_unit_warps(a);
     if (!W) {
         if (!p->ws || !aligned16p(p->ws) || p->ws_bytes < int4_workspace(a)) return cudaErrorInvalidValue;
         lay_workspace(&a, p->ws, max_ctas);

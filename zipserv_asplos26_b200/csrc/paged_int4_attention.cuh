@@ -42,12 +42,12 @@ struct Q4Places {
 };
 struct Q4Args : PaArgs {          // kp and vp: the codes (for page size, blocks and heads)
     Q4Places kcode, vcode, kpar, vpar;
-    int packed;                   // rows of a page's head follow one another, 32 or more of them
+    int packed;                   // rows of a page's head follow one another
 };
 
 namespace {
 
-constexpr int kQ4Parts = 2;     // a step takes 32 tokens: see Q4Ring
+constexpr int kPaChunkShift = 4;
 constexpr int kNoTop = -100, kMostTop = 100;        // of scales that count: 2^-100 to 2^100
 constexpr uint32_t kLowCodes = 0x000F000Fu, kHighCodes = 0x00F000F0u;
 
@@ -63,12 +63,18 @@ struct Q4Tile {
     }
 };
 
-template <int D, int NT>
+// A step's parts, CTAs an SM and stages of a warp's ring. In runs of up to 8 heads a step
+// takes 64 tokens: what it costs beside the products counts once for four parts, and the
+// parts' sums do not wait for one another (B=32 T=4129: 38.7 us with 8 warps an SM, 41.0
+// with 12 of 32 tokens, 50 with 16 of 16). With 16 heads the registers hold two parts.
+// Units are short and get two parts, so that more warps share them.
+template <int D, int NT, bool kUnits>
 struct Q4Cfg {
-    static constexpr int kCtas = NT == 1 ? 3 : 2;
-    static constexpr int kStages = 3;
+    static constexpr int kParts = NT == 1 && !kUnits ? 4 : 2;
+    static constexpr int kCtas = NT == 1 && kUnits ? 3 : 2;
+    static constexpr int kStages = kParts == 4 ? 2 : 3;
     static constexpr int kPartBytes = 2 * Q4Tile<D>::kTile;
-    static constexpr int kChunkBytes = kQ4Parts * kPartBytes;
+    static constexpr int kChunkBytes = kParts * kPartBytes;
     static constexpr int kPiece = kPaRows * (D + 2) * 4;     // a warp's piece in the units kernel
     static constexpr int kRing = kStages * kChunkBytes > kPiece ? kStages * kChunkBytes : kPiece;
     static constexpr int kSmem = kPaWarps * kRing;
@@ -78,6 +84,18 @@ __device__ __forceinline__ float exp2_fast(float x) {        // 2 ulp; below 2^-
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// 16 bytes, or zeros; without a hint to fetch what lies around (other heads' rows, where
+// rows do not follow one another).
+__device__ __forceinline__ void cp16_row(uint32_t dst, const void* src, bool on, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0),
+                 "l"(policy)
+                 : "memory");
+}
+__device__ __forceinline__ uint64_t evict_normal_policy() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+    return p;
 }
 __device__ __forceinline__ void cp16_all(uint32_t dst, const void* src, uint64_t policy) {
     asm volatile("cp.async.cg.shared.global.L2::cache_hint.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy)
@@ -150,12 +168,12 @@ __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e 
 // What a warp holds of a unit of up to NT x 8 heads. A lane has heads 2 (lane % 4) and
 // the next of each eight; of scores, tokens lane / 4 and lane / 4 + 8; of outputs the
 // four channels from 4 (lane / 4) on of each 32.
-template <typename T, int D, int NG, int NT>
+template <typename T, int D, int NG, int NT, int kParts>
 struct Q4State {
     static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     static constexpr int kBlocks = D / 32, kPer = kBlocks / NG;      // 32 channels: a 16-byte piece of a row
     static constexpr int kTerms = kBf16 ? 1 : 2;                     // fp16 parts of p s
-    static constexpr int kSettle = kBf16 ? 4 : 2;                    // steps after which codes are centred
+    static constexpr int kSettle = (kBf16 ? 8 : 4) / kParts;         // steps after which codes are centred
     using Bf = __nv_bfloat16;
     uint32_t qf[NT][kBlocks][2][2];    // q of the even, odd channels (these a sixteenth)
     uint32_t zf[NT][3];                // of what meets the parameters: -8 sum(q_g), sum(q_g), times scale2, in three parts
@@ -312,17 +330,17 @@ struct Q4State {
 
     // From scores x - ref to weights 2^(x - ref), of the first lim[i] tokens of each part, whose
     // values have the scales v.
-    __device__ __forceinline__ void weigh(Four (&x)[kQ4Parts], const int (&lim)[kQ4Parts], const Scales (&v)[kQ4Parts]) {
+    __device__ __forceinline__ void weigh(Four (&x)[kParts], const int (&lim)[kParts], const Scales (&v)[kParts]) {
         const int t = (threadIdx.x & 31) >> 2;
         uint32_t big = 0u;
 #pragma unroll
-        for (int i = 0; i < kQ4Parts; ++i)
+        for (int i = 0; i < kParts; ++i)
 #pragma unroll
             for (int w = 0; w < (NG + 1) / 2; ++w) big = max2(big, max2(v[i][0][w], v[i][1][w]));
         const uint32_t room = (uint32_t)(((top + 127) << 7) - 1) * 0x10001u;       // the largest bf16 below 2^top
         bool up = max2(big, room) != room;
 #pragma unroll
-        for (int i = 0; i < kQ4Parts; ++i) {
+        for (int i = 0; i < kParts; ++i) {
             if (lim[i] < kPaChunk) {                   // the same for the warp: a unit's last part
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -345,7 +363,7 @@ struct Q4State {
                 for (int j = 0; j < 2; ++j) {
                     float mx = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < kQ4Parts; ++i) mx = fmaxf(mx, fmaxf(x[i][nt][j], x[i][nt][2 + j]));
+                    for (int i = 0; i < kParts; ++i) mx = fmaxf(mx, fmaxf(x[i][nt][j], x[i][nt][2 + j]));
 #pragma unroll
                     for (int k = 4; k < 32; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, k));
                     m[nt][j] = fmaxf(m[nt][j], mx - less[nt][j]);
@@ -355,7 +373,7 @@ struct Q4State {
                     less[nt][j] = -now;
                     most[nt][j] = none ? -INFINITY : (float)(15 - top);
 #pragma unroll
-                    for (int i = 0; i < kQ4Parts; ++i) {
+                    for (int i = 0; i < kParts; ++i) {
                         x[i][nt][j] += by;
                         x[i][nt][2 + j] += by;
                     }
@@ -375,7 +393,7 @@ struct Q4State {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < kQ4Parts; ++i)
+            for (int i = 0; i < kParts; ++i)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     x[i][nt][j] = exp2_fast(x[i][nt][j]);
@@ -384,15 +402,15 @@ struct Q4State {
                 }
     }
 
-    // Four weights (a lane's tokens and heads) as fragments of kParts 16-bit parts.
-    template <typename P, int kParts>
-    __device__ __forceinline__ static void split(float a, float b, float c, float d, uint32_t (&f)[kParts][2]) {
+    // Four weights (a lane's tokens and heads) as fragments of kN 16-bit numbers that add up.
+    template <typename P, int kN>
+    __device__ __forceinline__ static void split(float a, float b, float c, float d, uint32_t (&f)[kN][2]) {
 #pragma unroll
-        for (int i = 0; i < kParts; ++i) {
+        for (int i = 0; i < kN; ++i) {
             const uint32_t x = pack2<P>(a, b), y = pack2<P>(c, d);
             f[i][0] = transpose8(x);
             f[i][1] = transpose8(y);
-            if (i + 1 < kParts) {
+            if (i + 1 < kN) {
                 const float2 xb = unpack2<P>(x), yb = unpack2<P>(y);
                 a -= xb.x;
                 b -= xb.y;
@@ -528,31 +546,33 @@ struct Q4State {
     }
 };
 
-// A warp's ring: kStages - 1 chunks are on their way while one is worked on. A chunk is
-// two parts of 16 tokens: their sums do not wait for one another, and what a step costs
-// beside the products is shared.
-template <int D, int NG, int NT>
+// A warp's ring: kStages - 1 chunks are on their way while one is worked on.
+template <int D, int NG, int NT, bool kUnits>
 struct Q4Ring {
-    using C = Q4Cfg<D, NT>;
+    using C = Q4Cfg<D, NT, kUnits>;
     using Tile = Q4Tile<D>;
+    static constexpr int kParts = C::kParts;
     static constexpr int kPieces = D / 32;             // 16-byte pieces a row
     static constexpr int kEach = kPaChunk * kPieces / 32;      // of K, and of V, a lane and part
     uint32_t base;
     uint64_t policy;
     int steps, head;
     const uint8_t *kfrom, *vfrom, *pfrom;              // a lane's places in the present head's rows
-    int lims[C::kStages - 1][kQ4Parts];                // of the chunks on their way, oldest first
+    int lims[C::kStages - 1][kParts];                // of the chunks on their way, oldest first
 
-    __device__ __forceinline__ void start(uint32_t at, int n) {
+    // Rows that follow one another pass through L2 once; of others, the lines are shared with
+    // other heads' rows (61 sequences of 0..16417 in pages by token, marked to leave first and
+    // fetched 256 bytes at a time: 1.96 GB read for 0.65).
+    __device__ __forceinline__ void start(const Q4Args& a, uint32_t at, int n) {
         base = at;
-        policy = evict_first_policy();
+        policy = a.packed ? evict_first_policy() : evict_normal_policy();
         steps = n;
         head = -1;
         // rows of parameters shorter than 16 bytes end in zeros
         if constexpr (NG < 4) {
             const int lane = threadIdx.x & 31;
 #pragma unroll
-            for (int s = 0; s < C::kStages * kQ4Parts; ++s)
+            for (int s = 0; s < C::kStages * kParts; ++s)
                 asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(
                                  base + s * C::kPartBytes + (lane >> 4) * Tile::kTile + Tile::kCodes + (lane & 15) * 16),
                              "r"(0)
@@ -576,62 +596,65 @@ struct Q4Ring {
         else pfrom = at(at(a.vpar.base, h, a.vpar.head), lane - 16, a.vpar.token);
     }
     static constexpr int kStep = 32 / kPieces;                 // rows that a warp's 16-byte pieces make
-    // 16 rows (the first `lim` of them, zeros behind) to dst; steps: bytes between the rows of a lane's pieces.
-    __device__ __forceinline__ void copy_part(uint32_t dst, const uint8_t* ks, const uint8_t* vs, const uint8_t* ps,
-                                              uint64_t kstep, uint64_t vstep, int lim) {
-        const int lane = threadIdx.x & 31, r0 = lane / kPieces;
-        const uint32_t to = dst + Tile::place(r0, lane % kPieces);
-        const uint32_t par = dst + (lane >> 4) * Tile::kTile + Tile::kCodes + (lane & 15) * 16;
-        if (lim == kPaChunk) {                                 // the same for the warp
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {                  // 8 or 16 rows on, a piece's place is as many rows on
-                cp16_all(to + i * kStep * Tile::kRow, ks + i * kstep, policy);
-                cp16_all(to + i * kStep * Tile::kRow + Tile::kTile, vs + i * vstep, policy);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                cp16(to + i * kStep * Tile::kRow, ks + i * kstep, r0 + i * kStep < lim, policy);
-                cp16(to + i * kStep * Tile::kRow + Tile::kTile, vs + i * vstep, r0 + i * kStep < lim, policy);
-            }
-        }
-        cp_params<4 * NG>(par, ps, (lane & 15) < lim, policy);
+    // A lane's places in a part at dst: of its first piece of a key row (8 or 16 rows on, a
+    // piece's place is as many rows on), and of its row of parameters.
+    __device__ __forceinline__ static uint32_t piece_place(uint32_t dst) {
+        const int lane = threadIdx.x & 31;
+        return dst + Tile::place(lane / kPieces, lane % kPieces);
     }
-    // The parts of a chunk: the second one's rows follow the first one's in pages of 32 tokens or more.
-    __device__ __forceinline__ void copy(const Q4Args& a, uint32_t dst, const int (&blk)[kQ4Parts], int ch,
-                                         const int (&lim)[kQ4Parts]) {
+    __device__ __forceinline__ static uint32_t params_place(uint32_t dst) {
+        const int lane = threadIdx.x & 31;
+        return dst + (lane >> 4) * Tile::kTile + Tile::kCodes + (lane & 15) * 16;
+    }
+    // The parts of a chunk. In pages that hold whole chunks the parts' rows follow one another.
+    __device__ __forceinline__ void copy(const Q4Args& a, uint32_t dst, const int (&blk)[kParts], int ch,
+                                         const int (&lim)[kParts]) {
         const bool key = (threadIdx.x & 31) < 16;
         const uint32_t p_block = key ? a.kpar.block : a.vpar.block, p_token = key ? a.kpar.token : a.vpar.token;
         const uint32_t row0 = (ch & ((1 << (a.kp.page_shift - 4)) - 1)) * kPaChunk;
         const uint8_t* ks = at(at(kfrom, blk[0], a.kcode.block), row0, a.kcode.token);
         const uint8_t* vs = at(at(vfrom, blk[0], a.vcode.block), row0, a.vcode.token);
         const uint8_t* ps = at(at(pfrom, blk[0], p_block), row0, p_token);
-        if (a.packed && lim[kQ4Parts - 1] == kPaChunk) {       // whole chunks whose rows follow one another
+        if (a.packed && a.kp.page_shift >= kPaChunkShift + (kParts == 4 ? 2 : 1) && lim[kParts - 1] == kPaChunk) {       // whole chunks whose rows follow one another
 #pragma unroll
-            for (int j = 0; j < kQ4Parts; ++j)
-                copy_part(dst + j * C::kPartBytes, ks + j * kPaChunk * Tile::kRow, vs + j * kPaChunk * Tile::kRow,
-                          ps + j * kPaChunk * 4 * NG, kStep * Tile::kRow, kStep * Tile::kRow, kPaChunk);
+            for (int j = 0; j < kParts; ++j) {
+                const uint32_t to = piece_place(dst) + j * C::kPartBytes;
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    const int on = (j * kPaChunk + i * kStep) * Tile::kRow;
+                    cp16_all(to + i * kStep * Tile::kRow, ks + on, policy);
+                    cp16_all(to + i * kStep * Tile::kRow + Tile::kTile, vs + on, policy);
+                }
+                cp_params<4 * NG>(params_place(dst) + j * C::kPartBytes, ps + j * kPaChunk * 4 * NG, true, policy);
+            }
             return;
         }
+        const int r0 = (threadIdx.x & 31) / kPieces;
 #pragma unroll
-        for (int j = 0; j < kQ4Parts; ++j) {
+        for (int j = 0; j < kParts; ++j) {
             if (j > 0) {
-                const uint32_t row = a.kp.page_shift > 4 ? row0 + j * kPaChunk : 0u;
+                const uint32_t row = ((ch + j) & ((1 << (a.kp.page_shift - 4)) - 1)) * kPaChunk;
                 ks = at(at(kfrom, blk[j], a.kcode.block), row, a.kcode.token);
                 vs = at(at(vfrom, blk[j], a.vcode.block), row, a.vcode.token);
                 ps = at(at(pfrom, blk[j], p_block), row, p_token);
             }
-            copy_part(dst + j * C::kPartBytes, ks, vs, ps, (uint64_t)kStep * a.kcode.token, (uint64_t)kStep * a.vcode.token,
-                      lim[j]);
+            const uint32_t to = piece_place(dst) + j * C::kPartBytes;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const bool on = r0 + i * kStep < lim[j];
+                cp16_row(to + i * kStep * Tile::kRow, at(ks, i * kStep, a.kcode.token), on, policy);
+                cp16_row(to + i * kStep * Tile::kRow + Tile::kTile, at(vs, i * kStep, a.vcode.token), on, policy);
+            }
+            cp_params<4 * NG>(params_place(dst) + j * C::kPartBytes, ps, (int)(threadIdx.x & 15) < lim[j], policy);
         }
     }
     template <typename Find>
     __device__ __forceinline__ void ask(const Q4Args& a, int s, Find&& find) {
-        int lim[kQ4Parts] = {};
+        int lim[kParts] = {};
         if (s < steps) {
-            int blk[kQ4Parts], ch0 = 0;
+            int blk[kParts], ch0 = 0;
 #pragma unroll
-            for (int j = 0; j < kQ4Parts; ++j) {
+            for (int j = 0; j < kParts; ++j) {
                 int ch, h;
                 lim[j] = find(blk[j], ch, h, s, j);
                 if (j == 0) {
@@ -644,9 +667,9 @@ struct Q4Ring {
 #pragma unroll
         for (int i = 0; i + 2 < C::kStages; ++i)
 #pragma unroll
-            for (int j = 0; j < kQ4Parts; ++j) lims[i][j] = lims[i + 1][j];
+            for (int j = 0; j < kParts; ++j) lims[i][j] = lims[i + 1][j];
 #pragma unroll
-        for (int j = 0; j < kQ4Parts; ++j) lims[C::kStages - 2][j] = lim[j];
+        for (int j = 0; j < kParts; ++j) lims[C::kStages - 2][j] = lim[j];
         cp_commit();
     }
     // Step s of a unit.
@@ -654,37 +677,38 @@ struct Q4Ring {
     __device__ __forceinline__ void step(const Q4Args& a, int s, State& st, Find&& find) {
         cp_wait<C::kStages - 2>();
         __syncwarp();
-        int lim[kQ4Parts];
+        int lim[kParts];
 #pragma unroll
-        for (int j = 0; j < kQ4Parts; ++j) lim[j] = lims[0][j];
+        for (int j = 0; j < kParts; ++j) lim[j] = lims[0][j];
         ask(a, s + C::kStages - 1, find);
-        typename State::Four x[kQ4Parts];
+        typename State::Four x[kParts];
 #pragma unroll
-        for (int j = 0; j < kQ4Parts; ++j) st.scores(slot(s) + j * C::kPartBytes, x[j]);
-        typename State::Scales v[kQ4Parts];
+        for (int j = 0; j < kParts; ++j) st.scores(slot(s) + j * C::kPartBytes, x[j]);
+        typename State::Scales v[kParts];
 #pragma unroll
-        for (int j = 0; j < kQ4Parts; ++j) st.look(slot(s) + j * C::kPartBytes + Tile::kTile, v[j]);
+        for (int j = 0; j < kParts; ++j) st.look(slot(s) + j * C::kPartBytes + Tile::kTile, v[j]);
         st.weigh(x, lim, v);
 #pragma unroll
-        for (int j = 0; j < kQ4Parts; ++j) st.add(slot(s) + j * C::kPartBytes + Tile::kTile, x[j], v[j]);
+        for (int j = 0; j < kParts; ++j) st.add(slot(s) + j * C::kPartBytes + Tile::kTile, x[j], v[j]);
         if (++st.owed == State::kSettle) st.settle();
         __syncwarp();
     }
 };
 
-template <typename T_, int D_, bool kListed_>
+template <typename T_, int D_, bool kListed_, int kParts_>
 struct Q4Base {
     using T = T_;
     using Args = Q4Args;
-    static constexpr int D = D_, kParts = kQ4Parts;
-    static constexpr bool kListed = kListed_, kOdd = false;
+    static constexpr int D = D_, kParts = kParts_;
+    static constexpr bool kListed = kListed_, kOdd = false, kGrouped = !kListed;
     static constexpr float kBias = 0.f;
 };
-template <typename T, int D, int NG, int NT, bool kListed>
-struct Q4Form : Q4Base<T, D, kListed>, Q4Cfg<D, NT> {
-    using Joined = Q4Base<T, D, kListed>;
-    using State = Q4State<T, D, NG, NT>;
-    using Ring = Q4Ring<D, NG, NT>;
+template <typename T, int D, int NG, int NT, bool kListed, bool kUnits, class C = Q4Cfg<D, NT, kUnits>>
+struct Q4Form : Q4Base<T, D, kListed, C::kParts> {
+    using Joined = Q4Base<T, D, kListed, C::kParts>;
+    using State = Q4State<T, D, NG, NT, C::kParts>;
+    using Ring = Q4Ring<D, NG, NT, kUnits>;
+    static constexpr int kCtas = C::kCtas, kStages = C::kStages, kRing = C::kRing, kSmem = C::kSmem;
     __device__ __forceinline__ static void start(State& st, const Q4Args& a, const uint16_t* q, int rows) {
         st.start(q, rows, a.scale2);
     }
@@ -692,7 +716,8 @@ struct Q4Form : Q4Base<T, D, kListed>, Q4Cfg<D, NT> {
 
 template <typename T, int D, int NG, bool kListed>
 cudaError_t launch_heads(const Q4Args& a, int W, cudaStream_t s) {
-    return a.G <= 8 ? launch_paged<Q4Form<T, D, NG, 1, kListed>>(a, W, s) : launch_paged<Q4Form<T, D, NG, 2, kListed>>(a, W, s);
+    return a.G <= 8 ? launch_paged<Q4Form<T, D, NG, 1, kListed, false>, Q4Form<T, D, NG, 1, kListed, true>>(a, W, s)
+                    : launch_paged<Q4Form<T, D, NG, 2, kListed, false>, Q4Form<T, D, NG, 2, kListed, true>>(a, W, s);
 }
 
 template <typename T, bool kListed>

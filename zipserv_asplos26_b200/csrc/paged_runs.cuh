@@ -8,7 +8,9 @@
 //     runs, found by a prefix sum over the lengths in the kernel, so ragged
 //     batches and single long sequences load every SM alike and no length is
 //     needed on the host. A run that ends inside a unit leaves its (m, l, O) in a
-//     workspace, and paged_join_kernel joins a unit's pieces in order.
+//     workspace, and paged_join_kernel joins a unit's pieces in order. Where rows of
+//     neighbouring heads share lines, a run goes to a CTA whose warps take the same
+//     tokens of a head each (PaArgs::group).
 //   * paged_attn_units_kernel: a fixed number of warps a unit, joined through
 //     distributed shared memory in the same kernel: short units and page lists.
 // Sums are always in the same order for the same sizes on the host and the same
@@ -16,7 +18,7 @@
 // those of 16-bit keys and values.
 //
 // A form F says what a warp does: T (of q and the output), D, kListed (page lists),
-// kParts (of a chunk), Args (PaArgs or more), kCtas, kStages, kRing, kSmem, Ring (start,
+// kParts (of a chunk), kGrouped (whether PaArgs::group is looked at), Args (PaArgs or more), kCtas, kStages, kRing, kSmem, Ring (start,
 // ask, step), State (what a warp holds of a unit: finish, write, park), start (of a
 // State), kBias (of its exponentials), kOdd (whether infinite values are looked at again,
 // by odd_values and State's odd and mend) and Joined (a form of the same T, D, kListed,
@@ -51,6 +53,7 @@ struct PaArgs {
     float* part_ml;           // [2 W][prow][2], W warps
     float* part_o;            // [2 W][prow][D]
     unsigned* err;
+    int group;                // units that a run's warps take side by side: 1, or a CTA's warps one each
 };
 
 namespace {
@@ -220,7 +223,8 @@ __global__ void __launch_bounds__(kPaThreads, F::kCtas) paged_attn_kernel(const 
 
     // ---- each warp's run of chunks
     const int entries = kListed ? a.B * a.Hkv : a.B;
-    const int per_entry = kListed ? a.tiles : a.Hkv * a.tiles;     // units an entry
+    const int group = F::kGrouped ? a.group : 1;
+    const int per_entry = (kListed ? a.tiles : a.Hkv * a.tiles) / group;     // groups of units an entry
     // Each warp by itself: lane i sums the chunks of entries [i per, (i + 1) per),
     // a prefix over the lanes gives the total and the lane whose entries hold the
     // warp's first chunk, a second one over those entries the entry.
@@ -235,13 +239,14 @@ __global__ void __launch_bounds__(kPaThreads, F::kCtas) paged_attn_kernel(const 
     }
     const long long inc = warp_prefix(mine);
     const long long total = __shfl_sync(~0u, inc, 31) * per_entry;
-    const int warps = gridDim.x * kPaWarps;
+    const int warps = gridDim.x * (kPaWarps / group);              // that take runs of their own
     // two chunks or more: pieces of one would double what is joined (48 pages for 8
     // pairs 17.5 us, 16.3 so)
     const long long run = max(div_nonneg(total + warps - 1, warps), 2ll);
     if (blockIdx.x == 0 && tid == 0) a.plan[0] = run;
     // neighbouring runs go to different CTAs, so that few chunks spread over the SMs
-    const int id = warp * (int)gridDim.x + (int)blockIdx.x;
+    const int mine_of = group > 1 ? warp : 0;                      // the warp's unit of a group
+    const int id = (group > 1 ? 0 : warp) * (int)gridDim.x + (int)blockIdx.x;
     const long long c_begin = run * id;
     if (c_begin >= total) return;
     const int steps = (int)min(run, total - c_begin);
@@ -288,7 +293,7 @@ __global__ void __launch_bounds__(kPaThreads, F::kCtas) paged_attn_kernel(const 
         t.ids = 0;
         t.lims = 0;
         t.ch = at.ch;
-        t.h = kListed ? at.e % a.Hkv : at.in_e / a.tiles;
+        t.h = kListed ? at.e % a.Hkv : (at.in_e * group + mine_of) / a.tiles;
         if (t.count <= 0) return;
         if (lane < t.count * kParts && (kParts == 1 || at.ch * kParts + lane < entry_parts<kListed>(a, at.e))) {
             const int b = kListed ? at.e / a.Hkv : at.e;
@@ -313,7 +318,7 @@ __global__ void __launch_bounds__(kPaThreads, F::kCtas) paged_attn_kernel(const 
         return __shfl_sync(~0u, now.lims, in_batch++);
     };
     typename F::Ring ring;
-    ring.start(smem_u32(pa_smem) + warp * F::kRing, steps);
+    ring.start(a, smem_u32(pa_smem) + warp * F::kRing, steps);
 #pragma unroll
     for (int s = 0; s < F::kStages - 1; ++s) {
         ring.ask(a, s, find);
@@ -325,8 +330,9 @@ __global__ void __launch_bounds__(kPaThreads, F::kCtas) paged_attn_kernel(const 
         // ---- a unit, or the part of it in this run
         const int first = cur.ch, count = min(cur.n - first, steps - s);
         const int b = kListed ? cur.e / a.Hkv : cur.e;
-        const int h = kListed ? cur.e % a.Hkv : cur.in_e / a.tiles;
-        const int tile = kListed ? cur.in_e : cur.in_e % a.tiles;
+        const int of = cur.in_e * group + mine_of;
+        const int h = kListed ? cur.e % a.Hkv : of / a.tiles;
+        const int tile = kListed ? cur.in_e : of % a.tiles;
         const int g0 = tile * kPaRows, rows = min(kPaRows, a.G - g0);
         if (first == 0 && lane == 0) a.plan[1 + (b * a.Hkv + h) * a.tiles + tile] = u_lo;
         const long long head0 = (long long)b * a.Hq + (long long)h * a.G + g0;
@@ -335,7 +341,7 @@ __global__ void __launch_bounds__(kPaThreads, F::kCtas) paged_attn_kernel(const 
         for (const int end = s + count; s < end; ++s) ring.step(a, s, st, find);
         // ---- out, or to the workspace where the run cuts the unit
         const bool whole = first == 0 && count == cur.n;
-        const long long slot = 2ll * id + (s == count ? 0 : 1);       // the run's first part, or its last
+        const long long slot = (2ll * id + (s == count ? 0 : 1)) * group + mine_of;    // the run's first part, or its last
         st.finish();
         if (whole) {
             if constexpr (F::kOdd) {
@@ -397,7 +403,7 @@ __global__ void __launch_bounds__(kPaThreads, F::kCtas) paged_attn_units_kernel(
         return __shfl_sync(~0u, lims, x & 31);
     };
     typename F::Ring ring;
-    ring.start(smem_u32(pa_smem) + warp * F::kRing, steps);
+    ring.start(a, smem_u32(pa_smem) + warp * F::kRing, steps);
 #pragma unroll
     for (int s = 0; s < F::kStages - 1; ++s) ring.ask(a, s, find);
     F::start(st, a, a.q + head0 * D, rows);
@@ -506,6 +512,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const typen
     grid_dep_wait();
     const long long run = a.plan[0], lo = a.plan[1 + (b * a.Hkv + h) * a.tiles + tile];
     const int n = entry_chunks<F>(a, kListed ? b * a.Hkv + h : b);
+    const int group = F::kGrouped ? a.group : 1, of = group > 1 ? (h * a.tiles + tile) % group : 0;
     float m = -INFINITY, l = 0.f, acc[kVec];
 #pragma unroll
     for (int j = 0; j < kVec; ++j) acc[j] = 0.f;
@@ -521,7 +528,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const typen
 #pragma unroll
             for (int x = 0; x < kJoinBatch; ++x) {
                 const int w = v + x * by;
-                const long long s = (2ll * w + (w == w0 && second ? 1 : 0)) * a.prow + row;
+                const long long s = ((2ll * w + (w == w0 && second ? 1 : 0)) * group + of) * a.prow + row;
                 ml[x] = make_float2(-INFINITY, 0.f);
 #pragma unroll
                 for (int j = 0; j < kVec; ++j) o[x][j] = 0.f;
@@ -695,10 +702,10 @@ cudaError_t launch_units(const typename F::Args& a, int W, cudaStream_t s) {
     return cudaLaunchKernelEx(&cfg, kernel, a, W);
 }
 
-// a's attention by form F; `W` is unit_warps' answer.
-template <class F>
+// a's attention by form F in runs, or by U in units where W, unit_warps' answer, is not 0.
+template <class F, class U>
 cudaError_t launch_paged(const typename F::Args& a, int W, cudaStream_t s) {
-    if (W) return launch_units<F>(a, W, s);
+    if (W) return launch_units<U>(a, W, s);
     int ctas = 0;
     cudaError_t e = resident_ctas<F>(&ctas);
     if (e != cudaSuccess) return e;
