@@ -460,6 +460,37 @@ typedef struct ZsPagedAttentionInt4 {
 size_t zs_paged_attention_int4_workspace(const ZsPagedAttentionInt4* args);
 int zs_paged_attention_int4(const ZsPagedAttentionInt4* args);
 
+/* ---- Sampling ------------------------------------------------------------
+ * One token per row of logits [B][V] (row_stride elements apart, V up to 2^20; any
+ * alignment of their type) from a random number u in [0, 1). With w_i = exp((x_i - max x)
+ * / temperature) and the tokens in the order of x, largest first and equal ones by index:
+ * the first top_k are kept (0: all), of these the shortest beginning whose weights reach
+ * top_p of theirs (1: all), of these the tokens with w_i >= min_p (0: all), the first token
+ * in any case. The token is the first, by index, at which the running sum of the kept
+ * weights passes u times their sum; sums do not depend on an order. temperature <= 0: the
+ * first of the largest. A logit of -inf is never chosen; where some are +inf, these have
+ * weight 1 and the others none. Each setting is a device array [B], or, where that is NULL,
+ * the value in ...1 for all rows. out [B]: the tokens; -1, and bit 8 in *err (nullable), for
+ * a row with a NaN or of -inf alone. Settings that are NaN count as off (temperature: as
+ * 0), u outside [0, 1) as its nearest end. */
+enum { ZS_FP32 = 2 };
+typedef struct ZsSample {
+    void* stream;
+    const void* logits;
+    int64_t row_stride;
+    const float* u;
+    const float* temperature;
+    const int* top_k;
+    const float* top_p;
+    const float* min_p;
+    int64_t* out;
+    unsigned* err;
+    int B, V, dtype;                /* ZS_BF16, ZS_FP16 or ZS_FP32 */
+    int top_k1;
+    double temperature1, top_p1, min_p1;
+} ZsSample;
+int zs_sample(const ZsSample* args);
+
 /* ---- On-disk TCA-TBE container (file format version 1) -------------------
  * No counterpart in the reference, which keeps no serialised compressed form
  * (its benchmarks re-encode the dense checkpoint at start-up,

@@ -19,3 +19,6 @@ from .paged import (Int4Pages, PagedKVCache, StepPlan, TokenRows, int4_pages, pa
 __all__ += ["PagedKVCache", "StepPlan", "TokenRows", "page_bounds", "paged_attention", "plan_step", "rope_write", "select_pages",
             "sparse_attention"]
 __all__ += ["Int4Pages", "int4_pages", "paged_attention_int4", "read_int4", "rope_write_int4"]
+from .sampling import sample  # noqa: E402,F401
+
+__all__ += ["sample"]

@@ -756,6 +756,61 @@ PyObject* paged_attention_int4(PyObject* const* a) {
     return THPVariable_Wrap(std::move(out));
 }
 
+// -------------------------------------------------------------- sampling
+// A setting for all rows (a number), or a row each (a tensor of B elements).
+const float* setting(PyObject* o, int64_t B, const char* name, int index, double& one) {
+    if (THPVariable_Check(o)) return vec<float>(o, B, at::kFloat, name, index);
+    one = number(o);
+    return nullptr;
+}
+
+// logits, u, temperature, top_k, top_p, min_p, out, err
+PyObject* sample(PyObject* const* a) {
+    const at::Tensor& x = cuda_tensor(a[0], "logits");
+    const int index = static_cast<int>(x.get_device());
+    const at::ScalarType type = x.scalar_type();
+    need(x.dim() == 2 && (type == at::kFloat || dtype_code(type) >= 0), "logits must be a bf16, fp16 or float32 tensor [B, V]");
+    const int64_t B = x.size(0), V = x.size(1);
+    need(V > 0 && V <= (1 << 20) && B <= INT32_MAX / 8, "at most 2**20 tokens a row, and one at least");
+    need(x.stride(1) == 1 || V == 1, "logits must have contiguous rows");
+    ZsSample p{};
+    p.logits = ptr(x);
+    p.row_stride = B > 1 ? x.stride(0) : V;
+    p.u = vec<float>(a[1], B, at::kFloat, "u", index);
+    p.temperature = setting(a[2], B, "temperature", index, p.temperature1);
+    if (!THPVariable_Check(a[3])) {
+        const int64_t k = integer(a[3]);
+        need(k >= 0, "top_k must not be negative");
+        p.top_k1 = static_cast<int>(std::min<int64_t>(k, INT32_MAX));
+    } else {
+        p.top_k = vec<int>(a[3], B, at::kInt, "top_k", index);
+    }
+    p.top_p = setting(a[4], B, "top_p", index, p.top_p1);
+    p.min_p = setting(a[5], B, "min_p", index, p.min_p1);
+    need(p.temperature || (p.temperature1 >= 0 && std::isfinite(p.temperature1)), "temperature must be 0 or more");
+    need(p.top_p || (p.top_p1 >= 0 && p.top_p1 <= 1), "top_p must be from 0 to 1");
+    need(p.min_p || (p.min_p1 >= 0 && p.min_p1 <= 1), "min_p must be from 0 to 1");
+    at::Tensor out;
+    OnDevice on(index);
+    if (given(a[6])) {
+        p.out = vec<int64_t>(a[6], B, at::kLong, "out", index);
+    } else {
+        out = fresh({B}, at::kLong, index);
+        p.out = ptr<int64_t>(out);
+    }
+    p.err = err_word(a[7], index);
+    p.stream = current_stream(index);
+    p.B = static_cast<int>(B);
+    p.V = static_cast<int>(V);
+    p.dtype = type == at::kFloat ? ZS_FP32 : dtype_code(type);
+    call(zs_sample, p, "zs_sample");
+    if (given(a[6])) {
+        Py_INCREF(a[6]);
+        return a[6];
+    }
+    return THPVariable_Wrap(std::move(out));
+}
+
 // No C++ exception leaves a C entry: refusals are ValueErrors, the rest RuntimeErrors.
 template <PyObject* (*F)(PyObject* const*), int N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -781,6 +836,7 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef methods[] = {ZS_ENTRY(plan_step, 10),    ZS_ENTRY(rope_write, 12),  ZS_ENTRY(paged_attention, 12),
                          ZS_ENTRY(page_bounds, 9),  ZS_ENTRY(select_pages, 10), ZS_ENTRY(sparse_attention, 13),
                          ZS_ENTRY(rope_write_int4, 12), ZS_ENTRY(read_int4, 6), ZS_ENTRY(paged_attention_int4, 12),
+                         ZS_ENTRY(sample, 8),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_paged_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
