@@ -15,13 +15,14 @@
 // Of the weights themselves 2^-49 is lost in 2^(-t): t's nearest multiple of 1 / 2048 from
 // a table, the rest by a polynomial of degree three.
 //
-// Borders are found by three passes over 12, 12 and 8 bits of the logits' order (16-bit
-// logits: two), each a histogram in shared memory of how many, or how much weight, the
-// tokens hold that share the bits found so far. A row is read once for its maximum, twice
-// or three times for each border, and once for sums of blocks of 1024, from which the
-// token's block is found; all but the first come from L2. A row goes to a cluster of up to
-// 8 CTAs where there are few, its histograms joined through distributed shared memory.
-// Bound by instructions: some 30 for a weight in a histogram, 10 of them in 64 bits.
+// Borders are found by the logits' order, its first 12 bits first: a histogram in shared
+// memory of how many, or how much weight, the tokens hold. A second reading gathers the tokens from there on; up to 2048 of them are
+// all that remains to be looked at, by the next 12 and 8 bits. Where there are more, further
+// readings find the other bits, and sums of blocks of 1024 tokens. In the end the block in
+// which the running sum passes its target is read once more. All readings but the first come
+// from L2. A row goes to a cluster of up to 8 CTAs where there are few, its histograms joined
+// through distributed shared memory. Bound by instructions: some 33 for a weight, 10 of them
+// in 64 bits.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -39,6 +40,7 @@ constexpr int kSampBlock = 1024;            // tokens of a sum
 constexpr int kSampMaxBlocks = 1024;        // so 2^20 tokens at most
 constexpr int kBins = 4096;
 constexpr int kPowers = 2048;
+constexpr int kList = 2048;                 // gathered tokens, at most
 constexpr unsigned kErrSampleNothing = 8u;  // a row had nothing to choose from
 using u64 = unsigned long long;
 
@@ -65,11 +67,15 @@ struct SampShared {
             unsigned lo[kBins], hi[kBins];
         };
     };
-    u64 mass[kSampMaxBlocks];               // of the CTA's blocks: weights above the border
+    u64 mass[kSampMaxBlocks];               // of the CTA's blocks (the row's, from a list): weights above the border
     unsigned ties[kSampMaxBlocks];          // and tokens on it
+    unsigned list_key[kList];
+    int list_at[kList];
+    int listed;                             // tokens that the CTA gathered, more than kList where they did not fit
+    int merged;                             // tokens of the row's list
     u64 part[kSampWarps], part2[kSampWarps];
-    u64 best;                               // the CTA's first largest token
-    int bad;
+    float peak;                             // the CTA's largest logit, NaN where it has one
+    int first;                              // its first token of the largest logit
     // what the first CTA found, for the others
     unsigned bin;
     u64 rest, total;
@@ -81,7 +87,12 @@ __device__ __forceinline__ unsigned order_of(float x) {
     return b >> 31 ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(unsigned k) { return __uint_as_float(k >> 31 ? k & 0x7FFFFFFFu : ~k); }
-constexpr unsigned kOrderInf = 0xFF800000u, kOrderMinusInf = 0x007FFFFFu;
+
+__device__ __forceinline__ float max_nan(float a, float b) {         // NaN where one is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 
 struct Weigher {
     const double* powers;
@@ -170,8 +181,7 @@ struct alignas(sizeof(T) * kVec) Several {
     T x[kVec];
 };
 
-// kVec logits a load where rows start on 16 bytes, else one.
-template <typename T, int kVec>
+template <typename T>
 __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs a) {
     extern __shared__ __align__(16) uint8_t samp_smem[];
     SampShared& sh = *reinterpret_cast<SampShared*>(samp_smem);
@@ -186,172 +196,280 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
         if (size > 1) cluster_sync();
         else __syncthreads();
     };
-    for (int j = tid; j < kPowers; j += kSampThreads) sh.powers[j] = exp2(-(double)j / kPowers);
-
-    // f(logit, index) for the logits from `from` to `to`, four loads on their way.
-    auto each = [&](int from, int to, int first, int threads, auto&& f) {
-        constexpr int kBatch = kVec > 1 ? 4 : 8;
-        for (int i = from + first * kVec; i < to; i += kBatch * threads * kVec) {
+    // f(logit, index) for the logits from `from` to `to`, by threads 0 to `threads`: 16 bytes a
+    // load between the first and the last boundary of 16, four loads on their way.
+    auto each = [&](int from, int to, int me, int threads, auto&& f) {
+        constexpr int kVec = 16 / sizeof(T), kBatch = 4;
+        const int off = (int)(reinterpret_cast<uintptr_t>(x + from) & 15) / (int)sizeof(T);
+        const int head = min(to - from, off ? kVec - off : 0);
+        if (me < head) f(to_float<T>(x[from + me]), from + me);
+        const int start = from + head, vecs = (to - start) / kVec, last = start + vecs * kVec;
+        const Several<T, kVec>* p = reinterpret_cast<const Several<T, kVec>*>(x + start);
+        int i = me;
+        for (; i + (kBatch - 1) * threads < vecs; i += kBatch * threads) {
             Several<T, kVec> v[kBatch];
 #pragma unroll
-            for (int y = 0; y < kBatch; ++y) {
-                const int at = i + y * threads * kVec;
-                if (at + kVec <= to) v[y] = *reinterpret_cast<const Several<T, kVec>*>(x + at);
-                else
-#pragma unroll
-                    for (int j = 0; j < kVec; ++j)
-                        if (at + j < to) v[y].x[j] = x[at + j];
-            }
+            for (int y = 0; y < kBatch; ++y) v[y] = p[i + y * threads];
 #pragma unroll
             for (int y = 0; y < kBatch; ++y)
 #pragma unroll
-                for (int j = 0; j < kVec; ++j) {
-                    const int at = i + y * threads * kVec + j;
-                    if (at < to) f(to_float<T>(v[y].x[j]), at);
-                }
+                for (int j = 0; j < kVec; ++j) f(to_float<T>(v[y].x[j]), start + (i + y * threads) * kVec + j);
         }
+        for (; i < vecs; i += threads) {
+            const Several<T, kVec> v = p[i];
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) f(to_float<T>(v.x[j]), start + i * kVec + j);
+        }
+        if (me < to - last) f(to_float<T>(x[last + me]), last + me);
     };
 
-    // ---- the first of the largest tokens; whether there is a NaN
-    u64 best = 0;
-    bool nan = false;
-    each(e0, e1, tid, kSampThreads, [&](float v, int i) {
-        const unsigned k = order_of(v);
-        nan |= isnan(v);
-        best = max(best, (u64)k << 32 | (unsigned)~i);
-    });
+    // ---- the largest logit, NaN if any is
+    float peak = -INFINITY;
+    each(e0, e1, tid, kSampThreads, [&](float v, int) { peak = max_nan(peak, v); });
 #pragma unroll
-    for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(~0u, best, o));
-    nan = __syncthreads_or(nan);
-    if (lane == 0) sh.part[warp] = best;
+    for (int o = 16; o; o >>= 1) peak = max_nan(peak, __shfl_xor_sync(~0u, peak, o));
+    float* peaks = reinterpret_cast<float*>(sh.part);
+    if (lane == 0) peaks[warp] = peak;
     __syncthreads();
     if (tid == 0) {
-        for (int w = 0; w < kSampWarps; ++w) best = max(best, sh.part[w]);
-        sh.best = best;
-        sh.bad = nan;
+        for (int w = 0; w < kSampWarps; ++w) peak = max_nan(peak, peaks[w]);
+        sh.peak = peak;
+        sh.first = INT_MAX;
+        sh.listed = 0;
     }
     all_sync();
-    best = sh.best;
-    bool bad = sh.bad;
-    for (unsigned r = 0; r < size && size > 1; ++r) {
-        best = max(best, ld_peer64(&sh.best, r));
-        bad |= ld_peer32(&sh.bad, r) != 0;
-    }
-    const unsigned top = (unsigned)(best >> 32);
-    bad |= top <= kOrderMinusInf;
+    peak = sh.peak;
+    for (unsigned r = 0; r < size && size > 1; ++r) peak = max_nan(peak, __uint_as_float(ld_peer32(&sh.peak, r)));
+    const bool bad = isnan(peak) || peak == -INFINITY;
     const double temperature = a.temperature ? (double)a.temperature[row] : a.temperature1;
     const int top_k = a.top_k ? a.top_k[row] : a.top_k1;
     const double top_p = a.top_p ? (double)a.top_p[row] : a.top_p1;
     const double min_p = a.min_p ? (double)a.min_p[row] : a.min_p1;
     if (bad || !(temperature > 0.0) || top_k == 1 || top_p <= 0.0) {           // the same for the row
+        int first = INT_MAX;
+        if (!bad) each(e0, e1, tid, kSampThreads, [&](float v, int i) { first = min(first, v == peak ? i : INT_MAX); });
+        first = __reduce_min_sync(~0u, first);
+        if (lane == 0) atomicMin(&sh.first, first);
+        all_sync();
         if (rank == 0 && tid == 0) {
+            first = sh.first;
+            for (unsigned r = 1; r < size; ++r) first = min(first, (int)ld_peer32(&sh.first, r));
             if (bad) set_err(a.err, kErrSampleNothing);
-            a.out[row] = bad ? -1 : (long long)(unsigned)~(unsigned)best;
+            a.out[row] = bad ? -1 : first;
         }
-        if (size > 1) cluster_sync();                                         // peers read this CTA's numbers
+        if (size > 1) cluster_sync();                                         // the first CTA has read the others' numbers
         return;
     }
 
+    // 2^(-j / 2048) as products of 2^(-i / 32) and 2^(-i / 2048)
+    double* few = reinterpret_cast<double*>(sh.count);
+    if (tid < 96) few[tid] = exp2(-(tid < 32 ? (double)tid / 32 : (double)(tid - 32) / kPowers));
+    __syncthreads();
+    for (int j = tid; j < kPowers; j += kSampThreads) sh.powers[j] = few[j >> 6] * few[32 + (j & 63)];
+    __syncthreads();
     Weigher weigh;
     weigh.powers = sh.powers;
-    weigh.peak = (double)value_of(top);
+    weigh.peak = (double)peak;
     weigh.rate = 1.4426950408889634 / temperature;
     weigh.steps = a.steps;
     weigh.least = 0.0;
     constexpr int kLevels = std::is_same<T, float>::value ? 3 : 2;            // 16-bit types: 24 bits tell all apart
     constexpr int kDigit[3] = {20, 8, 0}, kWidth[3] = {12, 12, 8};
+    const auto whole = [&](auto&& f) { each(e0, e1, tid, kSampThreads, [&](float v, int) { f(order_of(v), v); }); };
+    const auto list = [&](auto&& f) {
+        for (int i = tid; i < sh.merged; i += kSampThreads) f(sh.list_key[i], value_of(sh.list_key[i]));
+    };
 
-    // The place of a border in the order: kCount: of the `want`-th token; else where weights,
-    // of the tokens above `floor_key` and floor_ties times the one on it, reach top_p of their
-    // sum. rest: what is wanted of the tokens on the border (tokens, or weight).
-    auto border = [&](auto count_c, u64 want, unsigned floor_key, u64 floor_ties, u64& rest) {
-        constexpr bool kCount = decltype(count_c)::value;
-        unsigned found = 0;
-#pragma unroll 1
-        for (int level = 0; level < kLevels; ++level) {
-            const int shift = kDigit[level], width = kWidth[level], bins = 1 << width;
-            for (int j = tid; j < bins; j += kSampThreads) {
-                if constexpr (kCount) sh.count[j] = 0;
-                else sh.lo[j] = sh.hi[j] = 0;
-            }
-            __syncthreads();
-            auto put = [&](unsigned k, u64 w) {
-                const unsigned b = k >> shift & (bins - 1);
-                if constexpr (kCount) atomicAdd(&sh.count[b], 1u);
-                else if (w) {
-                    const unsigned lo = (unsigned)w, old = atomicAdd(&sh.lo[b], lo);
-                    const unsigned hi = (unsigned)(w >> 32) + (old + lo < old ? 1u : 0u);
-                    if (hi) atomicAdd(&sh.hi[b], hi);
-                }
-            };
-            each(e0, e1, tid, kSampThreads, [&](float v, int) {
-                const unsigned k = order_of(v);
-                if (level && k >> (shift + width) != found) return;
-                if constexpr (kCount) put(k, 0);
-                else if (k > floor_key) put(k, weigh(v));
-            });
-            if (!kCount && rank == 0 && tid == 0 && floor_ties && (!level || floor_key >> (shift + width) == found))
-                put(floor_key, weigh(value_of(floor_key)) * floor_ties);
-            all_sync();
-            if (rank == 0) {
-                // a thread's bins, from the highest down
-                const int per = max(1, bins / kSampThreads);
-                const int high = bins - 1 - tid * per;
-                u64 sum = 0, each_bin[kBins / kSampThreads];
-#pragma unroll
-                for (int j = 0; j < kBins / kSampThreads; ++j) {
-                    each_bin[j] = 0;
-                    if (j >= per || high - j < 0) continue;
-                    for (unsigned r = 0; r < size; ++r) {
-                        if constexpr (kCount) each_bin[j] += size > 1 ? ld_peer32(&sh.count[high - j], r) : sh.count[high - j];
-                        else if (size > 1)
-                            each_bin[j] += (u64)ld_peer32(&sh.hi[high - j], r) << 32;
-                        else each_bin[j] += (u64)sh.hi[high - j] << 32;
-                        if constexpr (!kCount) each_bin[j] += size > 1 ? ld_peer32(&sh.lo[high - j], r) : sh.lo[high - j];
-                    }
-                    sum += each_bin[j];
-                }
-                u64 total;
-                u64 before = block_prefix(sum, sh.part, total) - sum;
-                if (!kCount && level == 0) want = times(top_p, total, true);
-#pragma unroll
-                for (int j = 0; j < kBins / kSampThreads; ++j) {
-                    if (before < want && want <= before + each_bin[j]) {
-                        sh.bin = high - j;
-                        sh.rest = want - before;
-                    }
-                    before += each_bin[j];
-                }
-            }
-            all_sync();
-            const unsigned bin = size > 1 ? ld_peer32(&sh.bin, 0) : sh.bin;
-            want = size > 1 ? ld_peer64(&sh.rest, 0) : sh.rest;
-            found = found << width | bin;
+    // One digit of a border in the order, `found` being the digits before it. Count: of the
+    // `want`-th token of `from`; else where weights, of the tokens above `floor` and floor_ties
+    // times the one on it, reach `want` (at the first digit: top_p of their sum). `from` is the
+    // CTA's share of the row (cluster true) or the list, which the first CTA has to itself.
+    auto digit = [&](auto count_c, auto cluster_c, int level, auto&& from, unsigned floor, u64 floor_ties, unsigned& found,
+                     u64& want) {
+        constexpr bool kCount = decltype(count_c)::value, kCluster = decltype(cluster_c)::value;
+        const unsigned many = kCluster ? size : 1u;
+        const int shift = kDigit[level], width = kWidth[level], bins = 1 << width;
+        auto sync = [&] {
+            if (many > 1) cluster_sync();
+            else __syncthreads();
+        };
+        for (int j = tid; j < bins; j += kSampThreads) {
+            if constexpr (kCount) sh.count[j] = 0;
+            else sh.lo[j] = sh.hi[j] = 0;
         }
-        // peers have read the first CTA's numbers before it writes new ones: its histogram
-        // and the next all_sync lie in between
-        rest = want;
+        __syncthreads();
+        auto put = [&](unsigned k, u64 w) {
+            const unsigned b = k >> shift & (bins - 1);
+            if constexpr (kCount) atomicAdd(&sh.count[b], 1u);
+            else if (w) {
+                const unsigned lo = (unsigned)w, old = atomicAdd(&sh.lo[b], lo);
+                const unsigned hi = (unsigned)(w >> 32) + (old + lo < old ? 1u : 0u);
+                if (hi) atomicAdd(&sh.hi[b], hi);
+            }
+        };
+        from([&](unsigned k, float v) {
+            if (level && k >> (shift + width) != found) return;
+            if constexpr (kCount) put(k, 0);
+            else if (k > floor) put(k, weigh(v));
+        });
+        if (!kCount && rank == 0 && tid == 0 && floor_ties && (!level || floor >> (shift + width) == found))
+            put(floor, weigh(value_of(floor)) * floor_ties);
+        sync();
+        if (rank == 0) {
+            if (many > 1) {                    // the others' histograms to the first CTA's
+                for (int j = tid; j < bins; j += kSampThreads) {
+                    u64 n = 0;
+                    for (unsigned r = 0; r < many; ++r) {
+                        if constexpr (kCount) n += ld_peer32(&sh.count[j], r);
+                        else n += ((u64)ld_peer32(&sh.hi[j], r) << 32) + ld_peer32(&sh.lo[j], r);
+                    }
+                    if constexpr (kCount) sh.count[j] = (unsigned)n;
+                    else {
+                        sh.lo[j] = (unsigned)n;
+                        sh.hi[j] = (unsigned)(n >> 32);
+                    }
+                }
+                __syncthreads();
+            }
+            // a warp's bins, from the highest down
+            const int per = bins / kSampWarps, end = bins - 1 - warp * per;
+            u64 v[kBins / kSampThreads], sum = 0;
+#pragma unroll
+            for (int i = 0; i < kBins / kSampThreads; ++i) {
+                const int b = end - (i * 32 + lane);
+                v[i] = 0;
+                if (i * 32 + lane < per) {
+                    if constexpr (kCount) v[i] = sh.count[b];
+                    else v[i] = ((u64)sh.hi[b] << 32) + sh.lo[b];
+                }
+                sum += v[i];
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+            if (lane == 0) sh.part[warp] = sum;
+            __syncthreads();
+            u64 before = 0, total = 0;
+            for (int w = 0; w < kSampWarps; ++w) {
+                if (w < warp) before += sh.part[w];
+                total += sh.part[w];
+            }
+            if (!kCount && level == 0) want = times(top_p, total, true);
+            if (before < want && want <= before + sum) {
+#pragma unroll
+                for (int i = 0; i < kBins / kSampThreads; ++i) {
+                    u64 up_to = v[i];
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const u64 x = __shfl_up_sync(~0u, up_to, o);
+                        if (lane >= o) up_to += x;
+                    }
+                    up_to += before;
+                    if (up_to - v[i] < want && want <= up_to) {
+                        sh.bin = end - (i * 32 + lane);
+                        sh.rest = want - (up_to - v[i]);
+                    }
+                    before = __shfl_sync(~0u, up_to, 31);
+                }
+            }
+        }
+        sync();
+        const unsigned bin = many > 1 ? ld_peer32(&sh.bin, 0) : sh.bin;
+        want = many > 1 ? ld_peer64(&sh.rest, 0) : sh.rest;
+        found = found << width | bin;
+    };
+    // A border from digit `level` on; `want` in the end: of the tokens on it.
+    auto border = [&](auto count_c, auto cluster_c, int level, auto&& from, unsigned floor, u64 floor_ties, unsigned found,
+                      u64& want) {
+#pragma unroll 1
+        for (; level < kLevels; ++level) digit(count_c, cluster_c, level, from, floor, floor_ties, found, want);
         if constexpr (kLevels == 2) found = found << 8 | (found >> 23 ? 0u : 0xFFu);
         return found;
     };
-
+    const std::true_type yes{};
+    const std::false_type no{};
+    const bool by_count = top_k > 0 && top_k < a.V, by_weight = top_p < 1.0;
+    const double least = min_p > 0.0 ? fmin(min_p, 1.0) * __hiloint2double((1023 + a.steps) << 20, 0) : 0.0;
     unsigned edge = 0;             // tokens above it are kept, and of those on it the first `ties`
-    u64 ties = 0, rest;
-    if (top_k > 0 && top_k < a.V) {
-        edge = border(std::true_type(), (u64)top_k, 0u, 0ull, rest);
-        ties = rest;
+    u64 ties = 0, on_edge = 0;     // its weight
+    bool from_list = false;
+    if (by_count || by_weight) {
+        // ---- the first digit, and the tokens from it on
+        unsigned found = 0;
+        u64 want = (u64)top_k;
+        if (by_count) digit(yes, yes, 0, whole, 0u, 0ull, found, want);
+        else digit(no, yes, 0, whole, 0u, 0ull, found, want);
+        const unsigned low = found << kDigit[0];
+        each(e0, e1, tid, kSampThreads, [&](float v, int i) {
+            const unsigned k = order_of(v);
+            if (k < low) return;
+            const int at = atomicAdd(&sh.listed, 1);
+            if (at < kList) {
+                sh.list_key[at] = k;
+                sh.list_at[at] = i;
+            }
+        });
+        all_sync();
+        int listed = 0;
+        for (unsigned r = 0; r < size; ++r) listed += min(size > 1 ? (int)ld_peer32(&sh.listed, r) : sh.listed, kList + 1);
+        from_list = listed <= kList;
+        if (from_list && rank == 0) {
+            // the others' tokens behind the first CTA's
+            int n = sh.listed;
+            for (unsigned r = 1; r < size; ++r) {
+                const int more = (int)ld_peer32(&sh.listed, r);
+                for (int i = tid; i < more; i += kSampThreads) {
+                    sh.list_key[n + i] = ld_peer32(&sh.list_key[i], r);
+                    sh.list_at[n + i] = (int)ld_peer32(&sh.list_at[i], r);
+                }
+                n += more;
+            }
+            __syncthreads();
+            if (tid == 0) sh.merged = n;
+            for (int b = tid; b < (int)size * a.blocks; b += kSampThreads) {
+                sh.mass[b] = 0;
+                sh.ties[b] = 0;
+            }
+            __syncthreads();
+            if (by_count) {
+                edge = border(yes, no, 1, list, 0u, 0ull, found, want);
+                ties = want;
+            }
+            if (by_weight) {
+                if (by_count) edge = border(no, no, 0, list, edge, ties, 0u, want);
+                else edge = border(no, no, 1, list, 0u, 0ull, found, want);
+                const u64 w = weigh(value_of(edge));
+                ties = (want + w - 1) / w;
+            }
+            weigh.least = least;
+            on_edge = weigh(value_of(edge));
+            for (int i = tid; i < sh.merged; i += kSampThreads) {
+                const unsigned k = sh.list_key[i];
+                const int b = sh.list_at[i] / kSampBlock;
+                if (k > edge) atomicAdd(&sh.mass[b], weigh(value_of(k)));
+                else if (k == edge) atomicAdd(&sh.ties[b], 1u);
+            }
+            __syncthreads();
+        }
+        if (!from_list) {
+            if (by_count) {
+                edge = border(yes, yes, 1, whole, 0u, 0ull, found, want);
+                ties = want;
+            }
+            if (by_weight) {
+                if (by_count) edge = border(no, yes, 0, whole, edge, ties, 0u, want);
+                else edge = border(no, yes, 1, whole, 0u, 0ull, found, want);
+                const u64 w = weigh(value_of(edge));
+                ties = (want + w - 1) / w;
+            }
+        }
     }
-    if (top_p < 1.0) {
-        const unsigned e = border(std::false_type(), 0ull, edge, ties, rest);
-        const u64 w = weigh(value_of(e));
-        ties = (rest + w - 1) / w;
-        edge = e;
+    if (!from_list) {
+        weigh.least = least;
+        on_edge = edge ? weigh(value_of(edge)) : 0ull;
     }
-    if (min_p > 0.0) weigh.least = fmin(min_p, 1.0) * __hiloint2double((1023 + a.steps) << 20, 0);
 
     // ---- sums of blocks, a warp a block
-    const u64 on_edge = edge ? weigh(value_of(edge)) : 0ull;
-    for (int b = warp; b < a.blocks; b += kSampWarps) {
+    for (int b = warp; b < a.blocks && !from_list; b += kSampWarps) {
         const int from = e0 + b * kSampBlock;
         if (from >= e1) {
             if (lane == 0) {
@@ -377,14 +495,15 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
             sh.ties[b] = t;
         }
     }
-    all_sync();
+    if (!from_list) all_sync();
     if (rank == 0) {
         // a thread's blocks in order; the block in which the running sum passes u times the sum
         const int all = (int)size * a.blocks, per = (all + kSampThreads - 1) / kSampThreads;
         auto at = [&](int b, u64& m, unsigned& t) {
             const int r = b / a.blocks, i = b % a.blocks;
-            m = size > 1 ? ld_peer64(&sh.mass[i], r) : sh.mass[i];
-            t = size > 1 ? ld_peer32(&sh.ties[i], r) : sh.ties[i];
+            const bool own = size == 1 || from_list;
+            m = own ? sh.mass[from_list ? b : i] : ld_peer64(&sh.mass[i], r);
+            t = own ? sh.ties[from_list ? b : i] : ld_peer32(&sh.ties[i], r);
         };
         u64 sum = 0, tied = 0, total;
         for (int b = tid * per; b < min(all, (tid + 1) * per); ++b) {
@@ -455,9 +574,9 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
     if (size > 1) cluster_sync();          // the first CTA has read the others' sums
 }
 
-template <typename T, int kVec>
+template <typename T>
 cudaError_t launch_sample(const SampArgs& a, int B, int cluster, cudaStream_t s) {
-    const auto kernel = sample_kernel<T, kVec>;
+    const auto kernel = sample_kernel<T>;
     static std::atomic<unsigned long long> ready{0};      // a bit a device
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -480,13 +599,6 @@ cudaError_t launch_sample(const SampArgs& a, int B, int cluster, cudaStream_t s)
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, a);
-}
-
-template <typename T>
-cudaError_t launch_type(const SampArgs& a, int B, int cluster, cudaStream_t s) {
-    constexpr int kVec = 16 / sizeof(T);
-    const bool aligned = aligned16p(a.logits) && (B == 1 || a.stride % kVec == 0);
-    return aligned ? launch_sample<T, kVec>(a, B, cluster, s) : launch_sample<T, 1>(a, B, cluster, s);
 }
 
 }  // namespace
@@ -526,8 +638,8 @@ extern "C" int zs_sample(const ZsSample* p) {
     a.blocks = (blocks + cluster - 1) / cluster;
     cudaStream_t s = (cudaStream_t)p->stream;
     switch (p->dtype) {
-        case ZS_BF16: return launch_type<__nv_bfloat16>(a, p->B, cluster, s);
-        case ZS_FP16: return launch_type<__half>(a, p->B, cluster, s);
-        default: return launch_type<float>(a, p->B, cluster, s);
+        case ZS_BF16: return launch_sample<__nv_bfloat16>(a, p->B, cluster, s);
+        case ZS_FP16: return launch_sample<__half>(a, p->B, cluster, s);
+        default: return launch_sample<float>(a, p->B, cluster, s);
     }
 }
