@@ -25,6 +25,7 @@
 // in 64 bits.
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -42,6 +43,7 @@ constexpr int kBins = 4096;
 constexpr int kPowers = 2048;
 constexpr int kList = 2048;                 // gathered tokens, at most
 constexpr unsigned kErrSampleNothing = 8u;  // a row had nothing to choose from
+constexpr unsigned kOrderOfMost = 0xFF7FFFFFu, kOrderOfMinusInf = 0x007FFFFFu;     // of the largest finite number
 using u64 = unsigned long long;
 
 struct SampArgs {
@@ -83,8 +85,8 @@ struct SampShared {
 
 // Logits in their order as unsigned numbers; both zeros are one.
 __device__ __forceinline__ unsigned order_of(float x) {
-    const unsigned b = __float_as_uint(x + 0.f);
-    return b >> 31 ? ~b : b | 0x80000000u;
+    const int b = __float_as_int(x + 0.f);
+    return (unsigned)(b ^ (b >> 31 | INT_MIN));
 }
 __device__ __forceinline__ float value_of(unsigned k) { return __uint_as_float(k >> 31 ? k & 0x7FFFFFFFu : ~k); }
 
@@ -97,14 +99,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {         // NaN wher
 struct Weigher {
     const double* powers;
     double peak, rate, least;      // largest logit; log2(e) / T; min_p in steps
+    float top, cut;                // peak; a logit whose weight is 0, as are those below
     int steps;
 
-    // The weight of a logit in steps of 2^-S; 0 where min_p leaves it out.
-    __device__ __forceinline__ u64 operator()(float x) const {
-        const double d = peak - (double)x;              // NaN where both are infinite: not below 0
-        const double t = d * rate;
-        if (!(d > 0.0)) return 1ull << steps;
-        if (!(t < 64.0)) return 0ull;                   // x is -inf among them
+    // The weight of a logit in steps of 2^-S; with kMin, 0 where min_p leaves it out.
+    template <bool kMin = false>
+    __device__ __forceinline__ u64 of(float x) const {
+        const double t = (peak - (double)fminf(fmaxf(x, cut), top)) * rate;    // below 131
         const double m = fma(t, (double)kPowers, 6755399441055744.0);          // 1.5 2^52: rounds to a whole number
         const int k = __double2loint(m);
         const double r = fma(m - 6755399441055744.0, -1.0 / kPowers, t);
@@ -113,10 +114,11 @@ struct Weigher {
         const double p = powers[k & (kPowers - 1)];
         const double v = fma(p, e, p);
         const double w = __hiloint2double(__double2hiint(v) + ((steps - (k >> 11)) << 20), __double2loint(v));
-        if (w < least) return 0ull;
         const double whole = w + 4503599627370496.0;    // 2^52: its low bits are w rounded
-        return (u64)__double_as_longlong(whole) & 0xFFFFFFFFFFFFFull;
+        const u64 n = (u64)__double_as_longlong(whole) & 0xFFFFFFFFFFFFFull;
+        return kMin && w < least ? 0ull : n;
     }
+    __device__ __forceinline__ u64 of_kept(float x) const { return least > 0.0 ? of<true>(x) : of<false>(x); }
 };
 
 // Inclusive prefix over the block's threads, and the total.
@@ -269,8 +271,19 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
     __syncthreads();
     Weigher weigh;
     weigh.powers = sh.powers;
+    // Logits 64 T ln 2 below the largest, and -inf, weigh nothing. A T so small that the next
+    // number below the largest is further down than that counts as one that puts it at 130.
+    unsigned none = kOrderOfMinusInf;          // logits up to here are not weighed at all
     weigh.peak = (double)peak;
-    weigh.rate = 1.4426950408889634 / temperature;
+    weigh.top = peak;
+    weigh.cut = __double2float_rd((double)peak - 44.3614195558365 * temperature);
+    weigh.cut = fmaxf(fminf(weigh.cut, nextafterf(peak, -INFINITY)), -FLT_MAX);
+    weigh.rate = fmin(1.4426950408889634 / temperature, 130.0 / ((double)peak - (double)weigh.cut));
+    if (isinf(peak)) {                         // infinite ones weigh 1, others nothing
+        none = kOrderOfMost;
+        weigh.peak = weigh.top = weigh.cut = 0.f;
+        weigh.rate = 0.0;
+    }
     weigh.steps = a.steps;
     weigh.least = 0.0;
     constexpr int kLevels = std::is_same<T, float>::value ? 3 : 2;            // 16-bit types: 24 bits tell all apart
@@ -310,10 +323,10 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
         from([&](unsigned k, float v) {
             if (level && k >> (shift + width) != found) return;
             if constexpr (kCount) put(k, 0);
-            else if (k > floor) put(k, weigh(v));
+            else if (k > floor) put(k, weigh.of(v));
         });
         if (!kCount && rank == 0 && tid == 0 && floor_ties && (!level || floor >> (shift + width) == found))
-            put(floor, weigh(value_of(floor)) * floor_ties);
+            put(floor, weigh.of(value_of(floor)) * floor_ties);
         sync();
         if (rank == 0) {
             if (many > 1) {                    // the others' histograms to the first CTA's
@@ -389,19 +402,23 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
     const std::false_type no{};
     const bool by_count = top_k > 0 && top_k < a.V, by_weight = top_p < 1.0;
     const double least = min_p > 0.0 ? fmin(min_p, 1.0) * __hiloint2double((1023 + a.steps) << 20, 0) : 0.0;
-    unsigned edge = 0;             // tokens above it are kept, and of those on it the first `ties`
+    unsigned edge = none;          // tokens above it are kept, and of those on it the first `ties`
     u64 ties = 0, on_edge = 0;     // its weight
     bool from_list = false;
+    auto above_none = [&](u64 want) {          // top_k's border, where weights begin
+        ties = edge > none ? want : 0;
+        edge = max(edge, none);
+    };
     if (by_count || by_weight) {
         // ---- the first digit, and the tokens from it on
         unsigned found = 0;
         u64 want = (u64)top_k;
         if (by_count) digit(yes, yes, 0, whole, 0u, 0ull, found, want);
-        else digit(no, yes, 0, whole, 0u, 0ull, found, want);
+        else digit(no, yes, 0, whole, none, 0ull, found, want);
         const unsigned low = found << kDigit[0];
         each(e0, e1, tid, kSampThreads, [&](float v, int i) {
             const unsigned k = order_of(v);
-            if (k < low) return;
+            if (k < low || *static_cast<volatile int*>(&sh.listed) > kList) return;      // enough is known
             const int at = atomicAdd(&sh.listed, 1);
             if (at < kList) {
                 sh.list_key[at] = k;
@@ -432,20 +449,20 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
             __syncthreads();
             if (by_count) {
                 edge = border(yes, no, 1, list, 0u, 0ull, found, want);
-                ties = want;
+                above_none(want);
             }
             if (by_weight) {
                 if (by_count) edge = border(no, no, 0, list, edge, ties, 0u, want);
-                else edge = border(no, no, 1, list, 0u, 0ull, found, want);
-                const u64 w = weigh(value_of(edge));
+                else edge = border(no, no, 1, list, none, 0ull, found, want);
+                const u64 w = weigh.of(value_of(edge));
                 ties = (want + w - 1) / w;
             }
             weigh.least = least;
-            on_edge = weigh(value_of(edge));
+            on_edge = weigh.of_kept(value_of(edge));
             for (int i = tid; i < sh.merged; i += kSampThreads) {
                 const unsigned k = sh.list_key[i];
                 const int b = sh.list_at[i] / kSampBlock;
-                if (k > edge) atomicAdd(&sh.mass[b], weigh(value_of(k)));
+                if (k > edge) atomicAdd(&sh.mass[b], weigh.of_kept(value_of(k)));
                 else if (k == edge) atomicAdd(&sh.ties[b], 1u);
             }
             __syncthreads();
@@ -453,19 +470,19 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
         if (!from_list) {
             if (by_count) {
                 edge = border(yes, yes, 1, whole, 0u, 0ull, found, want);
-                ties = want;
+                above_none(want);
             }
             if (by_weight) {
                 if (by_count) edge = border(no, yes, 0, whole, edge, ties, 0u, want);
-                else edge = border(no, yes, 1, whole, 0u, 0ull, found, want);
-                const u64 w = weigh(value_of(edge));
+                else edge = border(no, yes, 1, whole, none, 0ull, found, want);
+                const u64 w = weigh.of(value_of(edge));
                 ties = (want + w - 1) / w;
             }
         }
     }
     if (!from_list) {
         weigh.least = least;
-        on_edge = edge ? weigh(value_of(edge)) : 0ull;
+        on_edge = weigh.of_kept(value_of(edge));
     }
 
     // ---- sums of blocks, a warp a block
@@ -482,7 +499,7 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
         unsigned t = 0;
         each(from, min(from + kSampBlock, e1), lane, 32, [&](float v, int) {
             const unsigned k = order_of(v);
-            if (k > edge) m += weigh(v);
+            if (k > edge) m += weigh.of_kept(v);
             t += k == edge;
         });
 #pragma unroll
@@ -553,14 +570,14 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
             if (first + j < a.V) {
                 const float v = to_float<T>(x[first + j]);
                 key[j] = order_of(v);
-                w[j] = key[j] > edge ? weigh(v) : 0ull;
-                here += edge && key[j] == edge;
+                w[j] = key[j] > edge ? weigh.of_kept(v) : 0ull;
+                here += key[j] == edge;
             }
         }
         u64 rank_of = sh.total + block_prefix(here, sh.part, total) - here;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-            if (edge && key[j] == edge) {
+            if (key[j] == edge) {
                 if (rank_of < ties) w[j] = on_edge;
                 ++rank_of;
             }
@@ -631,10 +648,14 @@ extern "C" int zs_sample(const ZsSample* p) {
     int log2v = 0;
     while ((1 << log2v) < p->V) ++log2v;
     a.steps = std::min(50, 62 - log2v);
-    // a CTA has four blocks or more, and all CTAs fit the GPU (two an SM)
+    // A CTA has four blocks or more, and either all CTAs fit the GPU (two an SM), or the rows
+    // at hand L2 (256 rows of 131071 in fp32: 681 MB read from HBM where all were).
     const int blocks = (p->V + kSampBlock - 1) / kSampBlock;
+    const long long row_bytes = (long long)p->V * (p->dtype == ZS_FP32 ? 4 : 2);
     int cluster = 1;
-    while (cluster < 8 && (long long)p->B * cluster * 2 <= 296 && blocks >= cluster * 8) cluster *= 2;
+    while (cluster < 8 && blocks >= cluster * 8 &&
+           ((long long)p->B * cluster * 2 <= 296 || std::min<long long>(p->B, 296 / cluster) * row_bytes > (96ll << 20)))
+        cluster *= 2;
     a.blocks = (blocks + cluster - 1) / cluster;
     cudaStream_t s = (cudaStream_t)p->stream;
     switch (p->dtype) {
