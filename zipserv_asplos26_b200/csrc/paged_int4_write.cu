@@ -11,14 +11,14 @@
 //     one (no fused multiply-add): codes are whole numbers, and the plain formula gives
 //     the same ones. (x - c) / s is a product with 1 / s, and a quotient only near the
 //     middle of two codes, where the two could round apart.
-//   * Reading back, a lane turns 4 bytes of codes into 16 bytes.
+//   * Reading back, a lane turns 8 bytes of codes into 32 bytes, of K and of V.
 #include "paged_int4.cuh"
 #include "paged_rope.cuh"
 
 namespace zs {
 namespace {
 
-constexpr int kInt4Batch = 2;       // passes whose loads are in flight together
+constexpr int kInt4QBatch = 4, kInt4Batch = 2;       // passes (of q, of k and v) whose loads are in flight together
 
 struct RopeInt4Args : RopeArgs {
     Int4View kp, vp;
@@ -47,44 +47,54 @@ __global__ void __launch_bounds__(kRopeThreads) rope_write_int4_kernel(const Rop
     if ((slot < -1 || slot >= cap) && lane == 0) set_err(a.err, kErrPagedIndex);     // -1: padding
     const long long blk = slot >> a.kp.page_shift, row = slot & ((1 << a.kp.page_shift) - 1);
     float* mine = s_rows[threadIdx.x >> 5] + sub * (a.D / 16 * 20);
-    const int rows = a.Hq + 2 * a.Hkv;                       // heads of q, then k, then v
-    const int passes = (rows + heads_per - 1) / heads_per;
-    for (int i0 = part; i0 < passes; i0 += kInt4Batch * a.parts) {
-        uint4 x[kInt4Batch], y[kInt4Batch];
+    // ---- q
+    const int q_passes = (a.Hq + heads_per - 1) / heads_per, rows = 2 * a.Hkv;           // heads of k, then v
+    int i0 = part;
+    for (; i0 < q_passes; i0 += kInt4QBatch * a.parts) {
+        uint4 x[kInt4QBatch], y[kInt4QBatch];
 #pragma unroll
-        for (int u = 0; u < kInt4Batch; ++u) {
+        for (int u = 0; u < kInt4QBatch; ++u) {
             const int h = (i0 + u * a.parts) * heads_per + sub;
-            const uint16_t* src = nullptr;
-            int c0 = me.c0, c1 = me.c1;
-            if (h < a.Hq) {
-                src = a.q + n * a.q_tok + h * a.q_head;
-            } else if (h < rows && live) {
-                if (h < a.Hq + a.Hkv) {
-                    src = a.k + n * a.k_tok + (h - a.Hq) * a.k_head;
-                } else {
-                    src = a.v + n * a.v_tok + (h - a.Hq - a.Hkv) * a.v_head;
-                    c0 = c * 16;
-                    c1 = c0 + 8;
-                }
-            }
-            x[u] = y[u] = make_uint4(0u, 0u, 0u, 0u);
-            if (src) {               // plain loads: q may be turned in place
-                x[u] = __ldcs(reinterpret_cast<const uint4*>(src + c0));
-                y[u] = __ldcs(reinterpret_cast<const uint4*>(src + c1));
+            if (h < a.Hq) {          // plain loads: q may be turned in place
+                const uint16_t* src = a.q + n * a.q_tok + h * a.q_head;
+                x[u] = __ldcs(reinterpret_cast<const uint4*>(src + me.c0));
+                y[u] = __ldcs(reinterpret_cast<const uint4*>(src + me.c1));
             }
         }
 #pragma unroll
-        for (int u = 0; u < kInt4Batch; ++u) {
-            const int pass = i0 + u * a.parts, h = pass * heads_per + sub;
+        for (int u = 0; u < kInt4QBatch; ++u) {
+            const int h = (i0 + u * a.parts) * heads_per + sub;
             if (h < a.Hq) {
                 if (me.turns) me.turn<T>(x[u], y[u], a.interleaved);
                 uint16_t* dst = a.q_out + n * a.qo_tok + h * a.qo_head;
                 __stcs(reinterpret_cast<uint4*>(dst + me.c0), x[u]);
                 __stcs(reinterpret_cast<uint4*>(dst + me.c1), y[u]);
             }
-            if (!live || pass >= passes || (pass + 1) * heads_per <= a.Hq) continue;      // the same for the warp
+        }
+    }
+    if (!live) return;
+    // ---- k and v, passes q_passes on of the token's
+    const int passes = (rows + heads_per - 1) / heads_per;
+    i0 = q_passes <= part ? part - q_passes : (part + a.parts - q_passes % a.parts) % a.parts;
+    for (; i0 < passes; i0 += kInt4Batch * a.parts) {
+        uint4 x[kInt4Batch], y[kInt4Batch];
+#pragma unroll
+        for (int u = 0; u < kInt4Batch; ++u) {
+            const int h = (i0 + u * a.parts) * heads_per + sub;
+            x[u] = y[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (h < rows) {
+                const bool key = h < a.Hkv;
+                const uint16_t* src = key ? a.k + n * a.k_tok + h * a.k_head : a.v + n * a.v_tok + (h - a.Hkv) * a.v_head;
+                x[u] = __ldcs(reinterpret_cast<const uint4*>(src + (key ? me.c0 : c * 16)));
+                y[u] = __ldcs(reinterpret_cast<const uint4*>(src + (key ? me.c1 : c * 16 + 8)));
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kInt4Batch; ++u) {
+            const int pass = i0 + u * a.parts, h = pass * heads_per + sub;
+            if (pass >= passes) continue;      // the same for the warp
             // ---- keys and values: 16 neighbouring channels a lane, in fp32
-            const bool key = h < a.Hq + a.Hkv;
+            const bool key = h < a.Hkv;
             float f[16];
             {
                 const uint32_t w[8] = {x[u].x, x[u].y, x[u].z, x[u].w, y[u].x, y[u].y, y[u].z, y[u].w};
@@ -160,11 +170,12 @@ __global__ void __launch_bounds__(kRopeThreads) rope_write_int4_kernel(const Rop
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
                 const float d = __fsub_rn(f[j], centre);
-                float t = __fmul_rn(d, by), r = rintf(t);
-                if (fabsf(t - r) > 0.4999f) r = rintf(__fdiv_rn(d, s));
-                r = s > 0.f ? fminf(fmaxf(r, -8.f), 7.f) : 0.f;
-                code[j / 8] |= (uint32_t)((int)r + 8) << (j % 8 * 4);
+                const float t = fminf(fmaxf(__fmul_rn(d, by), -8.f), 7.f);      // the clamped ones are far from a middle
+                float r = rintf(t);
+                if (fabsf(t - r) > 0.4999f) r = fminf(fmaxf(rintf(__fdiv_rn(d, s)), -8.f), 7.f);
+                code[j / 8] |= (uint32_t)(__float_as_int(r + 12582920.f) & 15) << (j % 8 * 4);     // 1.5 2^23 + 8
             }
+            if (!(s > 0.f)) code[0] = code[1] = 0x88888888u;
             // ---- the head's groups to its first lane
             const uint32_t sb = __bfloat16_as_ushort(__float2bfloat16_rn(s));
             const uint32_t cb = isnan(centre) ? 0x7FC0u : __bfloat16_as_ushort(__float2bfloat16_rn(centre));
@@ -175,9 +186,9 @@ __global__ void __launch_bounds__(kRopeThreads) rope_write_int4_kernel(const Rop
                 ss[g] = __shfl_sync(~0u, sb, from);
                 cc[g] = __shfl_sync(~0u, cb, from);
             }
-            if (h < a.Hq || h >= rows) continue;
+            if (h >= rows) continue;
             const Int4View& to = key ? a.kp : a.vp;
-            const long long head = h - a.Hq - (key ? 0 : a.Hkv);
+            const long long head = h - (key ? 0 : a.Hkv);
             *reinterpret_cast<uint2*>(to.codes + blk * to.c_block + row * to.c_token + head * to.c_head + c * 8) =
                 make_uint2(code[0], code[1]);
             if (c == 0) {
@@ -194,66 +205,71 @@ __global__ void __launch_bounds__(kRopeThreads) rope_write_int4_kernel(const Rop
     }
 }
 
-// ---- reading back
+// ---- reading back: a lane has 16 channels of a row of K and of V, 8 bytes of codes each,
+// and writes 32 bytes at once
 constexpr int kReadThreads = 256;
-constexpr int kReadBatch = 4;       // items of a thread, their loads in flight together
 
 struct ReadArgs {
     Int4View kp, vp;
     const long long* slots;
     uint16_t* k_out;
     uint16_t* v_out;
-    long long items;              // of 8 channels, of K or of V
-    int piece_shift;              // log2(D / 8)
-    int group_shift;              // log2(group / 8)
+    long long items;              // of 16 channels of K and of V
+    int per_token;                // items a token
+    int piece_shift;              // log2(D / 16)
+    int group_shift;              // log2(group / 16)
     unsigned* err;
 };
 
+struct Read16 {
+    uint2 w;
+    uint32_t s, c;                // scale and centre
+};
+
+__device__ __forceinline__ Read16 read16(const Int4View& p, long long blk, long long row, int h, int piece, int g) {
+    Read16 r;
+    r.w = __ldcs(reinterpret_cast<const uint2*>(p.codes + blk * p.c_block + row * p.c_token + h * p.c_head + piece * 8));
+    const uint16_t* par = p.params + blk * p.p_block + row * p.p_token + h * p.p_head + g;
+    r.s = __ldg(par);
+    r.c = __ldg(par + p.groups);
+    return r;
+}
+
 template <typename T>
-__device__ __forceinline__ uint4 values_of(uint32_t w, float s, float c) {
-    uint32_t r[4];
+__device__ __forceinline__ void write16(uint16_t* to, const Read16& x, bool live) {
+    const float s = bf16_bits_to_float(x.s), c = bf16_bits_to_float(x.c);
+    uint32_t r[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float lo = (float)((int)(w >> (8 * j) & 15u) - 8), hi = (float)((int)(w >> (8 * j + 4) & 15u) - 8);
-        r[j] = pack2<T>(__fadd_rn(c, s * lo), __fadd_rn(c, s * hi));          // s times a code is exact
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t w = j < 4 ? x.w.x : x.w.y;
+        // codes as floats: 2^23 + u, less 2^23 + 8
+        const float lo = __uint_as_float((w >> (j % 4 * 8) & 15u) | 0x4B000000u) - 8388616.f;
+        const float hi = __uint_as_float((w >> (j % 4 * 8 + 4) & 15u) | 0x4B000000u) - 8388616.f;
+        r[j] = live ? pack2<T>(__fmaf_rn(s, lo, c), __fmaf_rn(s, hi, c)) : 0u;       // s times a code is exact
     }
-    return make_uint4(r[0], r[1], r[2], r[3]);
+    asm volatile("st.global.cs.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(to), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+    asm volatile("st.global.cs.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(to + 8), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kReadThreads) read_int4_kernel(const ReadArgs a) {
-    const bool values = blockIdx.y;           // of K, or of V
-    const Int4View& p = values ? a.vp : a.kp;
-    uint16_t* out = values ? a.v_out : a.k_out;
-    const long long cap = (long long)p.num_blocks << p.page_shift;
-    const long long first = (long long)blockIdx.x * (kReadThreads * kReadBatch) + threadIdx.x;
-    uint32_t w[kReadBatch], s[kReadBatch], c[kReadBatch];
-#pragma unroll
-    for (int i = 0; i < kReadBatch; ++i) {
-        const long long item = first + i * kReadThreads;
-        w[i] = s[i] = c[i] = 0u;
-        if (item >= a.items) continue;
-        const long long head_row = item >> a.piece_shift;      // token and head
-        const int piece = (int)(item & ((1 << a.piece_shift) - 1));
-        const long long n = div_nonneg(head_row, p.heads), h = head_row - n * p.heads;
-        const long long slot = a.slots[n];
-        if (slot < 0 || slot >= cap) {
-            if (slot != -1) set_err(a.err, kErrPagedIndex);
-            continue;
-        }
-        const long long blk = slot >> p.page_shift, row = slot & ((1 << p.page_shift) - 1);
-        w[i] = __ldg(reinterpret_cast<const uint32_t*>(p.codes + blk * p.c_block + row * p.c_token + h * p.c_head + piece * 4));
-        const uint16_t* par = p.params + blk * p.p_block + row * p.p_token + h * p.p_head + (piece >> a.group_shift);
-        s[i] = __ldg(par);
-        c[i] = __ldg(par + p.groups);
+    const long long item = (long long)blockIdx.x * kReadThreads + threadIdx.x;
+    if (item >= a.items) return;
+    const long long n = div_nonneg(item, a.per_token);
+    const int in_token = (int)(item - n * a.per_token);
+    const int h = in_token >> a.piece_shift, piece = in_token & ((1 << a.piece_shift) - 1);
+    const long long slot = a.slots[n], cap = (long long)a.kp.num_blocks << a.kp.page_shift;
+    const bool live = slot >= 0 && slot < cap;
+    Read16 k{}, v{};
+    if (live) {
+        const long long blk = slot >> a.kp.page_shift, row = slot & ((1 << a.kp.page_shift) - 1);
+        k = read16(a.kp, blk, row, h, piece, piece >> a.group_shift);
+        v = read16(a.vp, blk, row, h, piece, piece >> a.group_shift);
+    } else if (slot != -1) {
+        set_err(a.err, kErrPagedIndex);
     }
-#pragma unroll
-    for (int i = 0; i < kReadBatch; ++i) {
-        const long long item = first + i * kReadThreads;
-        if (item < a.items)
-            __stcs(reinterpret_cast<uint4*>(out) + item,
-                   values_of<T>(w[i], bf16_bits_to_float(s[i]), bf16_bits_to_float(c[i])));
-    }
+    write16<T>(a.k_out + item * 16, k, live);
+    write16<T>(a.v_out + item * 16, v, live);
 }
 
 }  // namespace
@@ -291,14 +307,14 @@ extern "C" int zs_read_int4(const ZsReadInt4* p) {
     a.slots = reinterpret_cast<const long long*>(p->slots);
     a.k_out = p->k_out;
     a.v_out = p->v_out;
-    a.piece_shift = a.kp.dim == 64 ? 3 : 4;
-    a.group_shift = p->k_pool.group == 32 ? 2 : 3;
-    a.items = ((long long)p->N * a.kp.heads) << a.piece_shift;
+    a.piece_shift = a.kp.dim == 64 ? 2 : 3;
+    a.group_shift = p->k_pool.group == 32 ? 1 : 2;
+    a.per_token = a.kp.heads << a.piece_shift;
+    a.items = (long long)p->N * a.per_token;
     a.err = p->err;
-    const long long ctas = (a.items + kReadThreads * kReadBatch - 1) / (kReadThreads * kReadBatch);
-    if (ctas > INT32_MAX) return cudaErrorInvalidValue;
-    const dim3 grid((unsigned)ctas, 2);
-    if (p->dtype == ZS_BF16) read_int4_kernel<__nv_bfloat16><<<grid, kReadThreads, 0, (cudaStream_t)p->stream>>>(a);
-    else read_int4_kernel<__half><<<grid, kReadThreads, 0, (cudaStream_t)p->stream>>>(a);
+    const long long grid = (a.items + kReadThreads - 1) / kReadThreads;
+    if (a.kp.heads > INT32_MAX >> 3 || grid > INT32_MAX) return cudaErrorInvalidValue;
+    if (p->dtype == ZS_BF16) read_int4_kernel<__nv_bfloat16><<<(unsigned)grid, kReadThreads, 0, (cudaStream_t)p->stream>>>(a);
+    else read_int4_kernel<__half><<<(unsigned)grid, kReadThreads, 0, (cudaStream_t)p->stream>>>(a);
     return cudaGetLastError();
 }
