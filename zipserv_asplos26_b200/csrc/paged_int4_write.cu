@@ -29,6 +29,17 @@ struct RopeInt4Args : RopeArgs {
 constexpr int kHeadWords = 128 / 16 * 20;
 __device__ __forceinline__ float* place16(float* head, int channel) { return head + channel / 16 * 20 + channel % 16; }
 
+__device__ __forceinline__ float min_nan(float a, float b) {         // NaN where one is
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 template <typename T, int kLanes>      // kLanes: lanes a group (16 channels each)
 __global__ void __launch_bounds__(kRopeThreads) rope_write_int4_kernel(const RopeInt4Args a) {
     __shared__ __align__(16) float s_rows[kRopeThreads / 32][4 * kHeadWords];
@@ -120,7 +131,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_write_int4_kernel(const Rop
                     for (int j = 0; j < 8; ++j) turn(f[j], f[8 + j], j);
                 }
             }
-            if (!a.interleaved) {              // the same for the warp
+            if (!a.interleaved && pass * heads_per < a.Hkv) {      // the same for the warp
                 const int c0 = key ? me.c0 : c * 16, c1 = key ? me.c1 : c * 16 + 8;
                 __syncwarp();
 #pragma unroll
@@ -140,18 +151,16 @@ __global__ void __launch_bounds__(kRopeThreads) rope_write_int4_kernel(const Rop
                 }
             }
             // ---- the group's scale and centre
-            float low = f[0], high = f[0], odd = 0.f;
+            float low = f[0], high = f[0];             // NaN once a value is
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                low = fminf(low, f[j]);
-                high = fmaxf(high, f[j]);
-                odd += f[j] * 0.f;             // NaN once a value is not finite
+            for (int j = 1; j < 16; ++j) {
+                low = min_nan(low, f[j]);
+                high = max_nan(high, f[j]);
             }
 #pragma unroll
             for (int o = 1; o < kLanes; o <<= 1) {
-                low = fminf(low, __shfl_xor_sync(~0u, low, o));
-                high = fmaxf(high, __shfl_xor_sync(~0u, high, o));
-                odd += __shfl_xor_sync(~0u, odd, o);
+                low = min_nan(low, __shfl_xor_sync(~0u, low, o));
+                high = max_nan(high, __shfl_xor_sync(~0u, high, o));
             }
             const float range = __fsub_rn(high, low);
             float s = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(range, 15.f)));
@@ -160,20 +169,22 @@ __global__ void __launch_bounds__(kRopeThreads) rope_write_int4_kernel(const Rop
                 s = 0.f;
                 centre = __bfloat162float(__float2bfloat16_rn(low));
             }
-            if (!(odd == 0.f && range < INFINITY)) {
+            if (!(range < INFINITY)) {
                 s = 0.f;
                 centre = NAN;
             }
-            // ---- codes
+            // ---- codes: rounded by adding 1.5 2^23 (and 8), whose bits add up to as many times a constant
             const float by = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
-            uint32_t code[2] = {0u, 0u};
+            constexpr float kWhole = 12582920.f, kLeast = 12582912.f, kMost = 12582927.f;
+            uint32_t code[2] = {0u - 0x4B400000u * 0x11111111u, 0u - 0x4B400000u * 0x11111111u};
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
                 const float d = __fsub_rn(f[j], centre);
-                const float t = fminf(fmaxf(__fmul_rn(d, by), -8.f), 7.f);      // the clamped ones are far from a middle
-                float r = rintf(t);
-                if (fabsf(t - r) > 0.4999f) r = fminf(fmaxf(rintf(__fdiv_rn(d, s)), -8.f), 7.f);
-                code[j / 8] |= (uint32_t)(__float_as_int(r + 12582920.f) & 15) << (j % 8 * 4);     // 1.5 2^23 + 8
+                float m = fmaf(d, by, kWhole);
+                // off by 2^-20 at most before it was rounded: near the middle of two codes the quotient tells
+                if (fabsf(fmaf(d, by, kWhole - m)) > 0.499998f) m = rintf(__fdiv_rn(d, s)) + kWhole;
+                m = fminf(fmaxf(m, kLeast), kMost);
+                code[j / 8] += (uint32_t)__float_as_int(m) << (j % 8 * 4);
             }
             if (!(s > 0.f)) code[0] = code[1] = 0x88888888u;
             // ---- the head's groups to its first lane
