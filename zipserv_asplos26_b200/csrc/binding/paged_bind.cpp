@@ -631,24 +631,23 @@ PyObject* sparse_attention(PyObject* const* a) {
 // ------------------------------------------------------------ 4-bit cache
 // codes uint8 [num_blocks, page_size, heads, dim / 2] and params bf16 [num_blocks,
 // page_size, heads, 2, dim / group] of one pool.
-ZsInt4Pool int4_pool(PyObject* codes_o, PyObject* params_o, const char* name) {
-    const std::string n(name);
-    const at::Tensor &c = cuda_tensor(codes_o, (n + ".codes").c_str()), &t = cuda_tensor(params_o, (n + ".params").c_str());
+ZsInt4Pool int4_pool(PyObject* pages, const char* name, const char* codes, const char* params) {
+    const at::Tensor &c = cuda_tensor(PyTuple_GET_ITEM(pages, 0), codes), &t = cuda_tensor(PyTuple_GET_ITEM(pages, 1), params);
     if (c.scalar_type() != at::kByte || c.dim() != 4 || t.scalar_type() != at::kBFloat16 || t.dim() != 5 ||
         t.get_device() != c.get_device())
-        refuse(n + " must be uint8 codes [num_blocks, page_size, heads, dim / 2] and bfloat16 params [num_blocks, "
+        refuse(std::string(name) + " must be uint8 codes [num_blocks, page_size, heads, dim / 2] and bfloat16 params [num_blocks, "
                    "page_size, heads, 2, dim / group] on one CUDA device");
     check_page_size(c.size(1));
     const int64_t dim = c.size(3) * 2, groups = t.size(4);
     need(dim == 64 || dim == 128, "head dim must be 64 or 128");
     need(groups > 0 && (groups * 32 == dim || groups * 64 == dim), "params must have a scale and a centre for every 32 or 64 channels");
-    if (c.numel() == 0 || c.size(0) > INT32_MAX || c.size(2) > INT32_MAX) refuse(n + " must not be empty");
+    if (c.numel() == 0 || c.size(0) > INT32_MAX || c.size(2) > INT32_MAX) refuse(std::string(name) + " must not be empty");
     if (t.size(0) != c.size(0) || t.size(1) != c.size(1) || t.size(2) != c.size(2) || t.size(3) != 2)
-        refuse(n + ": codes and params must agree in blocks, page size and heads");
+        refuse(std::string(name) + ": codes and params must agree in blocks, page size and heads");
     if (c.stride(3) != 1 || (c.stride(0) | c.stride(1) | c.stride(2)) % 16 || !aligned16(c) ||
         (t.stride(4) != 1 && groups > 1) || t.stride(3) != groups ||
         (t.stride(0) | t.stride(1) | t.stride(2)) % (2 * groups) || !aligned16(t))
-        refuse(n + ": rows must be contiguous and aligned (codes to 16 bytes, params to a row's)");
+        refuse(std::string(name) + ": rows must be contiguous and aligned (codes to 16 bytes, params to a row's)");
     return {ptr<uint8_t>(c), ptr<uint16_t>(t), c.stride(0), c.stride(1), c.stride(2), t.stride(0), t.stride(1),
             t.stride(2), static_cast<int>(c.size(0)), static_cast<int>(c.size(1)), static_cast<int>(c.size(2)),
             static_cast<int>(dim), static_cast<int>(dim / groups), 0};
@@ -663,8 +662,8 @@ struct Int4Pools {
 Int4Pools int4_pools(PyObject* ko, PyObject* vo) {
     need(PyTuple_Check(ko) && PyTuple_GET_SIZE(ko) == 2 && PyTuple_Check(vo) && PyTuple_GET_SIZE(vo) == 2,
          "k_pages and v_pages must be Int4Pages");
-    Int4Pools p{int4_pool(PyTuple_GET_ITEM(ko, 0), PyTuple_GET_ITEM(ko, 1), "k_pages"),
-                int4_pool(PyTuple_GET_ITEM(vo, 0), PyTuple_GET_ITEM(vo, 1), "v_pages"),
+    Int4Pools p{int4_pool(ko, "k_pages", "k_pages.codes", "k_pages.params"),
+                int4_pool(vo, "v_pages", "v_pages.codes", "v_pages.params"),
                 static_cast<int>(THPVariable_Unpack(PyTuple_GET_ITEM(ko, 0)).get_device())};
     need(p.k.num_blocks == p.v.num_blocks && p.k.page_size == p.v.page_size && p.k.num_heads == p.v.num_heads &&
              p.k.head_dim == p.v.head_dim && p.k.group == p.v.group &&

@@ -18,7 +18,7 @@
 namespace zs {
 namespace {
 
-constexpr int kInt4QBatch = 4, kInt4Batch = 2;       // passes (of q, of k and v) whose loads are in flight together
+constexpr int kInt4QBatch = 4, kInt4Batch = 1;       // passes (of q, of k and v) whose loads are in flight together
 
 struct RopeInt4Args : RopeArgs {
     Int4View kp, vp;
@@ -41,7 +41,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 template <typename T, int kLanes>      // kLanes: lanes a group (16 channels each)
-__global__ void __launch_bounds__(kRopeThreads) rope_write_int4_kernel(const RopeInt4Args a) {
+__global__ void __launch_bounds__(kRopeThreads, 14) rope_write_int4_kernel(const RopeInt4Args a) {
     __shared__ __align__(16) float s_rows[kRopeThreads / 32][4 * kHeadWords];
     const int lane = threadIdx.x & 31;
     const long long warp = (long long)blockIdx.x * (kRopeThreads / 32) + (threadIdx.x >> 5);

@@ -16,13 +16,15 @@
 // a table, the rest by a polynomial of degree three.
 //
 // Borders are found by the logits' order, its first 12 bits first: a histogram in shared
-// memory of how many, or how much weight, the tokens hold. A second reading gathers the tokens from there on; up to 2048 of them are
-// all that remains to be looked at, by the next 12 and 8 bits. Where there are more, further
-// readings find the other bits, and sums of blocks of 1024 tokens. In the end the block in
-// which the running sum passes its target is read once more. All readings but the first come
-// from L2. A row goes to a cluster of up to 8 CTAs where there are few, its histograms joined
-// through distributed shared memory. Bound by instructions: some 33 for a weight, 10 of them
-// in 64 bits.
+// memory of how many, or how much weight, the tokens hold. The next reading, where there is
+// one border, sums the weights above its 4096th part of the order, for each block of 1024
+// tokens, and gathers the tokens in it; their next 12 and 8 bits find the border. With two
+// borders it gathers all tokens from the first one's part on; up to 4096 of them are all that
+// remains to be looked at. Where more are gathered, further readings find the other bits, and
+// the sums. In the end the block in which the running sum passes its target is read once
+// more. All readings but the first come from L2. A row goes to a cluster of up to 8 CTAs
+// where there are few, its histograms joined through distributed shared memory. Bound by
+// instructions: some 30 for a weight, 10 of them in 64 bits.
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
@@ -41,7 +43,7 @@ constexpr int kSampBlock = 1024;            // tokens of a sum
 constexpr int kSampMaxBlocks = 1024;        // so 2^20 tokens at most
 constexpr int kBins = 4096;
 constexpr int kPowers = 2048;
-constexpr int kList = 2048;                 // gathered tokens, at most
+constexpr int kList = 4096;                 // gathered tokens of a CTA, at most
 constexpr unsigned kErrSampleNothing = 8u;  // a row had nothing to choose from
 constexpr unsigned kOrderOfMost = 0xFF7FFFFFu, kOrderOfMinusInf = 0x007FFFFFu;     // of the largest finite number
 using u64 = unsigned long long;
@@ -285,7 +287,7 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
         weigh.rate = 0.0;
     }
     weigh.steps = a.steps;
-    weigh.least = 0.0;
+    weigh.least = min_p > 0.0 ? fmin(min_p, 1.0) * __hiloint2double((1023 + a.steps) << 20, 0) : 0.0;
     constexpr int kLevels = std::is_same<T, float>::value ? 3 : 2;            // 16-bit types: 24 bits tell all apart
     constexpr int kDigit[3] = {20, 8, 0}, kWidth[3] = {12, 12, 8};
     const auto whole = [&](auto&& f) { each(e0, e1, tid, kSampThreads, [&](float v, int) { f(order_of(v), v); }); };
@@ -401,10 +403,9 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
     const std::true_type yes{};
     const std::false_type no{};
     const bool by_count = top_k > 0 && top_k < a.V, by_weight = top_p < 1.0;
-    const double least = min_p > 0.0 ? fmin(min_p, 1.0) * __hiloint2double((1023 + a.steps) << 20, 0) : 0.0;
     unsigned edge = none;          // tokens above it are kept, and of those on it the first `ties`
     u64 ties = 0, on_edge = 0;     // its weight
-    bool from_list = false;
+    bool from_list = false, summed = false;        // the row is in the first CTA's list; the blocks are summed
     auto above_none = [&](u64 want) {          // top_k's border, where weights begin
         ties = edge > none ? want : 0;
         edge = max(edge, none);
@@ -415,59 +416,100 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
         u64 want = (u64)top_k;
         if (by_count) digit(yes, yes, 0, whole, 0u, 0ull, found, want);
         else digit(no, yes, 0, whole, none, 0ull, found, want);
-        const unsigned low = found << kDigit[0];
-        each(e0, e1, tid, kSampThreads, [&](float v, int i) {
-            const unsigned k = order_of(v);
-            if (k < low || *static_cast<volatile int*>(&sh.listed) > kList) return;      // enough is known
+        const unsigned first_part = found;
+        auto gather = [&](unsigned k, int i) {
             const int at = atomicAdd(&sh.listed, 1);
             if (at < kList) {
                 sh.list_key[at] = k;
                 sh.list_at[at] = i;
             }
-        });
-        all_sync();
-        int listed = 0;
-        for (unsigned r = 0; r < size; ++r) listed += min(size > 1 ? (int)ld_peer32(&sh.listed, r) : sh.listed, kList + 1);
-        from_list = listed <= kList;
-        if (from_list && rank == 0) {
-            // the others' tokens behind the first CTA's
-            int n = sh.listed;
-            for (unsigned r = 1; r < size; ++r) {
-                const int more = (int)ld_peer32(&sh.listed, r);
-                for (int i = tid; i < more; i += kSampThreads) {
-                    sh.list_key[n + i] = ld_peer32(&sh.list_key[i], r);
-                    sh.list_at[n + i] = (int)ld_peer32(&sh.list_at[i], r);
+        };
+        auto overflown = [&] { return *static_cast<volatile int*>(&sh.listed) > kList; };
+        if (by_count != by_weight) {
+            // ---- one border: sums of blocks above its part of the order, a warp a block
+            for (int b = warp; b < a.blocks; b += kSampWarps) {
+                const int from = e0 + b * kSampBlock;
+                u64 m = 0;
+                if (from < e1 && !overflown())
+                    each(from, min(from + kSampBlock, e1), lane, 32, [&](float v, int i) {
+                        const unsigned k = order_of(v), part = k >> kDigit[0];
+                        if (part > first_part && k > none) m += weigh.of_kept(v);
+                        if (part == first_part) gather(k, i);
+                    });
+#pragma unroll
+                for (int o = 16; o; o >>= 1) m += __shfl_xor_sync(~0u, m, o);
+                if (lane == 0) {
+                    sh.mass[b] = m;
+                    sh.ties[b] = 0;
                 }
-                n += more;
             }
-            __syncthreads();
-            if (tid == 0) sh.merged = n;
-            for (int b = tid; b < (int)size * a.blocks; b += kSampThreads) {
-                sh.mass[b] = 0;
-                sh.ties[b] = 0;
+            all_sync();
+            bool fits = true;
+            for (unsigned r = 0; r < size; ++r) fits &= (size > 1 ? (int)ld_peer32(&sh.listed, r) : sh.listed) <= kList;
+            if (fits) {
+                const auto mine = [&](auto&& f) {
+                    for (int i = tid; i < sh.listed; i += kSampThreads) f(sh.list_key[i], value_of(sh.list_key[i]));
+                };
+                if (by_count) {
+                    edge = border(yes, yes, 1, mine, 0u, 0ull, found, want);
+                    above_none(want);
+                } else {
+                    edge = border(no, yes, 1, mine, none, 0ull, found, want);
+                    const u64 w = weigh.of(value_of(edge));
+                    ties = (want + w - 1) / w;
+                }
+                on_edge = weigh.of_kept(value_of(edge));
+                for (int i = tid; i < sh.listed; i += kSampThreads) {
+                    const unsigned k = sh.list_key[i];
+                    const int b = (sh.list_at[i] - e0) / kSampBlock;
+                    if (k > edge) atomicAdd(&sh.mass[b], weigh.of_kept(value_of(k)));
+                    else if (k == edge) atomicAdd(&sh.ties[b], 1u);
+                }
+                summed = true;
             }
-            __syncthreads();
-            if (by_count) {
+        } else {
+            each(e0, e1, tid, kSampThreads, [&](float v, int i) {
+                const unsigned k = order_of(v);
+                if (k >> kDigit[0] >= first_part && !overflown()) gather(k, i);
+            });
+            all_sync();
+            int listed = 0;
+            for (unsigned r = 0; r < size; ++r) listed += min(size > 1 ? (int)ld_peer32(&sh.listed, r) : sh.listed, kList + 1);
+            from_list = listed <= kList;
+            if (from_list && rank == 0) {
+                // the others' tokens behind the first CTA's
+                int n = sh.listed;
+                for (unsigned r = 1; r < size; ++r) {
+                    const int more = (int)ld_peer32(&sh.listed, r);
+                    for (int i = tid; i < more; i += kSampThreads) {
+                        sh.list_key[n + i] = ld_peer32(&sh.list_key[i], r);
+                        sh.list_at[n + i] = (int)ld_peer32(&sh.list_at[i], r);
+                    }
+                    n += more;
+                }
+                __syncthreads();
+                if (tid == 0) sh.merged = n;
+                for (int b = tid; b < (int)size * a.blocks; b += kSampThreads) {
+                    sh.mass[b] = 0;
+                    sh.ties[b] = 0;
+                }
+                __syncthreads();
                 edge = border(yes, no, 1, list, 0u, 0ull, found, want);
                 above_none(want);
-            }
-            if (by_weight) {
-                if (by_count) edge = border(no, no, 0, list, edge, ties, 0u, want);
-                else edge = border(no, no, 1, list, none, 0ull, found, want);
+                edge = border(no, no, 0, list, edge, ties, 0u, want);
                 const u64 w = weigh.of(value_of(edge));
                 ties = (want + w - 1) / w;
+                on_edge = weigh.of_kept(value_of(edge));
+                for (int i = tid; i < sh.merged; i += kSampThreads) {
+                    const unsigned k = sh.list_key[i];
+                    const int b = sh.list_at[i] / kSampBlock;
+                    if (k > edge) atomicAdd(&sh.mass[b], weigh.of_kept(value_of(k)));
+                    else if (k == edge) atomicAdd(&sh.ties[b], 1u);
+                }
+                __syncthreads();
             }
-            weigh.least = least;
-            on_edge = weigh.of_kept(value_of(edge));
-            for (int i = tid; i < sh.merged; i += kSampThreads) {
-                const unsigned k = sh.list_key[i];
-                const int b = sh.list_at[i] / kSampBlock;
-                if (k > edge) atomicAdd(&sh.mass[b], weigh.of_kept(value_of(k)));
-                else if (k == edge) atomicAdd(&sh.ties[b], 1u);
-            }
-            __syncthreads();
         }
-        if (!from_list) {
+        if (!from_list && !summed) {
             if (by_count) {
                 edge = border(yes, yes, 1, whole, 0u, 0ull, found, want);
                 above_none(want);
@@ -480,13 +522,12 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
             }
         }
     }
-    if (!from_list) {
-        weigh.least = least;
+    if (!from_list && !summed) {
         on_edge = weigh.of_kept(value_of(edge));
     }
 
     // ---- sums of blocks, a warp a block
-    for (int b = warp; b < a.blocks && !from_list; b += kSampWarps) {
+    for (int b = warp; b < a.blocks && !from_list && !summed; b += kSampWarps) {
         const int from = e0 + b * kSampBlock;
         if (from >= e1) {
             if (lane == 0) {
