@@ -76,7 +76,6 @@ struct SampShared {
     unsigned list_key[kList];
     int list_at[kList];
     int listed;                             // tokens that the CTA gathered, more than kList where they did not fit
-    int merged;                             // tokens of the row's list
     u64 part[kSampWarps], part2[kSampWarps];
     float peak;                             // the CTA's largest logit, NaN where it has one
     int first;                              // its first token of the largest logit
@@ -200,31 +199,31 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
         if (size > 1) cluster_sync();
         else __syncthreads();
     };
-    // f(logit, index) for the logits from `from` to `to`, by threads 0 to `threads`: 16 bytes a
-    // load between the first and the last boundary of 16, four loads on their way.
+    // f(logit, index) for the logits from `from` to `to`, by `threads` threads, this one being
+    // `me` of them: four a load between the first and the last boundary of four, two loads on
+    // their way. (The loops are kept short: their bodies are most of the kernel's instructions,
+    // and for a row of 32000 reading those took longer than the row.)
     auto each = [&](int from, int to, int me, int threads, auto&& f) {
-        constexpr int kVec = 16 / sizeof(T), kBatch = 4;
-        const int off = (int)(reinterpret_cast<uintptr_t>(x + from) & 15) / (int)sizeof(T);
+        constexpr int kVec = 4;
+        using Vec = Several<T, kVec>;
+        const int off = (int)(reinterpret_cast<uintptr_t>(x + from) % sizeof(Vec)) / (int)sizeof(T);
         const int head = min(to - from, off ? kVec - off : 0);
-        if (me < head) f(to_float<T>(x[from + me]), from + me);
         const int start = from + head, vecs = (to - start) / kVec, last = start + vecs * kVec;
-        const Several<T, kVec>* p = reinterpret_cast<const Several<T, kVec>*>(x + start);
-        int i = me;
-        for (; i + (kBatch - 1) * threads < vecs; i += kBatch * threads) {
-            Several<T, kVec> v[kBatch];
-#pragma unroll
-            for (int y = 0; y < kBatch; ++y) v[y] = p[i + y * threads];
-#pragma unroll
-            for (int y = 0; y < kBatch; ++y)
-#pragma unroll
-                for (int j = 0; j < kVec; ++j) f(to_float<T>(v[y].x[j]), start + (i + y * threads) * kVec + j);
-        }
-        for (; i < vecs; i += threads) {
-            const Several<T, kVec> v = p[i];
+        const Vec* p = reinterpret_cast<const Vec*>(x + start);
+#pragma unroll 1
+        for (int i = me; i < vecs; i += 2 * threads) {
+            const int two = i + threads < vecs ? threads : 0;          // else the first again, not looked at
+            const Vec v = p[i], w = p[i + two];
 #pragma unroll
             for (int j = 0; j < kVec; ++j) f(to_float<T>(v.x[j]), start + i * kVec + j);
+            if (two) {
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) f(to_float<T>(w.x[j]), start + (i + threads) * kVec + j);
+            }
         }
-        if (me < to - last) f(to_float<T>(x[last + me]), last + me);
+        // before the first boundary and behind the last
+        const int at = me < head ? from + me : last + me - head;
+        if (me < head + to - last) f(to_float<T>(x[at]), at);
     };
 
     // ---- the largest logit, NaN if any is
@@ -290,19 +289,13 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
     weigh.least = min_p > 0.0 ? fmin(min_p, 1.0) * __hiloint2double((1023 + a.steps) << 20, 0) : 0.0;
     constexpr int kLevels = std::is_same<T, float>::value ? 3 : 2;            // 16-bit types: 24 bits tell all apart
     constexpr int kDigit[3] = {20, 8, 0}, kWidth[3] = {12, 12, 8};
-    const auto whole = [&](auto&& f) { each(e0, e1, tid, kSampThreads, [&](float v, int) { f(order_of(v), v); }); };
-    const auto list = [&](auto&& f) {
-        for (int i = tid; i < sh.merged; i += kSampThreads) f(sh.list_key[i], value_of(sh.list_key[i]));
-    };
-
     // One digit of a border in the order, `found` being the digits before it. Count: of the
-    // `want`-th token of `from`; else where weights, of the tokens above `floor` and floor_ties
-    // times the one on it, reach `want` (at the first digit: top_p of their sum). `from` is the
-    // CTA's share of the row (cluster true) or the list, which the first CTA has to itself.
-    auto digit = [&](auto count_c, auto cluster_c, int level, auto&& from, unsigned floor, u64 floor_ties, unsigned& found,
+    // `want`-th token; else where weights, of the tokens above `floor` and floor_ties times the
+    // one on it, reach `want` (at the first digit: top_p of their sum). The tokens are the
+    // CTA's share of the row or, with listed >= 0, so many of its list; `many` CTAs take part.
+    auto digit = [&](auto count_c, unsigned many, int level, int listed, unsigned floor, u64 floor_ties, unsigned& found,
                      u64& want) {
-        constexpr bool kCount = decltype(count_c)::value, kCluster = decltype(cluster_c)::value;
-        const unsigned many = kCluster ? size : 1u;
+        constexpr bool kCount = decltype(count_c)::value;
         const int shift = kDigit[level], width = kWidth[level], bins = 1 << width;
         auto sync = [&] {
             if (many > 1) cluster_sync();
@@ -322,11 +315,18 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
                 if (hi) atomicAdd(&sh.hi[b], hi);
             }
         };
-        from([&](unsigned k, float v) {
+        auto take = [&](unsigned k, float v) {
             if (level && k >> (shift + width) != found) return;
             if constexpr (kCount) put(k, 0);
-            else if (k > floor) put(k, weigh.of(v));
-        });
+            else {
+                const u64 w = weigh.of(v);             // without a branch around it
+                put(k, k > floor ? w : 0ull);
+            }
+        };
+        if (listed < 0) each(e0, e1, tid, kSampThreads, [&](float v, int) { take(order_of(v), v); });
+        else
+#pragma unroll 1
+            for (int i = tid; i < listed; i += kSampThreads) take(sh.list_key[i], value_of(sh.list_key[i]));
         if (!kCount && rank == 0 && tid == 0 && floor_ties && (!level || floor >> (shift + width) == found))
             put(floor, weigh.of(value_of(floor)) * floor_ties);
         sync();
@@ -392,176 +392,135 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
         want = many > 1 ? ld_peer64(&sh.rest, 0) : sh.rest;
         found = found << width | bin;
     };
-    // A border from digit `level` on; `want` in the end: of the tokens on it.
-    auto border = [&](auto count_c, auto cluster_c, int level, auto&& from, unsigned floor, u64 floor_ties, unsigned found,
-                      u64& want) {
-#pragma unroll 1
-        for (; level < kLevels; ++level) digit(count_c, cluster_c, level, from, floor, floor_ties, found, want);
-        if constexpr (kLevels == 2) found = found << 8 | (found >> 23 ? 0u : 0xFFu);
-        return found;
-    };
-    const std::true_type yes{};
-    const std::false_type no{};
     const bool by_count = top_k > 0 && top_k < a.V, by_weight = top_p < 1.0;
     unsigned edge = none;          // tokens above it are kept, and of those on it the first `ties`
-    u64 ties = 0, on_edge = 0;     // its weight
-    bool from_list = false, summed = false;        // the row is in the first CTA's list; the blocks are summed
-    auto above_none = [&](u64 want) {          // top_k's border, where weights begin
-        ties = edge > none ? want : 0;
-        edge = max(edge, none);
-    };
-    if (by_count || by_weight) {
-        // ---- the first digit, and the tokens from it on
-        unsigned found = 0;
-        u64 want = (u64)top_k;
-        if (by_count) digit(yes, yes, 0, whole, 0u, 0ull, found, want);
-        else digit(no, yes, 0, whole, none, 0ull, found, want);
-        const unsigned first_part = found;
-        auto gather = [&](unsigned k, int i) {
-            const int at = atomicAdd(&sh.listed, 1);
-            if (at < kList) {
-                sh.list_key[at] = k;
-                sh.list_at[at] = i;
-            }
-        };
-        auto overflown = [&] { return *static_cast<volatile int*>(&sh.listed) > kList; };
-        if (by_count != by_weight) {
-            // ---- one border: sums of blocks above its part of the order, a warp a block
-            for (int b = warp; b < a.blocks; b += kSampWarps) {
-                const int from = e0 + b * kSampBlock;
-                u64 m = 0;
-                if (from < e1 && !overflown())
-                    each(from, min(from + kSampBlock, e1), lane, 32, [&](float v, int i) {
-                        const unsigned k = order_of(v), part = k >> kDigit[0];
-                        if (part > first_part && k > none) m += weigh.of_kept(v);
-                        if (part == first_part) gather(k, i);
-                    });
-#pragma unroll
-                for (int o = 16; o; o >>= 1) m += __shfl_xor_sync(~0u, m, o);
-                if (lane == 0) {
-                    sh.mass[b] = m;
-                    sh.ties[b] = 0;
-                }
-            }
-            all_sync();
-            bool fits = true;
-            for (unsigned r = 0; r < size; ++r) fits &= (size > 1 ? (int)ld_peer32(&sh.listed, r) : sh.listed) <= kList;
-            if (fits) {
-                const auto mine = [&](auto&& f) {
-                    for (int i = tid; i < sh.listed; i += kSampThreads) f(sh.list_key[i], value_of(sh.list_key[i]));
-                };
-                if (by_count) {
-                    edge = border(yes, yes, 1, mine, 0u, 0ull, found, want);
-                    above_none(want);
-                } else {
-                    edge = border(no, yes, 1, mine, none, 0ull, found, want);
-                    const u64 w = weigh.of(value_of(edge));
-                    ties = (want + w - 1) / w;
-                }
-                on_edge = weigh.of_kept(value_of(edge));
-                for (int i = tid; i < sh.listed; i += kSampThreads) {
-                    const unsigned k = sh.list_key[i];
-                    const int b = (sh.list_at[i] - e0) / kSampBlock;
-                    if (k > edge) atomicAdd(&sh.mass[b], weigh.of_kept(value_of(k)));
-                    else if (k == edge) atomicAdd(&sh.ties[b], 1u);
-                }
-                summed = true;
-            }
-        } else {
-            each(e0, e1, tid, kSampThreads, [&](float v, int i) {
-                const unsigned k = order_of(v);
-                if (k >> kDigit[0] >= first_part && !overflown()) gather(k, i);
-            });
-            all_sync();
-            int listed = 0;
-            for (unsigned r = 0; r < size; ++r) listed += min(size > 1 ? (int)ld_peer32(&sh.listed, r) : sh.listed, kList + 1);
-            from_list = listed <= kList;
-            if (from_list && rank == 0) {
-                // the others' tokens behind the first CTA's
-                int n = sh.listed;
-                for (unsigned r = 1; r < size; ++r) {
-                    const int more = (int)ld_peer32(&sh.listed, r);
-                    for (int i = tid; i < more; i += kSampThreads) {
-                        sh.list_key[n + i] = ld_peer32(&sh.list_key[i], r);
-                        sh.list_at[n + i] = (int)ld_peer32(&sh.list_at[i], r);
-                    }
-                    n += more;
-                }
-                __syncthreads();
-                if (tid == 0) sh.merged = n;
-                for (int b = tid; b < (int)size * a.blocks; b += kSampThreads) {
-                    sh.mass[b] = 0;
-                    sh.ties[b] = 0;
-                }
-                __syncthreads();
-                edge = border(yes, no, 1, list, 0u, 0ull, found, want);
-                above_none(want);
-                edge = border(no, no, 0, list, edge, ties, 0u, want);
-                const u64 w = weigh.of(value_of(edge));
-                ties = (want + w - 1) / w;
-                on_edge = weigh.of_kept(value_of(edge));
-                for (int i = tid; i < sh.merged; i += kSampThreads) {
-                    const unsigned k = sh.list_key[i];
-                    const int b = sh.list_at[i] / kSampBlock;
-                    if (k > edge) atomicAdd(&sh.mass[b], weigh.of_kept(value_of(k)));
-                    else if (k == edge) atomicAdd(&sh.ties[b], 1u);
-                }
-                __syncthreads();
-            }
-        }
-        if (!from_list && !summed) {
-            if (by_count) {
-                edge = border(yes, yes, 1, whole, 0u, 0ull, found, want);
-                above_none(want);
-            }
-            if (by_weight) {
-                if (by_count) edge = border(no, yes, 0, whole, edge, ties, 0u, want);
-                else edge = border(no, yes, 1, whole, none, 0ull, found, want);
-                const u64 w = weigh.of(value_of(edge));
-                ties = (want + w - 1) / w;
-            }
-        }
-    }
-    if (!from_list && !summed) {
-        on_edge = weigh.of_kept(value_of(edge));
-    }
+    u64 ties = 0;
 
-    // ---- sums of blocks, a warp a block
-    for (int b = warp; b < a.blocks && !from_list && !summed; b += kSampWarps) {
-        const int from = e0 + b * kSampBlock;
-        if (from >= e1) {
-            if (lane == 0) {
-                sh.mass[b] = 0;
-                sh.ties[b] = 0;
-            }
-            continue;
-        }
-        u64 m = 0;
-        unsigned t = 0;
-        each(from, min(from + kSampBlock, e1), lane, 32, [&](float v, int) {
-            const unsigned k = order_of(v);
-            if (k > edge) m += weigh.of_kept(v);
-            t += k == edge;
-        });
+    // Sums of blocks, a warp a block: weights above `high`; tokens from `low` to `high` are
+    // gathered, or counted.
+    auto sum_blocks = [&](unsigned low, unsigned high, bool gather) {
+        for (int b = warp; b < a.blocks; b += kSampWarps) {
+            const int from = e0 + b * kSampBlock;
+            u64 m = 0;
+            unsigned t = 0;
+            // where more were gathered than fit, another reading follows
+            if (from < e1 && !(gather && *static_cast<volatile int*>(&sh.listed) > kList))
+                each(from, min(from + kSampBlock, e1), lane, 32, [&](float v, int i) {
+                    const unsigned k = order_of(v);
+                    if (k < low) return;
+                    if (k > high) {
+                        if (k > none) m += weigh.of_kept(v);
+                    } else if (gather) {
+                        const int at = atomicAdd(&sh.listed, 1);
+                        if (at < kList) {
+                            sh.list_key[at] = k;
+                            sh.list_at[at] = i;
+                        }
+                    } else {
+                        ++t;
+                    }
+                });
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            m += __shfl_xor_sync(~0u, m, o);
-            t += __shfl_xor_sync(~0u, t, o);
+            for (int o = 16; o; o >>= 1) {
+                m += __shfl_xor_sync(~0u, m, o);
+                t += __shfl_xor_sync(~0u, t, o);
+            }
+            if (lane == 0) {
+                sh.mass[b] = m;
+                sh.ties[b] = t;
+            }
         }
-        if (lane == 0) {
-            sh.mass[b] = m;
-            sh.ties[b] = t;
+    };
+
+    // ---- the borders. After the first digit of the first one: with one border the sums above
+    // its part of the order and the tokens in it; with two the tokens from its part on, which
+    // the first CTA goes on with alone.
+    bool summed = false, alone = false;
+    int listed = -1;
+    if (by_count || by_weight) {
+        unsigned found = 0, floor = none, many = size;
+        u64 want = (u64)top_k, floor_ties = 0;
+        bool weighing = !by_count, first = true;
+        int level = 0;
+#pragma unroll 1
+        while (true) {
+            if (weighing) digit(std::false_type(), many, level, listed, floor, floor_ties, found, want);
+            else digit(std::true_type(), many, level, listed, floor, floor_ties, found, want);
+            if (first) {
+                first = false;
+                const unsigned low = found << kDigit[0];
+                const bool one = by_count != by_weight;
+                sum_blocks(low, one ? low | ((1u << kDigit[0]) - 1) : 0xFFFFFFFFu, true);
+                all_sync();
+                int total = 0;
+                bool fits = true;
+                for (unsigned r = 0; r < size; ++r) {
+                    const int n = size > 1 ? (int)ld_peer32(&sh.listed, r) : sh.listed;
+                    fits &= n <= kList;
+                    total += min(n, kList + 1);
+                }
+                if (one && fits) {
+                    listed = sh.listed;
+                    summed = true;
+                } else if (!one && total <= kList) {
+                    alone = true;
+                    if (rank != 0) break;
+                    int n = sh.listed;
+#pragma unroll 1
+                    for (unsigned r = 1; r < size; ++r) {              // the others' tokens behind its own
+                        const int more = (int)ld_peer32(&sh.listed, r);
+                        for (int i = tid; i < more; i += kSampThreads) {
+                            sh.list_key[n + i] = ld_peer32(&sh.list_key[i], r);
+                            sh.list_at[n + i] = (int)ld_peer32(&sh.list_at[i], r);
+                        }
+                        n += more;
+                    }
+                    for (int b = tid; b < (int)size * a.blocks; b += kSampThreads) {
+                        sh.mass[b] = 0;
+                        sh.ties[b] = 0;
+                    }
+                    __syncthreads();
+                    listed = n;
+                    many = 1;
+                }
+            }
+            if (++level < kLevels) continue;
+            // 16-bit types: the last 8 bits follow from the sign
+            edge = kLevels == 3 ? found : found << 8 | (found >> 23 ? 0u : 0xFFu);
+            if (weighing) {
+                const u64 w = weigh.of(value_of(edge));
+                ties = (want + w - 1) / w;
+                break;
+            }
+            ties = edge > none ? want : 0;                 // weights begin above `none`
+            edge = max(edge, none);
+            if (!by_weight) break;
+            weighing = true;
+            level = 0;
+            found = 0;
+            floor = edge;
+            floor_ties = ties;
         }
     }
-    if (!from_list) all_sync();
+    const u64 on_edge = weigh.of_kept(value_of(edge));
+    if (!summed && !alone) sum_blocks(edge, edge, false);
+    else
+        for (int i = tid; i < listed; i += kSampThreads) {
+            const unsigned k = sh.list_key[i];
+            const int b = (sh.list_at[i] - (alone ? 0 : e0)) / kSampBlock;
+            if (k > edge) atomicAdd(&sh.mass[b], weigh.of_kept(value_of(k)));
+            else if (k == edge) atomicAdd(&sh.ties[b], 1u);
+        }
+    if (alone) __syncthreads();
+    else all_sync();
     if (rank == 0) {
         // a thread's blocks in order; the block in which the running sum passes u times the sum
         const int all = (int)size * a.blocks, per = (all + kSampThreads - 1) / kSampThreads;
         auto at = [&](int b, u64& m, unsigned& t) {
             const int r = b / a.blocks, i = b % a.blocks;
-            const bool own = size == 1 || from_list;
-            m = own ? sh.mass[from_list ? b : i] : ld_peer64(&sh.mass[i], r);
-            t = own ? sh.ties[from_list ? b : i] : ld_peer32(&sh.ties[i], r);
+            const bool own = size == 1 || alone;
+            m = own ? sh.mass[alone ? b : i] : ld_peer64(&sh.mass[i], r);
+            t = own ? sh.ties[alone ? b : i] : ld_peer32(&sh.ties[i], r);
         };
         u64 sum = 0, tied = 0, total;
         for (int b = tid * per; b < min(all, (tid + 1) * per); ++b) {
