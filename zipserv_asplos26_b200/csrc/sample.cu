@@ -20,7 +20,7 @@
 // one border, sums the weights above its 4096th part of the order, for each block of 1024
 // tokens, and gathers the tokens in it; their next 12 and 8 bits find the border. With two
 // borders it gathers all tokens from the first one's part on; up to 4096 of them are all that
-// remains to be looked at. Where more are gathered, further readings find the other bits, and
+// remains to be looked at, up to 512 each against all others. Where more are gathered, further readings find the other bits, and
 // the sums. In the end the block in which the running sum passes its target is read once
 // more. All readings but the first come from L2. A row goes to a cluster of up to 8 CTAs
 // where there are few, its histograms joined through distributed shared memory. Bound by
@@ -44,6 +44,7 @@ constexpr int kSampMaxBlocks = 1024;        // so 2^20 tokens at most
 constexpr int kBins = 4096;
 constexpr int kPowers = 2048;
 constexpr int kList = 4096;                 // gathered tokens of a CTA, at most
+constexpr int kFew = kSampThreads;          // of a row, so few that each is held against all others
 constexpr unsigned kErrSampleNothing = 8u;  // a row had nothing to choose from
 constexpr unsigned kOrderOfMost = 0xFF7FFFFFu, kOrderOfMinusInf = 0x007FFFFFu;     // of the largest finite number
 using u64 = unsigned long long;
@@ -70,6 +71,7 @@ struct SampShared {
         struct {
             unsigned lo[kBins], hi[kBins];
         };
+        ulonglong2 few[kSampThreads];       // a few gathered tokens: place in the order, weight
     };
     u64 mass[kSampMaxBlocks];               // of the CTA's blocks (the row's, from a list): weights above the border
     unsigned ties[kSampMaxBlocks];          // and tokens on it
@@ -332,16 +334,27 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
         sync();
         if (rank == 0) {
             if (many > 1) {                    // the others' histograms to the first CTA's
-                for (int j = tid; j < bins; j += kSampThreads) {
-                    u64 n = 0;
-                    for (unsigned r = 0; r < many; ++r) {
-                        if constexpr (kCount) n += ld_peer32(&sh.count[j], r);
-                        else n += ((u64)ld_peer32(&sh.hi[j], r) << 32) + ld_peer32(&sh.lo[j], r);
+                constexpr int kEach = kBins / kSampThreads;
+                u64 n[kEach];
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) n[i] = 0;
+#pragma unroll 1
+                for (unsigned r = 0; r < many; ++r)
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) {                  // all on their way together
+                        const int b = i * kSampThreads + tid;
+                        if (b >= bins) continue;
+                        if constexpr (kCount) n[i] += ld_peer32(&sh.count[b], r);
+                        else n[i] += ((u64)ld_peer32(&sh.hi[b], r) << 32) + ld_peer32(&sh.lo[b], r);
                     }
-                    if constexpr (kCount) sh.count[j] = (unsigned)n;
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    const int b = i * kSampThreads + tid;
+                    if (b >= bins) continue;
+                    if constexpr (kCount) sh.count[b] = (unsigned)n[i];
                     else {
-                        sh.lo[j] = (unsigned)n;
-                        sh.hi[j] = (unsigned)(n >> 32);
+                        sh.lo[b] = (unsigned)n[i];
+                        sh.hi[b] = (unsigned)(n[i] >> 32);
                     }
                 }
                 __syncthreads();
@@ -436,6 +449,13 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
     // its part of the order and the tokens in it; with two the tokens from its part on, which
     // the first CTA goes on with alone.
     bool summed = false, alone = false;
+    auto clear_blocks = [&] {
+        for (int b = tid; b < (int)size * a.blocks; b += kSampThreads) {
+            sh.mass[b] = 0;
+            sh.ties[b] = 0;
+        }
+        __syncthreads();
+    };
     int listed = -1;
     if (by_count || by_weight) {
         unsigned found = 0, floor = none, many = size;
@@ -452,12 +472,75 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
                 const bool one = by_count != by_weight;
                 sum_blocks(low, one ? low | ((1u << kDigit[0]) - 1) : 0xFFFFFFFFu, true);
                 all_sync();
-                int total = 0;
+                int before[9];                 // tokens that the CTAs before gathered
                 bool fits = true;
-                for (unsigned r = 0; r < size; ++r) {
-                    const int n = size > 1 ? (int)ld_peer32(&sh.listed, r) : sh.listed;
+                before[0] = 0;
+#pragma unroll
+                for (unsigned r = 0; r < 8; ++r) {
+                    const int n = r >= size ? 0 : size > 1 ? (int)ld_peer32(&sh.listed, r) : sh.listed;
                     fits &= n <= kList;
-                    total += min(n, kList + 1);
+                    before[r + 1] = before[r] + min(n, kList + 1);
+                }
+                const int total = before[8];
+                const bool few = total <= kFew;
+                if (rank == 0 && (few || (!one && total <= kList))) {          // the others' tokens behind its own
+                    for (int i = before[1] + tid; i < total; i += kSampThreads) {
+                        int r = 1, off = before[1];
+#pragma unroll
+                        for (int y = 2; y < 8; ++y)
+                            if (i >= before[y]) {
+                                r = y;
+                                off = before[y];
+                            }
+                        sh.list_key[i] = ld_peer32(&sh.list_key[i - off], r);
+                        sh.list_at[i] = (int)ld_peer32(&sh.list_at[i - off], r);
+                    }
+                    __syncthreads();
+                }
+                if (few) {
+                    // ---- each token against all others: how many come before it, of what weight
+                    if (rank == 0) {
+                        const bool on = tid < total;
+                        const unsigned key = on ? sh.list_key[tid] : 0u;
+                        const int at = on ? sh.list_at[tid] : INT_MAX;
+                        const u64 w = on && key > none ? weigh.of(value_of(key)) : 0ull;
+                        const u64 place = (u64)key << 32 | (unsigned)~at;              // larger comes first
+                        if (on) sh.few[tid] = make_ulonglong2(place, w);
+                        if (tid == 0) {
+                            sh.bin = 0xFFFFFFFFu;
+                            sh.rest = 0;
+                        }
+                        __syncthreads();
+                        u64 w_before = 0;
+                        unsigned n_before = 0;
+#pragma unroll 4
+                        for (int j = 0; j < total; ++j) {
+                            const ulonglong2 f = sh.few[j];
+                            const bool before = f.x > place;
+                            n_before += before;
+                            w_before += before ? f.y : 0ull;
+                        }
+                        // with one border `want` counts from the border's part on, as the list does
+                        bool kept = on && (by_count ? n_before < (one ? want : (u64)top_k) : w_before < want);
+                        if (by_count && by_weight) {
+                            u64 sum;
+                            block_prefix(kept ? w : 0ull, sh.part, sum);
+                            kept = kept && w_before < times(top_p, sum, true);
+                        }
+                        if (kept) atomicMin(&sh.bin, max(key, none));
+                        __syncthreads();
+                        if (kept && key > none && key == sh.bin) atomicAdd(&sh.rest, 1ull);
+                    }
+                    if (one) all_sync();
+                    else if (rank == 0) __syncthreads();
+                    alone = !one;
+                    summed = one;
+                    if (alone && rank != 0) break;
+                    edge = one && size > 1 ? ld_peer32(&sh.bin, 0) : sh.bin;
+                    ties = one && size > 1 ? ld_peer64(&sh.rest, 0) : sh.rest;
+                    listed = one ? sh.listed : total;
+                    if (!one) clear_blocks();
+                    break;
                 }
                 if (one && fits) {
                     listed = sh.listed;
@@ -465,22 +548,8 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
                 } else if (!one && total <= kList) {
                     alone = true;
                     if (rank != 0) break;
-                    int n = sh.listed;
-#pragma unroll 1
-                    for (unsigned r = 1; r < size; ++r) {              // the others' tokens behind its own
-                        const int more = (int)ld_peer32(&sh.listed, r);
-                        for (int i = tid; i < more; i += kSampThreads) {
-                            sh.list_key[n + i] = ld_peer32(&sh.list_key[i], r);
-                            sh.list_at[n + i] = (int)ld_peer32(&sh.list_at[i], r);
-                        }
-                        n += more;
-                    }
-                    for (int b = tid; b < (int)size * a.blocks; b += kSampThreads) {
-                        sh.mass[b] = 0;
-                        sh.ties[b] = 0;
-                    }
-                    __syncthreads();
-                    listed = n;
+                    clear_blocks();
+                    listed = total;
                     many = 1;
                 }
             }
@@ -648,12 +717,12 @@ extern "C" int zs_sample(const ZsSample* p) {
     int log2v = 0;
     while ((1 << log2v) < p->V) ++log2v;
     a.steps = std::min(50, 62 - log2v);
-    // A CTA has four blocks or more, and either all CTAs fit the GPU (two an SM), or the rows
+    // A CTA has eight blocks or more, and either all CTAs fit the GPU (two an SM), or the rows
     // at hand L2 (256 rows of 131071 in fp32: 681 MB read from HBM where all were).
     const int blocks = (p->V + kSampBlock - 1) / kSampBlock;
     const long long row_bytes = (long long)p->V * (p->dtype == ZS_FP32 ? 4 : 2);
     int cluster = 1;
-    while (cluster < 8 && blocks >= cluster * 8 &&
+    while (cluster < 8 && blocks >= cluster * 16 &&
            ((long long)p->B * cluster * 2 <= 296 || std::min<long long>(p->B, 296 / cluster) * row_bytes > (96ll << 20)))
         cluster *= 2;
     a.blocks = (blocks + cluster - 1) / cluster;
