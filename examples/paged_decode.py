@@ -1,14 +1,15 @@
-"""Greedy decoding with compressed weights over an uncompressed paged KV cache.
+"""Decoding with compressed weights over a paged KV cache, of 16-bit pages or 4-bit ones.
 
 A small decoder of random weights: every projection is a TCA-TBE compressed
 matrix multiplied by ZipGEMM, the KV cache is a PagedKVCache. Prompts of
 different lengths come in as one step (their attention in plain torch), then
 every decode step is one CUDA graph replay: plan_step gives the new tokens their
-slots, each layer turns q and k, writes k and v and attends, over the whole cache
-or, with --top, over chosen pages. One request ends on the way and another takes
-its row and its pages.
+slots, each layer turns q and k, writes k and v (with --bits 4 quantised) and attends,
+over the whole cache or, with --top, over chosen pages, and the rows' tokens are
+sampled (with --temperature 0, the largest logits' tokens). One request ends on the way
+and another takes its row and its pages.
 
-    python examples/paged_decode.py [--steps 48] [--top 4]
+    python examples/paged_decode.py [--steps 48] [--top 4 | --bits 4] [--temperature 0.8 --top-k 50 --top-p 0.95]
 """
 from __future__ import annotations
 
@@ -67,9 +68,7 @@ def prompt_attention(model, cache, plan):
         for r, (a, b) in enumerate(zip(cu, cu[1:])):
             if a == b:
                 continue
-            slot = plan.slots[a:b]
-            blk, row = slot // cache.page_size, slot % cache.page_size
-            k, v = cache.k[layer][blk, row].float(), cache.v[layer][blk, row].float()
+            k, v = (x.float() for x in cache.read(plan.slots[a:b], layer))
             g = model.hq // model.hkv
             s = torch.einsum("thd,shd->hts", q[a:b].float(), k.repeat_interleave(g, 1)) * model.dim ** -0.5
             s.masked_fill_(torch.ones(b - a, b - a, device=q.device, dtype=torch.bool).triu(1), -torch.inf)
@@ -79,7 +78,7 @@ def prompt_attention(model, cache, plan):
     return attend
 
 
-def run(steps=48, top=0, prompts=(33, 120, 7), seed=0, page=16):
+def run(steps=48, top=0, prompts=(33, 120, 7), seed=0, page=16, bits=16, temperature=0.0, top_k=0, top_p=1.0):
     """Decodes `steps` tokens for each prompt. Returns the tokens of each row and
     the logits of the last step."""
     torch.manual_seed(seed)
@@ -87,8 +86,12 @@ def run(steps=48, top=0, prompts=(33, 120, 7), seed=0, page=16):
     rows = len(prompts)
     longest = max(prompts) + 2 * steps + page
     pages = -(-longest // page)
-    cache = zs.PagedKVCache(rows * pages, rows, pages, model.hkv, model.dim, page, num_layers=len(model.layers))
+    cache = zs.PagedKVCache(rows * pages, rows, pages, model.hkv, model.dim, page, num_layers=len(model.layers), bits=bits)
     gen = torch.Generator(device="cuda").manual_seed(seed + 1)
+    luck = torch.Generator(device="cuda").manual_seed(seed + 2)
+
+    def choose(logits, u):
+        return zs.sample(logits, u, temperature, top_k, top_p)
 
     def admit(lens):
         """One step in which the rows of positive `lens` get a prompt; their first decoded tokens."""
@@ -98,12 +101,14 @@ def run(steps=48, top=0, prompts=(33, 120, 7), seed=0, page=16):
         tokens = torch.randint(0, model.embed.shape[0], (n,), device="cuda", generator=gen)
         logits = model.forward(tokens, plan, cache, prompt_attention(model, cache, plan))
         last = (plan.cu_tokens[1:] - 1)[new > 0].long()
-        return tokens, logits[last].argmax(-1), [r for r, t in enumerate(lens) if t > 0]
+        return tokens, choose(logits[last], torch.rand(len(last), device="cuda", generator=luck)), \
+            [r for r, t in enumerate(lens) if t > 0]
 
     prompt, first, _ = admit(list(prompts))
     history = [list(t) for t in (x.tolist() for x in prompt.split(list(prompts)))]
     tokens = first.clone()                                     # static input of the graph: row r's last token
     ones = torch.ones(rows, dtype=torch.int32, device="cuda")
+    u = torch.zeros(rows, device="cuda")                       # the step's random numbers
 
     def step():
         plan = cache.step(ones, rows)
@@ -114,7 +119,8 @@ def run(steps=48, top=0, prompts=(33, 120, 7), seed=0, page=16):
                 return cache.sparse_attention(q, top, layer, rows=own)[0]
             return cache.attention(q, layer, rows=own)
 
-        return model.forward(tokens, plan, cache, decode)
+        logits = model.forward(tokens, plan, cache, decode)
+        return logits, choose(logits, u)
 
     state = [cache.seqlens, cache.free_count, cache.block_table, cache.free_blocks]
     kept = [t.clone() for t in state]
@@ -127,7 +133,7 @@ def run(steps=48, top=0, prompts=(33, 120, 7), seed=0, page=16):
         t.copy_(k)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        logits = step()
+        logits, chosen = step()
 
     for i in range(steps):
         if i == steps // 2:                                    # row 0 ends; a new prompt takes its place
@@ -137,15 +143,25 @@ def run(steps=48, top=0, prompts=(33, 120, 7), seed=0, page=16):
             tokens[0] = first[0]
         for r, t in enumerate(tokens.tolist()):
             history[r].append(t)
+        u.uniform_(generator=luck)
         graph.replay()
-        tokens.copy_(logits.argmax(-1))
+        tokens.copy_(chosen)
     torch.cuda.synchronize()
     if cache.check_errors():
         raise RuntimeError(f"error bits {cache.check_errors()}")
     return model, history, logits
 
 
-def reference_logits(model, history):
+def held(x, group=64):
+    """Rows as a 4-bit cache holds them."""
+    y = x.unflatten(-1, (-1, group))
+    low, high = y.amin(-1, keepdim=True), y.amax(-1, keepdim=True)
+    s = ((high - low) / 15).bfloat16().float()
+    c = (low + 8 * s).bfloat16().float()
+    return (c + s * ((y - c) / s).round().clamp(-8, 7)).flatten(-2)
+
+
+def reference_logits(model, history, bits=16):
     """Last-token logits of each row in fp32 on the dense weights, without a cache."""
     out = []
     for tokens in history:
@@ -165,7 +181,10 @@ def reference_logits(model, history):
             qkv = (norm(x) @ w["qkv"].float().t()).view(n, -1, model.dim)
             q, k, v = qkv.split([model.hq, model.hkv, model.hkv], 1)
             g = model.hq // model.hkv
-            q, k, v = turn(q), turn(k).repeat_interleave(g, 1), v.repeat_interleave(g, 1)
+            q, k = turn(q), turn(k)
+            if bits == 4:
+                k, v = held(k), held(v)
+            k, v = k.repeat_interleave(g, 1), v.repeat_interleave(g, 1)
             s = torch.einsum("thd,shd->hts", q, k) * model.dim ** -0.5
             s.masked_fill_(torch.ones(n, n, device="cuda", dtype=torch.bool).triu(1), -torch.inf)
             x = x + torch.einsum("hts,shd->thd", s.softmax(-1), v).reshape(n, -1) @ w["o"].float().t()
@@ -179,9 +198,14 @@ def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--steps", type=int, default=48)
     ap.add_argument("--top", type=int, default=0, help="pages attended per KV head (0: all)")
+    ap.add_argument("--bits", type=int, default=16, choices=[4, 16], help="bits a value of the cache")
+    ap.add_argument("--temperature", type=float, default=0.0)
+    ap.add_argument("--top-k", type=int, default=0)
+    ap.add_argument("--top-p", type=float, default=1.0)
     args = ap.parse_args()
-    model, history, logits = run(args.steps, args.top)
-    ref = reference_logits(model, history)
+    model, history, logits = run(args.steps, args.top, bits=args.bits, temperature=args.temperature, top_k=args.top_k,
+                                 top_p=args.top_p)
+    ref = reference_logits(model, history, args.bits)
     err = float((logits.float() - ref).norm() / ref.norm())
     print(f"{len(history)} rows, {[len(h) for h in history]} tokens; last logits against fp32 without a cache: "
           f"rel-L2 {err:.4f}{' (sparse attention is an approximation)' if args.top else ''}")
