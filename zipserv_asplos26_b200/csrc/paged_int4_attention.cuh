@@ -21,10 +21,9 @@
 //     11 bits from there down to 2^-26 of it and vanishes below 2^-37. For bf16 outputs
 //     that is all: 2^-11 of a weight is an eighth of the output's own rounding. For fp16
 //     ones its remainder follows as a second part. The centres meet p in two bf16 parts.
-//     The codes are centred afterwards, every 128 tokens (64 for fp16): sums of codes from
-//     0 to 15 would in the end be far larger than the outputs that are left of them, and a
-//     tensor core's sums lose low bits. (Centring each code before its product took 32
-//     instructions of some 350 for every 16 tokens.)
+//     The codes are centred by a f16x2 add, exact: sums of codes from 0 to 15 would in the
+//     end be far larger than the outputs that are left of them, and a tensor core's sums
+//     lose low bits. (Centring the sums every 128 tokens instead took as long.)
 //
 // The maximum that exponents refer to follows the scores only where one passes it by 2
 // or more (base 2), so that most steps need no maximum over their lanes.
@@ -163,6 +162,10 @@ __device__ __forceinline__ void first_product(float (&d)[4], const uint32_t (&a)
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
+__device__ __forceinline__ uint32_t add_f16x2(uint32_t a, uint32_t b) {
+    const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }   // e from -126 to 127
 
 // What a warp holds of a unit of up to NT x 8 heads. A lane has heads 2 (lane % 4) and
@@ -173,7 +176,6 @@ struct Q4State {
     static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     static constexpr int kBlocks = D / 32, kPer = kBlocks / NG;      // 32 channels: a 16-byte piece of a row
     static constexpr int kTerms = kBf16 ? 1 : 2;                     // fp16 parts of p s
-    static constexpr int kSettle = (kBf16 ? 8 : 4) / kParts;         // steps after which codes are centred
     using Bf = __nv_bfloat16;
     uint32_t qf[NT][kBlocks][2][2];    // q of the even, odd channels (these a sixteenth)
     uint32_t zf[NT][3];                // of what meets the parameters: -8 sum(q_g), sum(q_g), times scale2, in three parts
@@ -183,14 +185,12 @@ struct Q4State {
     float m[NT][2], l[NT][2];          // largest score, sum of weights
     float less[NT][2], most[NT][2];    // scores count from ref = m + top - 13 = -less; at most `most` from there
     int top;                           // scales of values are below 2^top, weights times them below 2^15
-    int owed;                          // steps whose codes are still to be centred
 
     using Four = float[NT][4];         // of a lane's tokens of a part and heads
 
     __device__ __forceinline__ void start(const uint16_t* q, int rows, float scale2) {
         const int lane = threadIdx.x & 31;
         top = kNoTop;
-        owed = 0;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int head = nt * 8 + (lane >> 2);
@@ -451,8 +451,8 @@ struct Q4State {
                 uint32_t lo[4], hi[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    lo[j] = t[j] & kLowCodes;
-                    hi[j] = t[j] & kHighCodes;
+                    lo[j] = add_f16x2(t[j] & kLowCodes, 0x80088008u);        // - 8 steps
+                    hi[j] = add_f16x2(t[j] & kHighCodes, 0x80808080u);       // - 128 steps
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
@@ -465,32 +465,9 @@ struct Q4State {
         }
     }
 
-    // Centres the codes of the last steps: takes 8 sum(p s) off the sums over them.
-    __device__ __forceinline__ void settle() {
-        const int lane = threadIdx.x & 31;
-        owed = 0;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                for (int b = 0; b < kBlocks; ++b) {
-                    const float ps = __shfl_sync(~0u, z[nt][j], b / kPer * 4 + (lane & 3));
-#pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        const float by = y ? -power_of_two(7 - 24) : -power_of_two(3 - 24);
-                        o[nt][b][y][j] = fmaf(ps, by, o[nt][b][y][j]);
-                        o[nt][b][y][2 + j] = fmaf(ps, by, o[nt][b][y][2 + j]);
-                    }
-                }
-                if (lane >> 2 < NG) z[nt][j] = 0.f;
-            }
-    }
-
     // The sums of a head's eight lanes, and the outputs (unnormalised) from the sums.
     __device__ __forceinline__ void finish() {
         const int lane = threadIdx.x & 31;
-        settle();
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -690,7 +667,6 @@ struct Q4Ring {
         st.weigh(x, lim, v);
 #pragma unroll
         for (int j = 0; j < kParts; ++j) st.add(slot(s) + j * C::kPartBytes + Tile::kTile, x[j], v[j]);
-        if (++st.owed == State::kSettle) st.settle();
         __syncwarp();
     }
 };
