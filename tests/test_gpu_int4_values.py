@@ -1,0 +1,49 @@
+"""4-bit attention of values without a range of their own: groups that are one number have a
+scale of zero, so nothing but their centres says how large the sums get."""
+import pytest
+import torch
+
+import int4_plain as plain
+from test_gpu_int4 import BF, FP, U, TINY, filled, i32, randn, table_of, zs
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("value", [1.0, -1000.0, 2.0 ** 14])
+@pytest.mark.parametrize("lens", [[40], [20000, 3]])
+def test_constant_values_come_back(value, dtype, lens):
+    """The weighted mean of one number is that number: sums of T weights in two bf16 parts
+    (2^-16) over sums of the weights, each fp32 sum off by its T / 8 steps of 2^-23."""
+    page, dim = 64, 128
+    table, blocks = table_of(lens, page)
+    kp, vp = filled(blocks, page, 2, dim, 64, seed=3)
+    codes, params = plain.quantise(torch.full((blocks, page, 2, dim), value, device="cuda"), 64)
+    vp.codes.copy_(codes)
+    vp.params.copy_(params)
+    assert not vp.params[..., 0, :].any()
+    q = randn(len(lens), 8, dim, seed=2).to(dtype)
+    o = zs().paged_attention_int4(q, kp, vp, i32(table), i32(lens)).double()
+    tol = (U[dtype] + 2.0 ** -16 + 2 * (max(lens) / 8 + 16) * 2.0 ** -23) * abs(value) + TINY[dtype]
+    assert float((o - value).abs().max()) <= tol
+
+
+def test_zeros_and_one_live_group():
+    """One group of many has values, in some tokens only."""
+    page, dim, lens = 16, 64, [500]
+    table, blocks = table_of(lens, page)
+    kp, vp = filled(blocks, page, 1, dim, 32, seed=5)
+    x = torch.zeros(blocks, page, 1, dim, device="cuda")
+    x[::3, 5, 0, 32:] = randn(len(x[::3]), 32, seed=6) * 2.0 ** -20
+    codes, params = plain.quantise(x, 32)
+    vp.codes.copy_(codes)
+    vp.params.copy_(params)
+    q = randn(1, 4, dim, seed=2).to(BF)
+    o = zs().paged_attention_int4(q, kp, vp, i32(table), i32(lens))
+    i = torch.arange(500, device="cuda")
+    blk = torch.as_tensor(table[0], device="cuda").long()[i // page]
+    k, v = (plain.values(p.codes[blk, i % page], p.params[blk, i % page]) for p in (kp, vp))
+    want, _ = plain.attend(q[0], k, v, dim ** -0.5)
+    tol = U[BF] * want.abs() + plain.attention_error(q[0], k, v, kp.params, dim ** -0.5, 500) * float(v.abs().max())
+    assert bool(((o[0].double() - want).abs() <= tol).all())
+    assert not o[0, :, :32].any()

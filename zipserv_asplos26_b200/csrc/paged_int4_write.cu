@@ -2,7 +2,7 @@
 // slots of a paged KV cache (zs_rope_write_int4); rows of such a cache read back
 // (zs_read_int4). Format: paged_int4.cuh.
 //
-// Both are bound by HBM: every value is read once and written once.
+// Every value is read once and written once.
 //   * Writing goes as in paged_rope.cu (a warp walks a token's heads, 16 channels a
 //     lane). The halves of a turned head lie apart, so its fp32 values pass through
 //     shared memory and come back 16 neighbouring channels a lane; a group of 32 or 64
@@ -12,6 +12,12 @@
 //     the same ones. (x - c) / s is a product with 1 / s, and a quotient only near the
 //     middle of two codes, where the two could round apart.
 //   * Reading back, a lane turns 8 bytes of codes into 32 bytes, of K and of V.
+//
+// Measured in a graph (32 query and 8 KV heads of 128, bf16, groups of 64): 16411 tokens
+// written 82 us (375 MB, 4.6 TB/s; 3375 warp instructions a token, issued in 66% of the
+// cycles: quantising costs what is left of HBM; 72 registers, so 28 warps an SM: with 96
+// and 20, 96 us), read back 20; 65553 tokens read back 69.5 (345 MB, 5.0 TB/s); 32 tokens
+// 3.6 and 2.2.
 #include "paged_int4.cuh"
 #include "paged_rope.cuh"
 

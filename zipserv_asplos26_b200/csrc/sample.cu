@@ -25,6 +25,11 @@
 // more. All readings but the first come from L2. A row goes to a cluster of up to 8 CTAs
 // where there are few, its histograms joined through distributed shared memory. Bound by
 // instructions: some 30 for a weight, 10 of them in 64 bits.
+//
+// Measured: 256 rows of 131071 in fp32, nuclei of tens of thousands of tokens (two weights
+// for each) 243 us, 134 instructions a logit issued in 56% of the cycles, HBM read once; 64
+// rows of 128000 in bf16 with settings of their own 57 to 62; 3 of 32000 with top_k = 50 and
+// top_p = 0.95 22, a chain of some ten steps between barriers, 500 to 7000 cycles each.
 #include <algorithm>
 #include <atomic>
 #include <cfloat>

@@ -21,9 +21,8 @@ A page pool is a tensor of logical shape [num_blocks, page_size, heads, dim],
 bf16 or fp16, its last axis contiguous and the others of any strides that are
 multiples of 8 elements: `torch.empty(blocks, heads, page, dim).transpose(1, 2)`
 keeps each head's rows of a page together. A 4-bit pool is an Int4Pages, in either
-order too. Every call runs on the current
-stream of its tensors' device and synchronises nothing. `err` (optional, int32[1])
-collects error bits: 2 = an index was out of range (skipped; a position: taken as
+order too. Every call runs on the current stream of its tensors' device and synchronises
+nothing. `err` (optional, int32[1]) collects error bits: 2 = an index was out of range (skipped; a position: taken as
 0), 4 = a request was refused by plan_step.
 """
 from __future__ import annotations
@@ -220,8 +219,9 @@ def paged_attention_int4(q: torch.Tensor, k_pages: Int4Pages, v_pages: Int4Pages
                          out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
                          max_seqlen: Optional[int] = None, err: Optional[torch.Tensor] = None) -> torch.Tensor:
     """paged_attention over a 4-bit cache, q bf16 or fp16 (below 2**63 in magnitude). Keys and
-    values are what the codes stand for, not rounded to q's type in between. The arguments are
-    paged_attention's but for the pools."""
+    values are what the codes stand for, not rounded to q's type in between. A NaN among a
+    token's keys makes its head's outputs NaN, one among its values its group's channels. The
+    arguments are paged_attention's but for the pools."""
     o = (_native or _load()).paged_attention_int4(q, k_pages, v_pages, block_table, seq_lens, softmax_scale, pages,
                                                   counts, out, lse, max_seqlen, err)
     return o if q.dim() == 3 and out is None else o.view(q.shape)
