@@ -9,8 +9,8 @@
 //     channels is then 2 or 4 lanes, whose minimum and maximum take one or two shuffles
 //     each. k is quantised from the turned fp32 values, whose products are rounded one by
 //     one (no fused multiply-add): codes are whole numbers, and the plain formula gives
-//     the same ones. (x - c) / s is a product with 1 / s, and a quotient only near the
-//     middle of two codes, where the two could round apart.
+//     the same ones. (x - c) / s is a product with 1 / s, and a quotient only where one of
+//     a lane's is near the middle of two codes, where the two could round apart.
 //   * Reading back, a lane turns 8 bytes of codes into 32 bytes, of K and of V.
 //
 // Measured in a graph (32 query and 8 KV heads of 128, bf16, groups of 64): 16411 tokens
@@ -182,15 +182,23 @@ __global__ void __launch_bounds__(kRopeThreads, 14) rope_write_int4_kernel(const
             // ---- codes: rounded by adding 1.5 2^23 (and 8), whose bits add up to as many times a constant
             const float by = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
             constexpr float kWhole = 12582920.f, kLeast = 12582912.f, kMost = 12582927.f;
-            uint32_t code[2] = {0u - 0x4B400000u * 0x11111111u, 0u - 0x4B400000u * 0x11111111u};
+            constexpr uint32_t kNone = 0u - 0x4B400000u * 0x11111111u;
+            uint32_t code[2] = {kNone, kNone};
+            bool close = false;            // to the middle of two codes: products are off by 2^-20 at most
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-                const float d = __fsub_rn(f[j], centre);
-                float m = fmaf(d, by, kWhole);
-                // off by 2^-20 at most before it was rounded: near the middle of two codes the quotient tells
-                if (fabsf(fmaf(d, by, kWhole - m)) > 0.499998f) m = rintf(__fdiv_rn(d, s)) + kWhole;
-                m = fminf(fmaxf(m, kLeast), kMost);
-                code[j / 8] += (uint32_t)__float_as_int(m) << (j % 8 * 4);
+                f[j] = __fsub_rn(f[j], centre);
+                const float m = fmaf(f[j], by, kWhole);
+                close |= fabsf(fmaf(f[j], by, kWhole - m)) > 0.499998f;
+                code[j / 8] += (uint32_t)__float_as_int(fminf(fmaxf(m, kLeast), kMost)) << (j % 8 * 4);
+            }
+            if (close) {                   // again, by quotients
+                code[0] = code[1] = kNone;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float m = rintf(__fdiv_rn(f[j], s)) + kWhole;
+                    code[j / 8] += (uint32_t)__float_as_int(fminf(fmaxf(m, kLeast), kMost)) << (j % 8 * 4);
+                }
             }
             if (!(s > 0.f)) code[0] = code[1] = 0x88888888u;
             // ---- the head's groups to its first lane
