@@ -363,44 +363,30 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
                 }
                 __syncthreads();
             }
-            // a warp's bins, from the highest down
-            const int per = bins / kSampWarps, end = bins - 1 - warp * per;
-            u64 v[kBins / kSampThreads], sum = 0;
+            // a warp's bins from the highest down, neighbouring ones a lane
+            constexpr int kEach = kBins / kSampThreads;
+            const int per = max(1, bins / kSampThreads), end = bins - 1 - (warp * (bins / kSampWarps) + lane * per);
+            u64 v[kEach], mine = 0;
 #pragma unroll
-            for (int i = 0; i < kBins / kSampThreads; ++i) {
-                const int b = end - (i * 32 + lane);
+            for (int i = 0; i < kEach; ++i) {
                 v[i] = 0;
-                if (i * 32 + lane < per) {
-                    if constexpr (kCount) v[i] = sh.count[b];
-                    else v[i] = ((u64)sh.hi[b] << 32) + sh.lo[b];
+                if (i < per && lane * per < bins / kSampWarps) {
+                    if constexpr (kCount) v[i] = sh.count[end - i];
+                    else v[i] = ((u64)sh.hi[end - i] << 32) + sh.lo[end - i];
                 }
-                sum += v[i];
+                mine += v[i];
             }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-            if (lane == 0) sh.part[warp] = sum;
-            __syncthreads();
-            u64 before = 0, total = 0;
-            for (int w = 0; w < kSampWarps; ++w) {
-                if (w < warp) before += sh.part[w];
-                total += sh.part[w];
-            }
+            u64 total;
+            u64 before = block_prefix(mine, sh.part, total) - mine;
             if (!kCount && level == 0) want = times(top_p, total, true);
-            if (before < want && want <= before + sum) {
+            if (before < want && want <= before + mine) {
 #pragma unroll
-                for (int i = 0; i < kBins / kSampThreads; ++i) {
-                    u64 up_to = v[i];
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const u64 x = __shfl_up_sync(~0u, up_to, o);
-                        if (lane >= o) up_to += x;
+                for (int i = 0; i < kEach; ++i) {
+                    if (before < want && want <= before + v[i]) {
+                        sh.bin = end - i;
+                        sh.rest = want - before;
                     }
-                    up_to += before;
-                    if (up_to - v[i] < want && want <= up_to) {
-                        sh.bin = end - (i * 32 + lane);
-                        sh.rest = want - (up_to - v[i]);
-                    }
-                    before = __shfl_sync(~0u, up_to, 31);
+                    before += v[i];
                 }
             }
         }
@@ -413,26 +399,29 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
     unsigned edge = none;          // tokens above it are kept, and of those on it the first `ties`
     u64 ties = 0;
 
+    auto gather = [&](unsigned k, int i) {
+        const int at = atomicAdd(&sh.listed, 1);
+        if (at < kList) {
+            sh.list_key[at] = k;
+            sh.list_at[at] = i;
+        }
+    };
     // Sums of blocks, a warp a block: weights above `high`; tokens from `low` to `high` are
     // gathered, or counted.
-    auto sum_blocks = [&](unsigned low, unsigned high, bool gather) {
+    auto sum_blocks = [&](unsigned low, unsigned high, bool gathers) {
         for (int b = warp; b < a.blocks; b += kSampWarps) {
             const int from = e0 + b * kSampBlock;
             u64 m = 0;
             unsigned t = 0;
             // where more were gathered than fit, another reading follows
-            if (from < e1 && !(gather && *static_cast<volatile int*>(&sh.listed) > kList))
+            if (from < e1 && !(gathers && *static_cast<volatile int*>(&sh.listed) > kList))
                 each(from, min(from + kSampBlock, e1), lane, 32, [&](float v, int i) {
                     const unsigned k = order_of(v);
                     if (k < low) return;
                     if (k > high) {
                         if (k > none) m += weigh.of_kept(v);
-                    } else if (gather) {
-                        const int at = atomicAdd(&sh.listed, 1);
-                        if (at < kList) {
-                            sh.list_key[at] = k;
-                            sh.list_at[at] = i;
-                        }
+                    } else if (gathers) {
+                        gather(k, i);
                     } else {
                         ++t;
                     }
@@ -474,7 +463,11 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
                 first = false;
                 const unsigned low = found << kDigit[0];
                 const bool one = by_count != by_weight;
-                sum_blocks(low, one ? low | ((1u << kDigit[0]) - 1) : 0xFFFFFFFFu, true);
+                if (one) sum_blocks(low, low | ((1u << kDigit[0]) - 1), true);
+                else each(e0, e1, tid, kSampThreads, [&](float v, int i) {
+                    const unsigned k = order_of(v);
+                    if (k >= low && *static_cast<volatile int*>(&sh.listed) <= kList) gather(k, i);
+                });
                 all_sync();
                 int before[9];                 // tokens that the CTAs before gathered
                 bool fits = true;
