@@ -29,12 +29,13 @@
 // or more (base 2), so that most steps need no maximum over their lanes.
 //
 // Measured in a graph (bf16, 32 query and 8 KV heads of 128, groups of 64, pages of 64):
-// B=32 T=4129 38.7 us, 3.95 TB/s (60% of a plain copy's rate; 16-bit pages 85.5 us);
-// B=1 T=131105 38.0; 61 sequences of 0..16417 (fp16, 64 query heads, groups of 32, pages of
-// 16 by token) 182, 3.5 TB/s. 258 warp instructions for 16 tokens of a head, issued in half
-// of the cycles: a warp waits for its own results, and two warps a scheduler hide part of
-// it; arithmetic (ALU) 46% busy, tensor cores 29%. DRAM reads are the algorithm's bytes
-// (152.6 MB), but where rows lie by token 746 MB for 643.
+// B=32 T=4129 38.9 us, 3.9 TB/s (16-bit pages 85.5 us); B=128 122, 5.0 TB/s: 5.6 as a rate
+// (85% of a plain copy's) and some 12 us of start, first lookups and join. B=1 T=131105
+// 38.4; 61 sequences of 0..16417 (fp16, 64 query heads, groups of 32, pages of 16 by token)
+// 179, 3.6 TB/s. 282 warp instructions for 16 tokens of a head, issued in half of the
+// cycles: a warp waits for its own results, and two warps a scheduler hide part of it;
+// arithmetic (ALU) 44% busy, tensor cores 28%. DRAM reads are the algorithm's bytes (152.7
+// MB), but where rows lie by token 747 MB for 643.
 #pragma once
 
 #include "paged_int4.cuh"

@@ -14,10 +14,10 @@
 //   * Reading back, a lane turns 8 bytes of codes into 32 bytes, of K and of V.
 //
 // Measured in a graph (32 query and 8 KV heads of 128, bf16, groups of 64): 16411 tokens
-// written 82 us (375 MB, 4.6 TB/s; 3375 warp instructions a token, issued in 66% of the
+// written 80.5 us (364 MB, 4.5 TB/s; 3440 warp instructions a token, issued in 68% of the
 // cycles: quantising costs what is left of HBM; 72 registers, so 28 warps an SM: with 96
-// and 20, 96 us), read back 20; 65553 tokens read back 69.5 (345 MB, 5.0 TB/s); 32 tokens
-// 3.6 and 2.2.
+// and 20, 96 us), read back 20; 65553 tokens read back 69 (345 MB, 5.0 TB/s); 32 tokens
+// 3.6 and 2.3.
 #include "paged_int4.cuh"
 #include "paged_rope.cuh"
 

@@ -20,16 +20,16 @@
 // one border, sums the weights above its 4096th part of the order, for each block of 1024
 // tokens, and gathers the tokens in it; their next 12 and 8 bits find the border. With two
 // borders it gathers all tokens from the first one's part on; up to 4096 of them are all that
-// remains to be looked at, up to 512 each against all others. Where more are gathered, further readings find the other bits, and
-// the sums. In the end the block in which the running sum passes its target is read once
-// more. All readings but the first come from L2. A row goes to a cluster of up to 8 CTAs
+// remains to be looked at, up to 512 each against all others. Where more are gathered,
+// further readings find the other bits, and the sums. In the end the block in which the
+// running sum passes its target is read once more. All readings but the first come from L2. A row goes to a cluster of up to 8 CTAs
 // where there are few, its histograms joined through distributed shared memory. Bound by
 // instructions: some 30 for a weight, 10 of them in 64 bits.
 //
 // Measured: 256 rows of 131071 in fp32, nuclei of tens of thousands of tokens (two weights
-// for each) 243 us, 134 instructions a logit issued in 56% of the cycles, HBM read once; 64
-// rows of 128000 in bf16 with settings of their own 57 to 62; 3 of 32000 with top_k = 50 and
-// top_p = 0.95 22, a chain of some ten steps between barriers, 500 to 7000 cycles each.
+// for each) 246 us, 134 instructions a logit issued in 56% of the cycles, HBM read once; 64
+// rows of 128000 in bf16 with settings of their own 62; 3 of 32000 with top_k = 50 and top_p
+// = 0.95 19, a chain of some ten steps between barriers, 500 to 5000 cycles each.
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
