@@ -47,3 +47,26 @@ def test_zeros_and_one_live_group():
     tol = U[BF] * want.abs() + plain.attention_error(q[0], k, v, kp.params, dim ** -0.5, 500) * float(v.abs().max())
     assert bool(((o[0].double() - want).abs() <= tol).all())
     assert not o[0, :, :32].any()
+
+
+def test_read_refuses_one_output_for_both():
+    kp, vp = filled(2, 16, 1, 64, 32)
+    slots = torch.arange(4, device="cuda")
+    big = torch.empty(8, 1, 64, dtype=BF, device="cuda")
+    for out in ((big[:4], big[:4]), (big[:4], big[1:5]), (big[2:6], big[:4])):
+        with pytest.raises(ValueError):
+            zs().read_int4(kp, vp, slots, out=out)
+    k, v = zs().read_int4(kp, vp, slots, out=(big[:4], big[4:]))
+    assert torch.equal(torch.cat([k, v]), torch.cat(zs().read_int4(kp, vp, slots)))
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_read_of_slots_outside_a_cache(bits):
+    cache = zs().PagedKVCache(4, 1, 4, 2, 64, 16, bits=bits)
+    slots = torch.tensor([0, -1, 63], device="cuda")
+    cache.read(slots)
+    assert cache.check_errors() == 0
+    for bad in (-2, 64, 1 << 40):
+        cache.err.zero_()
+        k, v = cache.read(torch.tensor([3, bad], device="cuda"))
+        assert cache.check_errors() == 2 and not k[1].any() and not v[1].any()

@@ -719,6 +719,8 @@ PyObject* read_int4(PyObject* const* a) {
     }
     p.k_out = ptr<uint16_t>(out[0]);
     p.v_out = ptr<uint16_t>(out[1]);
+    const int64_t len = out[0].numel();
+    need(!zs::rows_meet(p.k_out, 1, 1, len, len, len, p.v_out, len), "out must be two tensors apart from one another");
     p.stream = current_stream(index);
     p.k_pool = pools.k;
     p.v_pool = pools.v;

@@ -329,6 +329,8 @@ extern "C" int zs_read_int4(const ZsReadInt4* p) {
         return cudaErrorInvalidValue;
     if (p->N == 0) return cudaSuccess;
     if (!p->slots || !p->k_out || !p->v_out || !aligned16p(p->k_out) || !aligned16p(p->v_out)) return cudaErrorInvalidValue;
+    const long long len = (long long)p->N * a.kp.heads * a.kp.dim;
+    if (rows_meet(p->k_out, 1, 1, len, len, len, p->v_out, len)) return cudaErrorInvalidValue;
     a.slots = reinterpret_cast<const long long*>(p->slots);
     a.k_out = p->k_out;
     a.v_out = p->v_out;

@@ -334,9 +334,11 @@ class PagedKVCache:
         [N, heads, dim] of the cache's dtype."""
         if self.bits == 4:
             return read_int4(self.k[layer], self.v[layer], slots, self.dtype, None, self.err)
-        at = slots.clamp(min=0)
+        most = self.k[layer].shape[0] * self.page_size
+        at = slots.clamp(0, most - 1)
         block, row = at // self.page_size, at % self.page_size
-        dead = (slots < 0).view(-1, 1, 1)
+        dead = (slots != at).view(-1, 1, 1)
+        self.err.bitwise_or_(((slots < -1) | (slots >= most)).any().int() * 2)
         return self.k[layer][block, row].masked_fill_(dead, 0), self.v[layer][block, row].masked_fill_(dead, 0)
 
     def token_rows(self, plan: StepPlan) -> TokenRows:
