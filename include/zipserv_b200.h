@@ -395,9 +395,9 @@ int zs_select_pages(const ZsSelectPages* args);
  * clamp(rint((x - c) / s) + 8, 0, 15) in fp32. A group whose scale is below 2^-126 has
  * s = 0, c = bf16(min) and codes of 8; one with a value that is not finite, or whose
  * max - min is not, c = NaN: it reads back as NaN. Row (block, token, head) starts at
- * codes + block * codes_block + ... (bytes, multiples of 16) and params + block *
- * params_block + ... (elements, multiples of 2 head_dim / group); both are 16-byte
- * aligned; pages as in ZsPagePool. */
+ * codes + block * codes_block + ... (bytes, multiples of 16, as is codes) and params +
+ * block * params_block + ... (elements, multiples of a row's 2 head_dim / group; params is
+ * aligned to a row's bytes); pages as in ZsPagePool. */
 typedef struct ZsInt4Pool {
     uint8_t* codes;
     uint16_t* params;

@@ -70,3 +70,26 @@ def test_read_of_slots_outside_a_cache(bits):
         cache.err.zero_()
         k, v = cache.read(torch.tensor([3, bad], device="cuda"))
         assert cache.check_errors() == 2 and not k[1].any() and not v[1].any()
+
+
+@pytest.mark.parametrize("group", [32, 64])
+def test_a_head_of_rows_by_token(group):
+    """Part of a larger pool, from an odd head on: parameters are aligned to a row of theirs."""
+    page, lens, dim = 16, [90], 128
+    table, blocks = table_of(lens, page)
+    kb, vb = filled(blocks, page, 5, dim, group, "tokens", seed=2)
+    kp, vp = (zs().Int4Pages(p.codes[:, :, 3:4], p.params[:, :, 3:4]) for p in (kb, vb))
+    own = [zs().Int4Pages(p.codes.contiguous(), p.params.contiguous()) for p in (kp, vp)]
+    q = randn(1, 4, dim, seed=2).to(BF)
+    o = zs().paged_attention_int4(q, kp, vp, i32(table), i32(lens))
+    assert torch.equal(o, zs().paged_attention_int4(q, *own, i32(table), i32(lens)))
+    slots = torch.arange(40, device="cuda")
+    assert torch.equal(zs().read_int4(kp, vp, slots)[0], zs().read_int4(*own, slots)[0])
+    kv = randn(40, 1, dim, seed=4).to(BF)
+    cos_sin = torch.cat([torch.ones(1, 64), torch.zeros(1, 64)], 1).cuda()
+    before = kb.codes.clone()
+    for pools in ((kp, vp), own):
+        zs().rope_write_int4(kv, kv, kv, torch.zeros(40, dtype=torch.int32, device="cuda"), cos_sin, slots, *pools)
+    assert torch.equal(kp.codes, own[0].codes) and torch.equal(vp.params, own[1].params)
+    before[:, :, 3] = kb.codes[:, :, 3]
+    assert torch.equal(kb.codes, before)

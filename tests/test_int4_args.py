@@ -63,7 +63,7 @@ def test_the_formulas_error():
             assert bool((off <= (s / 2 + (15 * s + c.abs()) / 256).unsqueeze(-1)).all())
 
 
-BAD_POOLS = [dict(codes=0), dict(params=0), dict(codes=8), dict(params=8), dict(codes_token=72), dict(params_token=6),
+BAD_POOLS = [dict(codes=0), dict(params=0), dict(codes=8), dict(params=4), dict(codes_token=72), dict(params_token=6),
              dict(codes_block=-64), dict(num_blocks=0), dict(page_size=24), dict(page_size=8), dict(num_heads=0),
              dict(head_dim=96), dict(head_dim=256), dict(group=16), dict(group=128)]
 

@@ -646,7 +646,8 @@ ZsInt4Pool int4_pool(PyObject* pages, const char* name, const char* codes, const
         refuse(std::string(name) + ": codes and params must agree in blocks, page size and heads");
     if (c.stride(3) != 1 || (c.stride(0) | c.stride(1) | c.stride(2)) % 16 || !aligned16(c) ||
         (t.stride(4) != 1 && groups > 1) || t.stride(3) != groups ||
-        (t.stride(0) | t.stride(1) | t.stride(2)) % (2 * groups) || !aligned16(t))
+        (t.stride(0) | t.stride(1) | t.stride(2)) % (2 * groups) ||
+        reinterpret_cast<uintptr_t>(t.data_ptr()) % (4 * groups))
         refuse(std::string(name) + ": rows must be contiguous and aligned (codes to 16 bytes, params to a row's)");
     return {ptr<uint8_t>(c), ptr<uint16_t>(t), c.stride(0), c.stride(1), c.stride(2), t.stride(0), t.stride(1),
             t.stride(2), static_cast<int>(c.size(0)), static_cast<int>(c.size(1)), static_cast<int>(c.size(2)),

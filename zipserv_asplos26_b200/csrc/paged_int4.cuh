@@ -41,7 +41,7 @@ inline bool make_int4_pool(const ZsInt4Pool* p, Int4View* v) {
     v->groups = p->head_dim / p->group;
     if ((p->codes_block | p->codes_token | p->codes_head) % 16) return false;
     if ((p->params_block | p->params_token | p->params_head) % (2 * v->groups)) return false;
-    if (!aligned16p(p->codes) || !aligned16p(p->params)) return false;
+    if (!aligned16p(p->codes) || reinterpret_cast<uintptr_t>(p->params) % (4 * v->groups)) return false;
     v->codes = p->codes;
     v->params = p->params;
     v->c_block = p->codes_block;
