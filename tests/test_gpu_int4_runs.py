@@ -67,3 +67,31 @@ def test_a_wide_table_with_short_sequences():
     check_attention(q, kp, vp, table, lens, page)
     check_attention(q, kp, vp, table, lens, page, max_seqlen=300)
     check_attention(q, kp, vp, table, lens, page, max_seqlen=100000)
+
+
+def test_two_graphs_replayed_side_by_side():
+    """Each call's workspace is its own, in a graph too: attention and sampling of two graphs on
+    two streams at once give what eager calls give."""
+    page, graphs = 64, []
+    for seed, lens in ((1, [9000, 100, 3000]), (2, [20000])):
+        table, blocks = table_of(lens, page, seed=seed)
+        kp, vp = filled(blocks, page, 2, 128, 64, seed=seed)
+        q = randn(len(lens), 8, 128, seed=seed).to(BF)
+        t, n = i32(table), i32(lens)
+        x = randn(len(lens), 40000, seed=seed) * 3
+        u = torch.rand(len(lens), device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed))
+        want = zs().paged_attention_int4(q, kp, vp, t, n), zs().sample(x, u, 0.9, 0, 0.9)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(side), torch.cuda.graph(g, stream=side):
+            got = zs().paged_attention_int4(q, kp, vp, t, n), zs().sample(x, u, 0.9, 0, 0.9)
+        graphs.append((g, side, got, want, (q, kp, vp, t, n, x, u)))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for g, side, *_ in graphs:
+            with torch.cuda.stream(side):
+                g.replay()
+    torch.cuda.synchronize()
+    for _, _, got, want, _ in graphs:
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
