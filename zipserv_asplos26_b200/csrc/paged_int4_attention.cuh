@@ -516,7 +516,8 @@ struct Q4State {
                 if (lse && lane < 4) lse[row] = log_sum(-less[nt][j], l[nt][j], 0.f);
             }
     }
-    // A piece: unnormalised rows [rows][D], and [rows][2] maxima and sums.
+    // A piece: unnormalised rows [rows][D], and [rows][2] references and sums. Where nothing
+    // weighs the reference is minus infinity, as the other pieces may lie far below zero.
     __device__ __forceinline__ void park(float* po, float* ml, int rows) const {
         const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -529,7 +530,9 @@ struct Q4State {
                 for (int b = 0; b < kBlocks; ++b)
                     *reinterpret_cast<float4*>(po + row * D + b * 32 + (lane >> 2) * 4) =
                         make_float4(o[nt][b][0][j], o[nt][b][1][j], o[nt][b][0][2 + j], o[nt][b][1][2 + j]);
-                if (lane < 4) *reinterpret_cast<float2*>(ml + row * 2) = make_float2(-less[nt][j], l[nt][j]);
+                if (lane < 4)
+                    *reinterpret_cast<float2*>(ml + row * 2) =
+                        make_float2(m[nt][j] == -INFINITY ? -INFINITY : -less[nt][j], l[nt][j]);
             }
     }
 };
