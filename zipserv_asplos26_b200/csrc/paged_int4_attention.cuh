@@ -377,6 +377,7 @@ struct Q4State {
                     for (int i = 0; i < kParts; ++i) mx = fmaxf(mx, fmaxf(x[i][nt][j], x[i][nt][2 + j]));
 #pragma unroll
                     for (int k = 4; k < 32; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, k));
+                    const bool held = m[nt][j] != -INFINITY;           // the same for a head's lanes
                     m[nt][j] = fmaxf(m[nt][j], mx - less[nt][j]);
                     const bool none = m[nt][j] == -INFINITY;
                     const float now = (none ? 0.f : m[nt][j]) + (float)(top - 13);
@@ -388,7 +389,7 @@ struct Q4State {
                         x[i][nt][j] += by;
                         x[i][nt][2 + j] += by;
                     }
-                    if (l[nt][j] != 0.f) {             // else nothing is held
+                    if (held) {                // by any lane: o and z sum all lanes' tokens, l this lane's
                         l[nt][j] *= keep;
                         z[nt][j] *= keep;
 #pragma unroll
