@@ -18,9 +18,10 @@
 //     power of two (bf16: 2^64; fp16: to its type's top), which loses nothing that counts.
 //   * Outputs: sum_t (p_t s_t) (u_t - 8) + sum_t p_t c_t. p s goes in as fp16, scaled by a
 //     power of two that follows the largest scale so far, so that it has all 11 bits from
-//     there down to 2^-26 of it and vanishes below 2^-37. For bf16 outputs
-//     that is all: 2^-11 of a weight is an eighth of the output's own rounding. For fp16
-//     ones its remainder follows as a second part. The centres meet p in two bf16 parts.
+//     there down to 2^-26 of it and vanishes below 2^-37, and its remainder follows as a
+//     second part: 22 bits, as rounding a weight must add nothing to outputs that are what
+//     is left of values that cancel (one part: 38.9 us for 42.9 at B=32 T=4129 in bf16, and such outputs
+//     off by an eighth). The centres meet p in two bf16 parts.
 //     The codes are centred by a f16x2 add, exact: sums of codes from 0 to 15 would in the
 //     end be far larger than the outputs that are left of them, and a tensor core's sums
 //     lose low bits. (Centring the sums every 128 tokens instead took as long.)
@@ -186,7 +187,6 @@ template <typename T, int D, int NG, int NT, int kParts>
 struct Q4State {
     static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     static constexpr int kBlocks = D / 32, kPer = kBlocks / NG;      // 32 channels: a 16-byte piece of a row
-    static constexpr int kTerms = kBf16 ? 1 : 2;                     // fp16 parts of p s
     using Bf = __nv_bfloat16;
     uint32_t qf[NT][kBlocks][2][2];    // q of the even, odd channels (these a sixteenth)
     uint32_t zf[NT][3];                // of what meets the parameters: -8 sum(q_g), sum(q_g), times scale2, in three parts
@@ -414,15 +414,15 @@ struct Q4State {
                 }
     }
 
-    // Four weights (a lane's tokens and heads) as fragments of kN 16-bit numbers that add up.
-    template <typename P, int kN>
-    __device__ __forceinline__ static void split(float a, float b, float c, float d, uint32_t (&f)[kN][2]) {
+    // Four weights (a lane's tokens and heads) as fragments of two 16-bit numbers that add up.
+    template <typename P>
+    __device__ __forceinline__ static void split(float a, float b, float c, float d, uint32_t (&f)[2][2]) {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
+        for (int i = 0; i < 2; ++i) {
             const uint32_t x = pack2<P>(a, b), y = pack2<P>(c, d);
             f[i][0] = transpose8(x);
             f[i][1] = transpose8(y);
-            if (i + 1 < kN) {
+            if (i == 0) {
                 const float2 xb = unpack2<P>(x), yb = unpack2<P>(y);
                 a -= xb.x;
                 b -= xb.y;
@@ -445,7 +445,7 @@ struct Q4State {
             product(z[nt], pr, f[0][0], f[0][1], Bf());
             product(z[nt], pr, f[1][0], f[1][1], Bf());
         }
-        uint32_t f[NT][kTerms][2];
+        uint32_t f[NT][2][2];
 #pragma unroll
         for (int b2 = 0; b2 < kBlocks / 2; ++b2) {
             uint32_t v[4];
@@ -469,7 +469,7 @@ struct Q4State {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int x = 0; x < kTerms; ++x) {
+                    for (int x = 0; x < 2; ++x) {
                         product(o[nt][b][0], lo, f[nt][x][0], f[nt][x][1], __half());
                         product(o[nt][b][1], hi, f[nt][x][0], f[nt][x][1], __half());
                     }
