@@ -10,12 +10,27 @@ inline int q4_max_ctas(int D, int G) {
     if (G <= 8) return 148 * (D == 64 ? Q4Cfg<64, 1, false>::kCtas : Q4Cfg<128, 1, false>::kCtas);
     return 148 * (D == 64 ? Q4Cfg<64, 2, false>::kCtas : Q4Cfg<128, 2, false>::kCtas);
 }
-// Warps a unit, or 0 for runs.
+// Warps a unit, or 0 for runs. A chunk is 32 tokens in units, so runs pay from fewer of
+// them on than with 16-bit pages (us in runs and in units, bf16, 32 query and 8 KV heads of
+// 128, page lists as batch x pages of 64):
+//   up to 5 a warp     B=1 T=2000 10.6 and 8.4; B=16 T=1000 12.2 and 12.4; 24 of 0..600
+//                      12.8 and 9.3; 8 x 16 12.4 and 10.2
+//   8 to 10            B=32 T=1000 16.9 and 19.0, T=800 16.9 and 15.9; B=128 T=300 19.5 and
+//                      23.8; 64 of 0..1000 23.3 and 21.0; 300 of 0..600 52.2 and 44.4;
+//                      512 of 300 61.3 and 56.1; 8 x 64 18.5 and 21.0
+//   12 to 16           B=32 T=1500 21.4 and 26.0, T=2000 26.4 and 33.0; B=64 T=2000 41.9 and
+//                      47.6; 100 of 0..1500 39.9 and 37.6; 200 x 8 41.7 and 36.1; 8 x 128
+//                      27.9 and 35.0
+//   32                 32 x 64 41.7 and 61.4; 128 x 16 47.3 and 62.5; 8 x 256 43.3 and 62.9
+// and where units leave SMs idle, 1 x 64 and 2 x 64 (8 chunks) 11.0 and 12.1, 12.3 and 12.6.
 inline int q4_unit_warps(const Q4Args& a) {
     using One = Q4Cfg<128, 1, true>;
     using Two = Q4Cfg<128, 2, true>;
     static_assert(One::kParts == 2 && Two::kParts == 2, "units' chunks are two parts");
-    return unit_warps(a, a.pages != nullptr, 148 * (a.G <= 8 ? One::kCtas : Two::kCtas), 2);
+    UnitLimits limits;
+    limits.whole = 10;
+    limits.listed = 16;
+    return unit_warps(a, a.pages != nullptr, 148 * (a.G <= 8 ? One::kCtas : Two::kCtas), 2, limits);
 }
 
 // The checked arguments of a call, but for its workspace.

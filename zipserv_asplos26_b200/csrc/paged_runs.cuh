@@ -1,7 +1,7 @@
 // How paged attention is dealt to the GPU and joined, whatever the cache holds
 // (paged_attention.cu: 16-bit keys and values; paged_int4_attention.cuh: 4-bit ones).
 //
-// The work is cut into chunks, a warp's step: one or two parts of 16 tokens of a unit
+// The work is cut into chunks, a warp's step: one to four parts of 16 tokens of a unit
 // (sequence, KV head, tile of up to 16 query heads). They are dealt in one of two ways,
 // chosen by sizes that the host has (unit_warps):
 //   * paged_attn_kernel: all chunks in order go to the warps of the GPU in equal
@@ -653,7 +653,8 @@ cudaError_t resident_ctas(int* ctas) {
 // of 0..1000: 26.4 and 34.6 at 36 chunks a warp; 16 of 2048: 27.1 and 28.5 at 17).
 // So they serve units that are bounded to 16 chunks a warp, to 64 for page lists,
 // whose units are alike (8 x 64 pages: 43.5 and 39.3), or to 5 where they leave SMs
-// idle (B=1 T=4096: 9.6 and 15.6). W fills the GPU once, with two chunks a warp or
+// idle (B=1 T=4096: 9.6 and 15.6). These are the limits for 16-bit keys and values,
+// whose chunks are 16 tokens; other forms bring their own (UnitLimits). W fills the GPU once, with two chunks a warp or
 // more; units of unlike lengths in more waves want shares of some 12 chunks (128
 // of 0..600: 41.1 us with one warp each, 28.7 with four, 31.4 in runs). Clusters of
 // more than 4 CTAs were slower in all of these.
@@ -665,14 +666,18 @@ inline long long unit_parts(const PaArgs& a, bool listed) {
     return a.max_len > 0 && !listed ? std::min(pages, ((long long)a.max_len + kPaChunk - 1) / kPaChunk) : pages;
 }
 
-inline int unit_warps(const PaArgs& a, bool listed, int max_ctas, int parts) {
+struct UnitLimits {
+    int whole = 16, listed = 64;       // chunks a warp, at most
+};
+
+inline int unit_warps(const PaArgs& a, bool listed, int max_ctas, int parts, UnitLimits limits = {}) {
     const long long units = (long long)a.B * a.Hkv * a.tiles, chunks = (unit_parts(a, listed) + parts - 1) / parts;
     const long long resident = (long long)max_ctas * kPaWarps;
     int W = 1;
     while (W < kPaMaxUnitWarps && units * W * 2 <= resident && W * 4 <= chunks) W *= 2;
     while (!listed && W < kPaWarps && W * 12 < chunks) W *= 2;
     const long long steps = (chunks + W - 1) / W;
-    const long long most = units * W < 148 * 4 ? 5 : listed ? 64 : 16;
+    const long long most = units * W < 148 * 4 ? 5 : listed ? limits.listed : limits.whole;
     return steps <= most && units * W <= INT32_MAX ? W : 0;
 }
 
