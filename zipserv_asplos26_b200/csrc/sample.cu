@@ -286,6 +286,7 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const SampArgs 
     weigh.cut = __double2float_rd((double)peak - 44.3614195558365 * temperature);
     weigh.cut = fmaxf(fminf(weigh.cut, nextafterf(peak, -INFINITY)), -FLT_MAX);
     weigh.rate = fmin(1.4426950408889634 / temperature, 130.0 / ((double)peak - (double)weigh.cut));
+    weigh.rate = fmin(weigh.rate, DBL_MAX);    // a row of -FLT_MAX, which has no number below, and T below 2^-1023
     if (isinf(peak)) {                         // infinite ones weigh 1, others nothing
         none = kOrderOfMost;
         weigh.peak = weigh.top = weigh.cut = 0.f;
