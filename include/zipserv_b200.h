@@ -472,7 +472,9 @@ int zs_paged_attention_int4(const ZsPagedAttentionInt4* args);
  * weights passes u times their sum; sums do not depend on an order. temperature <= 0: the
  * first of the largest. A logit of -inf is never chosen; where some are +inf, these have
  * weight 1 and the others none. Each setting is a device array [B], or, where that is NULL,
- * the value in ...1 for all rows. out [B]: the tokens; -1, and bit 8 in *err (nullable), for
+ * the value in ...1 for all rows (in 64 bits, where a device array's 0.95 is the nearest
+ * float). Settings outside their ranges count as the nearest end, an infinite temperature
+ * makes all weights 1. out [B]: the tokens; -1, and bit 8 in *err (nullable), for
  * a row with a NaN or of -inf alone. Settings that are NaN count as off (temperature: as
  * 0), u outside [0, 1) as its nearest end. */
 enum { ZS_FP32 = 2 };

@@ -24,6 +24,10 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torc
     an order of sums. temperature 0 takes the first of the largest.
 
     A setting is a number, or a tensor with one for each row (float32; top_k: int32). A
-    logit of -inf is never chosen. A row with a NaN, or of -inf alone, gives -1 and sets bit
+    number is taken in 64 bits, so a top_p of 0.95 may end a row's kept tokens one token from
+    where the float32 nearest to 0.95 does. A number outside its range is refused; a tensor's
+    counts as the nearest end (a top_k below 0 as 0), NaN as off (temperature: as 0), u
+    outside its own likewise, and an infinite temperature makes all weights 1. A logit of
+    -inf is never chosen. A row with a NaN, or of -inf alone, gives -1 and sets bit
     8 in err (int32 [1])."""
     return (paged._native or paged._load()).sample(logits, u, temperature, top_k, top_p, min_p, out, err)
