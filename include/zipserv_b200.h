@@ -437,7 +437,8 @@ typedef struct ZsReadInt4 {
 int zs_read_int4(const ZsReadInt4* args);
 
 /* zs_paged_attention over a 4-bit cache: keys and values are what the codes stand for, not
- * rounded to 16 bits in between. q is below 2^63 in magnitude, the values' scales below
+ * rounded to 16 bits in between. softmax_scale is below 2^57 in magnitude, q below 2^63 (a
+ * query all below 2^-57 loses bits) and times softmax_scale below 2^115, the values' scales below
  * 2^100 (those far below 2^-40 count less exactly), values of a scale of 0 below 2^40. A NaN among a token's keys makes its
  * head's outputs NaN, one among its values its group's channels. dtype is q's and out's.
  * The other arguments, and the workspace, are as there; strides are below 2^32 bytes. */

@@ -747,6 +747,7 @@ PyObject* paged_attention_int4(PyObject* const* a) {
     const Table table = block_table(a[3], B, index);
     const int* lens = vec<int>(a[4], B, at::kInt, "seq_lens", index);
     const Lists l = page_lists(a[6], a[7], B, hkv, pools.k.page_size, index);
+    need(!given(a[5]) || std::fabs(number(a[5])) < 0x1p57, "softmax_scale must be below 2**57 in magnitude");
     ZsPagedAttentionInt4 p{};
     p.k_pool = pools.k;
     p.v_pool = pools.v;

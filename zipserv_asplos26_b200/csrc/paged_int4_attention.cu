@@ -5,6 +5,8 @@
 namespace zs {
 namespace {
 
+constexpr float kMostScale = 0x1p57f;        // scores are brought up by 2^69 (Q4State::unit)
+
 // CTAs of the run kernel, at most.
 inline int q4_max_ctas(int D, int G) {
     if (G <= 8) return 148 * (D == 64 ? Q4Cfg<64, 1, false>::kCtas : Q4Cfg<128, 1, false>::kCtas);
@@ -39,7 +41,7 @@ bool int4_attention_args(const ZsPagedAttentionInt4* p, Q4Args* a, int* groups) 
     if (!p || !make_int4_pool(&p->k_pool, &k) || !make_int4_pool(&p->v_pool, &v) || !same_int4_pools(p->k_pool, p->v_pool))
         return false;
     const int B = p->B, Hq = p->Hq, Hkv = k.heads, top = p->top;
-    if (B < 0 || Hq <= 0 || Hq % Hkv || p->width <= 0 || p->table_stride < p->width || !std::isfinite(p->softmax_scale) ||
+    if (B < 0 || Hq <= 0 || Hq % Hkv || p->width <= 0 || p->table_stride < p->width || !(std::fabs(p->softmax_scale) < kMostScale) ||
         (p->dtype != ZS_BF16 && p->dtype != ZS_FP16))
         return false;
     if ((long long)B * Hq > INT32_MAX || (long long)p->width << k.page_shift > INT32_MAX) return false;

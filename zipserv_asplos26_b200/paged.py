@@ -218,8 +218,8 @@ def paged_attention_int4(q: torch.Tensor, k_pages: Int4Pages, v_pages: Int4Pages
                          pages: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
                          out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
                          max_seqlen: Optional[int] = None, err: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """paged_attention over a 4-bit cache, q bf16 or fp16 (below 2**63 in magnitude). Keys and
-    values are what the codes stand for, not rounded to q's type in between. A NaN among a
+    """paged_attention over a 4-bit cache, q bf16 or fp16 (below 2**63 in magnitude;
+    softmax_scale below 2**57, the product below 2**115). Keys and values are what the codes stand for, not rounded to q's type in between. A NaN among a
     token's keys makes its head's outputs NaN, one among its values its group's channels. The
     arguments are paged_attention's but for the pools."""
     o = (_native or _load()).paged_attention_int4(q, k_pages, v_pages, block_table, seq_lens, softmax_scale, pages,
