@@ -424,8 +424,8 @@ typedef struct ZsRopeWriteInt4 {
 int zs_rope_write_int4(const ZsRopeWriteInt4* args);
 
 /* Rows of a 4-bit cache by slot: k_out and v_out [N][num_heads][head_dim], contiguous,
- * 16-byte aligned and apart from one another, what the codes stand for rounded to dtype. Slots of -1 give zeros;
- * others out of range too, and set bit 2 in *err. A slot may be listed more than once. */
+ * 16-byte aligned and apart from one another and from the pools, what the codes stand for
+ * rounded to dtype. Slots of -1 give zeros; others out of range too, and set bit 2 in *err. A slot may be listed more than once. */
 typedef struct ZsReadInt4 {
     void* stream;
     const int64_t* slots;

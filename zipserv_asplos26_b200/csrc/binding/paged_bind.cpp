@@ -748,6 +748,10 @@ PyObject* paged_attention_int4(PyObject* const* a) {
     const int* lens = vec<int>(a[4], B, at::kInt, "seq_lens", index);
     const Lists l = page_lists(a[6], a[7], B, hkv, pools.k.page_size, index);
     need(!given(a[5]) || std::fabs(number(a[5])) < 0x1p57, "softmax_scale must be below 2**57 in magnitude");
+    for (const ZsInt4Pool* x : {&pools.k, &pools.v})
+        need(std::max({x->codes_block, x->codes_token, x->codes_head}) <= UINT32_MAX &&
+                 std::max({x->params_block, x->params_token, x->params_head}) <= UINT32_MAX / 2,
+             "attention takes pools with strides below 2**32 bytes");
     ZsPagedAttentionInt4 p{};
     p.k_pool = pools.k;
     p.v_pool = pools.v;

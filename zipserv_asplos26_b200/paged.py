@@ -170,7 +170,7 @@ class Int4Pages(NamedTuple):
     max - min is not) reads back as NaN.
 
     Both tensors have contiguous rows and any strides otherwise (codes: multiples of 16;
-    params: of a row's size)."""
+    params: of a row's size; for attention below 2**32 bytes)."""
     codes: torch.Tensor     # uint8 [num_blocks, page_size, heads, dim / 2], channel 2i in the low half of byte i
     params: torch.Tensor    # bfloat16 [num_blocks, page_size, heads, 2, dim / group]: scales, then centres
 
@@ -208,7 +208,8 @@ def read_int4(k_pages: Int4Pages, v_pages: Int4Pages, slots: torch.Tensor, dtype
               out=None, err: Optional[torch.Tensor] = None):
     """Rows of a 4-bit cache by slot (int64 [N], block * page_size + row): (k, v), each
     [N, heads, dim] of dtype (bf16 or fp16), what the codes stand for rounded once. A slot of
-    -1 gives zeros. out (optional) is a pair of contiguous tensors to write to."""
+    -1 gives zeros. out (optional) is a pair of contiguous tensors to write to, apart from one
+    another and from the pools."""
     kind = {torch.bfloat16: 0, torch.float16: 1}.get(dtype, -1)
     return (_native or _load()).read_int4(k_pages, v_pages, slots, kind, out, err)
 
