@@ -20,8 +20,8 @@
 //     power of two that follows the largest scale so far, so that it has all 11 bits from
 //     there down to 2^-26 of it and vanishes below 2^-37, and its remainder follows as a
 //     second part: 22 bits, as rounding a weight must add nothing to outputs that are what
-//     is left of values that cancel (one part: 38.9 us for 42.9 at B=32 T=4129 in bf16, and such outputs
-//     off by an eighth). The centres meet p in two bf16 parts.
+//     is left of values that cancel (one part: 38.8 us for 42.8 at B=32 T=4129 in bf16, and
+//     such outputs off by an eighth). The centres meet p in two bf16 parts.
 //     The codes are centred by a f16x2 add, exact: sums of codes from 0 to 15 would in the
 //     end be far larger than the outputs that are left of them, and a tensor core's sums
 //     lose low bits. (Centring the sums every 128 tokens instead took as long.)
@@ -30,12 +30,12 @@
 // or more (base 2), so that most steps need no maximum over their lanes.
 //
 // Measured in a graph (bf16, 32 query and 8 KV heads of 128, groups of 64, pages of 64):
-// B=32 T=4129 38.9 us, 3.9 TB/s (16-bit pages 85.5 us); B=128 122, 5.0 TB/s: 5.6 as a rate
-// (85% of a plain copy's) and some 12 us of start, first lookups and join. B=1 T=131105
-// 38.4; 61 sequences of 0..16417 (fp16, 64 query heads, groups of 32, pages of 16 by token)
-// 179, 3.6 TB/s. 282 warp instructions for 16 tokens of a head, issued in half of the
+// B=32 T=4129 42.8 us, 3.6 TB/s (16-bit pages 85.5 us); B=128 137, 4.5 TB/s: 4.9 as a rate
+// (75% of a plain copy's) and some 12 us of start, first lookups and join. B=1 T=131105
+// 41.5; 61 sequences of 0..16417 (fp16, 64 query heads, groups of 32, pages of 16 by token)
+// 176 to 185, 3.6 TB/s. 316 warp instructions for 16 tokens of a head, issued in half of the
 // cycles: a warp waits for its own results, and two warps a scheduler hide part of it;
-// arithmetic (ALU) 44% busy, tensor cores 28%. DRAM reads are the algorithm's bytes (152.7
+// arithmetic (ALU) 42% busy, tensor cores 35%. DRAM reads are the algorithm's bytes (152.7
 // MB), but where rows lie by token 747 MB for 643.
 #pragma once
 
@@ -76,8 +76,8 @@ struct Q4Tile {
 
 // A step's parts, CTAs an SM and stages of a warp's ring. In runs of up to 8 heads a step
 // takes 64 tokens: what it costs beside the products counts once for four parts, and the
-// parts' sums do not wait for one another (B=32 T=4129: 38.6 us with 8 warps an SM, 41.0
-// with 12 of 32 tokens, 49.8 with 16 of 16). With 16 heads the registers hold two parts.
+// parts' sums do not wait for one another (B=32 T=4129: 42.8 us with 8 warps an SM, 45.7
+// with 12 of 32 tokens, 54.9 with 16 of 16). With 16 heads the registers hold two parts.
 // Units are short and get two parts, so that more warps share them.
 template <int D, int NT, bool kUnits>
 struct Q4Cfg {
